@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-#define SB_ABI_VERSION 7
+#define SB_ABI_VERSION 8
 
 enum sb_status {
   SB_OK = 0,
@@ -239,6 +239,73 @@ int sb_wire_unpack(const void* q, const void* scale, int64_t rows, int64_t dim, 
  * fp32; weight NULL means ones; out NULL does the residual add alone. dim % 8 == 0. */
 int sb_residual_rmsnorm(void* x, const void* y, int64_t rows, int64_t dim, const float* weight, float eps, void* out,
                         void* stream);
+
+/* ── microscaled 4-bit operands on both sides (W4A4) ────────────────────────────────────────────────
+ * NVFP4 or MXFP4 activations, quantised per row, and their product with weights of the same format:
+ * what NVFP4 checkpoints are calibrated for (the M2.5 engine's experts, m25_stage.py:288-311; MXFP4 as
+ * in fp4_act_quant, kernel.py:128-200). fmt: SB_FMT_NVFP4 or SB_FMT_MXFP4.
+ *
+ * An operand of `rows` rows of K values: codes, row r at r * kp / 2 bytes, kp = K rounded up to 32, two
+ * e2m1 codes a byte, low nibble first, zero codes behind K; scales in 512-byte atoms of 128 rows x 4
+ * scales (row r's four bytes at 16 (r % 32) + 4 (r / 32 % 4) of its atom; the atoms of a row block lie
+ * along K, row blocks follow one another; an expert bank pads each matrix to whole row blocks); for
+ * NVFP4 an fp32 tensor scale: one, or one per row. With expert groups (row p of group e iff
+ * offsets[e] <= p < offsets[e+1]; int32 on the device, ascending, offsets[0] = 0), group e's scales
+ * start at row block offsets[e] / 128 + e. Codes and scales are 16-byte aligned. */
+enum sb_dtype { SB_BF16 = 0, SB_F16 = 1, SB_F32 = 2 };
+/* Bytes of an operand's scales: n_mat matrices of `rows` rows (groups = 0), or one of `rows` rows in
+ * `groups` expert groups (n_mat = 1). 0 for arguments that the calls below refuse. */
+size_t sb_fp4_scale_bytes(int fmt, int64_t n_mat, int64_t rows, int64_t k, int64_t groups);
+/* x [src_rows, K] of `dtype`, rows row_stride elements apart -> operand of `rows` rows, K in 1..65536.
+ * rows_in (int32 [rows], or NULL: row p is x's row p): the row of x that row p takes; outside
+ * [0, src_rows) the row is zero. tensor_scale (NVFP4): fp32 [1], or NULL for one per row,
+ * max(2^-126, amax / 2688), written to row_scale fp32 [rows]. Rows behind offsets[groups] are not
+ * written. A block that holds a non-finite value gets a NaN scale. */
+int sb_fp4_quant(int fmt, const void* x, int dtype, int64_t src_rows, int64_t k, int64_t row_stride,
+                 const int32_t* rows_in, int64_t rows, const float* tensor_scale, const int32_t* offsets,
+                 int64_t groups, void* codes, void* scales, float* row_scale, void* stream);
+/* The operand's values: y [rows, K] of `dtype` = code * scale * tensor scale (no expert groups).
+ * ts: fp32 [1], [rows] with ts_per_row, or NULL for 1. */
+int sb_fp4_dequant(int fmt, const void* codes, const void* scales, const float* ts, int ts_per_row, int64_t rows,
+                   int64_t k, void* y, int dtype, void* stream);
+/* Canonical scales (NVFP4 e4m3 [n_mat, N, K/16], MXFP4 e8m0 [n_mat, N, K/32]) -> atoms. K % 32 == 0. */
+int sb_fp4_tile_scales(int fmt, const void* src, void* dst, int64_t n_mat, int64_t n, int64_t k, void* stream);
+/* y [M, N] of `dtype`, rows ldy elements apart = A W^T, summed in fp32. w_ts: fp32 [1] or NULL. */
+int sb_fp4_gemm(int fmt, const void* a_codes, const void* a_scales, const float* a_ts, int a_ts_per_row, int64_t m,
+                const void* w_codes, const void* w_scales, const float* w_ts, int64_t n, int64_t k, void* y, int dtype,
+                int64_t ldy, void* stream);
+/* The same with one W [N, K] per expert of a bank and A's rows in expert groups. Rows behind
+ * offsets[n_experts] are left as they are. w_ts: fp32 [n_experts, w_ts_n] or NULL. row_weight: fp32 [M]
+ * (each output row times its weight) or NULL. swiglu: W holds w1's and w3's rows in turn (row 2i: w1,
+ * 2i + 1: w3; w_ts_n 2 gives each its scale) and y [M, N/2] = silu(min(g, limit)) * clip(u, +-limit)
+ * (limit 0: no clamp; Expert.forward, model.py:601-611). n_experts <= 1024. */
+int sb_fp4_grouped_gemm(int fmt, const void* a_codes, const void* a_scales, const float* a_ts, int a_ts_per_row,
+                        int64_t m, const int32_t* offsets, const void* w_codes, const void* w_scales,
+                        const float* w_ts, int w_ts_n, int64_t n_experts, int64_t n, int64_t k, int swiglu,
+                        float limit, const float* row_weight, void* y, int dtype, int64_t ldy, void* stream);
+/* *host_out = 1 if a kernel of the two products gave up a bounded wait on the current device since the
+ * last call (outputs since then may be incomplete), else 0. Synchronises the stream. */
+int sb_fp4_error(int* host_out, void* stream);
+
+/* ── routing from the caller's logits ───────────────────────────────────────────────────────────── */
+enum sb_group_score { SB_GROUP_MAX = 0, SB_GROUP_TOP2 = 1 };
+/* logits [T, E] of `dtype`, rows row_stride elements apart -> weights fp32 [T, k], indices int64 [T, k] in
+ * ranking order. score: sb_score of each logit; selection by score + bias (fp32 [E] or NULL) as real
+ * numbers, ties to the lower id; with n_group > 1 (a divisor of E, <= 32) only the experts of the
+ * topk_group best groups (scored by their best expert, or by the sum of their two best) compete. Weights
+ * are the unbiased scores, divided by their sum if renormalize, times route_scale. An expert whose logit
+ * is NaN, -inf or the type's lowest value is masked: it comes after every other of the kept groups, with
+ * weight 0. E <= 1024, k <= 16, k <= topk_group * E / n_group. */
+int sb_route_topk(const void* logits, int dtype, int64_t tokens, int64_t n_experts, int64_t row_stride,
+                  const float* bias, int topk, int score, int n_group, int topk_group, int group_score,
+                  int renormalize, float route_scale, float* weights, int64_t* indices, void* stream);
+/* The pairs (token, slot) of indices int64 [T, k] sorted by expert, stable: offsets int32 [E+1], tokens int32
+ * [T k] (the token of each place), places int32 [T, k] (each pair's place). Pairs whose id is outside
+ * [0, E) are left out: place -1, and tokens behind offsets[E] are -1. E <= 1024, T k < 2^31. The workspace
+ * holds sb_expert_order_workspace_bytes (0: NULL will do) and is the call's own until it has run. */
+size_t sb_expert_order_workspace_bytes(int64_t pairs, int64_t n_experts);
+int sb_expert_order(const int64_t* indices, int64_t tokens, int topk, int64_t n_experts, int32_t* offsets,
+                    int32_t* sorted_tokens, int32_t* places, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Routing alone (Gate.forward, model.py:569-589): weights fp32 [M, k], indices int64 [M, k]. */
 int sb_moe_route(const sb_moe_layer* layer, const void* x, int64_t m, const int64_t* input_ids,

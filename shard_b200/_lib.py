@@ -15,12 +15,13 @@ SB_OK = 0
 STATUS = {0: "SB_OK", -1: "SB_ERR_ARG", -2: "SB_ERR_SHAPE", -3: "SB_ERR_FORMAT", -4: "SB_ERR_WORKSPACE",
           -5: "SB_ERR_CUDA", -6: "SB_ERR_UNSUPPORTED"}
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 SCORE = {"softmax": 0, "sigmoid": 1, "sqrtsoftplus": 2}
 MAT_PLAIN, MAT_W13 = 0, 1
 KIND_TC = 4                      # OR'ed into a tiling kind: the tensor-core (tcgen05) layout
 LAYOUT_FRAGMENT, LAYOUT_TC = 0, 1
 MODE_V4, MODE_K3 = 0, 1
+BF16, F16, F32 = 0, 1, 2          # enum sb_dtype
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -70,6 +71,18 @@ SIGNATURES = {
     "sb_wire_unpack": (_int, [_vp, _vp, _i64, _i64, _vp, _vp]),
     "sb_selftest_formats": (_int, [_vp, _vp]),
     "sb_debug_set_wait_limit": (_int, [_i64]),
+    "sb_fp4_scale_bytes": (_sz, [_int, _i64, _i64, _i64, _i64]),
+    "sb_fp4_quant": (_int, [_int, _vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
+    "sb_fp4_dequant": (_int, [_int, _vp, _vp, _vp, _int, _i64, _i64, _vp, _int, _vp]),
+    "sb_fp4_tile_scales": (_int, [_int, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "sb_fp4_gemm": (_int, [_int, _vp, _vp, _vp, _int, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _int, _i64, _vp]),
+    "sb_fp4_grouped_gemm": (_int, [_int, _vp, _vp, _vp, _int, _i64, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _int,
+                                   ctypes.c_float, _vp, _vp, _int, _i64, _vp]),
+    "sb_fp4_error": (_int, [ctypes.POINTER(ctypes.c_int), _vp]),
+    "sb_route_topk": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _int, _int, _int, _int, _int, ctypes.c_float, _vp,
+                             _vp, _vp]),
+    "sb_expert_order_workspace_bytes": (_sz, [_i64, _i64]),
+    "sb_expert_order": (_int, [_vp, _i64, _int, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "sb_residual_rmsnorm": (_int, [_vp, _vp, _i64, _i64, _vp, ctypes.c_float, _vp, _vp]),
 }
 

@@ -10,6 +10,7 @@
 #include <string>
 
 #include "../../include/shard_b200.h"
+#include "sb_fp4.h"
 #include "sb_launch.h"
 
 namespace {
@@ -1077,6 +1078,261 @@ int sb_residual_rmsnorm(void* x, const void* y, int64_t rows, int64_t dim, const
   if (rows == 0) return SB_OK;
   return cuda_check(sb::launch_residual_rmsnorm(x, y, rows, dim, weight, eps, out, (cudaStream_t)stream),
                     "residual_rmsnorm");
+}
+
+namespace {
+
+constexpr int64_t FP4_MAX_K = 65536;      // a row's values stay in the registers of one CTA
+constexpr int64_t FP4_MAX_ROWS = 1 << 30;
+constexpr int64_t FP4_MAX_GROUPS = 1024;
+
+bool fp4_fmt(int fmt) { return fmt == SB_FMT_NVFP4 || fmt == SB_FMT_MXFP4; }
+bool fp4_dtype(int dtype) { return dtype == SB_BF16 || dtype == SB_F16 || dtype == SB_F32; }
+int64_t fp4_kp(int64_t k) { return (k + 31) / 32 * 32; }
+int64_t fp4_atoms(int fmt, int64_t k) { return (fp4_kp(k) / (fmt == SB_FMT_NVFP4 ? 16 : 32) + 3) / 4; }
+int64_t fp4_blocks(int64_t n_mat, int64_t rows, int64_t groups) {
+  return groups > 0 ? rows / 128 + groups : n_mat * ((rows + 127) / 128);
+}
+
+int fp4_common(const char* what, int fmt, int dtype, int64_t rows, int64_t k) {
+  if (!fp4_fmt(fmt)) return fail(SB_ERR_FORMAT, "%s: format %d is not NVFP4 or MXFP4", what, fmt);
+  if (!fp4_dtype(dtype)) return fail(SB_ERR_ARG, "%s: dtype %d", what, dtype);
+  if (rows < 0 || rows > FP4_MAX_ROWS || k < 1 || k > FP4_MAX_K)
+    return fail(SB_ERR_SHAPE, "%s: need 0 <= rows <= 2^30 and 1 <= K <= %lld (rows=%lld K=%lld)", what,
+                (long long)FP4_MAX_K, (long long)rows, (long long)k);
+  return SB_OK;
+}
+
+// the shapes of a product: `mats` matrices [n, k] and m token rows, y rows of `width` outputs
+int fp4_product(const char* what, int fmt, int dtype, const void* const* ptrs, int n_ptrs, int64_t m, int64_t mats,
+                int64_t n, int64_t k, int64_t width, int64_t ldy) {
+  if (int rc = fp4_common(what, fmt, dtype, m, k)) return rc;
+  if (n < 1 || mats < 1 || mats > FP4_MAX_GROUPS || mats * n > FP4_MAX_ROWS)
+    return fail(SB_ERR_SHAPE, "%s: need N >= 1, 1..%lld matrices and at most 2^30 weight rows (matrices=%lld N=%lld)",
+                what, (long long)FP4_MAX_GROUPS, (long long)mats, (long long)n);
+  if ((m / 128 + mats) * ((n + 127) / 128) > FP4_MAX_ROWS)
+    return fail(SB_ERR_SHAPE, "%s: more than 2^30 tiles (M=%lld N=%lld)", what, (long long)m, (long long)n);
+  if (ldy < width) return fail(SB_ERR_SHAPE, "%s: ldy %lld is less than a row of %lld", what, (long long)ldy, (long long)width);
+  if (m == 0) return SB_OK;
+  for (int i = 0; i < n_ptrs; ++i) {
+    if (!ptrs[i]) return fail(SB_ERR_ARG, "%s: NULL pointer", what);
+    if (i < 4 && !aligned16(ptrs[i])) return fail(SB_ERR_ARG, "%s: codes and scales must be 16-byte aligned", what);
+  }
+  return SB_OK;
+}
+
+}  // namespace
+
+size_t sb_fp4_scale_bytes(int fmt, int64_t n_mat, int64_t rows, int64_t k, int64_t groups) {
+  if (!fp4_fmt(fmt) || n_mat < 1 || rows < 0 || rows > FP4_MAX_ROWS || n_mat > FP4_MAX_ROWS || k < 1 ||
+      k > FP4_MAX_K || groups < 0 || groups > FP4_MAX_GROUPS || (groups > 0 && n_mat != 1))
+    return 0;
+  return (size_t)fp4_blocks(n_mat, rows, groups) * (size_t)fp4_atoms(fmt, k) * 512;
+}
+
+int sb_fp4_quant(int fmt, const void* x, int dtype, int64_t src_rows, int64_t k, int64_t row_stride,
+                 const int32_t* rows_in, int64_t rows, const float* tensor_scale, const int32_t* offsets,
+                 int64_t groups, void* codes, void* scales, float* row_scale, void* stream) {
+  if (int rc = fp4_common("fp4_quant", fmt, dtype, rows, k)) return rc;
+  if (src_rows < 0 || src_rows > FP4_MAX_ROWS || row_stride < 0)
+    return fail(SB_ERR_SHAPE, "fp4_quant: src_rows=%lld row_stride=%lld", (long long)src_rows, (long long)row_stride);
+  if (!rows_in && rows != src_rows) return fail(SB_ERR_SHAPE, "fp4_quant: rows and src_rows differ without rows_in");
+  if (groups < 0 || groups > FP4_MAX_GROUPS || (offsets != nullptr) != (groups > 0))
+    return fail(SB_ERR_ARG, "fp4_quant: offsets and 1..%lld groups go together (groups=%lld)", (long long)FP4_MAX_GROUPS,
+                (long long)groups);
+  const bool nv = fmt == SB_FMT_NVFP4;
+  if (!nv && tensor_scale) return fail(SB_ERR_ARG, "fp4_quant: MXFP4 has no tensor scale");
+  if (rows == 0) return SB_OK;
+  if ((!x && src_rows > 0) || !codes || !scales || (nv && !tensor_scale && !row_scale))
+    return fail(SB_ERR_ARG, "fp4_quant: NULL pointer");
+  if (!aligned16(codes) || !aligned16(scales)) return fail(SB_ERR_ARG, "fp4_quant: codes and scales must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(x) % (dtype == SB_F32 ? 4 : 2)) return fail(SB_ERR_ARG, "fp4_quant: x is misaligned");
+  sb::QuantArgs q = {};
+  q.x = x;
+  q.stride = row_stride;
+  q.rows = rows;
+  q.src_rows = src_rows;
+  q.k = (int)k;
+  q.units = (int)(fp4_kp(k) / 16);
+  q.nv = nv;
+  q.rows_in = rows_in;
+  q.offsets = offsets;
+  q.groups = (int)groups;
+  q.blocks = fp4_blocks(1, rows, groups);
+  q.ts = tensor_scale;
+  q.row_ts = row_scale;
+  q.codes = (uint8_t*)codes;
+  q.row_bytes = fp4_kp(k) / 2;
+  q.scales = (uint8_t*)scales;
+  q.atoms = fp4_atoms(fmt, k);
+  return cuda_check(sb::launch_fp4_quant(q, dtype, (cudaStream_t)stream), "fp4_quant");
+}
+
+int sb_fp4_dequant(int fmt, const void* codes, const void* scales, const float* ts, int ts_per_row, int64_t rows,
+                   int64_t k, void* y, int dtype, void* stream) {
+  if (int rc = fp4_common("fp4_dequant", fmt, dtype, rows, k)) return rc;
+  if (fmt == SB_FMT_MXFP4 && ts) return fail(SB_ERR_ARG, "fp4_dequant: MXFP4 has no tensor scale");
+  if (rows == 0) return SB_OK;
+  if (!codes || !scales || !y) return fail(SB_ERR_ARG, "fp4_dequant: NULL pointer");
+  if (!aligned16(codes) || !aligned16(scales)) return fail(SB_ERR_ARG, "fp4_dequant: codes and scales must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(y) % (dtype == SB_F32 ? 4 : 2)) return fail(SB_ERR_ARG, "fp4_dequant: y is misaligned");
+  sb::DequantArgs d = {};
+  d.codes = (const uint8_t*)codes;
+  d.scales = (const uint8_t*)scales;
+  d.ts = ts;
+  d.ts_row = ts_per_row;
+  d.rows = rows;
+  d.k = (int)k;
+  d.units = (int)(fp4_kp(k) / 16);
+  d.nv = fmt == SB_FMT_NVFP4;
+  d.row_bytes = fp4_kp(k) / 2;
+  d.atoms = fp4_atoms(fmt, k);
+  d.y = y;
+  return cuda_check(sb::launch_fp4_dequant(d, dtype, (cudaStream_t)stream), "fp4_dequant");
+}
+
+int sb_fp4_tile_scales(int fmt, const void* src, void* dst, int64_t n_mat, int64_t n, int64_t k, void* stream) {
+  if (int rc = fp4_common("fp4_tile_scales", fmt, SB_BF16, n, k)) return rc;
+  if (k % 32 || n_mat < 1 || n < 1 || n_mat * n > FP4_MAX_ROWS)
+    return fail(SB_ERR_SHAPE, "fp4_tile_scales: need K %% 32 == 0 and 1..2^30 rows (n_mat=%lld n=%lld k=%lld)",
+                (long long)n_mat, (long long)n, (long long)k);
+  if (!src || !dst) return fail(SB_ERR_ARG, "fp4_tile_scales: NULL pointer");
+  if (!aligned16(dst)) return fail(SB_ERR_ARG, "fp4_tile_scales: dst must be 16-byte aligned");
+  return cuda_check(sb::launch_fp4_tile_scales((const uint8_t*)src, (uint8_t*)dst, n_mat, n,
+                                               k / (fmt == SB_FMT_NVFP4 ? 16 : 32), (cudaStream_t)stream),
+                    "fp4_tile_scales");
+}
+
+int sb_fp4_gemm(int fmt, const void* a_codes, const void* a_scales, const float* a_ts, int a_ts_per_row, int64_t m,
+                const void* w_codes, const void* w_scales, const float* w_ts, int64_t n, int64_t k, void* y, int dtype,
+                int64_t ldy, void* stream) {
+  const void* ptrs[] = {a_codes, a_scales, w_codes, w_scales, y};
+  if (int rc = fp4_product("fp4_gemm", fmt, dtype, ptrs, 5, m, 1, n, k, n, ldy)) return rc;
+  if (fmt == SB_FMT_MXFP4 && (a_ts || w_ts)) return fail(SB_ERR_ARG, "fp4_gemm: MXFP4 has no tensor scale");
+  if (m == 0) return SB_OK;
+  sb::Fp4MmArgs g = {};
+  g.w = (const uint8_t*)w_codes;
+  g.w_s = (const uint8_t*)w_scales;
+  g.w_ts = w_ts;
+  g.w_ts_n = 1;
+  g.a = (const uint8_t*)a_codes;
+  g.a_s = (const uint8_t*)a_scales;
+  g.a_ts = a_ts;
+  g.a_ts_row = a_ts_per_row;
+  g.nv = fmt == SB_FMT_NVFP4;
+  g.mats = 1;
+  g.n = (int)n;
+  g.m = (int)m;
+  g.kp = (int)fp4_kp(k);
+  g.y = y;
+  g.ldy = ldy;
+  return cuda_check(sb::launch_fp4_mm(g, dtype, (cudaStream_t)stream), "fp4_gemm");
+}
+
+int sb_fp4_grouped_gemm(int fmt, const void* a_codes, const void* a_scales, const float* a_ts, int a_ts_per_row,
+                        int64_t m, const int32_t* offsets, const void* w_codes, const void* w_scales,
+                        const float* w_ts, int w_ts_n, int64_t n_experts, int64_t n, int64_t k, int swiglu,
+                        float limit, const float* row_weight, void* y, int dtype, int64_t ldy, void* stream) {
+  const void* ptrs[] = {a_codes, a_scales, w_codes, w_scales, y, offsets};
+  if (int rc = fp4_product("fp4_grouped_gemm", fmt, dtype, ptrs, 6, m, n_experts, n, k, swiglu ? n / 2 : n, ldy)) return rc;
+  if (fmt == SB_FMT_MXFP4 && (a_ts || w_ts)) return fail(SB_ERR_ARG, "fp4_grouped_gemm: MXFP4 has no tensor scale");
+  if (swiglu && n % 2) return fail(SB_ERR_SHAPE, "fp4_grouped_gemm: swiglu needs an even N (%lld)", (long long)n);
+  if (w_ts && w_ts_n != 1 && w_ts_n != 2) return fail(SB_ERR_ARG, "fp4_grouped_gemm: w_ts_n %d", w_ts_n);
+  if (!(limit >= 0.f)) return fail(SB_ERR_ARG, "fp4_grouped_gemm: limit must be >= 0");
+  if (m == 0) return SB_OK;
+  sb::Fp4MmArgs g = {};
+  g.w = (const uint8_t*)w_codes;
+  g.w_s = (const uint8_t*)w_scales;
+  g.w_ts = w_ts;
+  g.w_ts_n = w_ts_n;
+  g.a = (const uint8_t*)a_codes;
+  g.a_s = (const uint8_t*)a_scales;
+  g.a_ts = a_ts;
+  g.a_ts_row = a_ts_per_row;
+  g.row_weight = row_weight;
+  g.offsets = offsets;
+  g.nv = fmt == SB_FMT_NVFP4;
+  g.mats = (int)n_experts;
+  g.n = (int)n;
+  g.m = (int)m;
+  g.kp = (int)fp4_kp(k);
+  g.y = y;
+  g.ldy = ldy;
+  g.swiglu = swiglu;
+  g.limit = limit;
+  return cuda_check(sb::launch_fp4_mm(g, dtype, (cudaStream_t)stream), "fp4_grouped_gemm");
+}
+
+int sb_fp4_error(int* host_out, void* stream) {
+  if (!host_out) return fail(SB_ERR_ARG, "fp4_error: NULL pointer");
+  return cuda_check(sb::fp4_mm_error(host_out, (cudaStream_t)stream), "fp4_error");
+}
+
+int sb_route_topk(const void* logits, int dtype, int64_t tokens, int64_t n_experts, int64_t row_stride,
+                  const float* bias, int topk, int score, int n_group, int topk_group, int group_score,
+                  int renormalize, float route_scale, float* weights, int64_t* indices, void* stream) {
+  if (!fp4_dtype(dtype)) return fail(SB_ERR_ARG, "route_topk: dtype %d", dtype);
+  if (score != SB_SCORE_SOFTMAX && score != SB_SCORE_SIGMOID && score != SB_SCORE_SQRTSOFTPLUS)
+    return fail(SB_ERR_ARG, "route_topk: score %d", score);
+  if (group_score != SB_GROUP_MAX && group_score != SB_GROUP_TOP2)
+    return fail(SB_ERR_ARG, "route_topk: group_score %d", group_score);
+  if (tokens < 0 || tokens > (1 << 30) || n_experts < 1 || n_experts > 1024 || row_stride < 0)
+    return fail(SB_ERR_SHAPE, "route_topk: need 0 <= T <= 2^30 and 1 <= E <= 1024 (T=%lld E=%lld row_stride=%lld)",
+                (long long)tokens, (long long)n_experts, (long long)row_stride);
+  if (n_group < 1 || n_group > 32 || n_experts % n_group || topk_group < 1 || topk_group > n_group)
+    return fail(SB_ERR_SHAPE, "route_topk: n_group %d must divide E (<= 32), topk_group %d lie in 1..n_group", n_group,
+                topk_group);
+  if (topk < 1 || topk > 16 || topk > topk_group * (n_experts / n_group))
+    return fail(SB_ERR_SHAPE, "route_topk: topk %d must lie in 1..16 and in the kept groups' experts", topk);
+  if (tokens == 0) return SB_OK;
+  if (!logits || !weights || !indices) return fail(SB_ERR_ARG, "route_topk: NULL pointer");
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == SB_F32 ? 4 : 2)) return fail(SB_ERR_ARG, "route_topk: logits are misaligned");
+  sb::TopkArgs a = {};
+  a.logits = logits;
+  a.stride = row_stride;
+  a.tokens = tokens;
+  a.bias = bias;
+  a.experts = (int)n_experts;
+  a.topk = topk;
+  a.score = score;
+  a.groups = n_group;
+  a.kept = topk_group;
+  a.group_two = group_score == SB_GROUP_TOP2;
+  a.renorm = renormalize;
+  a.scale = route_scale;
+  a.weights = weights;
+  a.ids = indices;
+  return cuda_check(sb::launch_topk(a, dtype, (cudaStream_t)stream), "route_topk");
+}
+
+size_t sb_expert_order_workspace_bytes(int64_t pairs, int64_t n_experts) {
+  if (pairs < 0 || pairs > INT32_MAX || n_experts < 1 || n_experts > 1024) return 0;
+  const int64_t b = sb::order_blocks(pairs);
+  return b > 1 ? (size_t)b * (size_t)n_experts * sizeof(int32_t) : 0;
+}
+
+int sb_expert_order(const int64_t* indices, int64_t tokens, int topk, int64_t n_experts, int32_t* offsets,
+                    int32_t* sorted_tokens, int32_t* places, void* workspace, size_t workspace_bytes, void* stream) {
+  if (tokens < 0 || topk < 1 || tokens > INT32_MAX / topk || n_experts < 1 || n_experts > 1024)
+    return fail(SB_ERR_SHAPE, "expert_order: need T k < 2^31 and 1 <= E <= 1024 (T=%lld k=%d E=%lld)", (long long)tokens,
+                topk, (long long)n_experts);
+  const int64_t pairs = tokens * topk;
+  if (!offsets || (pairs > 0 && (!indices || !sorted_tokens || !places))) return fail(SB_ERR_ARG, "expert_order: NULL pointer");
+  const size_t need = sb_expert_order_workspace_bytes(pairs, n_experts);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(SB_ERR_WORKSPACE, "expert_order: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
+  if (reinterpret_cast<uintptr_t>(workspace) & 3u) return fail(SB_ERR_ARG, "expert_order: workspace must be 4-byte aligned");
+  sb::OrderArgs a = {};
+  a.ids = indices;
+  a.pairs = pairs;
+  a.topk = topk;
+  a.experts = (int)n_experts;
+  a.blocks = (int)(pairs > 0 ? sb::order_blocks(pairs) : 1);
+  a.hist = (int32_t*)workspace;
+  a.offsets = offsets;
+  a.tokens = sorted_tokens;
+  a.places = places;
+  return cuda_check(sb::launch_expert_order(a, (cudaStream_t)stream), "expert_order");
 }
 
 int sb_debug_set_wait_limit(int64_t polls) {

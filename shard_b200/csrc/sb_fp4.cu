@@ -1,0 +1,441 @@
+// Microscaled 4-bit floating point: quantisation of activations, its inverse, and the scale layout
+// of the fp4 x fp4 products (sb_fp4mm.cu).
+//
+//   MXFP4  per 32 values: s = 2^t, t the smallest integer with amax <= 6 2^t (t >= -126)
+//   NVFP4  per 16 values: s = e4m3(min(448, amax / (6 ts))), ts the fp32 tensor scale: the caller's, or
+//          one per row, max(2^-126, amax_row / 2688)
+//   q = e2m1(x / (s ts)) to nearest, ties to the even code, saturating at 6
+//
+// Quotients are rounded as the real quotient is: a plain fp32 division may land on a border between
+// two codes that the real number only comes near, so each value is rounded from both ends of an
+// interval around its quotient, and where these differ the border is compared exactly. A block that
+// holds a non-finite value gets a NaN scale and zero codes, and does not count for its row's scale.
+//
+// Operand layout. Codes are row-major, row r at r * kp / 2, kp = K rounded up to 32 (zero codes behind
+// K). Scales lie in atoms of 128 rows x 4 scales, 512 bytes, the source form of the scale-factor copy
+// into tensor memory: row r's word at 16 (r % 32) + 4 (r / 32 % 4); atoms along K, then row blocks.
+// With expert groups, group e starts at row block offsets[e] / 128 + e, so that every group starts
+// its own atoms and any row finds its place from the offsets alone.
+//
+// Both directions are bound by HBM at prompt sizes and by launch latency at one row.
+#include "sb_device.cuh"
+#include "sb_fp4.h"
+#include "sb_launch.h"
+
+namespace sb {
+namespace fp4 {
+
+// eight floats -> eight e2m1 codes, value 0 in the low nibble
+__device__ __forceinline__ uint32_t cvt8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n .reg .b8 b0, b1, b2, b3;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n"
+      " mov.b32 %0, {b0, b1, b2, b3};\n}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// the border between e2m1 magnitudes c and c + 1
+__device__ __forceinline__ float border(uint32_t c) {
+  return c < 4 ? 0.25f + 0.5f * (float)c : (c == 4 ? 2.5f : (c == 5 ? 3.5f : 5.0f));
+}
+
+// fp32 arithmetic decides exactly while nothing under- or overflows
+__device__ __forceinline__ bool mid_range(float v) { return v >= 7.9e-31f && v <= 1.2e30f; }
+
+// e4m3 code of min(448, a / (6 ts))
+__device__ __noinline__ uint32_t scale_exact(float a, float ts) {
+  const double v = (double)a / (6.0 * (double)ts);
+  uint32_t lo = 0, hi = 126;   // largest code not above v (e4m3 codes ascend with their values)
+  if (v >= 448.0) return 126;
+  while (hi - lo > 1) {
+    const uint32_t c = (lo + hi) >> 1;
+    if ((double)e4m3_to_f32(c) <= v) lo = c; else hi = c;
+  }
+  const double mid = 0.5 * ((double)e4m3_to_f32(lo) + (double)e4m3_to_f32(lo + 1));
+  return v > mid || (v == mid && (lo & 1u)) ? lo + 1 : lo;
+}
+
+__device__ __forceinline__ uint32_t scale_code(float a, float ts, float inv6ts, bool mid) {
+  const float v = a * inv6ts;
+  const uint32_t lo = f32_to_e4m3(v * (1.f - 9.6e-7f)), hi = f32_to_e4m3(v * (1.f + 9.6e-7f));
+  return (mid && lo == hi) ? lo : scale_exact(a, ts);
+}
+
+// magnitude code of |x| / (s ts)
+__device__ __noinline__ uint32_t code_exact(float x, float s, float ts) {
+  const double d = (double)s * (double)ts, v = fabs((double)x);
+  uint32_t c = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < 7; ++i) {
+    const double m = (double)border(i) * d;
+    if (v > m || (v == m && (i & 1u))) c = i + 1;
+  }
+  return c;
+}
+
+template <typename T>
+struct Traits;
+template <>
+struct Traits<__nv_bfloat16> {
+  static constexpr uint32_t INF = 0x7F80u;
+  static __device__ __forceinline__ float f(uint32_t h) { return __uint_as_float(h << 16); }
+};
+template <>
+struct Traits<__half> {
+  static constexpr uint32_t INF = 0x7C00u;
+  static __device__ __forceinline__ float f(uint32_t h) { return __half2float(__ushort_as_half((unsigned short)h)); }
+};
+
+// 16 consecutive values of a row
+template <typename T>
+struct Unit {
+  uint32_t w[8];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void load(const T* p) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  }
+  __device__ __forceinline__ void load_tail(const T* p, int n) {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t a = 2 * i < n ? q[2 * i] : 0u, b = 2 * i + 1 < n ? q[2 * i + 1] : 0u;
+      w[i] = a | (b << 16);
+    }
+  }
+  // bits of the largest magnitude as fp32 (0x7F800000 and above: not finite)
+  __device__ __forceinline__ uint32_t amax() const {
+    uint32_t m = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    const uint32_t h = max(m & 0xFFFFu, m >> 16);
+    return h >= Traits<T>::INF ? 0x7FC00000u : __float_as_uint(Traits<T>::f(h));
+  }
+  __device__ __forceinline__ float get(int i) const {
+    return Traits<T>::f((i & 1) ? (w[i >> 1] >> 16) : (w[i >> 1] & 0xFFFFu));
+  }
+};
+template <>
+struct Unit<float> {
+  float v[16];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.f;
+  }
+  __device__ __forceinline__ void load(const float* p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(p) + i);
+      v[4 * i] = a.x; v[4 * i + 1] = a.y; v[4 * i + 2] = a.z; v[4 * i + 3] = a.w;
+    }
+  }
+  __device__ __forceinline__ void load_tail(const float* p, int n) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = i < n ? p[i] : 0.f;
+  }
+  __device__ __forceinline__ uint32_t amax() const {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return m;
+  }
+  __device__ __forceinline__ float get(int i) const { return v[i]; }
+};
+
+constexpr uint32_t F32_INF = 0x7F800000u;
+
+// the unit's 16 codes for the scale s ts (NVFP4)
+template <typename T>
+__device__ __forceinline__ uint2 codes_nv(const Unit<T>& u, float s, float ts) {
+  const float p = s * ts;
+  if (!(p > 0.f) && s == 0.f) return make_uint2(0u, 0u);
+  uint32_t out[2];
+  if (mid_range(p) && mid_range(ts)) {
+    const float inv = __frcp_rn(p), lo = inv * (1.f - 9.6e-7f), hi = inv * (1.f + 9.6e-7f);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float a[8], b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = u.get(8 * h + i);
+        a[i] = x * lo;
+        b[i] = x * hi;
+      }
+      out[h] = cvt8(a);
+      const uint32_t diff = out[h] ^ cvt8(b);
+      if (diff != 0u) {
+        const float e = fmaf(s, ts, -p);   // s ts = p + e exactly
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if ((diff >> (4 * i)) & 0xFu) {
+            // |x| - m (p + e): the first difference is exact this near to the border m p
+            const uint32_t c = (out[h] >> (4 * i)) & 7u;
+            const float m = border(c), r = fmaf(-m, e, fmaf(-m, p, fabsf(u.get(8 * h + i))));
+            if (r > 0.f || (r == 0.f && (c & 1u))) out[h] += 1u << (4 * i);
+          }
+        }
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      out[h] = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = h ? u.get(8 + i) : u.get(i);
+        const uint32_t c = code_exact(x, s, ts) | (x < 0.f ? 8u : 0u);
+        out[h] |= c << (4 * i);
+      }
+    }
+  }
+  return make_uint2(out[0], out[1]);
+}
+
+template <typename T>
+__device__ __forceinline__ uint2 codes_mx(const Unit<T>& u, float inv) {
+  float a[8], b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    a[i] = u.get(i) * inv;
+    b[i] = u.get(8 + i) * inv;
+  }
+  return make_uint2(cvt8(a), cvt8(b));
+}
+
+// Warps [0, wpr) of each row's warps share the row; lane u of them takes units u, u + 32 wpr, ...
+// (16 values each, all loads issued before any is used). V units a thread: 4 keep enough bytes in
+// flight per thread for the large sizes, 1 spreads a few rows over more threads.
+template <typename T, bool NV, int V, bool VEC>
+__global__ void __launch_bounds__(1024) quant_kernel(QuantArgs a) {
+  __shared__ uint32_t red[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rpc = (blockDim.x >> 5) / a.wpr;
+  const int rw = warp / a.wpr, tr = threadIdx.x - rw * a.wpr * 32;
+  const int64_t row = (int64_t)blockIdx.x * rpc + rw;
+  pdl_wait();
+  pdl_trigger();
+  int64_t src = row;
+  int64_t pos = row;    // the row's place among the scale atoms' rows
+  bool live = row < a.rows;
+  if (a.offsets != nullptr) {
+    // group of the row: how many groups end at or before it
+    int g = 0;
+    for (int i = lane; i < a.groups; i += 32) g += a.offsets[i + 1] <= row ? 1 : 0;
+    g = __reduce_add_sync(0xffffffffu, g);
+    live = live && g < a.groups;
+    if (live) {
+      const int64_t o = a.offsets[g];
+      pos = ((o >> 7) + g) * 128 + (row - o);
+      if (o < 0 || o > row || pos >= a.blocks * 128) live = false;
+    }
+  }
+  bool has = live;
+  if (live && a.rows_in != nullptr) {
+    src = a.rows_in[row];
+    has = src >= 0 && src < a.src_rows;   // no such row: zeros
+  }
+  const T* xr = reinterpret_cast<const T*>(a.x) + (has ? src : 0) * a.stride;
+  const int step = a.wpr * 32;
+  Unit<T> u[V];
+  uint32_t am[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int k = tr + i * step;
+    u[i].zero();
+    if (has && k < a.units) {
+      if (VEC && (k + 1) * 16 <= a.k) {
+        u[i].load(xr + (int64_t)k * 16);
+      } else if (k * 16 < a.k) {
+        u[i].load_tail(xr + (int64_t)k * 16, a.k - k * 16);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) am[i] = u[i].amax();
+  float ts = 1.f;
+  if (NV) {
+    if (a.ts != nullptr) {
+      ts = *a.ts;
+    } else {
+      uint32_t m = 0u;
+#pragma unroll
+      for (int i = 0; i < V; ++i) m = max(m, am[i] < F32_INF ? am[i] : 0u);
+      m = __reduce_max_sync(0xffffffffu, m);
+      if (a.wpr > 1) {
+        if (lane == 0) red[warp] = m;
+        __syncthreads();
+        m = lane < a.wpr ? red[rw * a.wpr + lane] : 0u;
+        m = __reduce_max_sync(0xffffffffu, m);
+      }
+      ts = fmaxf(__fdiv_rn(__uint_as_float(m), 2688.f), 1.17549435e-38f);
+      if (live && tr == 0) a.row_ts[row] = ts;
+    }
+  }
+  if (!live) return;   // whole warps: a row's warps share `live`
+  const bool ts_ok = ts > 0.f && __float_as_uint(ts) < F32_INF;
+  const bool ts_mid = mid_range(ts);
+  const float inv6 = NV ? __frcp_rn(6.f * ts) : 0.f;
+  uint8_t* cr = a.codes + row * a.row_bytes;
+  uint8_t* sr = a.scales + ((pos >> 7) * a.atoms) * 512 + (pos & 31) * 16 + ((pos >> 5) & 3) * 4;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int k = tr + i * step;
+    uint32_t sc;
+    uint2 c = make_uint2(0u, 0u);
+    if (NV) {
+      const bool fine = am[i] < F32_INF && ts_ok;
+      sc = fine ? scale_code(__uint_as_float(am[i]), ts, inv6, ts_mid) : 0x7Fu;
+      if (fine) c = codes_nv<T>(u[i], e4m3_to_f32(sc), ts);
+      if (k >= a.units) sc = 0u;
+      uint32_t w = sc << (8 * (k & 3));
+      w |= __shfl_xor_sync(0xffffffffu, w, 1);
+      w |= __shfl_xor_sync(0xffffffffu, w, 2);
+      if (k < a.units && (k & 3) == 0) *reinterpret_cast<uint32_t*>(sr + (int64_t)(k >> 2) * 512) = w;
+    } else {
+      const uint32_t m = max(am[i], __shfl_xor_sync(0xffffffffu, am[i], 1));
+      // amax = f 2^e: t = e - 2 for f <= 1.5, else e - 1; biased and floored at 2^-126
+      sc = m < F32_INF ? (uint32_t)max((int)((m + 0x3FFFFFu) >> 23) - 2, 1) : 0xFFu;
+      if (m < F32_INF) c = codes_mx<T>(u[i], __uint_as_float((254u - sc) << 23));
+      if (k >= a.units) sc = 0u;
+      uint32_t w = sc << (8 * ((k >> 1) & 3));
+      w |= __shfl_xor_sync(0xffffffffu, w, 2);
+      w |= __shfl_xor_sync(0xffffffffu, w, 4);
+      if (k < a.units && (k & 7) == 0) *reinterpret_cast<uint32_t*>(sr + (int64_t)(k >> 3) * 512) = w;
+    }
+    if (k < a.units) *reinterpret_cast<uint2*>(cr + (int64_t)k * 8) = c;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ T to_out(float v);
+template <>
+__device__ __forceinline__ float to_out<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half to_out<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 to_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// y = code s ts: code s is exact in fp32 (6 significant bits), the product with ts rounds once. A thread
+// takes 16 values.
+template <typename T, bool NV>
+__global__ void __launch_bounds__(256) dequant_kernel(DequantArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t total = a.rows * a.units;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i / a.units;
+    const int k = (int)(i - row * a.units);
+    const uint2 c = *reinterpret_cast<const uint2*>(a.codes + row * a.row_bytes + (int64_t)k * 8);
+    const int b = NV ? k : k >> 1;
+    const uint32_t sb = a.scales[((row >> 7) * a.atoms + (b >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (b & 3)];
+    float s = NV ? e4m3_to_f32(sb) : (sb == 0xFFu ? __uint_as_float(0x7FC00000u) : e8m0_to_f32(sb));
+    const float ts = NV && a.ts != nullptr ? a.ts[a.ts_row ? row : 0] : 1.f;
+    T o[16];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t h = e2m1x2_to_f16x2((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      o[2 * j] = to_out<T>(f.x * s * ts);
+      o[2 * j + 1] = to_out<T>(f.y * s * ts);
+    }
+    T* y = reinterpret_cast<T*>(a.y) + row * a.k + (int64_t)k * 16;
+    const int left = a.k - k * 16;
+    if (a.vec && left >= 16) {
+#pragma unroll
+      for (int j = 0; j < (int)sizeof(T); ++j) reinterpret_cast<uint4*>(y)[j] = reinterpret_cast<const uint4*>(o)[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j < left) y[j] = o[j];
+    }
+  }
+}
+
+// canonical scales [mats][n][nb] bytes -> atoms, each matrix padded to whole row blocks (zero scales)
+__global__ void __launch_bounds__(256) tile_scales_kernel(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst,
+                                                          int64_t mats, int64_t n, int64_t nb, int64_t atoms) {
+  pdl_wait();
+  const int64_t blocks = (n + 127) >> 7;
+  const int64_t words = mats * blocks * atoms * 128;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < words; i += (int64_t)gridDim.x * blockDim.x) {
+    const int in = (int)(i & 127);                // word of the atom: row 32 (in % 4) + in / 4
+    const int64_t at = (i >> 7) % atoms, blk = (i >> 7) / atoms;
+    const int64_t mat = blk / blocks, r = (blk % blocks) * 128 + 32 * (in & 3) + (in >> 2);
+    uint32_t w = 0u;
+    if (r < n) {
+      const uint8_t* s = src + (mat * n + r) * nb + at * 4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (at * 4 + j < nb) w |= (uint32_t)s[j] << (8 * j);
+    }
+    reinterpret_cast<uint32_t*>(dst)[i] = w;
+  }
+}
+
+template <typename T, bool NV, bool VEC>
+static cudaError_t launch_quant_v(const QuantArgs& q, int v, dim3 grid, dim3 block, cudaStream_t st) {
+  if (v == 1) return launch_pdl(quant_kernel<T, NV, 1, VEC>, grid, block, 0, st, q);
+  if (v == 2) return launch_pdl(quant_kernel<T, NV, 2, VEC>, grid, block, 0, st, q);
+  return launch_pdl(quant_kernel<T, NV, 4, VEC>, grid, block, 0, st, q);
+}
+
+template <typename T>
+static cudaError_t launch_quant_t(const QuantArgs& q, int v, bool vec, dim3 grid, dim3 block, cudaStream_t st) {
+  if (q.nv) return vec ? launch_quant_v<T, true, true>(q, v, grid, block, st) : launch_quant_v<T, true, false>(q, v, grid, block, st);
+  return vec ? launch_quant_v<T, false, true>(q, v, grid, block, st) : launch_quant_v<T, false, false>(q, v, grid, block, st);
+}
+
+}  // namespace fp4
+
+cudaError_t launch_fp4_quant(const QuantArgs& args, int dtype, cudaStream_t st) {
+  QuantArgs q = args;
+  // units per thread: one while the rows do not fill the GPU, else four
+  const int64_t per = (int64_t)num_sms() * 1024;
+  int v = q.rows * q.units <= per ? 1 : (q.rows * q.units <= 2 * per ? 2 : 4);
+  while ((q.units + 32 * v - 1) / (32 * v) > 32) v *= 2;
+  q.wpr = (q.units + 32 * v - 1) / (32 * v);
+  const int rpc = q.wpr >= 8 ? 1 : 8 / q.wpr;
+  const dim3 grid((unsigned)((q.rows + rpc - 1) / rpc)), block(rpc * q.wpr * 32);
+  const int es = dtype == SB_F32 ? 4 : 2;
+  const bool vec = (reinterpret_cast<uintptr_t>(q.x) & 15u) == 0 && (q.stride * es) % 16 == 0;
+  if (dtype == SB_F32) return fp4::launch_quant_t<float>(q, v, vec, grid, block, st);
+  if (dtype == SB_F16) return fp4::launch_quant_t<__half>(q, v, vec, grid, block, st);
+  return fp4::launch_quant_t<__nv_bfloat16>(q, v, vec, grid, block, st);
+}
+
+template <typename T>
+static cudaError_t launch_dequant_t(const DequantArgs& a, dim3 grid, cudaStream_t st) {
+  if (a.nv) return launch_pdl(fp4::dequant_kernel<T, true>, grid, dim3(256), 0, st, a);
+  return launch_pdl(fp4::dequant_kernel<T, false>, grid, dim3(256), 0, st, a);
+}
+
+static unsigned grid_of(int64_t work, int64_t cap) {
+  const int64_t g = (work + 255) / 256;
+  return (unsigned)(g < 1 ? 1 : (g < cap ? g : cap));
+}
+
+cudaError_t launch_fp4_dequant(const DequantArgs& args, int dtype, cudaStream_t st) {
+  DequantArgs a = args;
+  const int es = dtype == SB_F32 ? 4 : 2;
+  a.vec = (reinterpret_cast<uintptr_t>(a.y) & 15u) == 0 && (a.k * es) % 16 == 0;
+  const dim3 grid(grid_of(a.rows * a.units, (int64_t)num_sms() * 64));
+  if (dtype == SB_F32) return launch_dequant_t<float>(a, grid, st);
+  if (dtype == SB_F16) return launch_dequant_t<__half>(a, grid, st);
+  return launch_dequant_t<__nv_bfloat16>(a, grid, st);
+}
+
+cudaError_t launch_fp4_tile_scales(const uint8_t* src, uint8_t* dst, int64_t mats, int64_t n, int64_t nb,
+                                   cudaStream_t st) {
+  const int64_t atoms = (nb + 3) / 4, words = mats * ((n + 127) / 128) * atoms * 128;
+  return launch_pdl(fp4::tile_scales_kernel, dim3(grid_of(words, (int64_t)num_sms() * 64)), dim3(256), 0, st, src, dst,
+                    mats, n, nb, atoms);
+}
+
+}  // namespace sb

@@ -1,0 +1,338 @@
+"""shard_b200.fp4 (W4A4) against plain 64-bit forms.
+
+Quantisation and its inverse are compared exactly. The products' tolerance, with S = sum_k |a_k w_k|: the
+tensor core adds K / 64 partial sums in fp32, each with an error of at most 2^-22 of the sums involved
+(<= S); the epilogue rounds twice in fp32 and once to the output type:
+
+    |y - exact| <= (K / 64 + 2) 2^-22 S + (eps_out / 2 + 2^-23) |exact|
+"""
+import math
+
+import pytest
+import torch
+
+import fp4_plain as P
+from shard_b200 import formats as F
+from shard_b200 import fp4
+
+NV, MX = F.FMT_NVFP4, F.FMT_MXFP4
+gpu = pytest.mark.gpu
+
+
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+
+
+def _acts(m, k, dtype, seed=0, spread=2.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(m, k, generator=g) * torch.exp(spread * torch.randn(m, 1, generator=g))).to(dtype)
+
+
+def _check_quant(x, q, fmt, ts=None):
+    codes, sb, t = P.quant(x, fmt, ts)
+    assert torch.equal(q.canonical_scales().cpu(), sb), "block scales"
+    if t is not None:
+        assert torch.equal(q.ts.cpu(), t), "row scales"
+    got = P.unpack(q.codes)
+    # a zero's sign is not part of its value
+    zero = (codes & 7) == 0
+    assert torch.equal(torch.where(zero, 0, got & 7), torch.where(zero, 0, codes & 7)) and \
+        torch.equal(torch.where(zero, 0, got), torch.where(zero, 0, codes)), "codes"
+    return codes, sb, t
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,k", [(1, 1), (3, 17), (5, 32), (2, 100), (130, 96), (33, 1056), (3, 7168), (1, 65536)])
+def test_quant_and_dequant_are_exact(fmt, dtype, m, k):
+    _need_gpu()
+    x = _acts(m, k, dtype, seed=m + k)
+    q = fp4.quant(x.cuda(), fmt)
+    codes, sb, t = _check_quant(x, q, fmt)
+    v = P.values(codes, sb, fmt, t)[:, :k]
+    y = fp4.dequant(q, torch.float32).cpu()
+    assert torch.equal(y, v.float())          # code * scale is exact, times ts rounds once
+    for out in (torch.bfloat16, torch.float16):
+        # fp32 first, then the output type: at most one step apart from rounding once, half a step off
+        d = (fp4.dequant(q, out).cpu().double() - v).abs()
+        lim = v.abs() * (torch.finfo(out).eps / 2 + 2.0 ** -24) + torch.finfo(out).smallest_normal * torch.finfo(out).eps
+        assert bool((d <= lim)[v.abs() < torch.finfo(out).max].all())
+
+
+@gpu
+@pytest.mark.parametrize("ts", [1.0, 0.0148810, 2.0 ** -10, 3.4e-38, 1e-42, 1e30])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quant_with_a_calibrated_scale(ts, dtype):
+    """Powers of two put many values exactly on a border; tiny and huge scales leave fp32's range."""
+    _need_gpu()
+    x = _acts(37, 256, dtype, seed=7, spread=1.0)
+    if ts < 1e-30 or ts > 1e20:
+        x = (x.double() * ts * 100).to(dtype)
+    t = torch.tensor([ts], dtype=torch.float32)
+    q = fp4.quant(x.cuda(), NV, tensor_scale=t.cuda())
+    _check_quant(x, q, NV, t)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+def test_quant_borders(fmt):
+    """Values on the borders between codes and one fp32 step to either side, under scales that divide
+    them exactly and scales that do not."""
+    _need_gpu()
+    rows = []
+    for s in (1.0, 0.75, 1 / 3, 1.1, 2.0 ** -20, 7e4):
+        mids = torch.tensor(F.E2M1_MID, dtype=torch.float64) * s
+        r = [torch.tensor([6.0 * s], dtype=torch.float64), mids, -mids]
+        f = torch.cat(r).float()
+        up, dn = torch.nextafter(f, torch.tensor(math.inf)), torch.nextafter(f, torch.tensor(-math.inf))
+        for v in (f, up, dn):
+            v = v.clone()
+            v[0] = f[0]
+            rows.append(torch.cat([v, f[:1]]))
+    x = torch.stack(rows)                       # [18, 16]
+    x = torch.cat([x, x.flip(1)], 1)
+    ts = torch.tensor([0.4], dtype=torch.float32)
+    _check_quant(x, fp4.quant(x.cuda(), fmt), fmt)
+    if fmt == NV:
+        _check_quant(x, fp4.quant(x.cuda(), fmt, tensor_scale=ts.cuda()), fmt, ts)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+def test_quant_of_empty_tiny_and_non_finite(fmt):
+    _need_gpu()
+    x = _acts(9, 128, torch.float32, seed=3)
+    x[0] = 0
+    x[1, 40] = math.nan
+    x[2, 0], x[2, 127] = math.inf, -math.inf
+    x[3] = 1e-45
+    x[4] = torch.finfo(torch.float32).max
+    x[5] = torch.finfo(torch.float32).min
+    x[6, 16:] = 0
+    x[7] = math.nan
+    x[8] = 2.0 ** -126
+    q = fp4.quant(x.cuda(), fmt)
+    codes, sb, t = _check_quant(x, q, fmt)
+    y = fp4.dequant(q, torch.float32).cpu()
+    g = 16 if fmt == NV else 32
+    bad = (~torch.isfinite(x)).view(9, -1, g).any(-1).repeat_interleave(g, 1)
+    assert torch.equal(torch.isnan(y), bad)
+    assert bool((y[0] == 0).all())
+    b = x[:3].to(torch.bfloat16)
+    _check_quant(b, fp4.quant(b.cuda(), fmt), fmt)
+    assert fp4.quant(torch.empty(0, 64, device="cuda", dtype=torch.bfloat16), fmt).rows == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+def test_quant_strides_gather_and_shape(fmt):
+    _need_gpu()
+    base = _acts(40, 333, torch.bfloat16, seed=5).cuda()
+    for x in (base[::3], base[:, 1:], base[:, 8:264], base[:1].expand(6, 333), base.t()[:64], base[5:6]):
+        _check_quant(x.cpu(), fp4.quant(x, fmt), fmt)
+    x3 = base[:, :320].reshape(4, 10, 320)
+    q = fp4.quant(x3, fmt)
+    assert q.shape == (4, 10) and fp4.dequant(q).shape == (4, 10, 320)
+    rows = torch.tensor([3, 3, 39, -1, 0, 40, 17], dtype=torch.int32)
+    want = torch.stack([base[r].cpu() if 0 <= r < 40 else torch.zeros(333, dtype=torch.bfloat16) for r in rows.tolist()])
+    _check_quant(want, fp4.quant(base, fmt, rows=rows.cuda()), fmt)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+def test_quant_rows_do_not_depend_on_the_batch(fmt):
+    _need_gpu()
+    x = _acts(300, 2080, torch.bfloat16, seed=9).cuda()
+    whole = fp4.dequant(fp4.quant(x, fmt), torch.float32)
+    for r in (0, 129, 299):
+        assert torch.equal(fp4.dequant(fp4.quant(x[r:r + 1], fmt), torch.float32)[0], whole[r])
+
+
+def _tol(av, wv, exact, k, out):
+    s = av.abs() @ wv.abs().T
+    return (k / 64 + 2) * 2.0 ** -22 * s + (torch.finfo(out).eps / 2 + 2.0 ** -23) * exact.abs()
+
+
+def _values(q):
+    return P.values(P.unpack(q.codes), q.canonical_scales().cpu(), q.fmt, q.ts)
+
+
+SHAPES = [(1, 1, 32), (1, 300, 4096), (7, 31, 64), (8, 128, 96), (9, 129, 1056), (64, 257, 256), (65, 64, 288),
+          (129, 256, 160), (192, 130, 512), (193, 128, 320), (257, 384, 64), (400, 100, 2048), (1025, 72, 128)]
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_gemm(fmt, m, n, k):
+    _need_gpu()
+    codes, s, ts, wv = P.weights(fmt, n, k, seed=n + k)
+    w = fp4.pack(fmt, codes[0].cuda(), s[0].cuda(), None if ts is None else ts[0].cuda())
+    a = fp4.quant(_acts(m, k, torch.bfloat16, seed=m).cuda(), fmt)
+    av = _values(a)
+    exact = av @ wv[0].T
+    for out in (torch.float32, torch.bfloat16):
+        y = fp4.gemm(a, w, out_dtype=out).cpu().double()
+        assert bool(((y - exact).abs() <= _tol(av, wv[0], exact, k, out)).all())
+    # fp16's range ends early: a tensor scale that keeps the outputs inside it
+    y = fp4.gemm(a, w, out_dtype=torch.float16).cpu().double()
+    fits = exact.abs() < 6e4
+    lim = _tol(av, wv[0], exact, k, torch.float16) + 2.0 ** -25
+    assert bool(((y - exact).abs() <= lim)[fits].all())
+    assert fp4.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+def test_gemm_of_an_odd_k_and_a_calibrated_scale(fmt):
+    """K 100: both operands are padded to 128 with zero codes, whatever the scale bytes behind K."""
+    _need_gpu()
+    x, wx = _acts(20, 100, torch.bfloat16, seed=1, spread=0.5), _acts(50, 100, torch.float32, seed=2, spread=0.5)
+    ts = torch.tensor([0.02], device="cuda") if fmt == NV else None
+    a, w = fp4.quant(x.cuda(), fmt, tensor_scale=ts), fp4.quant(wx.cuda(), fmt, tensor_scale=ts)
+    av, wv = _values(a), _values(w)
+    exact = av @ wv.T
+    y = fp4.gemm(a, w, out_dtype=torch.float32).cpu().double()
+    assert bool(((y - exact).abs() <= _tol(av, wv, exact, 128, torch.float32)).all())
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+def test_gemm_output_rows_and_non_finite_blocks(fmt):
+    _need_gpu()
+    codes, s, ts, wv = P.weights(fmt, 136, 256, seed=4)
+    w = fp4.pack(fmt, codes[0].cuda(), s[0].cuda(), None if ts is None else ts[0].cuda())
+    x = _acts(21, 256, torch.bfloat16, seed=4)
+    clean = fp4.gemm(fp4.quant(x.cuda(), fmt), w)
+    x[5, 77] = math.inf
+    a = fp4.quant(x.cuda(), fmt)
+    buf = torch.full((21, 200), 7.0, dtype=torch.bfloat16, device="cuda")
+    y = fp4.gemm(a, w, out=buf[:, 3:139])
+    assert y.data_ptr() == buf[:, 3:139].data_ptr()
+    assert bool((buf[:, :3] == 7).all()) and bool((buf[:, 139:] == 7).all())
+    assert bool(torch.isnan(y[5]).all()), "the row that held an infinity is NaN"
+    keep = [i for i in range(21) if i != 5]
+    assert torch.equal(y[keep], clean[keep]), "and no other row is touched"
+
+
+@gpu
+def test_gemm_rows_do_not_depend_on_the_batch():
+    _need_gpu()
+    codes, s, ts, _ = P.weights(NV, 256, 1024, seed=8)
+    w = fp4.pack(NV, codes[0].cuda(), s[0].cuda(), ts[0].cuda())
+    x = _acts(17, 1024, torch.bfloat16, seed=8).cuda()
+    whole = fp4.gemm(fp4.quant(x, NV), w)
+    for r in (0, 9, 16):
+        assert torch.equal(fp4.gemm(fp4.quant(x[r:r + 1], NV), w)[0], whole[r])
+
+
+COUNTS = [[5], [0, 3, 0, 0, 1], [127, 128, 129, 1, 0, 64], [300, 0, 193], [0, 0], [1] * 40, [700, 5, 0, 260]]
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+@pytest.mark.parametrize("w13", [False, True])
+@pytest.mark.parametrize("counts", COUNTS)
+def test_grouped_gemm(fmt, w13, counts):
+    """Rows in groups of any size, two rows behind the last group, with weights and a clamp for w13 banks.
+    silu(g) u of values with errors dg, du: off by 1.1 dg |u| + |silu(g)| du, and 2^-19 of the result for
+    the fast exponential and division at |g| <= 64."""
+    _need_gpu()
+    e, n, k = len(counts), 144, 224
+    codes, s, ts, wv = P.weights(fmt, n, k, seed=e, mats=e, halves=2 if w13 else 1)
+    bank = fp4.pack(fmt, codes.cuda(), s.cuda(), None if ts is None else ts.cuda(), kind=fp4.W13 if w13 else fp4.PLAIN)
+    p = sum(counts) + 2
+    off = torch.tensor([0] + counts).cumsum(0).to(torch.int32)
+    x = _acts(p, k, torch.bfloat16, seed=p, spread=0.3) * 0.05
+    x = x.to(torch.bfloat16)
+    a = fp4.quant(x.cuda(), fmt, offsets=off.cuda())
+    c, sb, t = P.quant(x, fmt)
+    assert torch.equal(P.unpack(a.codes)[:p - 2] & 7, c[:p - 2] & 7)
+    av = P.values(c, sb, fmt, t)
+    rw = torch.rand(p, generator=torch.Generator().manual_seed(1)) + 0.5
+    width = n // 2 if w13 else n
+    out = torch.full((p, width + 5), 3.0, device="cuda")
+    limit = 2.5 if w13 else 0.0
+    y = fp4.grouped_gemm(a, bank, out_dtype=torch.float32, row_weight=rw.cuda(), limit=limit, out=out[:, :width])
+    y = y.cpu().double()
+    assert bool((out[p - 2:] == 3).all()) and bool((out[:, width:] == 3).all()), "rows behind the last group stay"
+    for i in range(e):
+        lo, hi = int(off[i]), int(off[i + 1])
+        if lo == hi:
+            continue
+        r = av[lo:hi] @ wv[i].T
+        tol = _tol(av[lo:hi], wv[i], r, k, torch.float32)
+        if w13:
+            g, u = r[:, :n // 2], r[:, n // 2:]
+            dg, du = tol[:, :n // 2], tol[:, n // 2:]
+            g, u = g.clamp_max(limit), u.clamp(-limit, limit)
+            silu = g / (1 + torch.exp(-g))
+            assert float(g.abs().max()) < 64
+            r, tol = silu * u, 1.1 * dg * u.abs() + silu.abs() * du + 2.0 ** -19 * (silu * u).abs() + 1e-30
+        r, tol = r * rw[lo:hi, None].double(), tol * rw[lo:hi, None].double() + 2.0 ** -22 * r.abs()
+        assert bool(((y[lo:hi] - r).abs() <= tol).all()), f"expert {i}"
+    assert fp4.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+def test_pack_reads_the_canonical_form(fmt):
+    """Tiling and back; a plain product equals one with the operand that quant makes of the same values."""
+    _need_gpu()
+    codes, s, ts, _ = P.weights(fmt, 300, 160, seed=2, mats=3)
+    w = fp4.pack(fmt, codes.cuda(), s.cuda(), None if ts is None else ts.cuda())
+    assert torch.equal(w.canonical_scales().cpu(), s.view(900, -1)) and w.codes.data_ptr() != 0
+    v = fp4.pack(fmt, codes.cuda(), s.cuda(), kind=fp4.W13)
+    inter = torch.stack([s[:, :150], s[:, 150:]], 2).reshape(900, -1)
+    assert torch.equal(v.canonical_scales().cpu(), inter)
+
+
+def test_refusals_of_the_python_calls():
+    """Arguments that no kernel may see are refused before the library is touched (no GPU needed)."""
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        fp4.quant(x)                                        # not on a CUDA device
+    with pytest.raises(ValueError):
+        fp4.quant(x, "fp8")
+    with pytest.raises(ValueError):
+        fp4.pack("nvfp4", torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 4, dtype=torch.uint8))
+
+    def t(fmt=NV, mats=1, rows=4, k=64, ts=None, offsets=None, kind=fp4.PLAIN):
+        z = torch.zeros(1, dtype=torch.uint8)
+        return fp4.Fp4Tensor(fmt, mats, rows, k, z, z, ts, offsets, kind, (rows,))
+
+    off = torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: fp4.gemm(t(), t(fmt=MX)), lambda: fp4.gemm(t(), t(k=96)), lambda: fp4.gemm(t(), t(mats=2)),
+                 lambda: fp4.gemm(t(offsets=off), t()), lambda: fp4.gemm(t(), t(kind=fp4.W13)),
+                 lambda: fp4.gemm(t(mats=2), t()), lambda: fp4.gemm(t(), t(), out_dtype=torch.float64),
+                 lambda: fp4.grouped_gemm(t(), t(mats=2)), lambda: fp4.grouped_gemm(t(offsets=off), t(mats=3)),
+                 lambda: fp4.grouped_gemm(t(offsets=off), t(mats=2), limit=-1.0),
+                 lambda: fp4.grouped_gemm(t(offsets=off), t(mats=2), limit=math.nan),
+                 lambda: fp4.grouped_gemm(t(offsets=off), t(mats=2), row_weight=torch.ones(3)),
+                 lambda: fp4.dequant(t(offsets=off)), lambda: fp4.dequant(t(), torch.float64),
+                 lambda: t(offsets=off).canonical_scales()):
+        with pytest.raises(ValueError):
+            call()
+
+
+@gpu
+def test_refusals_of_tensors():
+    _need_gpu()
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+    i = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for kw in (dict(rows=i), dict(offsets=i), dict(offsets=i[:1].int()), dict(tensor_scale=torch.zeros(2, device="cuda")),
+               dict(tensor_scale=torch.zeros(1)), dict(fmt=MX, tensor_scale=torch.ones(1, device="cuda")),
+               dict(rows=torch.zeros(4, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            fp4.quant(x, **kw)
+    with pytest.raises(Exception, match="65536"):
+        fp4.quant(torch.zeros(1, 65537, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(ValueError):
+        fp4.quant(x.double())
+    a = fp4.quant(x)
+    with pytest.raises(ValueError):
+        fp4.gemm(a, a, out=torch.zeros(4, 5, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(ValueError):
+        fp4.gemm(a, a, out=torch.zeros(4, 4, dtype=torch.bfloat16, device="cuda").t()[:, :])

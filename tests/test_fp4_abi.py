@@ -1,0 +1,97 @@
+"""C-ABI validation of the fp4 and routing entry points: every refusal comes before any launch, so these run
+without a GPU."""
+import ctypes
+
+from shard_b200 import _lib
+from shard_b200 import formats as F
+
+FAKE = ctypes.c_void_p(1 << 12)   # an aligned address that these calls never dereference
+ODD = ctypes.c_void_p((1 << 12) + 8)
+NV, MX, FP8 = F.FMT_NVFP4, F.FMT_MXFP4, F.FMT_FP8
+
+
+def test_scale_bytes():
+    f = _lib.lib().sb_fp4_scale_bytes
+    assert f(NV, 1, 1, 32, 0) == 512 and f(MX, 1, 1, 32, 0) == 512
+    assert f(NV, 1, 129, 4096, 0) == 2 * 64 * 512 and f(MX, 1, 129, 4096, 0) == 2 * 32 * 512
+    assert f(NV, 3, 130, 64, 0) == 3 * 2 * 512
+    assert f(NV, 1, 300, 64, 7) == (300 // 128 + 7) * 512
+    assert f(NV, 1, 1, 33, 0) == 512 and f(MX, 1, 1, 129, 0) == 2 * 512
+    for bad in ((FP8, 1, 1, 64, 0), (NV, 0, 1, 64, 0), (NV, 1, -1, 64, 0), (NV, 1, 1, 0, 0), (NV, 1, 1, 65537, 0),
+                (NV, 1, 1, 64, 1025), (NV, 2, 1, 64, 3), (NV, 1, 1 << 31, 64, 0)):
+        assert f(*bad) == 0
+
+
+def _quant(fmt=NV, x=FAKE, dtype=0, src=4, k=64, stride=64, rows_in=None, rows=4, ts=None, off=None, groups=0, codes=FAKE,
+           scales=FAKE, rs=FAKE):
+    return _lib.lib().sb_fp4_quant(fmt, x, dtype, src, k, stride, rows_in, rows, ts, off, groups, codes, scales, rs, None)
+
+
+def test_quant_refusals():
+    assert _quant(fmt=FP8) == -3
+    assert _quant(dtype=3) == -1
+    for kw in (dict(k=0), dict(k=65537), dict(rows=-1), dict(rows=(1 << 30) + 1), dict(src=-1), dict(stride=-1), dict(src=5)):
+        assert _quant(**kw) == -2, kw
+    for kw in (dict(x=None), dict(codes=None), dict(scales=None), dict(rs=None), dict(codes=ODD), dict(scales=ODD),
+               dict(x=ctypes.c_void_p(4097)), dict(off=FAKE), dict(groups=2), dict(off=FAKE, groups=1025),
+               dict(fmt=MX, ts=FAKE)):
+        assert _quant(**kw) == -1, kw
+    assert _quant(rows=0, src=0, x=None, codes=None, scales=None) == 0
+
+
+def test_dequant_and_tile_refusals():
+    L = _lib.lib()
+    d = lambda fmt=NV, c=FAKE, s=FAKE, ts=None, rows=4, k=64, y=FAKE, dt=0: L.sb_fp4_dequant(  # noqa: E731
+        fmt, c, s, ts, 0, rows, k, y, dt, None)
+    assert d(fmt=FP8) == -3 and d(dt=7) == -1 and d(k=0) == -2
+    assert d(c=None) == -1 and d(s=ODD) == -1 and d(y=ctypes.c_void_p(4097)) == -1 and d(fmt=MX, ts=FAKE) == -1
+    assert d(rows=0, c=None) == 0
+    t = lambda fmt=NV, s=FAKE, o=FAKE, m=1, n=4, k=64: L.sb_fp4_tile_scales(fmt, s, o, m, n, k, None)  # noqa: E731
+    assert t(fmt=FP8) == -3 and t(k=48) == -2 and t(m=0) == -2 and t(n=0) == -2 and t(m=1 << 20, n=1 << 20) == -2
+    assert t(s=None) == -1 and t(o=ODD) == -1
+
+
+def test_product_refusals():
+    L = _lib.lib()
+
+    def g(fmt=NV, a=FAKE, s=FAKE, m=4, w=FAKE, ws=FAKE, wts=None, n=8, k=64, y=FAKE, dt=0, ld=8):
+        return L.sb_fp4_gemm(fmt, a, s, None, 0, m, w, ws, wts, n, k, y, dt, ld, None)
+
+    assert g(fmt=FP8) == -3 and g(dt=3) == -1
+    for kw in (dict(n=0), dict(k=0), dict(k=65537), dict(m=-1), dict(ld=7), dict(m=1 << 30, n=1 << 20, ld=1 << 20)):
+        assert g(**kw) == -2, kw
+    for kw in (dict(a=None), dict(s=ODD), dict(w=ODD), dict(ws=None), dict(y=None), dict(fmt=MX, wts=FAKE)):
+        assert g(**kw) == -1, kw
+    assert g(m=0, a=None, y=None) == 0
+
+    def gg(off=FAKE, wtsn=1, wts=None, e=4, n=8, sw=0, lim=0.0, m=4, ld=8):
+        return L.sb_fp4_grouped_gemm(NV, FAKE, FAKE, None, 0, m, off, FAKE, FAKE, wts, wtsn, e, n, 64, sw, lim, None, FAKE, 0,
+                                     ld, None)
+
+    assert gg(off=None) == -1 and gg(wts=FAKE, wtsn=3) == -1 and gg(lim=-1.0) == -1 and gg(lim=float("nan")) == -1
+    assert gg(e=0) == -2 and gg(e=1025) == -2 and gg(sw=1, n=7) == -2 and gg(e=1024, n=1 << 21) == -2 and gg(sw=1, ld=3) == -2
+    assert gg(m=0) == 0
+    assert L.sb_fp4_error(None, None) == -1
+
+
+def test_route_refusals():
+    L = _lib.lib()
+
+    def r(l=FAKE, dt=2, t=2, e=16, st=16, k=4, sc=1, g=1, kg=1, gs=0, w=FAKE, i=FAKE):
+        return L.sb_route_topk(l, dt, t, e, st, None, k, sc, g, kg, gs, 1, 1.0, w, i, None)
+
+    for kw in (dict(dt=3), dict(sc=3), dict(gs=2), dict(l=None), dict(w=None), dict(i=None), dict(l=ctypes.c_void_p(4098))):
+        assert r(**kw) == -1, kw
+    for kw in (dict(t=-1), dict(e=0), dict(e=1025), dict(st=-1), dict(g=0), dict(g=3), dict(g=64, e=64), dict(g=4, kg=5),
+               dict(g=4, kg=0), dict(k=0), dict(k=17), dict(k=5, g=4, kg=1)):
+        assert r(**kw) == -2, kw
+    assert r(t=0, l=None) == 0
+    assert L.sb_expert_order_workspace_bytes(2048, 256) == 0 and L.sb_expert_order_workspace_bytes(2049, 256) == 2 * 256 * 4
+
+    def o(ids=FAKE, t=4, k=2, e=8, off=FAKE, tok=FAKE, pl=FAKE, ws=None, n=0):
+        return L.sb_expert_order(ids, t, k, e, off, tok, pl, ws, n, None)
+
+    assert o(t=-1) == -2 and o(k=0) == -2 and o(e=1025) == -2 and o(t=1 << 30, k=4) == -2
+    assert o(ids=None) == -1 and o(off=None) == -1 and o(tok=None) == -1 and o(pl=None) == -1
+    assert o(t=4096, ws=None) == -4 and o(t=4096, ws=FAKE, n=4 * 8 * 4 - 1) == -4
+    assert o(t=4096, ws=ctypes.c_void_p(4097), n=1 << 20) == -1

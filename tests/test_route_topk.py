@@ -1,0 +1,167 @@
+"""shard_b200.route against a plain 64-bit router. Ids and the order are compared exactly; a weight is a few
+fp32 roundings from exact: the exponential's argument (|l - max| 2^-24 of the score), its value, the sums,
+the division, the scale, together below (16 + |l - max|) 2^-23 of the weight."""
+import math
+
+import pytest
+import torch
+
+import fp4_plain as P
+from shard_b200 import route
+
+gpu = pytest.mark.gpu
+
+
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+
+
+def _check(logits, k, bias=None, **kw):
+    w, ids = route.topk(logits.cuda(), k, bias=None if bias is None else bias.cuda(), **kw)
+    rw, rids = P.route(logits.cpu(), k, bias, **kw)
+    assert torch.equal(ids.cpu(), rids)
+    fin = logits.float().cpu()
+    fin = fin[torch.isfinite(fin) & (fin.abs() < 1e30)]
+    spread = float(fin.max() - fin.min()) if fin.numel() else 0.0
+    assert bool(((w.cpu().double() - rw).abs() <= (16 + spread) * 2.0 ** -23 * rw + 1e-37).all())
+
+
+GROUPS = [(1, 1, 1, 1), (5, 7, 3, 1), (16, 64, 6, 1), (33, 256, 8, 8), (130, 384, 8, 1), (9, 96, 4, 8), (6, 160, 8, 32),
+          (4, 1024, 16, 16), (3, 60, 5, 4), (2, 31, 16, 1), (7, 100, 8, 4), (3, 1000, 8, 8)]
+
+
+@gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid", "sqrtsoftplus"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,e,k,g", GROUPS)
+def test_topk(score, dtype, t, e, k, g):
+    _need_gpu()
+    gen = torch.Generator().manual_seed(t * e + k)
+    logits = (2 * torch.randn(t, e, generator=gen)).to(dtype)
+    bias = 0.2 * torch.randn(e, generator=gen)
+    kept = max(1, g // 2, -(-k * g // e))
+    for b in (None, bias):
+        for gs in ("max", "top2") if g > 1 else ("max",):
+            _check(logits, k, b, score=score, n_group=g, topk_group=kept, group_score=gs, renormalize=score != "softmax",
+                   scale=1.5)
+
+
+@gpu
+@pytest.mark.parametrize("bias", [None, "zero", "steps"])
+def test_topk_ties_go_to_the_lower_id(bias):
+    """Few distinct logits; biases that make the sums of unequal scores nearly or exactly equal."""
+    _need_gpu()
+    gen = torch.Generator().manual_seed(3)
+    logits = torch.randint(-2, 3, (64, 256), generator=gen).float()
+    b = None
+    if bias == "zero":
+        b = torch.zeros(256)
+    if bias == "steps":     # bias = 0.5 - sigmoid(l) rounded to fp32: the sums differ in the 8th digit only
+        logits = (0.5 * torch.arange(256).float() % 7 - 3).expand(64, 256).contiguous()
+        b = (0.5 - torch.sigmoid(logits[0].double())).float()
+    for g in (1, 8):
+        for gs in ("max", "top2"):
+            _check(logits, 8, b, score="sigmoid", n_group=g, topk_group=4 if g > 1 else 1, group_score=gs)
+            _check(logits.to(torch.bfloat16), 8, b, score="sigmoid", n_group=g, topk_group=4 if g > 1 else 1, group_score=gs)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid", "sqrtsoftplus"])
+def test_topk_masks(dtype, score):
+    """Rows masked in part and whole by -inf, NaN and the type's lowest value; +inf counts as the largest."""
+    _need_gpu()
+    gen = torch.Generator().manual_seed(5)
+    logits = torch.randn(12, 64, generator=gen).to(dtype)
+    low = torch.finfo(dtype).min
+    logits[0] = -math.inf
+    logits[1] = low
+    logits[2] = math.nan
+    logits[3, :62] = -math.inf
+    logits[4, ::2] = low
+    logits[5, 8:] = math.nan
+    logits[6, 7] = math.inf if score != "sqrtsoftplus" else 3.0
+    logits[7, :32] = -math.inf
+    logits[8] = 0
+    for b in (None, 0.1 * torch.randn(64, generator=gen)):
+        for g, kept in ((1, 1), (8, 3)):
+            for gs in ("max", "top2"):
+                _check(logits, 6, b, score=score, n_group=g, topk_group=kept, group_score=gs)
+
+
+@gpu
+def test_topk_strides_and_large_batches():
+    _need_gpu()
+    gen = torch.Generator().manual_seed(6)
+    base = torch.randn(40, 300, generator=gen)
+    _check(base[::2, :256], 8)
+    _check(base[:, 1:257], 8)
+    _check(base[:1].expand(5, 300), 4, score="softmax")
+    _check(base.t()[:64].contiguous().t()[:8], 4)
+    logits = torch.randn(20000, 64, generator=gen)
+    bias = torch.randn(64, generator=gen)
+    w, ids = route.topk(logits.cuda(), 6, bias=bias.cuda())
+    pick = torch.sigmoid(logits.double()) + bias.double()
+    want = torch.sort(pick, dim=1, descending=True, stable=True).indices[:, :6]
+    assert torch.equal(ids.cpu(), want)
+    assert route.topk(logits[:0].cuda(), 6)[1].shape == (0, 6)
+
+
+@gpu
+@pytest.mark.parametrize("t,k,e", [(0, 2, 4), (1, 1, 1), (3, 4, 16), (256, 8, 256), (257, 8, 7), (700, 8, 1024), (5000, 3, 100)])
+def test_expert_order(t, k, e):
+    _need_gpu()
+    gen = torch.Generator().manual_seed(t + e)
+    ids = (torch.rand(t, k, generator=gen) ** 2 * e).long()
+    if t > 2:
+        ids[1] = -1
+        ids[2, 0] = e
+        ids[0] = ids[0, 0]      # the same expert in every slot
+    o = route.expert_order(ids.cuda(), e)
+    offsets, tokens, places = P.order(ids, e) if t * k * e < 3_000_000 else _order_fast(ids, e)
+    assert o.offsets.tolist() == offsets
+    assert o.tokens.tolist() == tokens
+    assert o.places.reshape(-1).tolist() == places
+
+
+def _order_fast(ids, e):
+    flat = ids.reshape(-1)
+    good = (flat >= 0) & (flat < e)
+    at = torch.sort(torch.where(good, flat, e), stable=True).indices
+    n = int(good.sum())
+    places = torch.full_like(flat, -1)
+    places[at[:n]] = torch.arange(n)
+    offsets = torch.cat([torch.zeros(1, dtype=torch.long), torch.bincount(flat[good], minlength=e).cumsum(0)])
+    return offsets.tolist(), (at[:n] // ids.shape[1]).tolist() + [-1] * (flat.numel() - n), places.tolist()
+
+
+def test_refusals_of_the_python_calls():
+    l = torch.zeros(2, 8)
+    for call in (lambda: route.topk(l, 2), lambda: route.topk(l, 2, score="relu"), lambda: route.topk(l, 2, group_score="mean"),
+                 lambda: route.expert_order(torch.zeros(2, 2, dtype=torch.int64), 4)):
+        with pytest.raises(ValueError):
+            call()
+
+
+@gpu
+def test_refusals_of_tensors():
+    _need_gpu()
+    l = torch.zeros(2, 8, device="cuda")
+    for kw in (dict(bias=torch.zeros(7, device="cuda")), dict(bias=torch.zeros(8)), dict(bias=torch.zeros(8, device="cuda").half())):
+        with pytest.raises(ValueError):
+            route.topk(l, 2, **kw)
+    for kw in (dict(n_group=3), dict(n_group=4, topk_group=5), dict(n_group=4, topk_group=0)):
+        with pytest.raises(Exception, match="n_group"):
+            route.topk(l, 2, **kw)
+    for k in (0, 17, 9):
+        with pytest.raises(Exception, match="topk"):
+            route.topk(l, k)
+    with pytest.raises(Exception, match="topk"):
+        route.topk(l, 3, n_group=4, topk_group=1)
+    with pytest.raises(Exception, match="1024"):
+        route.topk(torch.zeros(1, 1025, device="cuda"), 2)
+    with pytest.raises(ValueError):
+        route.expert_order(torch.zeros(2, 2, dtype=torch.int32, device="cuda"), 4)
+    with pytest.raises(Exception, match="1024"):
+        route.expert_order(torch.zeros(2, 2, dtype=torch.int64, device="cuda"), 1025)
