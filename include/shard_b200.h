@@ -270,10 +270,11 @@ int sb_fp4_dequant(int fmt, const void* codes, const void* scales, const float* 
                    int64_t k, void* y, int dtype, void* stream);
 /* Canonical scales (NVFP4 e4m3 [n_mat, N, K/16], MXFP4 e8m0 [n_mat, N, K/32]) -> atoms. K % 32 == 0. */
 int sb_fp4_tile_scales(int fmt, const void* src, void* dst, int64_t n_mat, int64_t n, int64_t k, void* stream);
-/* y [M, N] of `dtype`, rows ldy elements apart = A W^T, summed in fp32. w_ts: fp32 [1] or NULL. */
+/* y [M, N] of `dtype`, rows ldy elements apart = A W^T, summed in fp32. w_ts: fp32 [1], [N] with w_ts_per_row,
+ * or NULL. */
 int sb_fp4_gemm(int fmt, const void* a_codes, const void* a_scales, const float* a_ts, int a_ts_per_row, int64_t m,
-                const void* w_codes, const void* w_scales, const float* w_ts, int64_t n, int64_t k, void* y, int dtype,
-                int64_t ldy, void* stream);
+                const void* w_codes, const void* w_scales, const float* w_ts, int w_ts_per_row, int64_t n, int64_t k,
+                void* y, int dtype, int64_t ldy, void* stream);
 /* The same with one W [N, K] per expert of a bank and A's rows in expert groups. Rows behind
  * offsets[n_experts] are left as they are. w_ts: fp32 [n_experts, w_ts_n] or NULL. row_weight: fp32 [M]
  * (each output row times its weight) or NULL. swiglu: W holds w1's and w3's rows in turn (row 2i: w1,

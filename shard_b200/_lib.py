@@ -75,7 +75,7 @@ SIGNATURES = {
     "sb_fp4_quant": (_int, [_int, _vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
     "sb_fp4_dequant": (_int, [_int, _vp, _vp, _vp, _int, _i64, _i64, _vp, _int, _vp]),
     "sb_fp4_tile_scales": (_int, [_int, _vp, _vp, _i64, _i64, _i64, _vp]),
-    "sb_fp4_gemm": (_int, [_int, _vp, _vp, _vp, _int, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _int, _i64, _vp]),
+    "sb_fp4_gemm": (_int, [_int, _vp, _vp, _vp, _int, _i64, _vp, _vp, _vp, _int, _i64, _i64, _vp, _int, _i64, _vp]),
     "sb_fp4_grouped_gemm": (_int, [_int, _vp, _vp, _vp, _int, _i64, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _int,
                                    ctypes.c_float, _vp, _vp, _int, _i64, _vp]),
     "sb_fp4_error": (_int, [ctypes.POINTER(ctypes.c_int), _vp]),

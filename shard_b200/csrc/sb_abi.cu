@@ -1204,8 +1204,8 @@ int sb_fp4_tile_scales(int fmt, const void* src, void* dst, int64_t n_mat, int64
 }
 
 int sb_fp4_gemm(int fmt, const void* a_codes, const void* a_scales, const float* a_ts, int a_ts_per_row, int64_t m,
-                const void* w_codes, const void* w_scales, const float* w_ts, int64_t n, int64_t k, void* y, int dtype,
-                int64_t ldy, void* stream) {
+                const void* w_codes, const void* w_scales, const float* w_ts, int w_ts_per_row, int64_t n, int64_t k,
+                void* y, int dtype, int64_t ldy, void* stream) {
   const void* ptrs[] = {a_codes, a_scales, w_codes, w_scales, y};
   if (int rc = fp4_product("fp4_gemm", fmt, dtype, ptrs, 5, m, 1, n, k, n, ldy)) return rc;
   if (fmt == SB_FMT_MXFP4 && (a_ts || w_ts)) return fail(SB_ERR_ARG, "fp4_gemm: MXFP4 has no tensor scale");
@@ -1214,7 +1214,7 @@ int sb_fp4_gemm(int fmt, const void* a_codes, const void* a_scales, const float*
   g.w = (const uint8_t*)w_codes;
   g.w_s = (const uint8_t*)w_scales;
   g.w_ts = w_ts;
-  g.w_ts_n = 1;
+  g.w_ts_n = w_ts_per_row ? 0 : 1;
   g.a = (const uint8_t*)a_codes;
   g.a_s = (const uint8_t*)a_scales;
   g.a_ts = a_ts;

@@ -37,6 +37,14 @@ __device__ __forceinline__ uint32_t cvt8(const float (&v)[8]) {
   return r;
 }
 
+// (a x, b x): two fp32 products in one instruction
+__device__ __forceinline__ void mul2(float a, float b, float x, float& ra, float& rb) {
+  asm("{\n .reg .b64 u, v, w;\n mov.b64 u, {%2, %3};\n mov.b64 v, {%4, %4};\n mul.rn.f32x2 w, u, v;\n"
+      " mov.b64 {%0, %1}, w;\n}"
+      : "=f"(ra), "=f"(rb)
+      : "f"(a), "f"(b), "f"(x));
+}
+
 // the border between e2m1 magnitudes c and c + 1
 __device__ __forceinline__ float border(uint32_t c) {
   return c < 4 ? 0.25f + 0.5f * (float)c : (c == 4 ? 2.5f : (c == 5 ? 3.5f : 5.0f));
@@ -163,10 +171,10 @@ __device__ __forceinline__ uint2 codes_nv(const Unit<T>& u, float s, float ts) {
     for (int h = 0; h < 2; ++h) {
       float a[8], b[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = u.get(8 * h + i);
-        a[i] = x * lo;
-        b[i] = x * hi;
+      for (int i = 0; i < 8; i += 2) {
+        const float x0 = u.get(8 * h + i), x1 = u.get(8 * h + i + 1);
+        mul2(x0, x1, lo, a[i], a[i + 1]);
+        mul2(x0, x1, hi, b[i], b[i + 1]);
       }
       out[h] = cvt8(a);
       const uint32_t diff = out[h] ^ cvt8(b);
@@ -202,9 +210,9 @@ template <typename T>
 __device__ __forceinline__ uint2 codes_mx(const Unit<T>& u, float inv) {
   float a[8], b[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    a[i] = u.get(i) * inv;
-    b[i] = u.get(8 + i) * inv;
+  for (int i = 0; i < 8; i += 2) {
+    mul2(u.get(i), u.get(i + 1), inv, a[i], a[i + 1]);
+    mul2(u.get(8 + i), u.get(9 + i), inv, b[i], b[i + 1]);
   }
   return make_uint2(cvt8(a), cvt8(b));
 }
@@ -323,27 +331,34 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 to_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // y = code s ts: code s is exact in fp32 (6 significant bits), the product with ts rounds once. A thread
-// takes 16 values.
+// takes 16 values at a time, the warps of a row as in quant_kernel.
 template <typename T, bool NV>
-__global__ void __launch_bounds__(256) dequant_kernel(DequantArgs a) {
+__global__ void __launch_bounds__(1024) dequant_kernel(DequantArgs a) {
+  const int warp = threadIdx.x >> 5;
+  const int rpc = (blockDim.x >> 5) / a.wpr;
+  const int rw = warp / a.wpr, tr = threadIdx.x - rw * a.wpr * 32;
+  const int64_t row = (int64_t)blockIdx.x * rpc + rw;
   pdl_wait();
   pdl_trigger();
-  const int64_t total = a.rows * a.units;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = i / a.units;
-    const int k = (int)(i - row * a.units);
-    const uint2 c = *reinterpret_cast<const uint2*>(a.codes + row * a.row_bytes + (int64_t)k * 8);
+  if (row >= a.rows) return;
+  const float ts = NV && a.ts != nullptr ? a.ts[a.ts_row ? row : 0] : 1.f;
+  const uint8_t* cr = a.codes + row * a.row_bytes;
+  const uint8_t* sr = a.scales + ((row >> 7) * a.atoms) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+  for (int k = tr; k < a.units; k += a.wpr * 32) {
+    const uint2 c = *reinterpret_cast<const uint2*>(cr + (int64_t)k * 8);
     const int b = NV ? k : k >> 1;
-    const uint32_t sb = a.scales[((row >> 7) * a.atoms + (b >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (b & 3)];
-    float s = NV ? e4m3_to_f32(sb) : (sb == 0xFFu ? __uint_as_float(0x7FC00000u) : e8m0_to_f32(sb));
-    const float ts = NV && a.ts != nullptr ? a.ts[a.ts_row ? row : 0] : 1.f;
-    T o[16];
+    const uint32_t sb = sr[(int64_t)(b >> 2) * 512 + (b & 3)];
+    const float s = NV ? e4m3_to_f32(sb) : (sb == 0xFFu ? __uint_as_float(0x7FC00000u) : e8m0_to_f32(sb));
+    alignas(16) T o[16];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t h = e2m1x2_to_f16x2((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-      o[2 * j] = to_out<T>(f.x * s * ts);
-      o[2 * j + 1] = to_out<T>(f.y * s * ts);
+      float v0, v1;
+      mul2(f.x, f.y, s, v0, v1);
+      if (NV) mul2(v0, v1, ts, v0, v1);
+      o[2 * j] = to_out<T>(v0);
+      o[2 * j + 1] = to_out<T>(v1);
     }
     T* y = reinterpret_cast<T*>(a.y) + row * a.k + (int64_t)k * 16;
     const int left = a.k - k * 16;
@@ -411,9 +426,9 @@ cudaError_t launch_fp4_quant(const QuantArgs& args, int dtype, cudaStream_t st) 
 }
 
 template <typename T>
-static cudaError_t launch_dequant_t(const DequantArgs& a, dim3 grid, cudaStream_t st) {
-  if (a.nv) return launch_pdl(fp4::dequant_kernel<T, true>, grid, dim3(256), 0, st, a);
-  return launch_pdl(fp4::dequant_kernel<T, false>, grid, dim3(256), 0, st, a);
+static cudaError_t launch_dequant_t(const DequantArgs& a, dim3 grid, dim3 block, cudaStream_t st) {
+  if (a.nv) return launch_pdl(fp4::dequant_kernel<T, true>, grid, block, 0, st, a);
+  return launch_pdl(fp4::dequant_kernel<T, false>, grid, block, 0, st, a);
 }
 
 static unsigned grid_of(int64_t work, int64_t cap) {
@@ -425,10 +440,14 @@ cudaError_t launch_fp4_dequant(const DequantArgs& args, int dtype, cudaStream_t 
   DequantArgs a = args;
   const int es = dtype == SB_F32 ? 4 : 2;
   a.vec = (reinterpret_cast<uintptr_t>(a.y) & 15u) == 0 && (a.k * es) % 16 == 0;
-  const dim3 grid(grid_of(a.rows * a.units, (int64_t)num_sms() * 64));
-  if (dtype == SB_F32) return launch_dequant_t<float>(a, grid, st);
-  if (dtype == SB_F16) return launch_dequant_t<__half>(a, grid, st);
-  return launch_dequant_t<__nv_bfloat16>(a, grid, st);
+  const int v = a.rows * a.units <= (int64_t)num_sms() * 1024 ? 1 : 4;
+  a.wpr = (a.units + 32 * v - 1) / (32 * v);
+  if (a.wpr > 32) a.wpr = 32;
+  const int rpc = a.wpr >= 8 ? 1 : 8 / a.wpr;
+  const dim3 grid((unsigned)((a.rows + rpc - 1) / rpc)), block(rpc * a.wpr * 32);
+  if (dtype == SB_F32) return launch_dequant_t<float>(a, grid, block, st);
+  if (dtype == SB_F16) return launch_dequant_t<__half>(a, grid, block, st);
+  return launch_dequant_t<__nv_bfloat16>(a, grid, block, st);
 }
 
 cudaError_t launch_fp4_tile_scales(const uint8_t* src, uint8_t* dst, int64_t mats, int64_t n, int64_t nb,

@@ -38,14 +38,14 @@ struct DequantArgs {
   int k, units, nv;
   int64_t row_bytes, atoms;
   void* y;
-  int vec;
+  int vec, wpr;              // set by the launch: y can be written 16 bytes at a time; warps per row
 };
 
 struct Fp4MmArgs {
   const uint8_t* w;          // codes [mats * n][row_bytes]
   const uint8_t* w_s;
   const float* w_ts;         // fp32 [mats][w_ts_n], or null
-  int w_ts_n;                // 2: one for the even rows (w1), one for the odd rows (w3)
+  int w_ts_n;                // 2: one for the even rows (w1), one for the odd rows (w3); 0: [n], one per row
   const uint8_t* a;          // codes [m][row_bytes]
   const uint8_t* a_s;
   const float* a_ts;         // fp32 [m] or [1], or null

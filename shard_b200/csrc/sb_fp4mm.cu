@@ -18,6 +18,8 @@
 #include <cudaTypedefs.h>
 #include <string.h>
 
+#include <atomic>
+
 #include "sb_fp4.h"
 #include "sb_launch.h"
 #include "sb_tcgen05.cuh"
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
       const int row = t.n0 + tid;
       const bool in = row < g.n;
       float wts = 1.f;
-      if (g.w_ts != nullptr) wts = g.w_ts[t.mat * g.w_ts_n + (g.w_ts_n == 2 ? (row & 1) : 0)];
+      if (g.w_ts != nullptr) wts = g.w_ts_n == 0 ? (in ? g.w_ts[row] : 0.f) : g.w_ts[t.mat * g.w_ts_n + (g.w_ts_n == 2 ? (row & 1) : 0)];
       if (!warp_wait(abortf, smem_addr(&c.accfull[q]), (n >> 1) & 1u)) break;
       fence_after();
       for (int c0 = 0; c0 < t.cnt; c0 += 32) {
@@ -397,10 +399,18 @@ static cudaError_t code_map(CUtensorMap* map, const void* base, uint64_t rows, u
 
 template <bool NV, bool SWIGLU, typename T>
 static cudaError_t launch_mm(const fp4mm::Args& a, int grid, size_t smem, cudaStream_t st) {
-  // (the limit belongs to the kernel on the current device)
-  const cudaError_t e = cudaFuncSetAttribute(fp4mm::fp4_mm_kernel<NV, SWIGLU, T>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, fp4mm::SMEM_LIMIT);
+  // the limit belongs to the kernel on one device: set once for each
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (!(done.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(fp4mm::fp4_mm_kernel<NV, SWIGLU, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             fp4mm::SMEM_LIMIT);
+    if (e != cudaSuccess) return e;
+    done.fetch_or(bit, std::memory_order_relaxed);
+  }
   return launch_pdl(fp4mm::fp4_mm_kernel<NV, SWIGLU, T>, dim3(grid), dim3(fp4mm::NTHREADS), smem, st, a);
 }
 

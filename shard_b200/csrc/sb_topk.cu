@@ -22,55 +22,43 @@ namespace topk {
 // order-preserving keys; 0: no candidate, 1: a masked expert
 __device__ __forceinline__ uint32_t key_of(float v) {
   const uint32_t b = __float_as_uint(v + 0.f);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ uint64_t key_of(double v) {
-  const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
-  return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
-}
-__device__ __forceinline__ uint32_t warp_kmax(uint32_t k) { return __reduce_max_sync(0xffffffffu, k); }
-__device__ __forceinline__ uint64_t warp_kmax(uint64_t k) {
-  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
-  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
-  return ((uint64_t)hi << 32) | lo;
-}
-template <typename V>
-struct KeyOf;
-template <>
-struct KeyOf<float> { using type = uint32_t; };
-template <>
-struct KeyOf<double> { using type = uint64_t; };
-
-__device__ __forceinline__ float ex(float v) { return expf(v); }
-__device__ __forceinline__ double ex(double v) { return exp(v); }
-__device__ __forceinline__ float lg1p(float v) { return log1pf(v); }
-__device__ __forceinline__ double lg1p(double v) { return log1p(v); }
-__device__ __forceinline__ float sq(float v) { return sqrtf(v); }
-__device__ __forceinline__ double sq(double v) { return sqrt(v); }
-
-// score of a logit; mx, sum: the row's softmax statistics
-template <typename V>
-__device__ __forceinline__ V score(int func, float l, V mx, V sum) {
-  const V x = (V)l;
-  if (func == SCORE_SOFTMAX) return ex(x - mx) / sum;
-  if (func == SCORE_SIGMOID) return (V)1 / ((V)1 + ex(-x));
-  return sq((x > (V)0 ? x : (V)0) + lg1p(ex(x > (V)0 ? -x : x)));
+__device__ __forceinline__ float value_of(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
+// the two best of (b1 >= b2) and (c1 >= c2)
 template <typename V>
-__device__ __forceinline__ V warp_add(V v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+__device__ __forceinline__ void merge(V& b1, V& b2, V c1, V c2) {
+  const V low = b1 < c1 ? b1 : c1, two = b2 > c2 ? b2 : c2;
+  b1 = b1 > c1 ? b1 : c1;
+  b2 = low > two ? low : two;
 }
-template <typename V>
-__device__ __forceinline__ V warp_most(V v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const V x = __shfl_xor_sync(0xffffffffu, v, o);
-    v = x > v ? x : v;
-  }
-  return v;
+
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// The score of a logit: for the selection (each within a few 2^-24 of itself, softmax of the row's largest), as an
+// output, and in 64 bits; mx, sum: the row's softmax statistics.
+__device__ __forceinline__ float score32(int func, float l, float mx, float rsum) {
+  if (func == SCORE_SOFTMAX) return l > -INFINITY ? __expf(l - mx) * rsum : 0.f;
+  if (func == SCORE_SIGMOID) return rcp(1.f + expf(-l));
+  return sqrtf(fmaxf(l, 0.f) + log1pf(expf(-fabsf(l))));
+}
+__device__ __forceinline__ float score_weight(int func, float l, float mx, float sum) {
+  if (func == SCORE_SOFTMAX) return __fdiv_rn(expf(l - mx), sum);
+  if (func == SCORE_SIGMOID) return __fdiv_rn(1.f, 1.f + expf(-l));
+  return sqrtf(fmaxf(l, 0.f) + log1pf(expf(-fabsf(l))));
+}
+__device__ __forceinline__ double score64(int func, float l, double mx, double sum) {
+  const double x = (double)l;
+  if (func == SCORE_SOFTMAX) return exp(x - mx) / sum;
+  if (func == SCORE_SIGMOID) return 1.0 / (1.0 + exp(-x));
+  return sqrt(fmax(x, 0.0) + log1p(exp(-fabs(x))));
 }
 
 __device__ __forceinline__ float logit(const float* p) { return *p; }
@@ -80,156 +68,6 @@ __device__ __forceinline__ float logit(const __nv_bfloat16* p) { return __bfloat
 // NaN: masked, like -inf and the type's lowest value; +inf counts as the largest fp32 value
 __device__ __forceinline__ float clean(float l, float lowest) {
   return l > lowest ? fminf(l, FLT_MAX) : -INFINITY;
-}
-
-// The k best (lane j < k: expert of rank j). Returns whether fp32 values may have decided it wrongly.
-template <typename V, int C, typename T>
-__device__ __forceinline__ bool select(const TopkArgs& a, const T* row, const float (&l)[C], int lane, float mxf,
-                                       int& mine) {
-  using K = typename KeyOf<V>::type;
-  constexpr bool FAST = sizeof(V) == 4;
-  const V NONE = -(V)INFINITY;
-  const bool biased = a.bias != nullptr;
-  const bool sums = a.groups > 1 && a.group_two;
-  bool doubt = false;
-  V mx = (V)mxf, sum = (V)1, most = (V)0;
-  if (a.score == SCORE_SOFTMAX && (biased || sums)) {
-    sum = (V)0;
-#pragma unroll
-    for (int i = 0; i < C; ++i) sum += l[i] > -INFINITY ? ex((V)l[i] - mx) : (V)0;
-    sum = warp_add(sum);
-  }
-  V v[C];      // selection values (NONE: masked or absent)
-  V gv[C];     // what the groups are scored by
-#pragma unroll
-  for (int i = 0; i < C; ++i) {
-    const int e = lane * C + i;
-    v[i] = NONE;
-    gv[i] = NONE;
-    if (e < a.experts && l[i] > -INFINITY) {
-      v[i] = (V)l[i];
-      gv[i] = v[i];
-      if (biased || sums) {
-        const V s = score<V>(a.score, l[i], mx, sum), b = biased ? (V)a.bias[e] : (V)0;
-        const V t = s + b;
-        if (biased) v[i] = t == t ? t : NONE;
-        gv[i] = biased ? v[i] : s;
-        const V mag = s + (b < (V)0 ? -b : b);
-        most = mag > most ? mag : most;
-      }
-    }
-  }
-  const V eps = FAST && (biased || sums) ? (V)2e-6f * warp_most(most) : (V)0;
-  uint32_t kept = 0xffffffffu;
-  if (a.groups > 1) {
-    const int size = a.experts / a.groups;
-    V gs = NONE;   // lane g: the score of group g
-    const int span = size / C;   // lanes per group when groups begin with lanes
-    if (size % C == 0 && (span & (span - 1)) == 0) {
-      V b1 = NONE, b2 = NONE;
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const V x = gv[i];
-        b2 = x > b1 ? b1 : (x > b2 ? x : b2);
-        b1 = x > b1 ? x : b1;
-      }
-      for (int o = 1; o < span; o <<= 1) {
-        const V c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
-        b2 = c1 > b1 ? (b1 > c2 ? b1 : c2) : (c1 > b2 ? c1 : b2);
-        b1 = c1 > b1 ? c1 : b1;
-      }
-      const V s = a.group_two && b2 > NONE ? b1 + b2 : b1;
-      gs = __shfl_sync(0xffffffffu, s, (lane * span) & 31);
-    } else {
-      for (int g = 0; g < a.groups; ++g) {
-        V b1 = NONE, b2 = NONE;
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-          const int e = lane * C + i;
-          const V x = e >= g * size && e < (g + 1) * size ? gv[i] : NONE;
-          b2 = x > b1 ? b1 : (x > b2 ? x : b2);
-          b1 = x > b1 ? x : b1;
-        }
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const V c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
-          b2 = c1 > b1 ? (b1 > c2 ? b1 : c2) : (c1 > b2 ? c1 : b2);
-          b1 = c1 > b1 ? c1 : b1;
-        }
-        if (lane == g) gs = a.group_two && b2 > NONE ? b1 + b2 : b1;
-      }
-    }
-    int rank = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      const V x = __shfl_sync(0xffffffffu, gs, g);
-      rank += x > gs || (x == gs && g < lane) ? 1 : 0;
-    }
-    const bool here = lane < a.groups, in = here && rank < a.kept;
-    kept = __ballot_sync(0xffffffffu, in);
-    if (FAST && (biased || sums) && a.kept < a.groups) {
-      const V low = -warp_most(in ? -gs : NONE), high = warp_most(here && !in ? gs : NONE);
-      doubt = !(low - high > eps) && high > NONE;
-    }
-  }
-  K key[C], best = 0;
-  int at = 0;
-  {
-    const int size = a.experts / a.groups;
-    int g = lane * C / size, left = (g + 1) * size - lane * C;   // the expert's group, experts left in it
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const bool in = lane * C + i < a.experts && ((kept >> g) & 1u);
-      if (--left == 0) {
-        ++g;
-        left = size;
-      }
-      key[i] = in ? (v[i] > NONE ? key_of(v[i]) : (K)1) : (K)0;
-      if (key[i] > best) {
-        best = key[i];
-        at = i;
-      }
-    }
-  }
-  const int rounds = FAST && biased ? a.topk + 1 : a.topk;
-  K got = 0;
-  for (int j = 0; j < rounds; ++j) {
-    const K top = warp_kmax(best);
-    const int e = (int)__reduce_min_sync(0xffffffffu, best == top ? (uint32_t)(lane * C + at) : 0x7fffffffu);
-    if (lane == j) {
-      mine = e;
-      got = top;
-    }
-    if (e / C == lane) {   // its owner drops it
-      best = 0;
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        if (i == at) key[i] = 0;
-      }
-      int na = 0;
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        if (key[i] > best) {
-          best = key[i];
-          na = i;
-        }
-      }
-      at = na;
-    }
-  }
-  if (FAST && biased) {
-    // neighbours in the ranking (lane j and j + 1, to the first one left out): far enough apart, or the
-    // same logit and bias, whose order is that of their ids
-    const K nk = __shfl_down_sync(0xffffffffu, got, 1);
-    const int ne = __shfl_down_sync(0xffffffffu, mine, 1);
-    bool near = false;
-    if (lane < a.topk && got > 1 && nk > 1) {
-      const auto val = [](uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); };
-      near = !(val((uint32_t)got) - val((uint32_t)nk) > (float)eps);
-      if (near && a.bias[mine] == a.bias[ne] && row[mine] == row[ne]) near = false;
-    }
-    doubt = doubt || __any_sync(0xffffffffu, near);
-  }
-  return doubt;
 }
 
 template <int C, typename T>
@@ -262,16 +100,235 @@ __device__ __forceinline__ float row_max(const float (&l)[C]) {
   return warp_max(mx);
 }
 
-// a token's selection in 64 bits (out of line: rare, and its registers are not the others')
+// A token's selection in 64 bits: lane j < k gets the expert of rank j. Out of line: it is rare, and its
+// registers are not the others'.
 template <int C, typename T>
 __device__ __noinline__ int select_exact(const TopkArgs& a, const T* row, int lane, float lowest) {
   float l[C];
   load_row<C, T>(a, row, lane, lowest, l);
+  const double NONE = -(double)INFINITY, mx = (double)row_max<C>(l);
+  double sum = 0.0;
+#pragma unroll 1
+  for (int i = 0; i < C; ++i) sum += l[i] > -INFINITY ? exp((double)l[i] - mx) : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  double v[C], gv[C];      // what the experts, and what their groups, are compared by
+#pragma unroll 1
+  for (int i = 0; i < C; ++i) {
+    const int e = lane * C + i;
+    v[i] = gv[i] = NONE;
+    if (e < a.experts && l[i] > -INFINITY) {
+      const double s = score64(a.score, l[i], mx, sum), t = a.bias != nullptr ? s + (double)a.bias[e] : (double)l[i];
+      v[i] = t == t ? t : NONE;
+      gv[i] = a.bias == nullptr && a.group_two ? s : v[i];
+    }
+  }
+  uint32_t kept = 0xffffffffu;
+  const int size = a.experts / a.groups;
+  if (a.groups > 1) {
+    double gs = NONE;   // lane g: the score of group g
+    for (int g = 0; g < a.groups; ++g) {
+      double b1 = NONE, b2 = NONE;
+#pragma unroll 1
+      for (int i = 0; i < C; ++i) {
+        const int e = lane * C + i;
+        if (e >= g * size && e < (g + 1) * size) merge(b1, b2, gv[i], NONE);
+      }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
+        merge(b1, b2, c1, c2);
+      }
+      if (lane == g) gs = a.group_two && b2 > NONE ? b1 + b2 : b1;
+    }
+    int rank = 0;
+    for (int g = 0; g < a.groups; ++g) {
+      const double x = __shfl_sync(0xffffffffu, gs, g);
+      rank += x > gs || (x == gs && g < lane) ? 1 : 0;
+    }
+    kept = __ballot_sync(0xffffffffu, lane < a.groups && rank < a.kept);
+  }
   int mine = 0;
-  select<double, C, T>(a, row, l, lane, row_max<C>(l), mine);
+  uint32_t taken = 0u;   // this lane's experts already chosen
+  for (int j = 0; j < a.topk; ++j) {
+    // the best left: 2 above masked, 1 masked, 0 none; then the value; then the lower id
+    int cls = 0, at = 0;
+    double best = NONE;
+#pragma unroll 1
+    for (int i = 0; i < C; ++i) {
+      const int e = lane * C + i;
+      const bool in = e < a.experts && ((kept >> (e / size)) & 1u) && !((taken >> i) & 1u);
+      const int c = in ? (v[i] > NONE ? 2 : 1) : 0;
+      if (c > cls || (c == 2 && v[i] > best)) {
+        cls = c;
+        best = v[i];
+        at = i;
+      }
+    }
+    const int top = __reduce_max_sync(0xffffffffu, cls);
+    double b = cls == top ? best : NONE;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) b = fmax(b, __shfl_xor_sync(0xffffffffu, b, o));
+    const int w = __ffs(__ballot_sync(0xffffffffu, cls == top && best == b)) - 1;
+    const int e = w * C + __shfl_sync(0xffffffffu, at, w);
+    if (lane == w) taken |= 1u << at;
+    if (lane == j) mine = e;
+  }
   return mine;
 }
 
+// Descending sorting network (odd-even merges).
+template <int C>
+__device__ __forceinline__ void sort_desc(uint32_t (&k)[C]) {
+#pragma unroll
+  for (int p = 1; p < C; p <<= 1)
+#pragma unroll
+    for (int q = p; q > 0; q >>= 1)
+#pragma unroll
+      for (int j = q % p; j + q < C; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < C && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t x = k[i + j], y = k[i + j + q];
+            k[i + j] = max(x, y);
+            k[i + j + q] = min(x, y);
+          }
+}
+
+// The k best from fp32 values; lane j < k gets the expert of rank j. Returns whether they may have decided
+// it wrongly. Each lane sorts its C keys once (without their ids: two instructions a step); a round then
+// takes the largest head of all lanes, and lanes hold consecutive experts, so that of equal keys the
+// lowest lane's is the lowest id. The places of the chosen keys in their lanes are found afterwards, for all
+// of them at once. (Rescanning the lane's
+// unsorted keys in every round took 1685 instructions a token at 256 experts.)
+template <int C, typename T>
+__device__ __forceinline__ bool select_fast(const TopkArgs& a, const T* row, const float (&l)[C], int lane, float mx,
+                                            float sum, int& mine) {
+  const bool biased = a.bias != nullptr, scored = biased || (a.groups > 1 && a.group_two);
+  float v[C], gv[C], most = 0.f;
+  if (scored) {
+    const float rsum = rcp(sum);
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int e = lane * C + i;
+      const float s = score32(a.score, l[i], mx, rsum);
+      const float b = biased && e < a.experts ? __ldg(a.bias + e) : 0.f;
+      const float t = s + b;
+      most = fmaxf(most, s + fabsf(b));
+      gv[i] = l[i] > -INFINITY && t == t ? t : -INFINITY;
+      v[i] = biased ? gv[i] : l[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = gv[i] = l[i];
+  }
+  // rounding errors of a score and its sum, twice (two of them are compared) and for pairs of experts
+  const float eps = scored ? 2e-6f * warp_max(most) : 0.f;
+  const int size = a.experts / a.groups;
+  uint32_t kept = 0xffffffffu;
+  bool doubt = false;
+  const int span = size / C;   // lanes per group when groups begin with lanes
+  const bool by_lane = size % C == 0 && (span & (span - 1)) == 0;
+  if (a.groups > 1) {
+    float gs = -INFINITY;   // lane g: the score of group g
+    if (by_lane) {
+      float b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < C; ++i) merge(b1, b2, gv[i], -INFINITY);
+      for (int o = 1; o < span; o <<= 1) {
+        const float c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
+        merge(b1, b2, c1, c2);
+      }
+      gs = __shfl_sync(0xffffffffu, a.group_two && b2 > -INFINITY ? b1 + b2 : b1, (lane * span) & 31);
+    } else {
+      for (int g = 0; g < a.groups; ++g) {
+        float b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          const int e = lane * C + i;
+          merge(b1, b2, e >= g * size && e < (g + 1) * size ? gv[i] : -INFINITY, -INFINITY);
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const float c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
+          merge(b1, b2, c1, c2);
+        }
+        if (lane == g) gs = a.group_two && b2 > -INFINITY ? b1 + b2 : b1;
+      }
+    }
+    uint32_t gk = lane < a.groups ? key_of(gs) : 0u, low = 0u;
+    kept = 0u;
+    for (int j = 0; j < a.kept; ++j) {
+      low = __reduce_max_sync(0xffffffffu, gk);
+      const int w = __ffs(__ballot_sync(0xffffffffu, gk == low)) - 1;
+      kept |= 1u << w;
+      if (lane == w) gk = 0u;
+    }
+    if (scored && a.kept < a.groups) {
+      const uint32_t high = __reduce_max_sync(0xffffffffu, gk);
+      doubt = high > key_of(-INFINITY) && !(value_of(low) - value_of(high) > eps);
+    }
+  }
+  uint32_t key[C], own[C];
+  if (by_lane || a.groups == 1) {
+    const bool in = a.groups == 1 || ((kept >> (lane / span & 31)) & 1u);
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      own[i] = in && lane * C + i < a.experts ? (v[i] > -INFINITY ? key_of(v[i]) : 1u) : 0u;
+  } else {
+    int g = lane * C / size, left = (g + 1) * size - lane * C;   // the expert's group, experts left in it
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const bool in = lane * C + i < a.experts && ((kept >> g) & 1u);
+      if (--left == 0) {
+        ++g;
+        left = size;
+      }
+      own[i] = in ? (v[i] > -INFINITY ? key_of(v[i]) : 1u) : 0u;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i) key[i] = own[i];
+  sort_desc<C>(key);
+  uint32_t got = 0u;
+  int from = 0;
+  const int rounds = biased ? a.topk + 1 : a.topk;
+  for (int j = 0; j < rounds; ++j) {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, key[0]);
+    const int w = __ffs(__ballot_sync(0xffffffffu, key[0] == top)) - 1;
+    if (lane == j) {
+      got = top;
+      from = w;
+    }
+    if (lane == w) {
+#pragma unroll
+      for (int i = 0; i + 1 < C; ++i) key[i] = key[i + 1];
+      key[C - 1] = 0u;
+    }
+  }
+  // the place of the chosen key in its lane: of several equal ones, taken in turn, the n-th
+  uint32_t at = 0u;
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+    if (__shfl_sync(0xffffffffu, own[i], from) == got) at |= 1u << i;
+  const bool picked = lane < rounds && got != 0u;
+  const uint32_t same = __match_any_sync(0xffffffffu, picked ? ((uint64_t)got << 5) | (uint64_t)from : (uint64_t)lane);
+  for (int n = __popc(same & ((1u << lane) - 1u)); n > 0; --n) at &= at - 1u;
+  mine = from * C + __ffs(at) - 1;
+  if (biased) {
+    // neighbours in the ranking, to the first one left out: far enough apart, or the same logit and bias, whose
+    // order is that of their ids
+    const uint32_t nk = __shfl_down_sync(0xffffffffu, got, 1);
+    const int ne = __shfl_down_sync(0xffffffffu, mine, 1);
+    bool near = lane < a.topk && got > 1u && nk > 1u && !(value_of(got) - value_of(nk) > eps);
+    if (near && a.bias[mine] == a.bias[ne] && row[mine] == row[ne]) near = false;
+    doubt = doubt || __any_sync(0xffffffffu, near);
+  }
+  return doubt;
+}
+
+// One warp per token; its instructions bound it (16384 tokens of 256 experts: see the sizes in the comment of
+// the file).
 template <int C, typename T>
 __global__ void __launch_bounds__(128) topk_kernel(TopkArgs a) {
   const int lane = threadIdx.x & 31;
@@ -283,24 +340,26 @@ __global__ void __launch_bounds__(128) topk_kernel(TopkArgs a) {
   const T* row = reinterpret_cast<const T*>(a.logits) + t * a.stride;
   float l[C];
   load_row<C, T>(a, row, lane, lowest, l);
-  const float mx = row_max<C>(l);
-  int mine = 0;
-  if (select<float, C, T>(a, row, l, lane, mx, mine)) mine = select_exact<C, T>(a, row, lane, lowest);
-  // weights of the chosen ones, from their unbiased scores
-  float sum = 1.f;
+  float mx = 0.f, sum = 1.f;
   if (a.score == SCORE_SOFTMAX) {
+    mx = row_max<C>(l);
     sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < C; ++i) sum += l[i] > -INFINITY ? expf(l[i] - mx) : 0.f;
+    for (int i = 0; i < C; ++i) sum += l[i] > -INFINITY ? __expf(l[i] - mx) : 0.f;
     sum = warp_sum(sum);
   }
+  int mine = 0;
+  if (select_fast<C, T>(a, row, l, lane, mx, sum, mine)) mine = select_exact<C, T>(a, row, lane, lowest);
+  // weights of the chosen ones, from their unbiased scores
   float w = 0.f;
   if (lane < a.topk) {
     const float x = clean(logit(row + mine), lowest);
-    if (x > -INFINITY) w = score<float>(a.score, x, mx, sum);
+    if (x > -INFINITY) w = score_weight(a.score, x, mx, sum);
   }
   if (a.renorm) {
-    const float s = warp_sum(w);
+    float s = w;   // lanes 16 and above hold zeros
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     w = s > 0.f ? __fdiv_rn(w, s) : 0.f;
   }
   if (lane < a.topk) {
@@ -311,33 +370,36 @@ __global__ void __launch_bounds__(128) topk_kernel(TopkArgs a) {
 
 // ── expert order ───────────────────────────────────────────────────────────────────────────────
 constexpr int OW = 8;               // warps of a block
-constexpr int OSEG = 256;           // consecutive pairs of a warp
+constexpr int OSTEP = 8;            // pairs of a thread
+constexpr int OSEG = 32 * OSTEP;    // consecutive pairs of a warp
 constexpr int OBLOCK = OW * OSEG;
 
-__device__ __forceinline__ int pair_expert(const OrderArgs& a, int64_t p) {
-  if (p >= a.pairs) return -1;
-  const int64_t e = a.ids[p];
-  return e >= 0 && e < a.experts ? (int)e : -1;
-}
-
-// cnt[w][e]: pairs of expert e in warp w's segment
-__device__ __forceinline__ void segment_counts(const OrderArgs& a, int* cnt, int64_t p0) {
+// The warp's pairs' experts (-1: none), all loads in flight at once, and cnt[w][e], the pairs of expert e
+// in warp w's segment.
+__device__ __forceinline__ void segment(const OrderArgs& a, int* cnt, int64_t p0, int (&ex)[OSTEP]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t id[OSTEP];
+#pragma unroll
+  for (int i = 0; i < OSTEP; ++i) {
+    const int64_t p = p0 + warp * OSEG + i * 32 + lane;
+    id[i] = p < a.pairs ? a.ids[p] : -1;
+  }
   for (int i = threadIdx.x; i < OW * a.experts; i += OW * 32) cnt[i] = 0;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < OSEG; i += 32) {
-    const int e = pair_expert(a, p0 + warp * OSEG + i + lane);
-    if (e >= 0) atomicAdd(&cnt[warp * a.experts + e], 1);
+  for (int i = 0; i < OSTEP; ++i) {
+    ex[i] = id[i] >= 0 && id[i] < a.experts ? (int)id[i] : -1;
+    if (ex[i] >= 0) atomicAdd(&cnt[warp * a.experts + ex[i]], 1);
   }
   __syncthreads();
 }
 
 __global__ void __launch_bounds__(OW * 32) order_count_kernel(OrderArgs a) {
   extern __shared__ int cnt[];
+  int ex[OSTEP];
   pdl_wait();
   pdl_trigger();
-  segment_counts(a, cnt, (int64_t)blockIdx.x * OBLOCK);
+  segment(a, cnt, (int64_t)blockIdx.x * OBLOCK, ex);
   for (int e = threadIdx.x; e < a.experts; e += OW * 32) {
     int s = 0;
 #pragma unroll
@@ -347,34 +409,44 @@ __global__ void __launch_bounds__(OW * 32) order_count_kernel(OrderArgs a) {
 }
 
 __global__ void __launch_bounds__(OW * 32) order_kernel(OrderArgs a) {
-  extern __shared__ int cnt[];
+  extern __shared__ int cnt[];               // [OW][experts] counts, then [experts] all pairs of each expert
   __shared__ int wsum[OW];
   __shared__ int total;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t p0 = (int64_t)blockIdx.x * OBLOCK;
+  int* all = cnt + OW * a.experts;
+  int ex[OSTEP];
   pdl_wait();
   pdl_trigger();
-  segment_counts(a, cnt, p0);
-  // four experts a thread: all pairs of each, and those in earlier blocks
-  int all[4], before[4], mine = 0;
+  segment(a, cnt, p0, ex);
+  // counts become each segment's first place after the expert's base (below)
+  for (int e = threadIdx.x; e < a.experts; e += OW * 32) {
+    int sum = 0, at = 0;
+    if (a.blocks > 1) {
+#pragma unroll 16
+      for (int b = 0; b < a.blocks; ++b) {
+        const int v = a.hist[(int64_t)b * a.experts + e];
+        sum += v;
+        at += b < (int)blockIdx.x ? v : 0;
+      }
+    }
+    int here = 0;
+#pragma unroll
+    for (int w = 0; w < OW; ++w) {
+      const int v = cnt[w * a.experts + e];
+      cnt[w * a.experts + e] = at + here;
+      here += v;
+    }
+    all[e] = a.blocks > 1 ? sum : here;
+  }
+  __syncthreads();
+  // exclusive scan of the experts' totals, four experts a thread
+  int four[4], mine = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int e = threadIdx.x * 4 + j;
-    all[j] = before[j] = 0;
-    if (e < a.experts) {
-      if (a.blocks == 1) {
-#pragma unroll
-        for (int w = 0; w < OW; ++w) all[j] += cnt[w * a.experts + e];
-      } else {
-#pragma unroll 8
-        for (int b = 0; b < a.blocks; ++b) {
-          const int v = a.hist[(int64_t)b * a.experts + e];
-          all[j] += v;
-          before[j] += b < (int)blockIdx.x ? v : 0;
-        }
-      }
-    }
-    mine += all[j];
+    four[j] = e < a.experts ? all[e] : 0;
+    mine += four[j];
   }
   int inc = mine;
 #pragma unroll
@@ -392,32 +464,31 @@ __global__ void __launch_bounds__(OW * 32) order_kernel(OrderArgs a) {
     const int e = threadIdx.x * 4 + j;
     if (e < a.experts) {
       if (blockIdx.x == 0) a.offsets[e] = base;
-      int at = base + before[j];
-#pragma unroll
-      for (int w = 0; w < OW; ++w) {   // counts become each segment's first place
-        const int v = cnt[w * a.experts + e];
-        cnt[w * a.experts + e] = at;
-        at += v;
-      }
+      all[e] = base;
     }
-    base += all[j];
+    base += four[j];
   }
   __syncthreads();
   if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[a.experts] = total;
   int* cursor = cnt + warp * a.experts;
-  for (int i = 0; i < OSEG; i += 32) {
-    const int64_t p = p0 + warp * OSEG + i + lane;
-    const int e = pair_expert(a, p);
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const int rank = __popc(same & ((1u << lane) - 1u));
+  unsigned same[OSTEP];
+#pragma unroll
+  for (int i = 0; i < OSTEP; ++i) same[i] = __match_any_sync(0xffffffffu, ex[i]);
+#pragma unroll
+  for (int i = 0; i < OSTEP; ++i) {
+    const int64_t p = p0 + warp * OSEG + i * 32 + lane;
+    const int rank = __popc(same[i] & ((1u << lane) - 1u));
     int at = -1;
-    if (e >= 0) at = cursor[e] + rank;
+    if (ex[i] >= 0) at = cursor[ex[i]] + rank;
     __syncwarp();
-    if (e >= 0 && rank == 0) cursor[e] += __popc(same);
+    if (ex[i] >= 0 && rank == 0) cursor[ex[i]] += __popc(same[i]);
     __syncwarp();
     if (p < a.pairs) {
+      if (at >= 0) {
+        at += all[ex[i]];
+        a.tokens[at] = (int)((unsigned)p / (unsigned)a.topk);
+      }
       a.places[p] = at;
-      if (at >= 0) a.tokens[at] = (int)(p / a.topk);
       if (p >= total) a.tokens[p] = -1;   // behind the last routed pair
     }
   }
@@ -451,7 +522,7 @@ int64_t order_blocks(int64_t pairs) { return (pairs + topk::OBLOCK - 1) / topk::
 
 cudaError_t launch_expert_order(const OrderArgs& a, cudaStream_t st) {
   const dim3 grid(a.blocks), block(topk::OW * 32);
-  const size_t smem = (size_t)topk::OW * a.experts * sizeof(int);
+  const size_t smem = (size_t)(topk::OW + 1) * a.experts * sizeof(int);
   if (a.blocks > 1) {
     const cudaError_t e = launch_pdl(topk::order_count_kernel, grid, block, smem, st, a);
     if (e != cudaSuccess) return e;

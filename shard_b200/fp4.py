@@ -29,7 +29,6 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import dataclasses
 from typing import Optional, Union
 
 import torch
@@ -40,37 +39,30 @@ from ._lib import check, lib, ptr
 
 PLAIN, W13 = _lib.MAT_PLAIN, _lib.MAT_W13
 DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
+_FMT = {"nvfp4": F.FMT_NVFP4, "mxfp4": F.FMT_MXFP4, F.FMT_NVFP4: F.FMT_NVFP4, F.FMT_MXFP4: F.FMT_MXFP4}
+
+# A decoded token's call is bound by its host side: these run once per call, without lookups by name.
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
+_empty = torch.empty
 
 
 def _fmt(fmt: Union[int, str]) -> int:
-    f = F.FMT_IDS.get(fmt, fmt) if isinstance(fmt, str) else fmt
-    if f not in (F.FMT_NVFP4, F.FMT_MXFP4):
+    f = _FMT.get(fmt)
+    if f is None:
         raise ValueError(f"format {fmt!r} is not nvfp4 or mxfp4")
     return f
 
 
 @contextlib.contextmanager
-def _other(device, stream):
+def _elsewhere(device, stream):
+    """`device` made current, and `stream` when one is given (also for the allocations of the call)."""
     with torch.cuda.device(device):
         if stream is None:
             yield
         else:
             with torch.cuda.stream(stream):
                 yield
-
-
-_HERE = contextlib.nullcontext()
-
-
-def _on(t: torch.Tensor, stream):
-    """The context in which a call on `t` runs: its device current, and `stream` when one is given."""
-    if stream is None and t.device.index == torch.cuda.current_device():
-        return _HERE
-    return _other(t.device, stream)
-
-
-def _sp(t: torch.Tensor) -> int:
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _same_device(what, ref, *tensors):
@@ -89,29 +81,45 @@ def _float_vec(what, name, t, n=None):
         raise ValueError(f"{what}: {name} must be contiguous fp32" + ("" if n is None else f" with {n} values"))
 
 
-@dataclasses.dataclass(eq=False)
 class Fp4Tensor:
     """A 4-bit operand on the device: `mats` matrices of `rows` rows of `k` values (activations: one).
 
     codes   uint8 [mats * rows, kp / 2], kp = k rounded up to 32; low nibble first
     scales  uint8, the atoms of 128 rows x 4 scales that the products read
-    ts      NVFP4: fp32 tensor scale, [1] or one per row (activations), [mats] or [mats, 2] (weights)
+    ts      NVFP4: fp32 tensor scale, [1] or one per row (activations), [mats, 1 or 2] (weights), or None
     offsets int32 [groups + 1]: the rows' expert groups (activations of grouped_gemm), else None
     """
-    fmt: int
-    mats: int
-    rows: int
-    k: int
-    codes: torch.Tensor
-    scales: torch.Tensor
-    ts: Optional[torch.Tensor] = None
-    offsets: Optional[torch.Tensor] = None
-    kind: int = PLAIN
-    shape: tuple = ()
+    __slots__ = ("fmt", "mats", "rows", "k", "kind", "shape", "offsets", "per_row", "_buf", "_parts", "_codes", "_scales",
+                 "_ts", "codes_ptr", "scales_ptr", "ts_ptr")
+
+    def __init__(self, fmt, mats, rows, k, codes, scales, ts=None, offsets=None, kind=PLAIN, shape=()):
+        self.fmt, self.mats, self.rows, self.k, self.kind, self.shape, self.offsets = fmt, mats, rows, k, kind, shape, offsets
+        self._buf, self._codes, self._scales, self._ts = codes, codes, scales, ts
+        self._parts = None
+        self.per_row = False
+        self.codes_ptr, self.scales_ptr, self.ts_ptr = codes.data_ptr(), scales.data_ptr(), ptr(ts)
 
     @property
     def device(self):
-        return self.codes.device
+        return self._buf.device
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._buf[:self._parts[0]].view(self.rows, -1)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._buf[self._parts[0]:self._parts[1]]
+        return self._scales
+
+    @property
+    def ts(self) -> Optional[torch.Tensor]:
+        if self._ts is None and self.per_row:
+            self._ts = self._buf[self._parts[1]:].view(torch.float32)
+        return self._ts
 
     def canonical_scales(self) -> torch.Tensor:
         """uint8 [mats * rows, K / 16 or K / 32]: the scales row by row (no expert groups)."""
@@ -131,42 +139,60 @@ def quant(x: torch.Tensor, fmt: Union[int, str] = F.FMT_NVFP4, tensor_scale: Opt
     rows          int32 [P]: operand row p is x's row rows[p] (a gather in the same pass); outside x: zeros
     offsets       int32 [E + 1]: expert e's rows are offsets[e] .. offsets[e + 1] - 1 (for grouped_gemm);
                   rows behind offsets[E] are left as they are"""
-    f = _fmt(fmt)
-    if not x.is_cuda or x.dtype not in DTYPES or x.dim() < 1:
+    f = _FMT.get(fmt)
+    if f is None:
+        _fmt(fmt)
+    dt = DTYPES.get(x.dtype)
+    if dt is None or not x.is_cuda or x.dim() < 1:
         raise ValueError("quant: x must be a CUDA tensor of bf16, fp16 or fp32")
-    k = x.shape[-1]
+    dev = x.get_device()
+    if stream is not None or dev != _current_device():
+        with _elsewhere(x.device, stream):
+            return quant(x, fmt, tensor_scale, rows, offsets)
+    shape = x.shape
+    k = shape[-1]
     z = x if x.dim() == 2 else x.reshape(-1, k)
-    if z.stride(1) != 1 and k > 1:
-        z = z.contiguous()
     m = z.shape[0]
-    p = m if rows is None else rows.shape[0]
-    _same_device("quant", x, tensor_scale, rows, offsets)
+    stride, inner = z.stride()
+    if inner != 1 and k > 1:
+        z = z.contiguous()
+        stride = k
+    p, groups, po, pr, pt = m, 0, None, None, None
     if rows is not None:
         _index("quant", "rows", rows)
-    groups = 0
+        _same_device("quant", x, rows)
+        p, pr = rows.shape[0], rows.data_ptr()
     if offsets is not None:
         _index("quant", "offsets", offsets)
-        groups = offsets.shape[0] - 1
+        _same_device("quant", x, offsets)
+        groups, po = offsets.shape[0] - 1, offsets.data_ptr()
         if groups < 1:
             raise ValueError("quant: offsets must hold at least two values")
     if tensor_scale is not None:
         if f != F.FMT_NVFP4:
             raise ValueError("quant: MXFP4 has no tensor scale")
         _float_vec("quant", "tensor_scale", tensor_scale, 1)
-    L = lib()
-    with _on(x, stream):
-        kp = (k + 31) // 32 * 32
-        dev = x.device
-        codes = torch.empty((p, kp // 2), dtype=torch.uint8, device=dev)
-        scales = torch.empty(L.sb_fp4_scale_bytes(f, 1, p, k, groups), dtype=torch.uint8, device=dev)
-        ts = tensor_scale
-        if f == F.FMT_NVFP4 and ts is None:
-            ts = torch.empty(p, dtype=torch.float32, device=dev)
-        check(L.sb_fp4_quant(f, z.data_ptr(), DTYPES[x.dtype], m, k, z.stride(0) if m > 1 else k, ptr(rows), p,
-                             ptr(tensor_scale), ptr(offsets), groups, codes.data_ptr(), scales.data_ptr(),
-                             None if ts is tensor_scale else ts.data_ptr(), _sp(x)), "sb_fp4_quant")
-    shape = tuple(x.shape[:-1]) if rows is None else (p,)
-    return Fp4Tensor(f, 1, p, k, codes, scales, ts, offsets, PLAIN, shape)
+        _same_device("quant", x, tensor_scale)
+        pt = tensor_scale.data_ptr()
+    # one allocation: codes, scale atoms (sb_fp4_scale_bytes), the rows' tensor scales
+    kp = (k + 31) >> 5
+    blocks = (p >> 7) + groups if groups else (p + 127) >> 7
+    end = p * kp * 16
+    per_row = f == F.FMT_NVFP4 and pt is None
+    atoms_end = end + blocks * ((kp + 1) >> 1 if f == F.FMT_NVFP4 else (kp + 3) >> 2) * 512
+    buf = _empty(atoms_end + 4 * p if per_row else atoms_end, dtype=torch.uint8, device=x.device)
+    base = buf.data_ptr()
+    q = Fp4Tensor.__new__(Fp4Tensor)
+    q.fmt, q.mats, q.rows, q.k, q.kind, q.offsets, q.per_row = f, 1, p, k, PLAIN, offsets, per_row
+    q.shape = shape[:-1] if rows is None else (p,)
+    q._buf, q._parts, q._codes, q._scales, q._ts = buf, (end, atoms_end), None, None, tensor_scale
+    q.codes_ptr, q.scales_ptr = base, base + end
+    q.ts_ptr = base + atoms_end if per_row else pt
+    rc = lib().sb_fp4_quant(f, z.data_ptr(), dt, m, k, stride if m > 1 else k, pr, p, pt, po, groups, base, base + end,
+                            q.ts_ptr if per_row else None, _current_stream(dev))
+    if rc:
+        check(rc, "sb_fp4_quant")
+    return q
 
 
 def dequant(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
@@ -174,13 +200,19 @@ def dequant(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, stream=None) -> t
     expert groups."""
     if q.offsets is not None or q.mats != 1 or q.kind != PLAIN:
         raise ValueError("dequant: a plain operand of one matrix, without expert groups")
-    if dtype not in DTYPES:
+    dt = DTYPES.get(dtype)
+    if dt is None:
         raise ValueError(f"dequant: dtype {dtype}")
-    with _on(q.codes, stream):
-        y = torch.empty((*q.shape, q.k), dtype=dtype, device=q.device)
-        per_row = q.ts is not None and q.ts.numel() == q.rows and q.rows > 1
-        check(lib().sb_fp4_dequant(q.fmt, q.codes.data_ptr(), q.scales.data_ptr(), ptr(q.ts), per_row, q.rows, q.k,
-                                   y.data_ptr(), DTYPES[dtype], _sp(q.codes)), "sb_fp4_dequant")
+    buf = q._buf
+    dev = buf.get_device()
+    if stream is not None or dev != _current_device():
+        with _elsewhere(buf.device, stream):
+            return dequant(q, dtype)
+    y = _empty((*q.shape, q.k), dtype=dtype, device=buf.device)
+    rc = lib().sb_fp4_dequant(q.fmt, q.codes_ptr, q.scales_ptr, q.ts_ptr, q.per_row, q.rows, q.k, y.data_ptr(), dt,
+                              _current_stream(dev))
+    if rc:
+        check(rc, "sb_fp4_dequant")
     return y
 
 
@@ -207,52 +239,67 @@ def pack(fmt: Union[int, str], codes: torch.Tensor, scales: torch.Tensor, ts: Op
             raise ValueError(f"pack: {ts.shape[1]} tensor scales a matrix")
     if kind not in (PLAIN, W13) or (kind == W13 and n % 2):
         raise ValueError("pack: kind is PLAIN, or W13 with an even number of rows")
-    with _on(codes, stream):
-        c, s = c.reshape(mats, n, k // 2), s.reshape(mats, n, nb)
-        if kind == W13:
-            c, s = (t.view(mats, 2, n // 2, -1).transpose(1, 2).reshape(mats, n, -1) for t in (c, s))
-        c, s = c.contiguous().view(mats * n, k // 2), s.contiguous()
-        L = lib()
-        out = torch.empty(L.sb_fp4_scale_bytes(f, mats, n, k, 0), dtype=torch.uint8, device=c.device)
-        check(L.sb_fp4_tile_scales(f, s.data_ptr(), out.data_ptr(), mats, n, k, _sp(c)), "sb_fp4_tile_scales")
+    if stream is not None or codes.get_device() != _current_device():
+        with _elsewhere(codes.device, stream):
+            return pack(fmt, codes, scales, ts, kind)
+    c, s = c.reshape(mats, n, k // 2), s.reshape(mats, n, nb)
+    if kind == W13:
+        c, s = (t.view(mats, 2, n // 2, -1).transpose(1, 2).reshape(mats, n, -1) for t in (c, s))
+    c, s = c.contiguous().view(mats * n, k // 2), s.contiguous()
+    L = lib()
+    out = torch.empty(L.sb_fp4_scale_bytes(f, mats, n, k, 0), dtype=torch.uint8, device=c.device)
+    check(L.sb_fp4_tile_scales(f, s.data_ptr(), out.data_ptr(), mats, n, k, _current_stream(c.get_device())),
+          "sb_fp4_tile_scales")
     return Fp4Tensor(f, mats, n, k, c, out, ts, None, kind, tuple(codes.shape[:-1]))
 
 
 def _operands(what, a, w, out_dtype):
+    """Checks shared by the products; the output type's code."""
     if a.fmt != w.fmt:
         raise ValueError(f"{what}: operands of two formats")
     if a.k != w.k:
         raise ValueError(f"{what}: K {a.k} and {w.k}")
     if a.mats != 1 or a.kind != PLAIN:
         raise ValueError(f"{what}: the first operand is one matrix of rows")
-    if out_dtype not in DTYPES:
+    dt = DTYPES.get(out_dtype)
+    if dt is None:
         raise ValueError(f"{what}: out_dtype {out_dtype}")
-    _same_device(what, a.codes, w.codes)
-    return a.ts is not None and a.ts.numel() == a.rows and a.rows > 1
+    if w._buf.get_device() != a._buf.get_device():
+        raise ValueError(f"{what}: operands on {a.device} and {w.device}")
+    return dt
 
 
-def _output(what, out, shape, dtype, like):
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != like.device or \
-            (out.numel() and out.stride(-1) != 1):
-        raise ValueError(f"{what}: out must be {tuple(shape)} {dtype} on {like.device}, rows contiguous")
-    return out
+def _check_out(what, out, shape, dtype, like):
+    if tuple(out.shape) != shape or out.dtype != dtype or out.device != like.device or \
+            (out.numel() and shape[1] > 1 and out.stride(-1) != 1) or (shape[0] > 1 and out.stride(0) < shape[1]):
+        raise ValueError(f"{what}: out must be {shape} {dtype} on {like.device}, with contiguous rows that do not overlap")
 
 
 def gemm(a: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None,
          stream=None) -> torch.Tensor:
-    """y [..., N] = A [..., K] W [N, K]^T, summed in fp32 and rounded once. `out` [M, N] may have any row stride."""
-    per_row = _operands("gemm", a, w, out_dtype)
-    if a.offsets is not None or w.mats != 1 or w.kind != PLAIN:
+    """y [..., N] = A [..., K] W [N, K]^T, summed in fp32 and rounded once. `out` [M, N] may have any row stride.
+    The tensor scale of `w` is one value or none (one per row, as quant makes them, multiplies its outputs)."""
+    dt = _operands("gemm", a, w, out_dtype)
+    if a.offsets is not None or w.offsets is not None or w.mats != 1 or w.kind != PLAIN:
         raise ValueError("gemm: plain operands of one matrix (grouped_gemm takes banks and expert groups)")
-    with _on(a.codes, stream):
-        y = _output("gemm", out, (*a.shape, w.rows) if out is None else (a.rows, w.rows), out_dtype, a.codes)
-        ld = w.rows if out is None or a.rows < 2 else out.stride(0)
-        check(lib().sb_fp4_gemm(a.fmt, a.codes.data_ptr(), a.scales.data_ptr(), ptr(a.ts), per_row, a.rows,
-                                w.codes.data_ptr(), w.scales.data_ptr(), ptr(w.ts), w.rows, a.k, y.data_ptr(),
-                                DTYPES[out_dtype], ld, _sp(a.codes)), "sb_fp4_gemm")
-    return y
+    buf = a._buf
+    dev = buf.get_device()
+    if stream is not None or dev != _current_device():
+        with _elsewhere(buf.device, stream):
+            return gemm(a, w, out_dtype, out)
+    m, n = a.rows, w.rows
+    ld = n
+    if out is None:
+        out = _empty((*a.shape, n), dtype=out_dtype, device=buf.device)
+    else:
+        _check_out("gemm", out, (m, n), out_dtype, buf)
+        if m > 1:
+            ld = out.stride(0)
+    rc = lib().sb_fp4_gemm(a.fmt, a.codes_ptr, a.scales_ptr, a.ts_ptr, a.per_row, m, w.codes_ptr, w.scales_ptr, w.ts_ptr,
+                           w.per_row, n, a.k, out.data_ptr(), dt, ld, _current_stream(dev))
+    if rc:
+        check(rc, "sb_fp4_gemm")
+    return out
 
 
 def grouped_gemm(a: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16,
@@ -261,25 +308,39 @@ def grouped_gemm(a: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bflo
     """Row p of expert e (offsets[e] <= p < offsets[e+1]) against W_e of the bank: y [P, N], or for a W13 bank
     y [P, N/2] = silu(min(g, limit)) * clip(u, -limit, limit) (limit 0: no clamp). row_weight fp32 [P]
     multiplies the output rows. Rows behind offsets[E] are left as they are."""
-    per_row = _operands("grouped_gemm", a, w, out_dtype)
-    if a.offsets is None or a.offsets.shape[0] != w.mats + 1:
-        raise ValueError(f"grouped_gemm: the rows need offsets [{w.mats + 1}] (quant(..., offsets=))")
+    dt = _operands("grouped_gemm", a, w, out_dtype)
+    off = a.offsets
+    if off is None or off.shape[0] != w.mats + 1 or w.per_row or w.offsets is not None:
+        raise ValueError(f"grouped_gemm: rows with offsets [{w.mats + 1}] (quant(..., offsets=)) and a bank (pack)")
     if not limit >= 0.0:
         raise ValueError("grouped_gemm: limit must be >= 0")
+    buf = a._buf
+    p = a.rows
+    pw = None
     if row_weight is not None:
-        _float_vec("grouped_gemm", "row_weight", row_weight, a.rows)
-        _same_device("grouped_gemm", a.codes, row_weight)
+        _float_vec("grouped_gemm", "row_weight", row_weight, p)
+        _same_device("grouped_gemm", buf, row_weight)
+        pw = row_weight.data_ptr()
+    dev = buf.get_device()
+    if stream is not None or dev != _current_device():
+        with _elsewhere(buf.device, stream):
+            return grouped_gemm(a, w, out_dtype, row_weight, limit, out)
     swiglu = w.kind == W13
-    width = w.rows // 2 if swiglu else w.rows
-    with _on(a.codes, stream):
-        y = _output("grouped_gemm", out, (a.rows, width), out_dtype, a.codes)
-        ld = y.stride(0) if a.rows > 1 else width
-        check(lib().sb_fp4_grouped_gemm(a.fmt, a.codes.data_ptr(), a.scales.data_ptr(), ptr(a.ts), per_row, a.rows,
-                                        a.offsets.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), ptr(w.ts),
-                                        1 if w.ts is None else w.ts.shape[1], w.mats, w.rows, a.k, swiglu, float(limit),
-                                        ptr(row_weight), y.data_ptr(), DTYPES[out_dtype], ld, _sp(a.codes)),
-              "sb_fp4_grouped_gemm")
-    return y
+    n = w.rows
+    width = n >> 1 if swiglu else n
+    ld = width
+    if out is None:
+        out = _empty((p, width), dtype=out_dtype, device=buf.device)
+    else:
+        _check_out("grouped_gemm", out, (p, width), out_dtype, buf)
+        if p > 1:
+            ld = out.stride(0)
+    rc = lib().sb_fp4_grouped_gemm(a.fmt, a.codes_ptr, a.scales_ptr, a.ts_ptr, a.per_row, p, off.data_ptr(), w.codes_ptr,
+                                   w.scales_ptr, w.ts_ptr, 1 if w._ts is None else w._ts.shape[1], w.mats, n, a.k, swiglu,
+                                   limit, pw, out.data_ptr(), dt, ld, _current_stream(dev))
+    if rc:
+        check(rc, "sb_fp4_grouped_gemm")
+    return out
 
 
 def device_error(device=None) -> int:

@@ -16,9 +16,10 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from ._lib import check, lib, ptr
-from .fp4 import DTYPES, _on, _same_device, _sp
+from ._lib import check, lib
+from .fp4 import DTYPES, _current_device, _current_stream, _elsewhere, _empty, _same_device
 
+_SCORE = _lib.SCORE
 _GROUP_SCORE = {"max": 0, "top2": 1}
 
 
@@ -42,23 +43,32 @@ def topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, scor
 
     Values are compared as real numbers, ties go to the lower id. An expert whose logit is NaN, -inf or the
     type's lowest value is masked: after all others of the kept groups, with weight 0."""
-    if score not in _lib.SCORE or group_score not in _GROUP_SCORE:
+    sc, gs, dt = _SCORE.get(score), _GROUP_SCORE.get(group_score), DTYPES.get(logits.dtype)
+    if sc is None or gs is None:
         raise ValueError(f"topk: score {score!r}, group_score {group_score!r}")
-    if not logits.is_cuda or logits.dtype not in DTYPES or logits.dim() != 2:
+    if dt is None or not logits.is_cuda or logits.dim() != 2:
         raise ValueError("topk: logits must be a CUDA tensor [T, E] of bf16, fp16 or fp32")
+    dev = logits.get_device()
+    if stream is not None or dev != _current_device():
+        with _elsewhere(logits.device, stream):
+            return topk(logits, k, bias, score, n_group, topk_group, group_score, renormalize, scale)
     t, e = logits.shape
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (e,) or not bias.is_contiguous()):
-        raise ValueError(f"topk: bias must be contiguous fp32 [{e}]")
-    _same_device("topk", logits, bias)
-    if logits.stride(1) != 1 and e > 1:
+    stride, inner = logits.stride()
+    if inner != 1 and e > 1:
         logits = logits.contiguous()
-    with _on(logits, stream):
-        w = torch.empty((t, k), dtype=torch.float32, device=logits.device)
-        ids = torch.empty((t, k), dtype=torch.int64, device=logits.device)
-        check(lib().sb_route_topk(logits.data_ptr(), DTYPES[logits.dtype], t, e, logits.stride(0) if t > 1 else e,
-                                  ptr(bias), k, _lib.SCORE[score], n_group, topk_group, _GROUP_SCORE[group_score],
-                                  bool(renormalize), float(scale), w.data_ptr(), ids.data_ptr(), _sp(logits)),
-              "sb_route_topk")
+        stride = e
+    pb = None
+    if bias is not None:
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (e,) or not bias.is_contiguous():
+            raise ValueError(f"topk: bias must be contiguous fp32 [{e}]")
+        _same_device("topk", logits, bias)
+        pb = bias.data_ptr()
+    w = _empty((t, k), dtype=torch.float32, device=logits.device)
+    ids = _empty((t, k), dtype=torch.int64, device=logits.device)
+    rc = lib().sb_route_topk(logits.data_ptr(), dt, t, e, stride if t > 1 else e, pb, k, sc, n_group, topk_group, gs,
+                             renormalize, scale, w.data_ptr(), ids.data_ptr(), _current_stream(dev))
+    if rc:
+        check(rc, "sb_route_topk")
     return w, ids
 
 
@@ -67,16 +77,23 @@ def expert_order(indices: torch.Tensor, n_experts: int, stream=None) -> ExpertOr
     left out."""
     if not indices.is_cuda or indices.dtype != torch.int64 or indices.dim() != 2 or not indices.is_contiguous():
         raise ValueError("expert_order: indices must be a contiguous CUDA int64 tensor [T, k]")
+    dev = indices.get_device()
+    if stream is not None or dev != _current_device():
+        with _elsewhere(indices.device, stream):
+            return expert_order(indices, n_experts)
     t, k = indices.shape
     if k < 1:
         raise ValueError("expert_order: no slots")
+    pairs = t * k
     L = lib()
-    with _on(indices, stream):
-        i32 = dict(dtype=torch.int32, device=indices.device)
-        offsets, tokens = torch.empty(n_experts + 1, **i32), torch.empty(t * k, **i32)
-        places = torch.empty((t, k), **i32)
-        need = L.sb_expert_order_workspace_bytes(t * k, n_experts)
-        ws = torch.empty(need, dtype=torch.uint8, device=indices.device) if need else None
-        check(L.sb_expert_order(indices.data_ptr(), t, k, n_experts, offsets.data_ptr(), tokens.data_ptr(),
-                                places.data_ptr(), ptr(ws), need, _sp(indices)), "sb_expert_order")
-    return ExpertOrder(offsets, tokens, places)
+    need = L.sb_expert_order_workspace_bytes(pairs, n_experts) if pairs > 1024 else 0
+    # one allocation: places, tokens, offsets, the kernels' counts
+    n0, n1, n2, n3 = pairs, pairs, n_experts + 1, need >> 2
+    buf = _empty(n0 + n1 + n2 + n3, dtype=torch.int32, device=indices.device)
+    base = buf.data_ptr()
+    rc = L.sb_expert_order(indices.data_ptr(), t, k, n_experts, base + 4 * (n0 + n1), base + 4 * n0, base,
+                           base + 4 * (n0 + n1 + n2) if need else None, need, _current_stream(dev))
+    if rc:
+        check(rc, "sb_expert_order")
+    places, tokens, offsets, _ = buf.split_with_sizes((n0, n1, n2, n3))
+    return ExpertOrder(offsets, tokens, places.view(t, k))

@@ -186,16 +186,19 @@ def test_gemm(fmt, m, n, k):
 
 @gpu
 @pytest.mark.parametrize("fmt", [NV, MX])
-def test_gemm_of_an_odd_k_and_a_calibrated_scale(fmt):
-    """K 100: both operands are padded to 128 with zero codes, whatever the scale bytes behind K."""
+@pytest.mark.parametrize("calibrated", [False, True])
+def test_gemm_of_two_quantised_matrices(fmt, calibrated):
+    """K 100: both operands are padded to 128 with zero codes. Tensor scales: one, or one per row of either."""
     _need_gpu()
-    x, wx = _acts(20, 100, torch.bfloat16, seed=1, spread=0.5), _acts(50, 100, torch.float32, seed=2, spread=0.5)
-    ts = torch.tensor([0.02], device="cuda") if fmt == NV else None
+    x, wx = _acts(20, 100, torch.bfloat16, seed=1, spread=0.5), _acts(150, 100, torch.float32, seed=2, spread=0.5)
+    ts = torch.tensor([0.02], device="cuda") if fmt == NV and calibrated else None
     a, w = fp4.quant(x.cuda(), fmt, tensor_scale=ts), fp4.quant(wx.cuda(), fmt, tensor_scale=ts)
     av, wv = _values(a), _values(w)
     exact = av @ wv.T
     y = fp4.gemm(a, w, out_dtype=torch.float32).cpu().double()
     assert bool(((y - exact).abs() <= _tol(av, wv, exact, 128, torch.float32)).all())
+    one = fp4.gemm(fp4.quant(x[0].cuda(), fmt, tensor_scale=ts), w)      # a vector
+    assert one.shape == (150,) and torch.equal(one, fp4.gemm(a, w)[0])
 
 
 @gpu

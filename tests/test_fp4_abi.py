@@ -55,7 +55,7 @@ def test_product_refusals():
     L = _lib.lib()
 
     def g(fmt=NV, a=FAKE, s=FAKE, m=4, w=FAKE, ws=FAKE, wts=None, n=8, k=64, y=FAKE, dt=0, ld=8):
-        return L.sb_fp4_gemm(fmt, a, s, None, 0, m, w, ws, wts, n, k, y, dt, ld, None)
+        return L.sb_fp4_gemm(fmt, a, s, None, 0, m, w, ws, wts, 0, n, k, y, dt, ld, None)
 
     assert g(fmt=FP8) == -3 and g(dt=3) == -1
     for kw in (dict(n=0), dict(k=0), dict(k=65537), dict(m=-1), dict(ld=7), dict(m=1 << 30, n=1 << 20, ld=1 << 20)):
