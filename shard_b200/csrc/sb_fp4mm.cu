@@ -5,14 +5,16 @@
 // (e8m0) values of either side and sums in fp32, so the whole K accumulates in tensor memory and is
 // read once; the fp32 tensor scales are applied there.
 //
-// The weights are the M operand (128 rows a tile), the tokens N: a token tile takes any multiple of 8
-// columns, so one decoded token costs an 8-column tile and ragged expert groups waste at most 7.
-// Stages hold 256 K: 128 weight rows and the tile's token rows of 128 bytes each, landed by TMA in the
-// 128-byte-swizzled K-major form, and their scale atoms by bulk copies. Roles (192 threads): warp 4
-// copies, warp 5 moves scale atoms to tensor memory and issues the MMAs, warps 0-3 read the
-// accumulator (thread = weight row) and store 32 consecutive outputs of one token per instruction.
-// Two accumulators of up to 192 columns alternate, so that one tile's readback overlaps the next
-// tile's products; 192 and not 256 leaves room for the scales beside two of them.
+// The weights are the M operand, the tokens N: a token tile takes any multiple of 8 columns, so one
+// decoded token costs an 8-column tile and ragged expert groups waste little. A CTA takes 128 weight
+// rows; where there are tiles for all SMs, two CTAs form a pair (cta_group::2) that shares the token
+// rows of a 256-row tile, each loading half of them, and one of them issues for both.
+// Stages hold 256 K: 128 weight rows and the token rows of 128 bytes each, landed by TMA in the 128-byte-
+// swizzled K-major form, and their scale atoms. Roles (352 threads): warp 8 copies codes, warp 9 scales,
+// warp 10 moves scale atoms to tensor memory and issues the MMAs, warps 0-7 read the accumulator (a
+// thread: one weight row, every other 32 columns) and store. Two accumulators of up to 192 columns
+// alternate, so that one tile's readback overlaps the next tile's products; 192 and not 256 leaves room
+// for the scales beside two of them.
 //
 // Every wait is bounded: on timeout the CTA sets the device's error word and winds down.
 #include <cudaTypedefs.h>
@@ -29,13 +31,14 @@ namespace fp4mm {
 
 using namespace tc5;
 
-constexpr int NTHREADS = 192;
-constexpr int PRODUCER_WARP = 4;
-constexpr int MMA_WARP = 5;
+constexpr int EPI_WARPS = 8;
+constexpr int CODE_WARP = 8;         // copies codes,
+constexpr int SCALE_WARP = 9;        // and their scales
+constexpr int MMA_WARP = 10;
+constexpr int NTHREADS = 352;
 constexpr int NT_MAX = 192;          // token columns of a tile
 constexpr int BOX = 32;              // token rows of one copy with expert groups
 constexpr int A_BYTES = 128 * 128;   // a stage's weight rows
-constexpr int SF_BLOCK = 4 * 512;    // a stage's scale atoms of 128 rows
 constexpr int MAX_STAGES = 10;
 constexpr int MAX_MATS = 1024;
 constexpr int TMEM_COLS = 512;
@@ -44,63 +47,163 @@ constexpr int SFB_COL = SFA_COL + 16;  // 4 atoms x 8 columns of the tokens (two
 constexpr uint32_t WAIT_LIMIT = 1u << 16;
 constexpr int SMEM_LIMIT = 232448;
 
+template <bool NV>
+constexpr int SF_BLOCK = NV ? 2048 : 1024;   // a stage's scale atoms of 128 rows
+
 __device__ int g_err;
 
 struct Args {
-  CUtensorMap map_w, map_a;
+  CUtensorMap map_w, map_a;     // codes
+  CUtensorMap map_ws, map_as;   // scale atoms
   Fp4MmArgs g;
   int nt;            // token columns of a full tile (a multiple of 64 when a matrix has several)
   int box;           // token rows of one copy
   int stages;
-  int b_bytes;       // token rows of a stage
-  int sfb_bytes;     // their scale atoms
-  int atoms;         // scale atoms along K
+  int b_bytes;       // token rows of a stage (of one CTA)
+  int sblk;          // row blocks of token scales that a copy brings
   int ksteps;        // MMAs along K (64 values each)
+  int vec;           // 16-byte stores to y
 };
 
 struct Ctl {
   uint64_t full[MAX_STAGES], empty[MAX_STAGES], accfull[2], accempty[2], drain;
   uint32_t tmem_base;
   int abort;
+  alignas(16) float scale[EPI_WARPS][NT_MAX / 2];   // of each warp's tokens: tensor scale,
+  alignas(16) float weight[EPI_WARPS][NT_MAX / 2];  // row weight
   int tiles[MAX_MATS + 1];   // tiles before each matrix
   int rows[MAX_MATS + 1];    // first token row of each matrix's group, and the end of the last
 };
 
 struct Tile {
   int mat, n0, t0, cnt, row0;   // matrix, first weight row, first token of the group, tokens, group's first row
-  int64_t blk;                  // group's first scale row block
+  int blk;                      // the tokens' first scale row block
 };
 
-// instruction descriptor: e2m1 x e2m1, M = 128, N = n, scale byte pair `id` of both sides' words
-template <bool NV>
-__device__ __forceinline__ uint32_t idesc(uint32_t n, uint32_t id) {
-  return (id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((NV ? 0u : 1u) << 23) | ((128u >> 4) << 24) | (id << 29);
+// instruction descriptor: e2m1 x e2m1, M = 128 (256 of a pair), N = n (bits 4 and 29 up: which scale bytes of either side's words)
+template <bool NV, bool PAIR>
+__device__ __forceinline__ uint32_t idesc(uint32_t n) {
+  return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((NV ? 0u : 1u) << 23) | (((PAIR ? 256u : 128u) >> 4) << 24);
 }
 
-template <bool NV>
+#define SB_MMA(group, kind)                                                                                        \
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"                                                       \
+               " tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, [%5], [%6], p;\n}\n" ::"r"(d),  \
+               "l"(ad), "l"(bd), "r"(id), "r"(acc), "r"(sfa), "r"(sfb))
+
+template <bool NV, bool PAIR>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t id, uint32_t sfa, uint32_t sfb,
                                     uint32_t acc) {
-  if constexpr (NV) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%5], [%6], p;\n}\n" ::"r"(d),
-        "l"(ad), "l"(bd), "r"(id), "r"(acc), "r"(sfa), "r"(sfb));
-  } else {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n}\n" ::"r"(d),
-        "l"(ad), "l"(bd), "r"(id), "r"(acc), "r"(sfa), "r"(sfb));
-  }
+  if constexpr (NV && PAIR) SB_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+  else if constexpr (NV) SB_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
+  else if constexpr (PAIR) SB_MMA("2", "mxf4.block_scale.scale_vec::2X");
+  else SB_MMA("1", "mxf4.block_scale.scale_vec::2X");
 }
+#undef SB_MMA
 
-// one scale atom into four tensor memory columns of every 32-lane quarter
-__device__ __forceinline__ void cp_sf(uint32_t taddr, uint32_t src) {
+// a scale atom as the source of a copy: 32 rows of 16 bytes, no swizzle
+__device__ __forceinline__ uint64_t sf_desc(uint32_t src) {
   uint64_t d = 0;
   d |= (uint64_t)((src >> 4) & 0x3FFFu);
   d |= (uint64_t)(128 >> 4) << 16;
   d |= (uint64_t)(128 >> 4) << 32;
   d |= (uint64_t)1 << 46;
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(taddr), "l"(d) : "memory");
+  return d;
+}
+// one scale atom into four tensor memory columns of every 32-lane quarter
+template <bool PAIR>
+__device__ __forceinline__ void cp_sf(uint32_t taddr, uint64_t desc) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// arrive, once all MMAs issued so far have finished, on `bar` (of both CTAs of a pair)
+template <bool PAIR>
+__device__ __forceinline__ void commit_to(uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    commit(bar);
+}
+
+// tensor copies into this CTA's shared memory; a pair's complete on the first CTA's barrier
+template <bool PAIR>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+  else
+    tma_load_2d(dst, map, c0, c1, bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+        "[%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+            dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+
+// the address of this shared memory location in CTA 0 of the pair
+__device__ __forceinline__ uint32_t in_first(uint32_t addr) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;\n" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
+}
+
+// One stage: its scale atoms, then `steps` MMAs of 64 K. Descriptors are made once per kernel and only
+// added to here, and a full stage's steps are unrolled: building each descriptor from its address made
+// the issuing thread the bound (203 ns a stage without scales, 122 so, at N = 8; the tensor pipe takes
+// 213 at N = 192).
+template <bool NV, bool PAIR, int SBLK>
+__device__ __forceinline__ void issue(uint32_t tbase, uint32_t acc, uint32_t sfb, uint64_t ad, uint64_t bd, uint64_t sd,
+                                      uint32_t id, int steps, bool first) {
+  constexpr int PER = NV ? 1 : 2;   // MMAs per scale atom
+  if (steps == 4) {
+#pragma unroll
+    for (int j = 0; j < 4 / PER; ++j) {
+      cp_sf<PAIR>(tbase + SFA_COL + 4 * j, sd + j * 32);
+#pragma unroll
+      for (int b = 0; b < SBLK; ++b) cp_sf<PAIR>(tbase + SFB_COL + 8 * j + 4 * b, sd + (SF_BLOCK<NV> >> 4) * (1 + b) + j * 32);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t h = NV ? 0u : (uint32_t)(j & 1) * 2u;
+      mma<NV, PAIR>(acc, ad + 2 * j, bd + 2 * j, id | (h << 4) | (h << 29), (tbase + SFA_COL + 4 * (j / PER)) | (h << 30),
+              (sfb + 8 * (j / PER)) | (h << 30), j > 0 || !first ? 1u : 0u);
+    }
+  } else {
+    for (int j = 0; j * PER < steps; ++j) {
+      cp_sf<PAIR>(tbase + SFA_COL + 4 * j, sd + j * 32);
+      for (int b = 0; b < SBLK; ++b) cp_sf<PAIR>(tbase + SFB_COL + 8 * j + 4 * b, sd + (SF_BLOCK<NV> >> 4) * (1 + b) + j * 32);
+    }
+    for (int j = 0; j < steps; ++j) {
+      const uint32_t h = NV ? 0u : (uint32_t)(j & 1) * 2u;
+      mma<NV, PAIR>(acc, ad + 2 * j, bd + 2 * j, id | (h << 4) | (h << 29), (tbase + SFA_COL + 4 * (j / PER)) | (h << 30),
+              (sfb + 8 * (j / PER)) | (h << 30), j > 0 || !first ? 1u : 0u);
+    }
+  }
 }
 
 // the first token row of matrix mat's group (mat == mats: the end), inside [0, m] whatever the offsets hold
@@ -115,24 +218,30 @@ __device__ __forceinline__ bool warp_wait(volatile int* abortf, uint32_t bar, ui
 
 // Tiles of one matrix run in bands of 12 weight blocks by all token tiles, so that the tiles in flight
 // share both operands in L2.
+template <bool PAIR>
 __device__ __forceinline__ Tile tile_at(const Args& a, const Ctl& c, int i) {
+  constexpr int MT = PAIR ? 256 : 128;
   int lo = 0, hi = a.g.mats;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (c.tiles[mid] <= i) lo = mid; else hi = mid;
   }
-  const int r = i - c.tiles[lo], nb = (a.g.n + 127) >> 7;
+  const int r = i - c.tiles[lo], nb = (a.g.n + MT - 1) / MT;
   const int tb = (c.tiles[lo + 1] - c.tiles[lo]) / nb;
   const int band = r / (12 * tb), left = r - band * 12 * tb, wide = min(12, nb - band * 12);
   Tile t;
   t.mat = lo;
-  t.n0 = (band * 12 + left % wide) * 128;
+  t.n0 = (band * 12 + left % wide) * MT;
   t.row0 = c.rows[lo];
   t.t0 = left / wide * a.nt;
   t.cnt = min(c.rows[lo + 1] - t.row0 - t.t0, a.nt);
-  t.blk = a.g.offsets ? (t.row0 >> 7) + lo : 0;
+  t.blk = (a.g.offsets ? (t.row0 >> 7) + lo : 0) + (t.t0 >> 7);
   return t;
 }
+
+// clamps that let NaN through
+__device__ __forceinline__ float clamp_hi(float v, float lim) { return v > lim ? lim : v; }
+__device__ __forceinline__ float clamp_lo(float v, float lim) { return v < lim ? lim : v; }
 
 template <typename T>
 __device__ __forceinline__ T to_out(float v);
@@ -143,46 +252,174 @@ __device__ __forceinline__ __half to_out<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 to_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <bool NV, bool SWIGLU, typename T>
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 r = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// v: one row's values of 8 columns, the lanes that differ in the bits M0, M1, M2 = M0 << 1, << 2 holding 8 rows.
+// Afterwards each of them holds 8 rows of one column (the one its three bits number), rounded.
+template <int M0, typename T>
+__device__ __forceinline__ uint4 transpose8(const float (&v)[8], int lane) {
+  const bool b0 = lane & M0, b1 = lane & (2 * M0), b2 = lane & (4 * M0);
+  uint32_t w[4], x[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const float o = __shfl_xor_sync(0xffffffffu, b0 ? v[2 * p] : v[2 * p + 1], M0);
+    w[p] = pack2<T>(b0 ? o : v[2 * p], b0 ? v[2 * p + 1] : o);
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const uint32_t o = __shfl_xor_sync(0xffffffffu, b1 ? w[2 * q] : w[2 * q + 1], 2 * M0);
+    x[2 * q] = b1 ? o : w[2 * q];
+    x[2 * q + 1] = b1 ? w[2 * q + 1] : o;
+  }
+  const uint32_t o0 = __shfl_xor_sync(0xffffffffu, b2 ? x[0] : x[2], 4 * M0);
+  const uint32_t o1 = __shfl_xor_sync(0xffffffffu, b2 ? x[1] : x[3], 4 * M0);
+  return b2 ? make_uint4(o0, o1, x[2], x[3]) : make_uint4(x[0], x[1], o0, o1);
+}
+
+// silu(gate) * up of one pair of rows: the even lane holds gate, the odd lane up, of two tokens; each lane
+// gets one of the tokens' results
+__device__ __forceinline__ float gated(float v0, float v1, int lane, float lim) {
+  const float o = __shfl_xor_sync(0xffffffffu, (lane & 1) ? v0 : v1, 1);
+  const float gate = clamp_hi((lane & 1) ? o : v0, lim), up = clamp_lo(clamp_hi((lane & 1) ? v1 : o, lim), -lim);
+  return __fdividef(gate, 1.f + __expf(-gate)) * up;
+}
+
+// 32 accumulator columns (tokens tok ..) of this thread's weight row to y; sc, wt: the tokens' scales and weights in
+// shared memory. 16-bit outputs are turned so that a lane stores 8 neighbouring ones at once: with a 2-byte
+// store per row and column the stores bound every tile of K <= 4096 (8.5 us a tile of 192 columns).
+template <bool SWIGLU, typename T>
+__device__ __forceinline__ void store_chunk(const Args& a, const uint32_t (&d)[32], int64_t tok, int row, int lane, int left,
+                                            bool vec, float wts, const float* sc, const float* wt) {
+  const Fp4MmArgs& g = a.g;
+  T* y = reinterpret_cast<T*>(g.y);
+  const int64_t ld = g.ldy;
+  const float lim = g.limit > 0.f ? g.limit : INFINITY;
+  if constexpr (sizeof(T) == 2) {
+    if (vec) {
+      if constexpr (SWIGLU) {
+        const int col = ((lane >> 1) & 7) * 2 + (lane & 1), base = ((row - lane) >> 1) + ((lane >> 4) << 3);
+        T* yp = y + (tok + col) * ld + base;
+#pragma unroll
+        for (int j = 0; j < 32; j += 16) {
+          if (j < left) {
+            float h[8];
+#pragma unroll
+            for (int m = 0; m < 8; ++m) {
+              const float2 s = *reinterpret_cast<const float2*>(sc + j + 2 * m);
+              h[m] = gated(__uint_as_float(d[j + 2 * m]) * (s.x * wts), __uint_as_float(d[j + 2 * m + 1]) * (s.y * wts),
+                           lane, lim) *
+                     wt[j + 2 * m + (lane & 1)];
+            }
+            const uint4 o = transpose8<2, T>(h, lane);
+            if (j + col < left && 2 * base < g.n) *reinterpret_cast<uint4*>(yp + (int64_t)j * ld) = o;
+          }
+        }
+      } else {
+        const int col = lane & 7, base = row - lane + (lane & ~7);
+        T* yp = y + (tok + col) * ld + base;
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          if (j < left) {
+            const float4 s0 = *reinterpret_cast<const float4*>(sc + j), s1 = *reinterpret_cast<const float4*>(sc + j + 4);
+            const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+            float v[8];
+#pragma unroll
+            for (int m = 0; m < 8; ++m) v[m] = __uint_as_float(d[j + m]) * (s[m] * wts);
+            const uint4 o = transpose8<1, T>(v, lane);
+            if (j + col < left && base < g.n) *reinterpret_cast<uint4*>(yp + (int64_t)j * ld) = o;
+          }
+        }
+      }
+      return;
+    }
+  }
+  const bool in = row < g.n;
+  if constexpr (SWIGLU) {
+    T* yp = y + (tok + (lane & 1)) * ld + (row >> 1);
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      if (j < left) {
+        const float2 s = *reinterpret_cast<const float2*>(sc + j);
+        const float h = gated(__uint_as_float(d[j]) * (s.x * wts), __uint_as_float(d[j + 1]) * (s.y * wts), lane, lim) *
+                        wt[j + (lane & 1)];
+        if (in && j + (lane & 1) < left) yp[(int64_t)j * ld] = to_out<T>(h);
+      }
+    }
+  } else {
+    T* yp = y + tok * ld + row;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      if (j < left) {
+        const float4 s = *reinterpret_cast<const float4*>(sc + j);
+        const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          if (in && j + m < left) yp[(int64_t)(j + m) * ld] = to_out<T>(__uint_as_float(d[j + m]) * (v[m] * wts));
+      }
+    }
+  }
+}
+
+template <bool NV, bool SWIGLU, bool PAIR, typename T>
 __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_constant__ Args a) {
   extern __shared__ uint8_t raw[];
+  // (both CTAs of a pair round the same address up, so that their stages lie at the same places)
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  const int s_bytes = SF_BLOCK<NV> * (1 + a.sblk);
   uint8_t* sA = base;
   uint8_t* sB = sA + a.stages * A_BYTES;
   uint8_t* sS = sB + a.stages * a.b_bytes;
-  const int s_bytes = SF_BLOCK + a.sfb_bytes;
   Ctl& c = *reinterpret_cast<Ctl*>(sS + a.stages * s_bytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
+  const int first = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, stride = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
   const Fp4MmArgs& g = a.g;
 
   if (tid == 0) {
     for (int s = 0; s < a.stages; ++s) {
-      mbar_init(smem_addr(&c.full[s]), 1);
+      mbar_init(smem_addr(&c.full[s]), 2);
       mbar_init(smem_addr(&c.empty[s]), 1);
     }
     for (int q = 0; q < 2; ++q) {
       mbar_init(smem_addr(&c.accfull[q]), 1);
-      mbar_init(smem_addr(&c.accempty[q]), 4);
+      mbar_init(smem_addr(&c.accempty[q]), PAIR ? 2 * EPI_WARPS : EPI_WARPS);
     }
     mbar_init(smem_addr(&c.drain), 1);
     c.abort = 0;
     mbar_init_fence();
   }
   if (warp == MMA_WARP) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(&c.tmem_base)),
-                 "n"(TMEM_COLS)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+    if constexpr (PAIR)
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(&c.tmem_base)),
+                   "n"(TMEM_COLS)
+                   : "memory");
+    else
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(&c.tmem_base)),
+                   "n"(TMEM_COLS)
+                   : "memory");
   }
-  if (warp == PRODUCER_WARP && lane == 0) {
+  if (warp == CODE_WARP && lane == 0) {
     prefetch_map(&a.map_w);
     prefetch_map(&a.map_a);
+    prefetch_map(&a.map_ws);
+    prefetch_map(&a.map_as);
   }
   pdl_wait();
   pdl_trigger();
   if (warp == 0) {
     // tiles before each matrix
-    const int nb = (g.n + 127) >> 7;
+    const int nb = (g.n + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
     int run = 0;
     for (int m0 = 0; m0 < g.mats; m0 += 32) {
       const int m = m0 + lane;
@@ -205,39 +442,44 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
   }
   fence_before();
   __syncthreads();
+  if constexpr (PAIR) pair_sync();
   fence_after();
   const uint32_t tbase = c.tmem_base;
   const int total = c.tiles[g.mats];
   const int kstages = (a.ksteps + 3) >> 2;
-  constexpr int STEPS_PER_ATOM = NV ? 1 : 2;
   volatile int* abortf = &c.abort;
 
-  if (warp == PRODUCER_WARP) {
-    uint32_t it = 0, s = 0, ph = 0;
+  if (warp == CODE_WARP || warp == SCALE_WARP) {
+    uint32_t it = 0, s = 0, ph = 1;
     bool ok = true;
-    for (int i = blockIdx.x; ok && i < total; i += gridDim.x) {
-      const Tile t = tile_at(a, c, i);
-      const int nbox = (t.cnt + a.box - 1) / a.box;
-      const int sblk = ((t.t0 & 127) + t.cnt + 127) >> 7;
-      const int wrow = t.mat * g.n + t.n0, arow = t.row0 + t.t0;
-      const uint8_t* ws = g.w_s + ((int64_t)t.mat * ((g.n + 127) >> 7) + (t.n0 >> 7)) * a.atoms * 512;
-      const uint8_t* as = g.a_s + (t.blk + (t.t0 >> 7)) * a.atoms * 512;
+    const uint32_t own0 = smem_addr(&c.full[0]), full0 = PAIR ? in_first(own0) : own0, empty0 = smem_addr(&c.empty[0]);
+    const uint32_t a0 = smem_addr(sA), b0 = smem_addr(sB), s0 = smem_addr(sS);
+    for (int i = first; ok && i < total; i += stride) {
+      const Tile t = tile_at<PAIR>(a, c, i);
+      // token rows that this CTA brings: all, or its half of the pair's columns
+      const int half = PAIR ? ((t.cnt + 15) >> 4) << 3 : t.cnt;
+      const int nbox = (half + a.box - 1) / a.box;
+      const int wrow = t.mat * g.n + t.n0 + rank * 128, arow = t.row0 + t.t0 + rank * half;
+      const int wblk = t.mat * ((g.n + 127) >> 7) + (t.n0 >> 7) + rank;
+      const uint32_t bytes = (PAIR ? 2u : 1u) * (warp == CODE_WARP ? A_BYTES + nbox * a.box * 128 : s_bytes);
       for (int k = 0; k < kstages; ++k, ++it) {
-        if (!warp_wait(abortf, smem_addr(&c.empty[s]), ph ^ 1u)) {
+        if (!warp_wait(abortf, empty0 + 8 * s, ph)) {
           ok = false;
           break;
         }
-        const int at0 = k * 4 / STEPS_PER_ATOM, nat = min(4 / STEPS_PER_ATOM, a.atoms - at0);
         if (elect_one()) {
-          const uint32_t full = smem_addr(&c.full[s]);
-          const uint32_t sf = smem_addr(sS + s * s_bytes);
-          mbar_expect_tx(full, A_BYTES + nbox * a.box * 128 + (1 + sblk) * nat * 512);
-          tma_load_2d(smem_addr(sA + s * A_BYTES), &a.map_w, k * 128, wrow, full);
-          for (int b = 0; b < nbox; ++b)
-            tma_load_2d(smem_addr(sB + s * a.b_bytes) + b * a.box * 128, &a.map_a, k * 128, arow + b * a.box, full);
-          bulk_g2s(sf, ws + (int64_t)at0 * 512, nat * 512, full);
-          for (int b = 0; b < sblk; ++b)
-            bulk_g2s(sf + SF_BLOCK * (1 + b), as + ((int64_t)b * a.atoms + at0) * 512, nat * 512, full);
+          const uint32_t full = full0 + 8 * s;
+          if (rank == 0) mbar_expect_tx(own0 + 8 * s, bytes);
+          if (warp == CODE_WARP) {
+            load_2d<PAIR>(a0 + s * A_BYTES, &a.map_w, k * 128, wrow, full);
+            const uint32_t dst = b0 + s * a.b_bytes;
+            for (int b = 0; b < nbox; ++b) load_2d<PAIR>(dst + b * a.box * 128, &a.map_a, k * 128, arow + b * a.box, full);
+          } else {
+            const uint32_t dst = s0 + s * s_bytes;
+            const int at = k * (NV ? 4 : 2);
+            load_3d<PAIR>(dst, &a.map_ws, 0, at, wblk, full);
+            load_3d<PAIR>(dst + SF_BLOCK<NV>, &a.map_as, 0, at, t.blk, full);
+          }
         }
         __syncwarp();
         if (++s == (uint32_t)a.stages) {
@@ -246,125 +488,128 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
         }
       }
     }
-    // the copies in flight land before the CTA's shared memory goes
-    if (!ok) {
+    // The copies in flight land before the CTA's shared memory goes (a stage that only one of the warps filled never
+    // completes: its wait ends by its limit).
+    if (!ok && rank == 0) {
       const uint32_t n = it < (uint32_t)a.stages ? it : (uint32_t)a.stages;
       for (uint32_t j = it - n; j < it; ++j)
-        for (uint32_t p = 0; p < WAIT_LIMIT; ++p)
-          if (mbar_try_wait_sleep(smem_addr(&c.full[j % a.stages]), (j / a.stages) & 1u, 1000u)) break;
+        for (uint32_t p = 0; p < WAIT_LIMIT / 16; ++p)
+          if (mbar_try_wait_sleep(own0 + 8 * (j % a.stages), (j / a.stages) & 1u, 1000u)) break;
     }
   } else if (warp == MMA_WARP) {
-    uint32_t s = 0, ph = 0, n = 0;
-    bool ok = true;
-    for (int i = blockIdx.x; ok && i < total; i += gridDim.x, ++n) {
-      const Tile t = tile_at(a, c, i);
-      const int sblk = ((t.t0 & 127) + t.cnt + 127) >> 7;
-      const uint32_t cols = (uint32_t)(t.cnt + 7) & ~7u;
-      const uint32_t q = n & 1u, acc = tbase + q * NT_MAX;
-      const uint32_t sfb = tbase + SFB_COL + ((t.t0 & 127) >> 5);
-      if (!warp_wait(abortf, smem_addr(&c.accempty[q]), ((n >> 1) & 1u) ^ 1u)) break;
-      fence_after();
-      for (int k = 0; k < kstages; ++k) {
-        if (!warp_wait(abortf, smem_addr(&c.full[s]), ph)) {
-          ok = false;
-          break;
-        }
+    if (rank == 0) {
+      uint32_t s = 0, ph = 0, n = 0;
+      bool ok = true;
+      const uint64_t ad0 = sdesc(smem_addr(sA)), bd0 = sdesc(smem_addr(sB)), sd0 = sf_desc(smem_addr(sS));
+      const uint32_t full0 = smem_addr(&c.full[0]), empty0 = smem_addr(&c.empty[0]);
+      for (int i = first; ok && i < total; i += stride, ++n) {
+        const Tile t = tile_at<PAIR>(a, c, i);
+        const bool two = ((t.t0 & 127) + t.cnt) > 128;
+        const uint32_t q = n & 1u, acc = tbase + q * NT_MAX;
+        const uint32_t sfb = tbase + SFB_COL + ((t.t0 & 127) >> 5);
+        const uint32_t id = idesc<NV, PAIR>(PAIR ? (uint32_t)(t.cnt + 15) & ~15u : (uint32_t)(t.cnt + 7) & ~7u);
+        if (!warp_wait(abortf, smem_addr(&c.accempty[q]), ((n >> 1) & 1u) ^ 1u)) break;
         fence_after();
-        if (elect_one()) {
-          const uint32_t sa = smem_addr(sA + s * A_BYTES), sb = smem_addr(sB + s * a.b_bytes);
-          const uint32_t sf = smem_addr(sS + s * s_bytes);
-          const int steps = min(4, a.ksteps - 4 * k), nat = (steps + STEPS_PER_ATOM - 1) / STEPS_PER_ATOM;
-          for (int j = 0; j < nat; ++j) {
-            cp_sf(tbase + SFA_COL + 4 * j, sf + j * 512);
-            for (int b = 0; b < sblk; ++b) cp_sf(tbase + SFB_COL + 8 * j + 4 * b, sf + SF_BLOCK * (1 + b) + j * 512);
+        for (int k = 0; k < kstages; ++k) {
+          if (!warp_wait(abortf, full0 + 8 * s, ph)) {
+            ok = false;
+            break;
           }
-          for (int j = 0; j < steps; ++j) {
-            const uint32_t id = NV ? 0u : (uint32_t)(j & 1) * 2u, at = (uint32_t)(j / STEPS_PER_ATOM);
-            mma<NV>(acc, sdesc(sa + j * 32), sdesc(sb + j * 32), idesc<NV>(cols, id),
-                    (tbase + SFA_COL + 4 * at) | (id << 30), (sfb + 8 * at) | (id << 30), (k | j) != 0 ? 1u : 0u);
+          fence_after();
+          if (elect_one()) {
+            const uint64_t ad = ad0 + s * (A_BYTES >> 4), bd = bd0 + s * (uint32_t)(a.b_bytes >> 4);
+            const uint64_t sd = sd0 + s * (uint32_t)(s_bytes >> 4);
+            const int steps = min(4, a.ksteps - 4 * k);
+            if (two) issue<NV, PAIR, 2>(tbase, acc, sfb, ad, bd, sd, id, steps, k == 0);
+            else issue<NV, PAIR, 1>(tbase, acc, sfb, ad, bd, sd, id, steps, k == 0);
+            commit_to<PAIR>(empty0 + 8 * s);
           }
-          commit(smem_addr(&c.empty[s]));
+          __syncwarp();
+          if (++s == (uint32_t)a.stages) {
+            s = 0;
+            ph ^= 1u;
+          }
         }
+        if (!ok) break;
+        if (elect_one()) commit_to<PAIR>(smem_addr(&c.accfull[q]));
         __syncwarp();
-        if (++s == (uint32_t)a.stages) {
-          s = 0;
-          ph ^= 1u;
-        }
       }
-      if (!ok) break;
-      if (elect_one()) commit(smem_addr(&c.accfull[q]));
+      // every MMA issued has completed once `drain` fires
+      if (elect_one()) commit_to<PAIR>(smem_addr(&c.drain));
       __syncwarp();
+      for (uint32_t p = 0; p < WAIT_LIMIT; ++p)
+        if (mbar_try_wait_sleep(smem_addr(&c.drain), 0, 1000u)) break;
     }
-    // every MMA issued has completed once `drain` fires
-    if (elect_one()) commit(smem_addr(&c.drain));
-    __syncwarp();
-    for (uint32_t p = 0; p < WAIT_LIMIT; ++p)
-      if (mbar_try_wait_sleep(smem_addr(&c.drain), 0, 1000u)) break;
   } else {
     uint32_t n = 0;
-    T* y = reinterpret_cast<T*>(g.y);
-    for (int i = blockIdx.x; i < total; i += gridDim.x, ++n) {
-      const Tile t = tile_at(a, c, i);
+    const int half = warp >> 2;   // this warp's 32-column chunks: half, half + 2, ...
+    const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
+    float* sc = c.scale[warp];
+    float* wt = c.weight[warp];
+    for (int i = first; i < total; i += stride, ++n) {
+      const Tile t = tile_at<PAIR>(a, c, i);
       const uint32_t q = n & 1u;
-      const uint32_t acc = tbase + q * NT_MAX + ((uint32_t)(warp * 32) << 16);
-      const int row = t.n0 + tid;
-      const bool in = row < g.n;
+      const uint32_t acc = tbase + q * NT_MAX + quarter;
+      const int row = t.n0 + rank * 128 + (warp & 3) * 32 + lane;
+      const bool vec = a.vec && (t.n0 + rank * 128 + 128 <= g.n || (SWIGLU ? g.n % 16 : g.n % 8) == 0);
       float wts = 1.f;
-      if (g.w_ts != nullptr) wts = g.w_ts_n == 0 ? (in ? g.w_ts[row] : 0.f) : g.w_ts[t.mat * g.w_ts_n + (g.w_ts_n == 2 ? (row & 1) : 0)];
+      if (g.w_ts != nullptr && row < g.n)
+        wts = g.w_ts[g.w_ts_n == 0 ? row : t.mat * g.w_ts_n + (g.w_ts_n == 2 ? (row & 1) : 0)];
+      // the tokens' scales and weights, in shared memory before the products are done
+      const int64_t tok0 = (int64_t)t.row0 + t.t0;
+#pragma unroll
+      for (int j = 0; j < NT_MAX / 64; ++j) {
+        const int col = 32 * (half + 2 * j) + lane;
+        float s = 1.f, w = 1.f;
+        if (col < t.cnt) {
+          if (g.a_ts != nullptr) s = g.a_ts[g.a_ts_row ? tok0 + col : 0];
+          if (g.row_weight != nullptr) w = g.row_weight[tok0 + col];
+        }
+        sc[32 * j + lane] = SWIGLU ? s : s * w;
+        if (SWIGLU) wt[32 * j + lane] = w;
+      }
+      __syncwarp();
       if (!warp_wait(abortf, smem_addr(&c.accfull[q]), (n >> 1) & 1u)) break;
       fence_after();
-      for (int c0 = 0; c0 < t.cnt; c0 += 32) {
+      bool held = true;   // this warp has yet to read the accumulator's last chunk
+      for (int ch = half, j = 0; ch * 32 < t.cnt; ch += 2, ++j) {
         uint32_t d[32];
-        ld32(acc + c0, d);
-        const int64_t tok = (int64_t)t.row0 + t.t0 + c0;
-        const int left = min(32, t.cnt - c0);
-        float ats = 1.f, rw = 1.f;
-        if (lane < left) {
-          if (g.a_ts != nullptr) ats = g.a_ts[g.a_ts_row ? tok + lane : 0];
-          if (g.row_weight != nullptr) rw = g.row_weight[tok + lane];
-        }
+        ld32(acc + ch * 32, d);
         ld_wait();
-        if (SWIGLU) {
-          T* yp = y + (tok + (lane & 1)) * g.ldy + (row >> 1);
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            if (j < left) {
-              const float s0 = __shfl_sync(0xffffffffu, ats, j), s1 = __shfl_sync(0xffffffffu, ats, j + 1);
-              const float w = __shfl_sync(0xffffffffu, rw, j + (lane & 1));
-              const float v0 = __uint_as_float(d[j]) * (s0 * wts), v1 = __uint_as_float(d[j + 1]) * (s1 * wts);
-              // the even lane holds gate, the odd lane up: each takes one of the two tokens
-              const float o = __shfl_xor_sync(0xffffffffu, (lane & 1) ? v0 : v1, 1);
-              float gate = (lane & 1) ? o : v0, up = (lane & 1) ? v1 : o;
-              if (g.limit > 0.f) {
-                gate = fminf(gate, g.limit);
-                up = fminf(fmaxf(up, -g.limit), g.limit);
-              }
-              const float h = __fdividef(gate, 1.f + __expf(-gate)) * up * w;
-              if (in && j + (lane & 1) < left) yp[(int64_t)j * g.ldy] = to_out<T>(h);
-            }
+        if ((ch + 2) * 32 >= t.cnt) {
+          held = false;
+          fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (PAIR) arrive_remote(in_first(smem_addr(&c.accempty[q])));
+            else arrive(smem_addr(&c.accempty[q]));
           }
-        } else {
-          T* yp = y + tok * g.ldy + row;
-          ats *= rw;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (j < left) {
-              const float s = __shfl_sync(0xffffffffu, ats, j);
-              if (in) yp[(int64_t)j * g.ldy] = to_out<T>(__uint_as_float(d[j]) * (s * wts));
-            }
-          }
+        }
+        store_chunk<SWIGLU, T>(a, d, tok0 + ch * 32, row, lane, min(32, t.cnt - ch * 32), vec, wts, sc + 32 * j, wt + 32 * j);
+      }
+      if (held) {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR) arrive_remote(in_first(smem_addr(&c.accempty[q])));
+          else arrive(smem_addr(&c.accempty[q]));
         }
       }
-      fence_before();
       __syncwarp();
-      if (lane == 0) arrive(smem_addr(&c.accempty[q]));
     }
   }
   fence_before();
   __syncthreads();
+  if constexpr (PAIR) pair_sync();   // the other CTA's products read this one's shared memory to the end
   if (warp == MMA_WARP) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tbase), "n"(TMEM_COLS));
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n");
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tbase), "n"(TMEM_COLS));
+    } else {
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tbase), "n"(TMEM_COLS));
+    }
   }
 }
 
@@ -386,7 +631,6 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 static cudaError_t code_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = encode_fn();
   if (enc == nullptr) return cudaErrorNotSupported;
-  memset(map, 0, sizeof *map);
   const cuuint64_t dims[2] = {row_bytes, rows};
   const cuuint64_t strides[1] = {row_bytes};
   const cuuint32_t boxes[2] = {128, box};
@@ -397,8 +641,24 @@ static cudaError_t code_map(CUtensorMap* map, const void* base, uint64_t rows, u
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-template <bool NV, bool SWIGLU, typename T>
+// scale atoms [blocks][atoms][512 bytes] in boxes of `row_blocks` blocks x `along` atoms
+static cudaError_t scale_map(CUtensorMap* map, const void* base, uint64_t blocks, uint64_t atoms, uint32_t row_blocks,
+                             uint32_t along) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = encode_fn();
+  if (enc == nullptr) return cudaErrorNotSupported;
+  const cuuint64_t dims[3] = {128, atoms, blocks};
+  const cuuint64_t strides[2] = {512, atoms * 512};
+  const cuuint32_t boxes[3] = {128, along, row_blocks};
+  const cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, boxes, es,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <bool NV, bool SWIGLU, bool PAIR, typename T>
 static cudaError_t launch_mm(const fp4mm::Args& a, int grid, size_t smem, cudaStream_t st) {
+  const auto kernel = fp4mm::fp4_mm_kernel<NV, SWIGLU, PAIR, T>;
   // the limit belongs to the kernel on one device: set once for each
   static std::atomic<uint64_t> done{0};
   int dev = 0;
@@ -406,58 +666,85 @@ static cudaError_t launch_mm(const fp4mm::Args& a, int grid, size_t smem, cudaSt
   if (e != cudaSuccess) return e;
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (!(done.load(std::memory_order_relaxed) & bit)) {
-    e = cudaFuncSetAttribute(fp4mm::fp4_mm_kernel<NV, SWIGLU, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             fp4mm::SMEM_LIMIT);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fp4mm::SMEM_LIMIT);
     if (e != cudaSuccess) return e;
     done.fetch_or(bit, std::memory_order_relaxed);
   }
-  return launch_pdl(fp4mm::fp4_mm_kernel<NV, SWIGLU, T>, dim3(grid), dim3(fp4mm::NTHREADS), smem, st, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(fp4mm::NTHREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-template <typename T>
+template <bool PAIR, typename T>
 static cudaError_t launch_mm_t(const fp4mm::Args& a, int grid, size_t smem, cudaStream_t st) {
-  if (a.g.nv) return a.g.swiglu ? launch_mm<true, true, T>(a, grid, smem, st) : launch_mm<true, false, T>(a, grid, smem, st);
-  return a.g.swiglu ? launch_mm<false, true, T>(a, grid, smem, st) : launch_mm<false, false, T>(a, grid, smem, st);
+  if (a.g.nv) return a.g.swiglu ? launch_mm<true, true, PAIR, T>(a, grid, smem, st) : launch_mm<true, false, PAIR, T>(a, grid, smem, st);
+  return a.g.swiglu ? launch_mm<false, true, PAIR, T>(a, grid, smem, st) : launch_mm<false, false, PAIR, T>(a, grid, smem, st);
+}
+
+template <bool PAIR>
+static cudaError_t launch_mm_p(const fp4mm::Args& a, int dtype, int grid, size_t smem, cudaStream_t st) {
+  if (dtype == SB_F32) return launch_mm_t<PAIR, float>(a, grid, smem, st);
+  if (dtype == SB_F16) return launch_mm_t<PAIR, __half>(a, grid, smem, st);
+  return launch_mm_t<PAIR, __nv_bfloat16>(a, grid, smem, st);
 }
 
 cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
   using namespace fp4mm;
   Args a;
+  memset(&a, 0, sizeof a);
   a.g = g;
   a.ksteps = (g.kp + 63) / 64;
-  a.atoms = g.nv ? a.ksteps : (a.ksteps + 1) / 2;
+  const int atoms = g.nv ? a.ksteps : (a.ksteps + 1) / 2, sms = num_sms();
   // Token columns of a tile: all of them when they fit one, else 128 or 192 (whole 64-row steps of the
   // scale atoms), whichever leaves fewer columns unused. With groups the counts are on the device: the
   // average decides.
   if (g.offsets != nullptr) {
     const int avg = (g.m + g.mats - 1) / g.mats;
-    a.nt = avg > 256 ? 192 : 128;
-    a.box = BOX;
+    a.nt = avg > 128 ? 192 : 128;
   } else if (g.m <= NT_MAX) {
-    a.nt = (g.m + 7) & ~7;
-    a.box = a.nt;
+    a.nt = (g.m + 15) & ~15;
   } else {
     const int c128 = (g.m + 127) / 128 * 128, c192 = (g.m + 191) / 192 * 192;
     a.nt = c128 < c192 - c192 / 8 ? 128 : 192;
-    a.box = a.nt;
   }
-  a.b_bytes = a.nt * 128;
-  a.sfb_bytes = (a.nt > 64 ? 2 : 1) * SF_BLOCK;
-  const int stage = A_BYTES + a.b_bytes + SF_BLOCK + a.sfb_bytes;
+  // tiles of 128 rows, or with groups the most there can be
+  const int64_t nb = (g.n + 127) / 128;
+  const int64_t tt = g.offsets ? (int64_t)g.m / a.nt + (g.mats < g.m ? g.mats : g.m) : (g.m + a.nt - 1) / a.nt;
+  const int64_t tiles = tt * nb;
+  // Pairs where tiles of full width are many: they halve the token bytes per product, which is what bounds
+  // those; narrow tiles are bound by the weights, which pairs do not share.
+  const bool pair = a.nt >= 128 && g.m >= 128 * (int64_t)g.mats && tiles >= 2 * sms;
+  a.box = g.offsets ? BOX : (pair ? a.nt / 2 : a.nt);
+  a.b_bytes = (pair ? a.nt / 2 : a.nt) * 128;
+  a.sblk = a.nt > 128 ? 2 : 1;
+  a.vec = (reinterpret_cast<uintptr_t>(g.y) & 15u) == 0 && g.ldy % 8 == 0;
+  const int sf = g.nv ? SF_BLOCK<true> : SF_BLOCK<false>;
+  const int stage = A_BYTES + a.b_bytes + sf * (1 + a.sblk);
   const int room = SMEM_LIMIT - 1024 - (int)sizeof(Ctl);
   a.stages = room / stage < MAX_STAGES ? room / stage : MAX_STAGES;
   const size_t smem = 1024 + (size_t)a.stages * stage + sizeof(Ctl);
   const uint64_t row_bytes = (uint64_t)g.kp / 2;
+  const uint64_t a_blocks = g.offsets ? (uint64_t)g.m / 128 + g.mats : ((uint64_t)g.m + 127) / 128;
+  const uint32_t along = g.nv ? 4 : 2;
   cudaError_t e = code_map(&a.map_w, g.w, (uint64_t)g.mats * g.n, row_bytes, 128);
   if (e == cudaSuccess) e = code_map(&a.map_a, g.a, (uint64_t)g.m, row_bytes, (uint32_t)a.box);
+  if (e == cudaSuccess) e = scale_map(&a.map_ws, g.w_s, (uint64_t)g.mats * nb, (uint64_t)atoms, 1, along);
+  if (e == cudaSuccess) e = scale_map(&a.map_as, g.a_s, a_blocks, (uint64_t)atoms, (uint32_t)a.sblk, along);
   if (e != cudaSuccess) return e;
-  const int64_t nb = (g.n + 127) / 128;
-  // tiles, or with groups the most there can be
-  const int64_t tiles = g.offsets ? ((int64_t)g.m / a.nt + (g.mats < g.m ? g.mats : g.m)) * nb : (g.m + a.nt - 1) / a.nt * nb;
-  const int grid = (int)(tiles < num_sms() ? tiles : num_sms());
-  if (dtype == SB_F32) return launch_mm_t<float>(a, grid, smem, st);
-  if (dtype == SB_F16) return launch_mm_t<__half>(a, grid, smem, st);
-  return launch_mm_t<__nv_bfloat16>(a, grid, smem, st);
+  if (pair) return launch_mm_p<true>(a, dtype, sms & ~1, smem, st);
+  return launch_mm_p<false>(a, dtype, (int)(tiles < sms ? tiles : sms), smem, st);
 }
 
 cudaError_t fp4_mm_error(int* host_out, cudaStream_t st) {
