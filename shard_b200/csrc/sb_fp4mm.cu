@@ -21,6 +21,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "sb_fp4.h"
 #include "sb_launch.h"
@@ -172,36 +173,27 @@ __device__ __forceinline__ void pair_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
 }
 
-// One stage: its scale atoms, then `steps` MMAs of 64 K. Descriptors are made once per kernel and only
-// added to here, and a full stage's steps are unrolled: building each descriptor from its address made
-// the issuing thread the bound (203 ns a stage without scales, 122 so, at N = 8; the tensor pipe takes
-// 213 at N = 192).
-template <bool NV, bool PAIR, int SBLK>
+// One stage: its scale atoms, then `steps` MMAs of 64 K (FULL: four). Descriptors are made once per kernel
+// and only added to, and a full stage is unrolled: building each descriptor from its address made the issuing
+// thread the bound (203 ns a stage without scales, 122 so, at N = 8; the tensor pipe takes 213 at N = 192).
+template <bool NV, bool PAIR, int SBLK, bool FULL>
 __device__ __forceinline__ void issue(uint32_t tbase, uint32_t acc, uint32_t sfb, uint64_t ad, uint64_t bd, uint64_t sd,
                                       uint32_t id, int steps, bool first) {
   constexpr int PER = NV ? 1 : 2;   // MMAs per scale atom
-  if (steps == 4) {
 #pragma unroll
-    for (int j = 0; j < 4 / PER; ++j) {
+  for (int j = 0; j < 4 / PER; ++j) {
+    if (FULL || j * PER < steps) {
       cp_sf<PAIR>(tbase + SFA_COL + 4 * j, sd + j * 32);
 #pragma unroll
       for (int b = 0; b < SBLK; ++b) cp_sf<PAIR>(tbase + SFB_COL + 8 * j + 4 * b, sd + (SF_BLOCK<NV> >> 4) * (1 + b) + j * 32);
     }
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 4; ++j) {
+    if (FULL || j < steps) {
       const uint32_t h = NV ? 0u : (uint32_t)(j & 1) * 2u;
       mma<NV, PAIR>(acc, ad + 2 * j, bd + 2 * j, id | (h << 4) | (h << 29), (tbase + SFA_COL + 4 * (j / PER)) | (h << 30),
-              (sfb + 8 * (j / PER)) | (h << 30), j > 0 || !first ? 1u : 0u);
-    }
-  } else {
-    for (int j = 0; j * PER < steps; ++j) {
-      cp_sf<PAIR>(tbase + SFA_COL + 4 * j, sd + j * 32);
-      for (int b = 0; b < SBLK; ++b) cp_sf<PAIR>(tbase + SFB_COL + 8 * j + 4 * b, sd + (SF_BLOCK<NV> >> 4) * (1 + b) + j * 32);
-    }
-    for (int j = 0; j < steps; ++j) {
-      const uint32_t h = NV ? 0u : (uint32_t)(j & 1) * 2u;
-      mma<NV, PAIR>(acc, ad + 2 * j, bd + 2 * j, id | (h << 4) | (h << 29), (tbase + SFA_COL + 4 * (j / PER)) | (h << 30),
-              (sfb + 8 * (j / PER)) | (h << 30), j > 0 || !first ? 1u : 0u);
+                    (sfb + 8 * (j / PER)) | (h << 30), j > 0 || !first ? 1u : 0u);
     }
   }
 }
@@ -211,6 +203,11 @@ __device__ __forceinline__ int group_begin(const Fp4MmArgs& g, int mat) {
   return g.offsets ? min(max(g.offsets[mat], 0), g.m) : (mat == 0 ? 0 : g.m);
 }
 
+// The copying and issuing warps each run on one elected thread, whose waits need no vote of the warp (a vote and
+// a re-election per stage cost the issuing warp 100 ns of 330).
+__device__ __forceinline__ bool wait(volatile int* abortf, uint32_t bar, uint32_t parity) {
+  return mbar_try_wait(bar, parity) || wait_bounded(abortf, &g_err, bar, parity, WAIT_LIMIT);
+}
 // one answer for the whole warp, whose next instructions need all of its lanes
 __device__ __forceinline__ bool warp_wait(volatile int* abortf, uint32_t bar, uint32_t parity) {
   return __all_sync(0xffffffffu, wait_bounded(abortf, &g_err, bar, parity, WAIT_LIMIT));
@@ -450,27 +447,28 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
   volatile int* abortf = &c.abort;
 
   if (warp == CODE_WARP || warp == SCALE_WARP) {
-    uint32_t it = 0, s = 0, ph = 1;
-    bool ok = true;
-    const uint32_t own0 = smem_addr(&c.full[0]), full0 = PAIR ? in_first(own0) : own0, empty0 = smem_addr(&c.empty[0]);
-    const uint32_t a0 = smem_addr(sA), b0 = smem_addr(sB), s0 = smem_addr(sS);
-    for (int i = first; ok && i < total; i += stride) {
-      const Tile t = tile_at<PAIR>(a, c, i);
-      // token rows that this CTA brings: all, or its half of the pair's columns
-      const int half = PAIR ? ((t.cnt + 15) >> 4) << 3 : t.cnt;
-      const int nbox = (half + a.box - 1) / a.box;
-      const int wrow = t.mat * g.n + t.n0 + rank * 128, arow = t.row0 + t.t0 + rank * half;
-      const int wblk = t.mat * ((g.n + 127) >> 7) + (t.n0 >> 7) + rank;
-      const uint32_t bytes = (PAIR ? 2u : 1u) * (warp == CODE_WARP ? A_BYTES + nbox * a.box * 128 : s_bytes);
-      for (int k = 0; k < kstages; ++k, ++it) {
-        if (!warp_wait(abortf, empty0 + 8 * s, ph)) {
-          ok = false;
-          break;
-        }
-        if (elect_one()) {
+    if (elect_one()) {
+      uint32_t it = 0, s = 0, ph = 1;
+      bool ok = true;
+      const bool codes = warp == CODE_WARP;
+      const uint32_t own0 = smem_addr(&c.full[0]), full0 = PAIR ? in_first(own0) : own0, empty0 = smem_addr(&c.empty[0]);
+      const uint32_t a0 = smem_addr(sA), b0 = smem_addr(sB), s0 = smem_addr(sS);
+      for (int i = first; ok && i < total; i += stride) {
+        const Tile t = tile_at<PAIR>(a, c, i);
+        // token rows that this CTA brings: all, or its half of the pair's columns
+        const int half = PAIR ? ((t.cnt + 15) >> 4) << 3 : t.cnt;
+        const int nbox = (half + a.box - 1) / a.box;
+        const int wrow = t.mat * g.n + t.n0 + rank * 128, arow = t.row0 + t.t0 + rank * half;
+        const int wblk = t.mat * ((g.n + 127) >> 7) + (t.n0 >> 7) + rank;
+        const uint32_t bytes = (PAIR ? 2u : 1u) * (codes ? A_BYTES + nbox * a.box * 128 : s_bytes);
+        for (int k = 0; k < kstages; ++k, ++it) {
+          if (!wait(abortf, empty0 + 8 * s, ph)) {
+            ok = false;
+            break;
+          }
           const uint32_t full = full0 + 8 * s;
           if (rank == 0) mbar_expect_tx(own0 + 8 * s, bytes);
-          if (warp == CODE_WARP) {
+          if (codes) {
             load_2d<PAIR>(a0 + s * A_BYTES, &a.map_w, k * 128, wrow, full);
             const uint32_t dst = b0 + s * a.b_bytes;
             for (int b = 0; b < nbox; ++b) load_2d<PAIR>(dst + b * a.box * 128, &a.map_a, k * 128, arow + b * a.box, full);
@@ -480,66 +478,65 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
             load_3d<PAIR>(dst, &a.map_ws, 0, at, wblk, full);
             load_3d<PAIR>(dst + SF_BLOCK<NV>, &a.map_as, 0, at, t.blk, full);
           }
-        }
-        __syncwarp();
-        if (++s == (uint32_t)a.stages) {
-          s = 0;
-          ph ^= 1u;
-        }
-      }
-    }
-    // The copies in flight land before the CTA's shared memory goes (a stage that only one of the warps filled never
-    // completes: its wait ends by its limit).
-    if (!ok && rank == 0) {
-      const uint32_t n = it < (uint32_t)a.stages ? it : (uint32_t)a.stages;
-      for (uint32_t j = it - n; j < it; ++j)
-        for (uint32_t p = 0; p < WAIT_LIMIT / 16; ++p)
-          if (mbar_try_wait_sleep(own0 + 8 * (j % a.stages), (j / a.stages) & 1u, 1000u)) break;
-    }
-  } else if (warp == MMA_WARP) {
-    if (rank == 0) {
-      uint32_t s = 0, ph = 0, n = 0;
-      bool ok = true;
-      const uint64_t ad0 = sdesc(smem_addr(sA)), bd0 = sdesc(smem_addr(sB)), sd0 = sf_desc(smem_addr(sS));
-      const uint32_t full0 = smem_addr(&c.full[0]), empty0 = smem_addr(&c.empty[0]);
-      for (int i = first; ok && i < total; i += stride, ++n) {
-        const Tile t = tile_at<PAIR>(a, c, i);
-        const bool two = ((t.t0 & 127) + t.cnt) > 128;
-        const uint32_t q = n & 1u, acc = tbase + q * NT_MAX;
-        const uint32_t sfb = tbase + SFB_COL + ((t.t0 & 127) >> 5);
-        const uint32_t id = idesc<NV, PAIR>(PAIR ? (uint32_t)(t.cnt + 15) & ~15u : (uint32_t)(t.cnt + 7) & ~7u);
-        if (!warp_wait(abortf, smem_addr(&c.accempty[q]), ((n >> 1) & 1u) ^ 1u)) break;
-        fence_after();
-        for (int k = 0; k < kstages; ++k) {
-          if (!warp_wait(abortf, full0 + 8 * s, ph)) {
-            ok = false;
-            break;
-          }
-          fence_after();
-          if (elect_one()) {
-            const uint64_t ad = ad0 + s * (A_BYTES >> 4), bd = bd0 + s * (uint32_t)(a.b_bytes >> 4);
-            const uint64_t sd = sd0 + s * (uint32_t)(s_bytes >> 4);
-            const int steps = min(4, a.ksteps - 4 * k);
-            if (two) issue<NV, PAIR, 2>(tbase, acc, sfb, ad, bd, sd, id, steps, k == 0);
-            else issue<NV, PAIR, 1>(tbase, acc, sfb, ad, bd, sd, id, steps, k == 0);
-            commit_to<PAIR>(empty0 + 8 * s);
-          }
-          __syncwarp();
           if (++s == (uint32_t)a.stages) {
             s = 0;
             ph ^= 1u;
           }
         }
-        if (!ok) break;
-        if (elect_one()) commit_to<PAIR>(smem_addr(&c.accfull[q]));
-        __syncwarp();
+      }
+      // The copies in flight land before the CTA's shared memory goes (a stage that only one of the warps filled
+      // never completes: its wait ends by its limit).
+      if (!ok && rank == 0) {
+        const uint32_t n = it < (uint32_t)a.stages ? it : (uint32_t)a.stages;
+        for (uint32_t j = it - n; j < it; ++j)
+          for (uint32_t p = 0; p < WAIT_LIMIT / 16; ++p)
+            if (mbar_try_wait_sleep(own0 + 8 * (j % a.stages), (j / a.stages) & 1u, 1000u)) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp == MMA_WARP) {
+    if (rank == 0 && elect_one()) {
+      uint32_t s = 0, ph = 0, n = 0;
+      bool ok = true;
+      const uint64_t ad0 = sdesc(smem_addr(sA)), bd0 = sdesc(smem_addr(sB)), sd0 = sf_desc(smem_addr(sS));
+      const uint32_t b_step = (uint32_t)(a.b_bytes >> 4), s_step = (uint32_t)(s_bytes >> 4);
+      const uint32_t full0 = smem_addr(&c.full[0]), empty0 = smem_addr(&c.empty[0]);
+      const int kfull = a.ksteps >> 2, ktail = a.ksteps & 3;
+      for (int i = first; ok && i < total; i += stride, ++n) {
+        const Tile t = tile_at<PAIR>(a, c, i);
+        const uint32_t q = n & 1u, acc = tbase + q * NT_MAX;
+        const uint32_t sfb = tbase + SFB_COL + ((t.t0 & 127) >> 5);
+        const uint32_t id = idesc<NV, PAIR>(PAIR ? (uint32_t)(t.cnt + 15) & ~15u : (uint32_t)(t.cnt + 7) & ~7u);
+        if (!wait(abortf, smem_addr(&c.accempty[q]), ((n >> 1) & 1u) ^ 1u)) break;
+        fence_after();
+        auto stage = [&](auto blocks, auto whole, int k) {
+          if (!wait(abortf, full0 + 8 * s, ph)) {
+            ok = false;
+            return;
+          }
+          fence_after();
+          issue<NV, PAIR, decltype(blocks)::value, decltype(whole)::value>(tbase, acc, sfb, ad0 + s * (A_BYTES >> 4),
+                                                                           bd0 + s * b_step, sd0 + s * s_step, id, ktail, k == 0);
+          commit_to<PAIR>(empty0 + 8 * s);
+          if (++s == (uint32_t)a.stages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        };
+        auto tile = [&](auto blocks) {
+          for (int k = 0; ok && k < kfull; ++k) stage(blocks, std::true_type{}, k);
+          if (ok && ktail > 0) stage(blocks, std::false_type{}, kfull);
+        };
+        if ((t.t0 & 127) + t.cnt > 128) tile(std::integral_constant<int, 2>{});
+        else tile(std::integral_constant<int, 1>{});
+        if (ok) commit_to<PAIR>(smem_addr(&c.accfull[q]));
       }
       // every MMA issued has completed once `drain` fires
-      if (elect_one()) commit_to<PAIR>(smem_addr(&c.drain));
-      __syncwarp();
+      commit_to<PAIR>(smem_addr(&c.drain));
       for (uint32_t p = 0; p < WAIT_LIMIT; ++p)
         if (mbar_try_wait_sleep(smem_addr(&c.drain), 0, 1000u)) break;
     }
+    __syncwarp();
   } else {
     uint32_t n = 0;
     const int half = warp >> 2;   // this warp's 32-column chunks: half, half + 2, ...
