@@ -72,6 +72,7 @@ struct TopkArgs {
   int64_t* ids;
   int vec;                   // set by the launch: rows can be read 16 bytes at a time
   float lowest;              // set by the launch: the lowest finite value of 16-bit logits
+  int size, span;            // set by the launch: experts and lanes of a group (span 0: groups share lanes)
 };
 
 struct OrderArgs {

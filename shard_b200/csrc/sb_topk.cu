@@ -3,10 +3,10 @@
 //
 // topk_kernel: one warp per token, lane l holds experts C l .. C l + C - 1. Selection values are exact
 // without a bias (the scores ascend with the logits, so the logits themselves are compared). With a
-// bias, or for groups scored by a sum, they are fp32 sums of rounded scores: after the selection the
-// gaps that decided it are compared with the error bound of those sums, and a token with a smaller
-// gap is selected again in 64 bits (a fraction of a percent of them). So a selection never hangs on
-// how an exponential rounds.
+// bias, or for groups scored by a sum, they are fp32 sums of rounded scores: the gaps that decide are
+// compared with the error bound of those sums, and where one is smaller the candidates in doubt are
+// compared again in 64 bits (a fraction of a percent of the tokens; selecting those tokens anew from 64-bit
+// scores of all experts took 20 us of 38). So a selection never hangs on how an exponential rounds.
 //
 // order_kernel: a stable counting sort of the pairs by expert, in blocks of 2048 pairs, no atomics
 // on anything the outputs depend on.
@@ -54,7 +54,7 @@ __device__ __forceinline__ float score_weight(int func, float l, float mx, float
   if (func == SCORE_SIGMOID) return __fdiv_rn(1.f, 1.f + expf(-l));
   return sqrtf(fmaxf(l, 0.f) + log1pf(expf(-fabsf(l))));
 }
-__device__ __forceinline__ double score64(int func, float l, double mx, double sum) {
+__device__ __noinline__ double score64(int func, float l, double mx, double sum) {
   const double x = (double)l;
   if (func == SCORE_SOFTMAX) return exp(x - mx) / sum;
   if (func == SCORE_SIGMOID) return 1.0 / (1.0 + exp(-x));
@@ -124,7 +124,7 @@ __device__ __noinline__ int select_exact(const TopkArgs& a, const T* row, int la
     }
   }
   uint32_t kept = 0xffffffffu;
-  const int size = a.experts / a.groups;
+  const int size = a.size;
   if (a.groups > 1) {
     double gs = NONE;   // lane g: the score of group g
     for (int g = 0; g < a.groups; ++g) {
@@ -195,15 +195,104 @@ __device__ __forceinline__ void sort_desc(uint32_t (&k)[C]) {
           }
 }
 
-// The k best from fp32 values; lane j < k gets the expert of rank j. Returns whether they may have decided
-// it wrongly. Each lane sorts its C keys once (without their ids: two instructions a step); a round then
-// takes the largest head of all lanes, and lanes hold consecutive experts, so that of equal keys the
-// lowest lane's is the lowest id. The places of the chosen keys in their lanes are found afterwards, for all
-// of them at once. (Rescanning the lane's
-// unsorted keys in every round took 1685 instructions a token at 256 experts.)
+// Exact values of this lane's experts in `mask` (bits: places in the lane), the two best of them.
 template <int C, typename T>
-__device__ __forceinline__ bool select_fast(const TopkArgs& a, const T* row, const float (&l)[C], int lane, float mx,
-                                            float sum, int& mine) {
+__device__ __forceinline__ void best_exact(const TopkArgs& a, const T* row, int lane, float lowest, uint32_t mask, double mx,
+                                           double sum, double& b1, double& b2) {
+  while (__any_sync(0xffffffffu, mask != 0u)) {
+    if (mask != 0u) {
+      const int e = lane * C + __ffs(mask) - 1;
+      mask &= mask - 1u;
+      const double s = score64(a.score, clean(logit(row + e), lowest), mx, sum);
+      merge(b1, b2, a.bias != nullptr ? s + (double)a.bias[e] : s, -(double)INFINITY);
+    }
+    __syncwarp();
+  }
+}
+
+// softmax statistics in 64 bits
+template <int C>
+__device__ __forceinline__ double sum_exact(const TopkArgs& a, const float (&l)[C], float mx) {
+  double sum = 0.0;
+  if (a.score == SCORE_SOFTMAX) {
+#pragma unroll 1
+    for (int i = 0; i < C; ++i) sum += l[i] > -INFINITY ? exp((double)l[i] - (double)mx) : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+  return sum;
+}
+
+// The groups kept, from exact scores of the experts that can be among a group's two best: near[i], those within eps
+// of its second best fp32 value (rare, out of line).
+template <int C, typename T>
+__device__ __noinline__ uint32_t kept_exact(const TopkArgs& a, const T* row, int lane, float lowest, float mx, uint32_t near) {
+  const double NONE = -(double)INFINITY;
+  float l[C];
+  load_row<C, T>(a, row, lane, lowest, l);
+  const double sum = sum_exact<C>(a, l, mx);
+  double gs = NONE;
+  if (a.span > 0) {
+    double b1 = NONE, b2 = NONE;
+    best_exact<C, T>(a, row, lane, lowest, near, (double)mx, sum, b1, b2);
+    for (int o = 1; o < a.span; o <<= 1) {
+      const double c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
+      merge(b1, b2, c1, c2);
+    }
+    gs = __shfl_sync(0xffffffffu, a.group_two && b2 > NONE ? b1 + b2 : b1, (lane * a.span) & 31);
+  } else {
+    for (int g = 0; g < a.groups; ++g) {
+      const int lo = min(max(g * a.size - lane * C, 0), C), hi = min(max((g + 1) * a.size - lane * C, 0), C);
+      const uint32_t in = (uint32_t)((1ull << hi) - (1ull << lo));
+      double b1 = NONE, b2 = NONE;
+      best_exact<C, T>(a, row, lane, lowest, near & in, (double)mx, sum, b1, b2);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
+        merge(b1, b2, c1, c2);
+      }
+      if (lane == g) gs = a.group_two && b2 > NONE ? b1 + b2 : b1;
+    }
+  }
+  int rank = 0;
+  for (int g = 0; g < a.groups; ++g) {
+    const double x = __shfl_sync(0xffffffffu, gs, g);
+    rank += x > gs || (x == gs && g < lane) ? 1 : 0;
+  }
+  return __ballot_sync(0xffffffffu, lane < a.groups && rank < a.kept);
+}
+
+// Lanes 0 .. n - 1 hold candidates in the order of their fp32 values (cls: 2 an expert, 1 a masked one, 0 none), all
+// that can be among the k best. Returns lane j's expert by exact values (rare, out of line).
+template <int C, typename T>
+__device__ __noinline__ int order_exact(const TopkArgs& a, const T* row, int lane, float lowest, float mx, int mine, int cls,
+                                        int n) {
+  float l[C];
+  load_row<C, T>(a, row, lane, lowest, l);
+  const double sum = sum_exact<C>(a, l, mx);
+  double v = -(double)INFINITY;
+  if (lane < n && cls == 2) v = score64(a.score, clean(logit(row + mine), lowest), (double)mx, sum) + (double)a.bias[mine];
+  int rank = 0;
+  for (int i = 0; i < n; ++i) {
+    const double x = __shfl_sync(0xffffffffu, v, i);
+    const int c = __shfl_sync(0xffffffffu, cls, i), e = __shfl_sync(0xffffffffu, mine, i);
+    rank += c > cls || (c == cls && (x > v || (x == v && e < mine))) ? 1 : 0;
+  }
+  int out = mine;
+  for (int i = 0; i < n; ++i) {
+    const int r = __shfl_sync(0xffffffffu, lane < n ? rank : -1, i), e = __shfl_sync(0xffffffffu, mine, i);
+    if (r == lane) out = e;
+  }
+  return out;
+}
+
+// The k best: lane j < k gets the expert of rank j. Each lane sorts its C keys once (without their ids: two
+// instructions a step); a round then takes the largest head of all lanes, and lanes hold consecutive experts, so
+// that of equal keys the lowest lane's is the lowest id. The places of the chosen keys in their lanes are found
+// afterwards, for all of them at once.
+template <int C, typename T>
+__device__ __forceinline__ int select(const TopkArgs& a, const T* row, const float (&l)[C], int lane, float lowest, float mx,
+                                      float sum) {
   const bool biased = a.bias != nullptr, scored = biased || (a.groups > 1 && a.group_two);
   float v[C], gv[C], most = 0.f;
   if (scored) {
@@ -223,30 +312,29 @@ __device__ __forceinline__ bool select_fast(const TopkArgs& a, const T* row, con
     for (int i = 0; i < C; ++i) v[i] = gv[i] = l[i];
   }
   // rounding errors of a score and its sum, twice (two of them are compared) and for pairs of experts
-  const float eps = scored ? 2e-6f * warp_max(most) : 0.f;
-  const int size = a.experts / a.groups;
+  const float eps = scored ? 2e-6f * __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most))) : 0.f;
   uint32_t kept = 0xffffffffu;
-  bool doubt = false;
-  const int span = size / C;   // lanes per group when groups begin with lanes
-  const bool by_lane = size % C == 0 && (span & (span - 1)) == 0;
   if (a.groups > 1) {
     float gs = -INFINITY;   // lane g: the score of group g
-    if (by_lane) {
+    uint32_t near = 0u;     // this lane's experts that may be among their group's two best
+    if (a.span > 0) {
       float b1 = -INFINITY, b2 = -INFINITY;
 #pragma unroll
       for (int i = 0; i < C; ++i) merge(b1, b2, gv[i], -INFINITY);
-      for (int o = 1; o < span; o <<= 1) {
+      for (int o = 1; o < a.span; o <<= 1) {
         const float c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
         merge(b1, b2, c1, c2);
       }
-      gs = __shfl_sync(0xffffffffu, a.group_two && b2 > -INFINITY ? b1 + b2 : b1, (lane * span) & 31);
+      gs = __shfl_sync(0xffffffffu, a.group_two && b2 > -INFINITY ? b1 + b2 : b1, (lane * a.span) & 31);
+#pragma unroll
+      for (int i = 0; i < C; ++i) near |= gv[i] > -INFINITY && gv[i] >= b2 - eps ? 1u << i : 0u;
     } else {
       for (int g = 0; g < a.groups; ++g) {
         float b1 = -INFINITY, b2 = -INFINITY;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           const int e = lane * C + i;
-          merge(b1, b2, e >= g * size && e < (g + 1) * size ? gv[i] : -INFINITY, -INFINITY);
+          merge(b1, b2, e >= g * a.size && e < (g + 1) * a.size ? gv[i] : -INFINITY, -INFINITY);
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -254,6 +342,11 @@ __device__ __forceinline__ bool select_fast(const TopkArgs& a, const T* row, con
           merge(b1, b2, c1, c2);
         }
         if (lane == g) gs = a.group_two && b2 > -INFINITY ? b1 + b2 : b1;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          const int e = lane * C + i;
+          if (e >= g * a.size && e < (g + 1) * a.size && gv[i] > -INFINITY && gv[i] >= b2 - eps) near |= 1u << i;
+        }
       }
     }
     uint32_t gk = lane < a.groups ? key_of(gs) : 0u, low = 0u;
@@ -266,23 +359,24 @@ __device__ __forceinline__ bool select_fast(const TopkArgs& a, const T* row, con
     }
     if (scored && a.kept < a.groups) {
       const uint32_t high = __reduce_max_sync(0xffffffffu, gk);
-      doubt = high > key_of(-INFINITY) && !(value_of(low) - value_of(high) > eps);
+      if (high > key_of(-INFINITY) && !(value_of(low) - value_of(high) > eps))
+        kept = kept_exact<C, T>(a, row, lane, lowest, mx, near);
     }
   }
   uint32_t key[C], own[C];
-  if (by_lane || a.groups == 1) {
-    const bool in = a.groups == 1 || ((kept >> (lane / span & 31)) & 1u);
+  if (a.span > 0) {
+    const bool in = (kept >> (a.groups == 1 ? 0 : lane / a.span & 31)) & 1u;
 #pragma unroll
     for (int i = 0; i < C; ++i)
       own[i] = in && lane * C + i < a.experts ? (v[i] > -INFINITY ? key_of(v[i]) : 1u) : 0u;
   } else {
-    int g = lane * C / size, left = (g + 1) * size - lane * C;   // the expert's group, experts left in it
+    int g = lane * C / a.size, left = (g + 1) * a.size - lane * C;   // the expert's group, experts left in it
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       const bool in = lane * C + i < a.experts && ((kept >> g) & 1u);
       if (--left == 0) {
         ++g;
-        left = size;
+        left = a.size;
       }
       own[i] = in ? (v[i] > -INFINITY ? key_of(v[i]) : 1u) : 0u;
     }
@@ -292,8 +386,7 @@ __device__ __forceinline__ bool select_fast(const TopkArgs& a, const T* row, con
   sort_desc<C>(key);
   uint32_t got = 0u;
   int from = 0;
-  const int rounds = biased ? a.topk + 1 : a.topk;
-  for (int j = 0; j < rounds; ++j) {
+  auto round = [&](int j) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, key[0]);
     const int w = __ffs(__ballot_sync(0xffffffffu, key[0] == top)) - 1;
     if (lane == j) {
@@ -305,30 +398,45 @@ __device__ __forceinline__ bool select_fast(const TopkArgs& a, const T* row, con
       for (int i = 0; i + 1 < C; ++i) key[i] = key[i + 1];
       key[C - 1] = 0u;
     }
-  }
+    return top;
+  };
   // the place of the chosen key in its lane: of several equal ones, taken in turn, the n-th
-  uint32_t at = 0u;
+  auto expert = [&]() {
+    uint32_t at = 0u;
 #pragma unroll
-  for (int i = 0; i < C; ++i)
-    if (__shfl_sync(0xffffffffu, own[i], from) == got) at |= 1u << i;
-  const bool picked = lane < rounds && got != 0u;
-  const uint32_t same = __match_any_sync(0xffffffffu, picked ? ((uint64_t)got << 5) | (uint64_t)from : (uint64_t)lane);
-  for (int n = __popc(same & ((1u << lane) - 1u)); n > 0; --n) at &= at - 1u;
-  mine = from * C + __ffs(at) - 1;
+    for (int i = 0; i < C; ++i)
+      if (__shfl_sync(0xffffffffu, own[i], from) == got) at |= 1u << i;
+    const bool several = got != 0u && (at & (at - 1u)) != 0u;
+    if (__any_sync(0xffffffffu, several)) {
+      const uint32_t same = __match_any_sync(0xffffffffu, several ? ((uint64_t)got << 5) | (uint64_t)from : (uint64_t)lane);
+      for (int n = __popc(same & ((1u << lane) - 1u)); n > 0; --n) at &= at - 1u;
+    }
+    return from * C + __ffs(at) - 1;
+  };
+  const int rounds = biased ? a.topk + 1 : a.topk;
+  for (int j = 0; j < rounds; ++j) round(j);
+  int mine = expert();
   if (biased) {
-    // neighbours in the ranking, to the first one left out: far enough apart, or the same logit and bias, whose
-    // order is that of their ids
+    // Neighbours in the ranking, to the first one left out: far enough apart, or the same logit and bias, whose
+    // order is that of their ids. Else all that may belong to the k best are ordered by their exact values.
     const uint32_t nk = __shfl_down_sync(0xffffffffu, got, 1);
     const int ne = __shfl_down_sync(0xffffffffu, mine, 1);
     bool near = lane < a.topk && got > 1u && nk > 1u && !(value_of(got) - value_of(nk) > eps);
     if (near && a.bias[mine] == a.bias[ne] && row[mine] == row[ne]) near = false;
-    doubt = doubt || __any_sync(0xffffffffu, near);
+    if (__any_sync(0xffffffffu, near)) {
+      const uint32_t last = __shfl_sync(0xffffffffu, got, a.topk - 1);
+      uint32_t top = __shfl_sync(0xffffffffu, got, a.topk);
+      int n = rounds;
+      while (n < 32 && last > 1u && top > 1u && !(value_of(last) - value_of(top) > eps)) top = round(n++);
+      if (last > 1u && top > 1u && !(value_of(last) - value_of(top) > eps)) return select_exact<C, T>(a, row, lane, lowest);
+      mine = expert();
+      mine = order_exact<C, T>(a, row, lane, lowest, mx, mine, lane < n ? (got > 1u ? 2 : (int)got) : 0, n);
+    }
   }
-  return doubt;
+  return mine;
 }
 
-// One warp per token; its instructions bound it (16384 tokens of 256 experts: see the sizes in the comment of
-// the file).
+// One warp per token; the chain of its rounds and its instructions bound it.
 template <int C, typename T>
 __global__ void __launch_bounds__(128) topk_kernel(TopkArgs a) {
   const int lane = threadIdx.x & 31;
@@ -348,8 +456,7 @@ __global__ void __launch_bounds__(128) topk_kernel(TopkArgs a) {
     for (int i = 0; i < C; ++i) sum += l[i] > -INFINITY ? __expf(l[i] - mx) : 0.f;
     sum = warp_sum(sum);
   }
-  int mine = 0;
-  if (select_fast<C, T>(a, row, l, lane, mx, sum, mine)) mine = select_exact<C, T>(a, row, lane, lowest);
+  const int mine = select<C, T>(a, row, l, lane, lowest, mx, sum);
   // weights of the chosen ones, from their unbiased scores
   float w = 0.f;
   if (lane < a.topk) {
@@ -513,6 +620,12 @@ cudaError_t launch_topk(const TopkArgs& args, int dtype, cudaStream_t st) {
   const int es = dtype == SB_F32 ? 4 : 2, per = 16 / es;
   a.vec = (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0 && a.experts % per == 0 && (a.stride * es) % 16 == 0;
   a.lowest = dtype == SB_F16 ? -65504.f : -3.3895313892515355e38f;
+  // lanes per group, when groups begin with lanes and a power of two of them makes one
+  int c = 1;
+  while (32 * c < a.experts) c *= 2;
+  a.size = a.experts / a.groups;
+  const int span = a.size / c;
+  a.span = a.groups == 1 ? 32 : (a.size % c == 0 && (span & (span - 1)) == 0 ? span : 0);
   if (dtype == SB_F32) return topk::launch_topk_t<float>(a, st);
   if (dtype == SB_F16) return topk::launch_topk_t<__half>(a, st);
   return topk::launch_topk_t<__nv_bfloat16>(a, st);
