@@ -1327,7 +1327,6 @@ int sb_expert_order(const int64_t* indices, int64_t tokens, int topk, int64_t n_
   a.pairs = pairs;
   a.topk = topk;
   a.experts = (int)n_experts;
-  a.blocks = (int)(pairs > 0 ? sb::order_blocks(pairs) : 1);
   a.hist = (int32_t*)workspace;
   a.offsets = offsets;
   a.tokens = sorted_tokens;

@@ -72,13 +72,15 @@ struct TopkArgs {
   int64_t* ids;
   int vec;                   // set by the launch: rows can be read 16 bytes at a time
   float lowest;              // set by the launch: the lowest finite value of 16-bit logits
-  int size, span;            // set by the launch: experts and lanes of a group (span 0: groups share lanes)
+  int size, span, span_log;  // set by the launch: experts and lanes of a group (span 0: groups share lanes)
+  int vec_bias;
 };
 
 struct OrderArgs {
   const int64_t* ids;        // [pairs]
   int64_t pairs;
-  int topk, experts, blocks;
+  int topk, experts;
+  int blocks;                // set by the launch
   int32_t* hist;             // [blocks][experts], blocks > 1
   int32_t* offsets;          // [experts + 1]
   int32_t* tokens;           // [pairs]

@@ -210,6 +210,31 @@ __device__ __forceinline__ void best_exact(const TopkArgs& a, const T* row, int 
   }
 }
 
+template <int C, int FUNC>
+__device__ __forceinline__ void scores32(const float (&l)[C], float mx, float rsum, float (&s)[C]) {
+#pragma unroll
+  for (int i = 0; i < C; ++i) s[i] = score32(FUNC, l[i], mx, rsum);
+}
+
+template <int C>
+__device__ __forceinline__ void load_bias(const TopkArgs& a, int lane, float (&b)[C]) {
+  if (C % 4 == 0 && a.vec_bias) {
+#pragma unroll
+    for (int i = 0; i < C; i += 4) {
+      const int e = lane * C + i;
+      float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (e < a.experts) w = __ldg(reinterpret_cast<const float4*>(a.bias + e));
+      b[i] = w.x;
+      b[i + (C > 1)] = w.y;
+      b[i + (C > 2) * 2] = w.z;
+      b[i + (C > 2) * 3] = w.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i) b[i] = lane * C + i < a.experts ? __ldg(a.bias + lane * C + i) : 0.f;
+  }
+}
+
 // softmax statistics in 64 bits
 template <int C>
 __device__ __forceinline__ double sum_exact(const TopkArgs& a, const float (&l)[C], float mx) {
@@ -296,16 +321,26 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
   const bool biased = a.bias != nullptr, scored = biased || (a.groups > 1 && a.group_two);
   float v[C], gv[C], most = 0.f;
   if (scored) {
-    const float rsum = rcp(sum);
+    // (one branch for the whole row, not one per expert)
+    if (a.score == SCORE_SOFTMAX) scores32<C, SCORE_SOFTMAX>(l, mx, rcp(sum), gv);
+    else if (a.score == SCORE_SIGMOID) scores32<C, SCORE_SIGMOID>(l, mx, 1.f, gv);
+    else scores32<C, SCORE_SQRTSOFTPLUS>(l, mx, 1.f, gv);
+    if (biased) {
+      float b[C];
+      load_bias<C>(a, lane, b);
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const int e = lane * C + i;
-      const float s = score32(a.score, l[i], mx, rsum);
-      const float b = biased && e < a.experts ? __ldg(a.bias + e) : 0.f;
-      const float t = s + b;
-      most = fmaxf(most, s + fabsf(b));
-      gv[i] = l[i] > -INFINITY && t == t ? t : -INFINITY;
-      v[i] = biased ? gv[i] : l[i];
+      for (int i = 0; i < C; ++i) {
+        const float t = gv[i] + b[i];
+        most = fmaxf(most, gv[i] + fabsf(b[i]));
+        v[i] = gv[i] = l[i] > -INFINITY && t == t ? t : -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        most = fmaxf(most, gv[i]);
+        gv[i] = l[i] > -INFINITY ? gv[i] : -INFINITY;
+        v[i] = l[i];
+      }
     }
   } else {
 #pragma unroll
@@ -365,7 +400,7 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
   }
   uint32_t key[C], own[C];
   if (a.span > 0) {
-    const bool in = (kept >> (a.groups == 1 ? 0 : lane / a.span & 31)) & 1u;
+    const bool in = (kept >> (a.groups == 1 ? 0 : lane >> a.span_log)) & 1u;
 #pragma unroll
     for (int i = 0; i < C; ++i)
       own[i] = in && lane * C + i < a.experts ? (v[i] > -INFINITY ? key_of(v[i]) : 1u) : 0u;
@@ -476,9 +511,9 @@ __global__ void __launch_bounds__(128) topk_kernel(TopkArgs a) {
 }
 
 // ── expert order ───────────────────────────────────────────────────────────────────────────────
-constexpr int OW = 8;               // warps of a block
 constexpr int OSTEP = 8;            // pairs of a thread
 constexpr int OSEG = 32 * OSTEP;    // consecutive pairs of a warp
+constexpr int OW = 8;               // warps of a block (one block of 32 for 8192 pairs: 16 us, four of 8: 6)
 constexpr int OBLOCK = OW * OSEG;
 
 // The warp's pairs' experts (-1: none), all loads in flight at once, and cnt[w][e], the pairs of expert e
@@ -523,9 +558,12 @@ __global__ void __launch_bounds__(OW * 32) order_kernel(OrderArgs a) {
   const int64_t p0 = (int64_t)blockIdx.x * OBLOCK;
   int* all = cnt + OW * a.experts;
   int ex[OSTEP];
-  pdl_wait();
-  pdl_trigger();
+  // After order_count_kernel this starts while that one runs, which in turn began when the ids were written: they
+  // can be read before the wait, the counts in memory after it.
+  if (a.blocks == 1) pdl_wait();
   segment(a, cnt, p0, ex);
+  if (a.blocks > 1) pdl_wait();
+  pdl_trigger();
   // counts become each segment's first place after the expert's base (below)
   for (int e = threadIdx.x; e < a.experts; e += OW * 32) {
     int sum = 0, at = 0;
@@ -547,11 +585,12 @@ __global__ void __launch_bounds__(OW * 32) order_kernel(OrderArgs a) {
     all[e] = a.blocks > 1 ? sum : here;
   }
   __syncthreads();
-  // exclusive scan of the experts' totals, four experts a thread
-  int four[4], mine = 0;
+  // exclusive scan of the experts' totals
+  constexpr int PER = 1024 / (OW * 32);   // experts a thread
+  int four[PER], mine = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int e = threadIdx.x * 4 + j;
+  for (int j = 0; j < PER; ++j) {
+    const int e = threadIdx.x * PER + j;
     four[j] = e < a.experts ? all[e] : 0;
     mine += four[j];
   }
@@ -567,8 +606,8 @@ __global__ void __launch_bounds__(OW * 32) order_kernel(OrderArgs a) {
   for (int w = 0; w < warp; ++w) base += wsum[w];
   if (threadIdx.x == OW * 32 - 1) total = base + mine;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int e = threadIdx.x * 4 + j;
+  for (int j = 0; j < PER; ++j) {
+    const int e = threadIdx.x * PER + j;
     if (e < a.experts) {
       if (blockIdx.x == 0) a.offsets[e] = base;
       all[e] = base;
@@ -620,12 +659,15 @@ cudaError_t launch_topk(const TopkArgs& args, int dtype, cudaStream_t st) {
   const int es = dtype == SB_F32 ? 4 : 2, per = 16 / es;
   a.vec = (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0 && a.experts % per == 0 && (a.stride * es) % 16 == 0;
   a.lowest = dtype == SB_F16 ? -65504.f : -3.3895313892515355e38f;
+  a.vec_bias = (reinterpret_cast<uintptr_t>(a.bias) & 15u) == 0 && a.experts % 4 == 0;
   // lanes per group, when groups begin with lanes and a power of two of them makes one
   int c = 1;
   while (32 * c < a.experts) c *= 2;
   a.size = a.experts / a.groups;
   const int span = a.size / c;
   a.span = a.groups == 1 ? 32 : (a.size % c == 0 && (span & (span - 1)) == 0 ? span : 0);
+  a.span_log = 0;
+  while ((2 << a.span_log) <= a.span) ++a.span_log;
   if (dtype == SB_F32) return topk::launch_topk_t<float>(a, st);
   if (dtype == SB_F16) return topk::launch_topk_t<__half>(a, st);
   return topk::launch_topk_t<__nv_bfloat16>(a, st);
@@ -633,7 +675,9 @@ cudaError_t launch_topk(const TopkArgs& args, int dtype, cudaStream_t st) {
 
 int64_t order_blocks(int64_t pairs) { return (pairs + topk::OBLOCK - 1) / topk::OBLOCK; }
 
-cudaError_t launch_expert_order(const OrderArgs& a, cudaStream_t st) {
+cudaError_t launch_expert_order(const OrderArgs& args, cudaStream_t st) {
+  OrderArgs a = args;
+  a.blocks = (int)(a.pairs > 0 ? order_blocks(a.pairs) : 1);
   const dim3 grid(a.blocks), block(topk::OW * 32);
   const size_t smem = (size_t)(topk::OW + 1) * a.experts * sizeof(int);
   if (a.blocks > 1) {

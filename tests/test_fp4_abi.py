@@ -93,5 +93,5 @@ def test_route_refusals():
 
     assert o(t=-1) == -2 and o(k=0) == -2 and o(e=1025) == -2 and o(t=1 << 30, k=4) == -2
     assert o(ids=None) == -1 and o(off=None) == -1 and o(tok=None) == -1 and o(pl=None) == -1
-    assert o(t=4096, ws=None) == -4 and o(t=4096, ws=FAKE, n=4 * 8 * 4 - 1) == -4
-    assert o(t=4096, ws=ctypes.c_void_p(4097), n=1 << 20) == -1
+    assert o(t=8192, ws=None) == -4 and o(t=8192, ws=FAKE, n=8 * 8 * 4 - 1) == -4
+    assert o(t=8192, ws=ctypes.c_void_p(4097), n=1 << 20) == -1
