@@ -50,8 +50,16 @@ __device__ __forceinline__ float border(uint32_t c) {
   return c < 4 ? 0.25f + 0.5f * (float)c : (c == 4 ? 2.5f : (c == 5 ? 3.5f : 5.0f));
 }
 
-// fp32 arithmetic decides exactly while nothing under- or overflows
-__device__ __forceinline__ bool mid_range(float v) { return v >= 7.9e-31f && v <= 1.2e30f; }
+// Tensor scales for which fp32 arithmetic decides exactly: neither they nor their products with any block scale
+// under- or overflow.
+__device__ __forceinline__ bool mid_range(float ts) { return ts >= 7.9e-28f && ts <= 1.2e27f; }
+
+// 1 / v within 2^-22, v in the middle of the range
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 
 // e4m3 code of min(448, a / (6 ts))
 __device__ __noinline__ uint32_t scale_exact(float a, float ts) {
@@ -67,9 +75,13 @@ __device__ __noinline__ uint32_t scale_exact(float a, float ts) {
 }
 
 __device__ __forceinline__ uint32_t scale_code(float a, float ts, float inv6ts, bool mid) {
+  if (!mid) return scale_exact(a, ts);
   const float v = a * inv6ts;
   const uint32_t lo = f32_to_e4m3(v * (1.f - 9.6e-7f)), hi = f32_to_e4m3(v * (1.f + 9.6e-7f));
-  return (mid && lo == hi) ? lo : scale_exact(a, ts);
+  if (lo == hi) return lo;
+  // a against 6 ts times the middle of the two: the product-sum rounds once, so its sign is exact
+  const float r = fmaf(-3.f * (e4m3_to_f32(lo) + e4m3_to_f32(hi)), ts, a);
+  return r > 0.f || (r == 0.f && (lo & 1u)) ? hi : lo;
 }
 
 // magnitude code of |x| / (s ts)
@@ -89,11 +101,13 @@ struct Traits;
 template <>
 struct Traits<__nv_bfloat16> {
   static constexpr uint32_t INF = 0x7F80u;
+  static constexpr uint32_t BELOW = 0xFFFFu;   // fp32 bits below the type's last one
   static __device__ __forceinline__ float f(uint32_t h) { return __uint_as_float(h << 16); }
 };
 template <>
 struct Traits<__half> {
   static constexpr uint32_t INF = 0x7C00u;
+  static constexpr uint32_t BELOW = 0x1FFFu;
   static __device__ __forceinline__ float f(uint32_t h) { return __half2float(__ushort_as_half((unsigned short)h)); }
 };
 
@@ -159,34 +173,69 @@ struct Unit<float> {
 
 constexpr uint32_t F32_INF = 0x7F800000u;
 
+// How 1 / p has to be turned so that one rounding of x / p decides as the real quotient does, for 16-bit x. The borders
+// between codes are p / 4 times 1, 3, 5, 7, 10, 14 and 20: four mantissas k p. The 16-bit values that come near a border
+// (2^-19 of it) all have the mantissa of the one grid point next to k p, so that its exact side of k (p + e)
+// decides for all of them; on the border itself the even code is the lower one for k = 1 and 5, the upper one for
+// 3 and 7. Other values are further than 2^-20 away. Returns 0 (no value comes near), 1 (down), 2 (up), 3 (both: no
+// one factor serves). With one scale per row such values are common: there 6 p is the row's largest value in
+// its own block.
+template <typename T>
+__device__ __forceinline__ uint32_t lean(float p, float e) {
+  uint32_t need = 0u;
+#pragma unroll
+  for (int m = 1; m < 8; m += 2) {
+    const float k = (float)m;
+    const uint32_t b = __float_as_uint(p * k);
+    const float g = __uint_as_float((b + (Traits<T>::BELOW + 1u) / 2u) & ~Traits<T>::BELOW);
+    const float r = fmaf(-k, e, fmaf(-k, p, g));
+    const uint32_t side = r > 0.f || (r == 0.f && (m & 2)) ? 2u : 1u;
+    if (((b + 16u) & Traits<T>::BELOW) <= 32u) need |= side;
+  }
+  return need;
+}
+template <>
+__device__ __forceinline__ uint32_t lean<float>(float, float) { return 3u; }
+
 // the unit's 16 codes for the scale s ts (NVFP4)
 template <typename T>
-__device__ __forceinline__ uint2 codes_nv(const Unit<T>& u, float s, float ts) {
-  const float p = s * ts;
-  if (!(p > 0.f) && s == 0.f) return make_uint2(0u, 0u);
+__device__ __forceinline__ uint2 codes_nv(const Unit<T>& u, float s, float ts, bool mid) {
+  if (s == 0.f) return make_uint2(0u, 0u);
   uint32_t out[2];
-  if (mid_range(p) && mid_range(ts)) {
-    const float inv = __frcp_rn(p), lo = inv * (1.f - 9.6e-7f), hi = inv * (1.f + 9.6e-7f);
+  if (mid) {
+    const float p = s * ts, e = fmaf(s, ts, -p), inv = rcp(p);   // s ts = p + e exactly
+    const uint32_t need = lean<T>(p, e);
+    if (need != 3u) {
+      const float f = need == 0u ? inv : (need == 1u ? inv * (1.f - 4.8e-7f) : inv * (1.f + 4.8e-7f));
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float a[8], b[8];
+      for (int h = 0; h < 2; ++h) {
+        float a[8];
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        const float x0 = u.get(8 * h + i), x1 = u.get(8 * h + i + 1);
-        mul2(x0, x1, lo, a[i], a[i + 1]);
-        mul2(x0, x1, hi, b[i], b[i + 1]);
+        for (int i = 0; i < 8; i += 2) mul2(u.get(8 * h + i), u.get(8 * h + i + 1), f, a[i], a[i + 1]);
+        out[h] = cvt8(a);
       }
-      out[h] = cvt8(a);
-      const uint32_t diff = out[h] ^ cvt8(b);
-      if (diff != 0u) {
-        const float e = fmaf(s, ts, -p);   // s ts = p + e exactly
+    } else {
+      const float lo = inv * (1.f - 9.6e-7f), hi = inv * (1.f + 9.6e-7f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if ((diff >> (4 * i)) & 0xFu) {
-            // |x| - m (p + e): the first difference is exact this near to the border m p
-            const uint32_t c = (out[h] >> (4 * i)) & 7u;
-            const float m = border(c), r = fmaf(-m, e, fmaf(-m, p, fabsf(u.get(8 * h + i))));
-            if (r > 0.f || (r == 0.f && (c & 1u))) out[h] += 1u << (4 * i);
+      for (int h = 0; h < 2; ++h) {
+        float a[8], b[8];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float x0 = u.get(8 * h + i), x1 = u.get(8 * h + i + 1);
+          mul2(x0, x1, lo, a[i], a[i + 1]);
+          mul2(x0, x1, hi, b[i], b[i + 1]);
+        }
+        out[h] = cvt8(a);
+        const uint32_t diff = out[h] ^ cvt8(b);
+        if (diff != 0u) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if ((diff >> (4 * i)) & 0xFu) {
+              // |x| - m (p + e): the first difference is exact this near to the border m p
+              const uint32_t c = (out[h] >> (4 * i)) & 7u;
+              const float m = border(c), r = fmaf(-m, e, fmaf(-m, p, fabsf(u.get(8 * h + i))));
+              if (r > 0.f || (r == 0.f && (c & 1u))) out[h] += 1u << (4 * i);
+            }
           }
         }
       }
@@ -217,9 +266,18 @@ __device__ __forceinline__ uint2 codes_mx(const Unit<T>& u, float inv) {
   return make_uint2(cvt8(a), cvt8(b));
 }
 
-// Warps [0, wpr) of each row's warps share the row; lane u of them takes units u, u + 32 wpr, ...
-// (16 values each, all loads issued before any is used). V units a thread: 4 keep enough bytes in
-// flight per thread for the large sizes, 1 spreads a few rows over more threads.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_unit(Unit<T>& u, const T* row, int k, const QuantArgs& a, bool has) {
+  u.zero();
+  if (has && k * 16 < a.k) {
+    if (VEC) u.load(row + (int64_t)k * 16);
+    else u.load_tail(row + (int64_t)k * 16, a.k - k * 16);
+  }
+}
+
+// A row's wpr warps take its units (16 values a thread) in turn, V at a time with their loads issued together. With
+// one tensor scale per row the row is read twice, first for its largest value, then, from L1, for its
+// codes.
 template <typename T, bool NV, int V, bool VEC>
 __global__ void __launch_bounds__(1024) quant_kernel(QuantArgs a) {
   __shared__ uint32_t red[32];
@@ -251,30 +309,22 @@ __global__ void __launch_bounds__(1024) quant_kernel(QuantArgs a) {
   }
   const T* xr = reinterpret_cast<const T*>(a.x) + (has ? src : 0) * a.stride;
   const int step = a.wpr * 32;
-  Unit<T> u[V];
-  uint32_t am[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int k = tr + i * step;
-    u[i].zero();
-    if (has && k < a.units) {
-      if (VEC && (k + 1) * 16 <= a.k) {
-        u[i].load(xr + (int64_t)k * 16);
-      } else if (k * 16 < a.k) {
-        u[i].load_tail(xr + (int64_t)k * 16, a.k - k * 16);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) am[i] = u[i].amax();
   float ts = 1.f;
   if (NV) {
     if (a.ts != nullptr) {
       ts = *a.ts;
     } else {
       uint32_t m = 0u;
+      for (int k0 = tr; k0 < a.units; k0 += step * V) {
+        Unit<T> u[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) m = max(m, am[i] < F32_INF ? am[i] : 0u);
+        for (int i = 0; i < V; ++i) load_unit<T, VEC>(u[i], xr, k0 + i * step, a, has);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const uint32_t am = u[i].amax();
+          m = max(m, am < F32_INF ? am : 0u);
+        }
+      }
       m = __reduce_max_sync(0xffffffffu, m);
       if (a.wpr > 1) {
         if (lane == 0) red[warp] = m;
@@ -289,35 +339,41 @@ __global__ void __launch_bounds__(1024) quant_kernel(QuantArgs a) {
   if (!live) return;   // whole warps: a row's warps share `live`
   const bool ts_ok = ts > 0.f && __float_as_uint(ts) < F32_INF;
   const bool ts_mid = mid_range(ts);
-  const float inv6 = NV ? __frcp_rn(6.f * ts) : 0.f;
+  const float inv6 = NV ? rcp(6.f * ts) : 0.f;
   uint8_t* cr = a.codes + row * a.row_bytes;
   uint8_t* sr = a.scales + ((pos >> 7) * a.atoms) * 512 + (pos & 31) * 16 + ((pos >> 5) & 3) * 4;
+  for (int base = 0; base < a.units; base += step * V) {
+    Unit<T> u[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int k = tr + i * step;
-    uint32_t sc;
-    uint2 c = make_uint2(0u, 0u);
-    if (NV) {
-      const bool fine = am[i] < F32_INF && ts_ok;
-      sc = fine ? scale_code(__uint_as_float(am[i]), ts, inv6, ts_mid) : 0x7Fu;
-      if (fine) c = codes_nv<T>(u[i], e4m3_to_f32(sc), ts);
-      if (k >= a.units) sc = 0u;
-      uint32_t w = sc << (8 * (k & 3));
-      w |= __shfl_xor_sync(0xffffffffu, w, 1);
-      w |= __shfl_xor_sync(0xffffffffu, w, 2);
-      if (k < a.units && (k & 3) == 0) *reinterpret_cast<uint32_t*>(sr + (int64_t)(k >> 2) * 512) = w;
-    } else {
-      const uint32_t m = max(am[i], __shfl_xor_sync(0xffffffffu, am[i], 1));
-      // amax = f 2^e: t = e - 2 for f <= 1.5, else e - 1; biased and floored at 2^-126
-      sc = m < F32_INF ? (uint32_t)max((int)((m + 0x3FFFFFu) >> 23) - 2, 1) : 0xFFu;
-      if (m < F32_INF) c = codes_mx<T>(u[i], __uint_as_float((254u - sc) << 23));
-      if (k >= a.units) sc = 0u;
-      uint32_t w = sc << (8 * ((k >> 1) & 3));
-      w |= __shfl_xor_sync(0xffffffffu, w, 2);
-      w |= __shfl_xor_sync(0xffffffffu, w, 4);
-      if (k < a.units && (k & 7) == 0) *reinterpret_cast<uint32_t*>(sr + (int64_t)(k >> 3) * 512) = w;
+    for (int i = 0; i < V; ++i) load_unit<T, VEC>(u[i], xr, base + tr + i * step, a, has);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int k = base + tr + i * step;
+      const uint32_t am = u[i].amax();
+      uint32_t sc;
+      uint2 c = make_uint2(0u, 0u);
+      if (NV) {
+        const bool fine = am < F32_INF && ts_ok;
+        sc = fine ? scale_code(__uint_as_float(am), ts, inv6, ts_mid) : 0x7Fu;
+        if (fine) c = codes_nv<T>(u[i], e4m3_to_f32(sc), ts, ts_mid);
+        if (k >= a.units) sc = 0u;
+        uint32_t w = sc << (8 * (k & 3));
+        w |= __shfl_xor_sync(0xffffffffu, w, 1);
+        w |= __shfl_xor_sync(0xffffffffu, w, 2);
+        if (k < a.units && (k & 3) == 0) *reinterpret_cast<uint32_t*>(sr + (int64_t)(k >> 2) * 512) = w;
+      } else {
+        const uint32_t m = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
+        // amax = f 2^e: t = e - 2 for f <= 1.5, else e - 1; biased and floored at 2^-126
+        sc = m < F32_INF ? (uint32_t)max((int)((m + 0x3FFFFFu) >> 23) - 2, 1) : 0xFFu;
+        if (m < F32_INF) c = codes_mx<T>(u[i], __uint_as_float((254u - sc) << 23));
+        if (k >= a.units) sc = 0u;
+        uint32_t w = sc << (8 * ((k >> 1) & 3));
+        w |= __shfl_xor_sync(0xffffffffu, w, 2);
+        w |= __shfl_xor_sync(0xffffffffu, w, 4);
+        if (k < a.units && (k & 7) == 0) *reinterpret_cast<uint32_t*>(sr + (int64_t)(k >> 3) * 512) = w;
+      }
+      if (k < a.units) *reinterpret_cast<uint2*>(cr + (int64_t)k * 8) = c;
     }
-    if (k < a.units) *reinterpret_cast<uint2*>(cr + (int64_t)k * 8) = c;
   }
 }
 
@@ -397,8 +453,7 @@ __global__ void __launch_bounds__(256) tile_scales_kernel(const uint8_t* __restr
 template <typename T, bool NV, bool VEC>
 static cudaError_t launch_quant_v(const QuantArgs& q, int v, dim3 grid, dim3 block, cudaStream_t st) {
   if (v == 1) return launch_pdl(quant_kernel<T, NV, 1, VEC>, grid, block, 0, st, q);
-  if (v == 2) return launch_pdl(quant_kernel<T, NV, 2, VEC>, grid, block, 0, st, q);
-  return launch_pdl(quant_kernel<T, NV, 4, VEC>, grid, block, 0, st, q);
+  return launch_pdl(quant_kernel<T, NV, 2, VEC>, grid, block, 0, st, q);
 }
 
 template <typename T>
@@ -411,15 +466,14 @@ static cudaError_t launch_quant_t(const QuantArgs& q, int v, bool vec, dim3 grid
 
 cudaError_t launch_fp4_quant(const QuantArgs& args, int dtype, cudaStream_t st) {
   QuantArgs q = args;
-  // units per thread: one while the rows do not fill the GPU, else four
-  const int64_t per = (int64_t)num_sms() * 1024;
-  int v = q.rows * q.units <= per ? 1 : (q.rows * q.units <= 2 * per ? 2 : 4);
-  while ((q.units + 32 * v - 1) / (32 * v) > 32) v *= 2;
+  // units in flight per thread: one while the rows do not fill the GPU, else two
+  const int v = q.rows * q.units <= (int64_t)num_sms() * 1024 ? 1 : 2;
   q.wpr = (q.units + 32 * v - 1) / (32 * v);
+  if (q.wpr > 32) q.wpr = 32;
   const int rpc = q.wpr >= 8 ? 1 : 8 / q.wpr;
   const dim3 grid((unsigned)((q.rows + rpc - 1) / rpc)), block(rpc * q.wpr * 32);
   const int es = dtype == SB_F32 ? 4 : 2;
-  const bool vec = (reinterpret_cast<uintptr_t>(q.x) & 15u) == 0 && (q.stride * es) % 16 == 0;
+  const bool vec = (reinterpret_cast<uintptr_t>(q.x) & 15u) == 0 && (q.stride * es) % 16 == 0 && q.k % 16 == 0;
   if (dtype == SB_F32) return fp4::launch_quant_t<float>(q, v, vec, grid, block, st);
   if (dtype == SB_F16) return fp4::launch_quant_t<__half>(q, v, vec, grid, block, st);
   return fp4::launch_quant_t<__nv_bfloat16>(q, v, vec, grid, block, st);
