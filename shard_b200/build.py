@@ -4,7 +4,8 @@
     python -m shard_b200.build --force
 
 Each .cu under shard_b200/csrc is compiled to an object in parallel, then linked into
-shard_b200/libshard_b200.so, next to the Python package that loads it.
+shard_b200/libshard_b200.so, next to the Python package that loads it. csrc/sb_host.cpp, the torch side of
+shard_b200.fp4 and shard_b200.route, becomes the extension module shard_b200/_host.so, linked to it.
 """
 from __future__ import annotations
 
@@ -20,6 +21,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libshard_b200.so")
+HOST = os.path.join(PKG, "_host.so")
+HOST_SRC = os.path.join(CSRC, "sb_host.cpp")
 BUILD = os.path.join(PKG, "_build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-warn-spills",
@@ -39,13 +42,13 @@ def sources():
 
 def _deps():
     return sources() + sorted(glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h"))) + \
-        [os.path.join(ROOT, "include", "shard_b200.h")]
+        [HOST_SRC, os.path.join(ROOT, "include", "shard_b200.h")]
 
 
 def up_to_date() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(HOST):
         return False
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(HOST))
     return all(os.path.getmtime(d) <= t for d in _deps())
 
 
@@ -56,6 +59,24 @@ def _compile(src: str) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"nvcc failed on {src}:\n{r.stdout}\n{r.stderr}")
     return obj
+
+
+def _compile_host() -> None:
+    import sysconfig
+
+    import torch
+    t = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    inc = [os.path.join(t, "include"), os.path.join(t, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include"), sysconfig.get_paths()["include"], os.path.join(ROOT, "include")]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + d for d in inc), HOST_SRC, "-o",
+           HOST + ".tmp", "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-L" + PKG,
+           "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {HOST_SRC}:\n{r.stdout}\n{r.stderr}")
+    os.replace(HOST + ".tmp", HOST)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -70,8 +91,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    _compile_host()
     if verbose:
-        print(f"built {LIB}")
+        print(f"built {LIB} and {HOST}")
     return LIB
 
 

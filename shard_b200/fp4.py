@@ -35,16 +35,29 @@ import torch
 
 from . import _lib
 from . import formats as F
-from ._lib import check, lib, ptr
+from ._lib import ShardB200Error, check, lib, ptr
 
 PLAIN, W13 = _lib.MAT_PLAIN, _lib.MAT_W13
 DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
 _FMT = {"nvfp4": F.FMT_NVFP4, "mxfp4": F.FMT_MXFP4, F.FMT_NVFP4: F.FMT_NVFP4, F.FMT_MXFP4: F.FMT_MXFP4}
 
-# A decoded token's call is bound by its host side: these run once per call, without lookups by name.
 _current_device = torch._C._cuda_getDevice
-_current_stream = torch._C._cuda_getCurrentRawStream
-_empty = torch.empty
+_new = object.__new__
+_HOST = None
+
+
+def host():
+    """The extension module that checks, allocates and launches (csrc/sb_host.cpp). Like the library it has no
+    substitute: a missing one raises."""
+    global _HOST
+    if _HOST is None:
+        lib()
+        try:
+            from . import _host
+        except ImportError as e:
+            raise ShardB200Error(f"shard_b200/_host.so cannot be loaded ({e}); build it with `python -m shard_b200.build`")
+        _HOST = _host
+    return _HOST
 
 
 def _fmt(fmt: Union[int, str]) -> int:
@@ -63,22 +76,6 @@ def _elsewhere(device, stream):
         else:
             with torch.cuda.stream(stream):
                 yield
-
-
-def _same_device(what, ref, *tensors):
-    for t in tensors:
-        if t is not None and t.device != ref.device:
-            raise ValueError(f"{what}: tensors on {t.device} and {ref.device}")
-
-
-def _index(what, name, t, n=None):
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{what}: {name} must be a contiguous int32 vector" + ("" if n is None else f" of {n}"))
-
-
-def _float_vec(what, name, t, n=None):
-    if t.dtype != torch.float32 or not t.is_contiguous() or (n is not None and t.numel() != n):
-        raise ValueError(f"{what}: {name} must be contiguous fp32" + ("" if n is None else f" with {n} values"))
 
 
 class Fp4Tensor:
@@ -141,57 +138,21 @@ def quant(x: torch.Tensor, fmt: Union[int, str] = F.FMT_NVFP4, tensor_scale: Opt
                   rows behind offsets[E] are left as they are"""
     f = _FMT.get(fmt)
     if f is None:
-        _fmt(fmt)
-    dt = DTYPES.get(x.dtype)
-    if dt is None or not x.is_cuda or x.dim() < 1:
-        raise ValueError("quant: x must be a CUDA tensor of bf16, fp16 or fp32")
-    dev = x.get_device()
-    if stream is not None or dev != _current_device():
+        f = _fmt(fmt)
+    if stream is not None or x.get_device() != _current_device():
+        if not x.is_cuda:
+            raise ValueError("quant: x must be a CUDA tensor of bf16, fp16 or fp32")
         with _elsewhere(x.device, stream):
-            return quant(x, fmt, tensor_scale, rows, offsets)
-    shape = x.shape
-    k = shape[-1]
-    z = x if x.dim() == 2 else x.reshape(-1, k)
-    m = z.shape[0]
-    stride, inner = z.stride()
-    if inner != 1 and k > 1:
-        z = z.contiguous()
-        stride = k
-    p, groups, po, pr, pt = m, 0, None, None, None
-    if rows is not None:
-        _index("quant", "rows", rows)
-        _same_device("quant", x, rows)
-        p, pr = rows.shape[0], rows.data_ptr()
-    if offsets is not None:
-        _index("quant", "offsets", offsets)
-        _same_device("quant", x, offsets)
-        groups, po = offsets.shape[0] - 1, offsets.data_ptr()
-        if groups < 1:
-            raise ValueError("quant: offsets must hold at least two values")
-    if tensor_scale is not None:
-        if f != F.FMT_NVFP4:
-            raise ValueError("quant: MXFP4 has no tensor scale")
-        _float_vec("quant", "tensor_scale", tensor_scale, 1)
-        _same_device("quant", x, tensor_scale)
-        pt = tensor_scale.data_ptr()
-    # one allocation: codes, scale atoms (sb_fp4_scale_bytes), the rows' tensor scales
-    kp = (k + 31) >> 5
-    blocks = (p >> 7) + groups if groups else (p + 127) >> 7
-    end = p * kp * 16
-    per_row = f == F.FMT_NVFP4 and pt is None
-    atoms_end = end + blocks * ((kp + 1) >> 1 if f == F.FMT_NVFP4 else (kp + 3) >> 2) * 512
-    buf = _empty(atoms_end + 4 * p if per_row else atoms_end, dtype=torch.uint8, device=x.device)
-    base = buf.data_ptr()
-    q = Fp4Tensor.__new__(Fp4Tensor)
-    q.fmt, q.mats, q.rows, q.k, q.kind, q.offsets, q.per_row = f, 1, p, k, PLAIN, offsets, per_row
-    q.shape = shape[:-1] if rows is None else (p,)
-    q._buf, q._parts, q._codes, q._scales, q._ts = buf, (end, atoms_end), None, None, tensor_scale
+            return quant(x, f, tensor_scale, rows, offsets)
+    r = (_HOST or host()).quant(x, f, tensor_scale, rows, offsets)
+    if type(r) is int:
+        check(r, "sb_fp4_quant")
+    q = _new(Fp4Tensor)
+    q._buf, q.rows, q.k, q.per_row, end, atoms_end, base, q.shape = r
+    q.fmt, q.mats, q.kind, q.offsets = f, 1, PLAIN, offsets
+    q._parts, q._codes, q._scales, q._ts = (end, atoms_end), None, None, tensor_scale
     q.codes_ptr, q.scales_ptr = base, base + end
-    q.ts_ptr = base + atoms_end if per_row else pt
-    rc = lib().sb_fp4_quant(f, z.data_ptr(), dt, m, k, stride if m > 1 else k, pr, p, pt, po, groups, base, base + end,
-                            q.ts_ptr if per_row else None, _current_stream(dev))
-    if rc:
-        check(rc, "sb_fp4_quant")
+    q.ts_ptr = base + atoms_end if q.per_row else ptr(tensor_scale)
     return q
 
 
@@ -204,15 +165,12 @@ def dequant(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, stream=None) -> t
     if dt is None:
         raise ValueError(f"dequant: dtype {dtype}")
     buf = q._buf
-    dev = buf.get_device()
-    if stream is not None or dev != _current_device():
+    if stream is not None or buf.get_device() != _current_device():
         with _elsewhere(buf.device, stream):
             return dequant(q, dtype)
-    y = _empty((*q.shape, q.k), dtype=dtype, device=buf.device)
-    rc = lib().sb_fp4_dequant(q.fmt, q.codes_ptr, q.scales_ptr, q.ts_ptr, q.per_row, q.rows, q.k, y.data_ptr(), dt,
-                              _current_stream(dev))
-    if rc:
-        check(rc, "sb_fp4_dequant")
+    y = (_HOST or host()).dequant(buf, q.fmt, q.codes_ptr, q.scales_ptr, q.ts_ptr, q.per_row, q.rows, q.k, q.shape, dt)
+    if type(y) is int:
+        check(y, "sb_fp4_dequant")
     return y
 
 
@@ -226,7 +184,9 @@ def pack(fmt: Union[int, str], codes: torch.Tensor, scales: torch.Tensor, ts: Op
     if not codes.is_cuda or codes.dim() not in (2, 3):
         raise ValueError("pack: codes must be a CUDA tensor [N, K/2] or [E, N, K/2]")
     c, s = codes.view(torch.uint8), scales.view(torch.uint8)
-    _same_device("pack", codes, scales, ts)
+    for t in (scales, ts):
+        if t is not None and t.device != codes.device:
+            raise ValueError(f"pack: tensors on {t.device} and {codes.device}")
     mats, n, k = (1 if c.dim() == 2 else c.shape[0]), c.shape[-2], 2 * c.shape[-1]
     nb = k // (16 if f == F.FMT_NVFP4 else 32)
     if k % 32 or tuple(s.shape) != (*c.shape[:-1], nb):
@@ -248,7 +208,7 @@ def pack(fmt: Union[int, str], codes: torch.Tensor, scales: torch.Tensor, ts: Op
     c, s = c.contiguous().view(mats * n, k // 2), s.contiguous()
     L = lib()
     out = torch.empty(L.sb_fp4_scale_bytes(f, mats, n, k, 0), dtype=torch.uint8, device=c.device)
-    check(L.sb_fp4_tile_scales(f, s.data_ptr(), out.data_ptr(), mats, n, k, _current_stream(c.get_device())),
+    check(L.sb_fp4_tile_scales(f, s.data_ptr(), out.data_ptr(), mats, n, k, torch.cuda.current_stream().cuda_stream),
           "sb_fp4_tile_scales")
     return Fp4Tensor(f, mats, n, k, c, out, ts, None, kind, tuple(codes.shape[:-1]))
 
@@ -269,12 +229,6 @@ def _operands(what, a, w, out_dtype):
     return dt
 
 
-def _check_out(what, out, shape, dtype, like):
-    if tuple(out.shape) != shape or out.dtype != dtype or out.device != like.device or \
-            (out.numel() and shape[1] > 1 and out.stride(-1) != 1) or (shape[0] > 1 and out.stride(0) < shape[1]):
-        raise ValueError(f"{what}: out must be {shape} {dtype} on {like.device}, with contiguous rows that do not overlap")
-
-
 def gemm(a: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None,
          stream=None) -> torch.Tensor:
     """y [..., N] = A [..., K] W [N, K]^T, summed in fp32 and rounded once. `out` [M, N] may have any row stride.
@@ -283,23 +237,14 @@ def gemm(a: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, ou
     if a.offsets is not None or w.offsets is not None or w.mats != 1 or w.kind != PLAIN:
         raise ValueError("gemm: plain operands of one matrix (grouped_gemm takes banks and expert groups)")
     buf = a._buf
-    dev = buf.get_device()
-    if stream is not None or dev != _current_device():
+    if stream is not None or buf.get_device() != _current_device():
         with _elsewhere(buf.device, stream):
             return gemm(a, w, out_dtype, out)
-    m, n = a.rows, w.rows
-    ld = n
-    if out is None:
-        out = _empty((*a.shape, n), dtype=out_dtype, device=buf.device)
-    else:
-        _check_out("gemm", out, (m, n), out_dtype, buf)
-        if m > 1:
-            ld = out.stride(0)
-    rc = lib().sb_fp4_gemm(a.fmt, a.codes_ptr, a.scales_ptr, a.ts_ptr, a.per_row, m, w.codes_ptr, w.scales_ptr, w.ts_ptr,
-                           w.per_row, n, a.k, out.data_ptr(), dt, ld, _current_stream(dev))
-    if rc:
-        check(rc, "sb_fp4_gemm")
-    return out
+    y = (_HOST or host()).gemm(buf, a.fmt, a.codes_ptr, a.scales_ptr, a.ts_ptr, a.per_row, a.rows, a.shape, a.k, w.codes_ptr,
+                               w.scales_ptr, w.ts_ptr, w.per_row, w.rows, dt, out)
+    if type(y) is int:
+        check(y, "sb_fp4_gemm")
+    return y
 
 
 def grouped_gemm(a: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16,
@@ -315,32 +260,15 @@ def grouped_gemm(a: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bflo
     if not limit >= 0.0:
         raise ValueError("grouped_gemm: limit must be >= 0")
     buf = a._buf
-    p = a.rows
-    pw = None
-    if row_weight is not None:
-        _float_vec("grouped_gemm", "row_weight", row_weight, p)
-        _same_device("grouped_gemm", buf, row_weight)
-        pw = row_weight.data_ptr()
-    dev = buf.get_device()
-    if stream is not None or dev != _current_device():
+    if stream is not None or buf.get_device() != _current_device():
         with _elsewhere(buf.device, stream):
             return grouped_gemm(a, w, out_dtype, row_weight, limit, out)
-    swiglu = w.kind == W13
-    n = w.rows
-    width = n >> 1 if swiglu else n
-    ld = width
-    if out is None:
-        out = _empty((p, width), dtype=out_dtype, device=buf.device)
-    else:
-        _check_out("grouped_gemm", out, (p, width), out_dtype, buf)
-        if p > 1:
-            ld = out.stride(0)
-    rc = lib().sb_fp4_grouped_gemm(a.fmt, a.codes_ptr, a.scales_ptr, a.ts_ptr, a.per_row, p, off.data_ptr(), w.codes_ptr,
-                                   w.scales_ptr, w.ts_ptr, 1 if w._ts is None else w._ts.shape[1], w.mats, n, a.k, swiglu,
-                                   limit, pw, out.data_ptr(), dt, ld, _current_stream(dev))
-    if rc:
-        check(rc, "sb_fp4_grouped_gemm")
-    return out
+    y = (_HOST or host()).grouped_gemm(buf, a.fmt, a.codes_ptr, a.scales_ptr, a.ts_ptr, a.per_row, a.rows, a.k, off, w.codes_ptr,
+                                       w.scales_ptr, w.ts_ptr, 1 if w._ts is None else w._ts.shape[1], w.mats, w.rows,
+                                       w.kind == W13, limit, row_weight, dt, out)
+    if type(y) is int:
+        check(y, "sb_fp4_grouped_gemm")
+    return y
 
 
 def device_error(device=None) -> int:

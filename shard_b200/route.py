@@ -16,8 +16,9 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from ._lib import check, lib
-from .fp4 import DTYPES, _current_device, _current_stream, _elsewhere, _empty, _same_device
+from ._lib import check
+from . import fp4
+from .fp4 import _current_device, _elsewhere
 
 _SCORE = _lib.SCORE
 _GROUP_SCORE = {"max": 0, "top2": 1}
@@ -43,57 +44,29 @@ def topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, scor
 
     Values are compared as real numbers, ties go to the lower id. An expert whose logit is NaN, -inf or the
     type's lowest value is masked: after all others of the kept groups, with weight 0."""
-    sc, gs, dt = _SCORE.get(score), _GROUP_SCORE.get(group_score), DTYPES.get(logits.dtype)
+    sc, gs = _SCORE.get(score), _GROUP_SCORE.get(group_score)
     if sc is None or gs is None:
         raise ValueError(f"topk: score {score!r}, group_score {group_score!r}")
-    if dt is None or not logits.is_cuda or logits.dim() != 2:
-        raise ValueError("topk: logits must be a CUDA tensor [T, E] of bf16, fp16 or fp32")
-    dev = logits.get_device()
-    if stream is not None or dev != _current_device():
+    if stream is not None or logits.get_device() != _current_device():
+        if not logits.is_cuda:
+            raise ValueError("topk: logits must be a CUDA tensor [T, E] of bf16, fp16 or fp32")
         with _elsewhere(logits.device, stream):
             return topk(logits, k, bias, score, n_group, topk_group, group_score, renormalize, scale)
-    t, e = logits.shape
-    stride, inner = logits.stride()
-    if inner != 1 and e > 1:
-        logits = logits.contiguous()
-        stride = e
-    pb = None
-    if bias is not None:
-        if bias.dtype != torch.float32 or tuple(bias.shape) != (e,) or not bias.is_contiguous():
-            raise ValueError(f"topk: bias must be contiguous fp32 [{e}]")
-        _same_device("topk", logits, bias)
-        pb = bias.data_ptr()
-    w = _empty((t, k), dtype=torch.float32, device=logits.device)
-    ids = _empty((t, k), dtype=torch.int64, device=logits.device)
-    rc = lib().sb_route_topk(logits.data_ptr(), dt, t, e, stride if t > 1 else e, pb, k, sc, n_group, topk_group, gs,
-                             renormalize, scale, w.data_ptr(), ids.data_ptr(), _current_stream(dev))
-    if rc:
-        check(rc, "sb_route_topk")
-    return w, ids
+    r = (fp4._HOST or fp4.host()).topk(logits, k, bias, sc, n_group, topk_group, gs, renormalize, scale)
+    if type(r) is int:
+        check(r, "sb_route_topk")
+    return r
 
 
 def expert_order(indices: torch.Tensor, n_experts: int, stream=None) -> ExpertOrder:
     """indices int64 [T, k] -> ExpertOrder. Pairs whose id is outside [0, n_experts) (dropped tokens, padding) are
     left out."""
-    if not indices.is_cuda or indices.dtype != torch.int64 or indices.dim() != 2 or not indices.is_contiguous():
-        raise ValueError("expert_order: indices must be a contiguous CUDA int64 tensor [T, k]")
-    dev = indices.get_device()
-    if stream is not None or dev != _current_device():
+    if stream is not None or indices.get_device() != _current_device():
+        if not indices.is_cuda:
+            raise ValueError("expert_order: indices must be a contiguous CUDA int64 tensor [T, k]")
         with _elsewhere(indices.device, stream):
             return expert_order(indices, n_experts)
-    t, k = indices.shape
-    if k < 1:
-        raise ValueError("expert_order: no slots")
-    pairs = t * k
-    L = lib()
-    need = L.sb_expert_order_workspace_bytes(pairs, n_experts) if pairs > 1024 else 0
-    # one allocation: places, tokens, offsets, the kernels' counts
-    n0, n1, n2, n3 = pairs, pairs, n_experts + 1, need >> 2
-    buf = _empty(n0 + n1 + n2 + n3, dtype=torch.int32, device=indices.device)
-    base = buf.data_ptr()
-    rc = L.sb_expert_order(indices.data_ptr(), t, k, n_experts, base + 4 * (n0 + n1), base + 4 * n0, base,
-                           base + 4 * (n0 + n1 + n2) if need else None, need, _current_stream(dev))
-    if rc:
-        check(rc, "sb_expert_order")
-    places, tokens, offsets, _ = buf.split_with_sizes((n0, n1, n2, n3))
-    return ExpertOrder(offsets, tokens, places.view(t, k))
+    r = (fp4._HOST or fp4.host()).expert_order(indices, n_experts)
+    if type(r) is int:
+        check(r, "sb_expert_order")
+    return ExpertOrder(*r)
