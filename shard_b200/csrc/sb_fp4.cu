@@ -77,7 +77,8 @@ __device__ __noinline__ uint32_t scale_exact(float a, float ts) {
 __device__ __forceinline__ uint32_t scale_code(float a, float ts, float inv6ts, bool mid) {
   if (!mid) return scale_exact(a, ts);
   const float v = a * inv6ts;
-  const uint32_t lo = f32_to_e4m3(v * (1.f - 9.6e-7f)), hi = f32_to_e4m3(v * (1.f + 9.6e-7f));
+  const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(v * (1.f - 9.6e-7f), v * (1.f + 9.6e-7f)), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t lo = two & 0xFFu, hi = two >> 8;
   if (lo == hi) return lo;
   // a against 6 ts times the middle of the two: the product-sum rounds once, so its sign is exact
   const float r = fmaf(-3.f * (e4m3_to_f32(lo) + e4m3_to_f32(hi)), ts, a);
@@ -103,12 +104,23 @@ struct Traits<__nv_bfloat16> {
   static constexpr uint32_t INF = 0x7F80u;
   static constexpr uint32_t BELOW = 0xFFFFu;   // fp32 bits below the type's last one
   static __device__ __forceinline__ float f(uint32_t h) { return __uint_as_float(h << 16); }
+  // of two pairs, the larger magnitudes (their signs are of no account; NaN stays)
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
 };
 template <>
 struct Traits<__half> {
   static constexpr uint32_t INF = 0x7C00u;
   static constexpr uint32_t BELOW = 0x1FFFu;
   static __device__ __forceinline__ float f(uint32_t h) { return __half2float(__ushort_as_half((unsigned short)h)); }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
 };
 
 // 16 consecutive values of a row
@@ -134,10 +146,10 @@ struct Unit {
   }
   // bits of the largest magnitude as fp32 (0x7F800000 and above: not finite)
   __device__ __forceinline__ uint32_t amax() const {
-    uint32_t m = w[0] & 0x7FFF7FFFu;
+    uint32_t m = w[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
-    const uint32_t h = max(m & 0xFFFFu, m >> 16);
+    for (int i = 1; i < 8; ++i) m = Traits<T>::max2(m, w[i]);
+    const uint32_t h = max(m & 0x7FFFu, (m >> 16) & 0x7FFFu);
     return h >= Traits<T>::INF ? 0x7FC00000u : __float_as_uint(Traits<T>::f(h));
   }
   __device__ __forceinline__ float get(int i) const {
@@ -266,12 +278,15 @@ __device__ __forceinline__ uint2 codes_mx(const Unit<T>& u, float inv) {
   return make_uint2(cvt8(a), cvt8(b));
 }
 
+// unit k of a row; VEC: rows of whole units at 16-byte addresses, where a unit behind the row's last is the last again
+// (it adds nothing to the row's largest value, and nothing of it is stored)
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_unit(Unit<T>& u, const T* row, int k, const QuantArgs& a, bool has) {
-  u.zero();
-  if (has && k * 16 < a.k) {
-    if (VEC) u.load(row + (int64_t)k * 16);
-    else u.load_tail(row + (int64_t)k * 16, a.k - k * 16);
+  if (VEC) {
+    u.load(row + (int64_t)min(k, a.k / 16 - 1) * 16);
+  } else {
+    u.zero();
+    if (has && k * 16 < a.k) u.load_tail(row + (int64_t)k * 16, a.k - k * 16);
   }
 }
 
@@ -307,8 +322,9 @@ __global__ void __launch_bounds__(1024) quant_kernel(QuantArgs a) {
     src = a.rows_in[row];
     has = src >= 0 && src < a.src_rows;   // no such row: zeros
   }
+  // (a row without a source reads row 0, and its values count as zeros)
   const T* xr = reinterpret_cast<const T*>(a.x) + (has ? src : 0) * a.stride;
-  const int step = a.wpr * 32;
+  const int step = a.wpr * 32, whole = has ? (a.k + 15) / 16 : 0;   // units with values
   float ts = 1.f;
   if (NV) {
     if (a.ts != nullptr) {
@@ -332,7 +348,7 @@ __global__ void __launch_bounds__(1024) quant_kernel(QuantArgs a) {
         m = lane < a.wpr ? red[rw * a.wpr + lane] : 0u;
         m = __reduce_max_sync(0xffffffffu, m);
       }
-      ts = fmaxf(__fdiv_rn(__uint_as_float(m), 2688.f), 1.17549435e-38f);
+      ts = fmaxf(__fdiv_rn(has ? __uint_as_float(m) : 0.f, 2688.f), 1.17549435e-38f);
       if (live && tr == 0) a.row_ts[row] = ts;
     }
   }
@@ -349,7 +365,7 @@ __global__ void __launch_bounds__(1024) quant_kernel(QuantArgs a) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int k = base + tr + i * step;
-      const uint32_t am = u[i].amax();
+      const uint32_t am = k < whole ? u[i].amax() : 0u;
       uint32_t sc;
       uint2 c = make_uint2(0u, 0u);
       if (NV) {
@@ -365,7 +381,7 @@ __global__ void __launch_bounds__(1024) quant_kernel(QuantArgs a) {
         const uint32_t m = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
         // amax = f 2^e: t = e - 2 for f <= 1.5, else e - 1; biased and floored at 2^-126
         sc = m < F32_INF ? (uint32_t)max((int)((m + 0x3FFFFFu) >> 23) - 2, 1) : 0xFFu;
-        if (m < F32_INF) c = codes_mx<T>(u[i], __uint_as_float((254u - sc) << 23));
+        if (m < F32_INF && k < whole) c = codes_mx<T>(u[i], __uint_as_float((254u - sc) << 23));
         if (k >= a.units) sc = 0u;
         uint32_t w = sc << (8 * ((k >> 1) & 3));
         w |= __shfl_xor_sync(0xffffffffu, w, 2);
@@ -466,14 +482,16 @@ static cudaError_t launch_quant_t(const QuantArgs& q, int v, bool vec, dim3 grid
 
 cudaError_t launch_fp4_quant(const QuantArgs& args, int dtype, cudaStream_t st) {
   QuantArgs q = args;
-  // units in flight per thread: one while the rows do not fill the GPU, else two
-  const int v = q.rows * q.units <= (int64_t)num_sms() * 1024 ? 1 : 2;
-  q.wpr = (q.units + 32 * v - 1) / (32 * v);
+  // Units per thread: one while the rows do not fill the GPU, up to eight at large sizes, where what a warp does once
+  // per row counts (8192 x 7168 NVFP4: two units 49 us, eight 45; 1021 x 7168: 8.5 and 11.4). Two are in flight.
+  const int64_t per = q.rows * q.units / ((int64_t)num_sms() * 3072);
+  const int each = per < 1 ? 1 : (per > 8 ? 8 : (int)per), v = each == 1 ? 1 : 2;
+  q.wpr = (q.units + 32 * each - 1) / (32 * each);
   if (q.wpr > 32) q.wpr = 32;
   const int rpc = q.wpr >= 8 ? 1 : 8 / q.wpr;
   const dim3 grid((unsigned)((q.rows + rpc - 1) / rpc)), block(rpc * q.wpr * 32);
   const int es = dtype == SB_F32 ? 4 : 2;
-  const bool vec = (reinterpret_cast<uintptr_t>(q.x) & 15u) == 0 && (q.stride * es) % 16 == 0 && q.k % 16 == 0;
+  const bool vec = (reinterpret_cast<uintptr_t>(q.x) & 15u) == 0 && (q.stride * es) % 16 == 0 && q.k % 16 == 0 && q.src_rows > 0;
   if (dtype == SB_F32) return fp4::launch_quant_t<float>(q, v, vec, grid, block, st);
   if (dtype == SB_F16) return fp4::launch_quant_t<__half>(q, v, vec, grid, block, st);
   return fp4::launch_quant_t<__nv_bfloat16>(q, v, vec, grid, block, st);

@@ -9,6 +9,8 @@
 // decoded token costs an 8-column tile and ragged expert groups waste little. A CTA takes 128 weight
 // rows; where there are tiles for all SMs, two CTAs form a pair (cta_group::2) that shares the token
 // rows of a 256-row tile, each loading half of them, and one of them issues for both.
+// Where one token tile's weight rows are too few for the SMs, a cluster of CTAs splits K between them and adds its
+// sums through distributed shared memory, in the order of K.
 // Stages hold 256 K: 128 weight rows and the token rows of 128 bytes each, landed by TMA in the 128-byte-
 // swizzled K-major form, and their scale atoms. Roles (352 threads): warp 8 copies codes, warp 9 scales,
 // warp 10 moves scale atoms to tensor memory and issues the MMAs, warps 0-7 read the accumulator (a
@@ -48,6 +50,8 @@ constexpr int SFB_COL = SFA_COL + 16;  // 4 atoms x 8 columns of the tokens (two
 constexpr uint32_t WAIT_LIMIT = 1u << 16;
 constexpr int SMEM_LIMIT = 232448;
 
+enum Form { SINGLE = 0, PAIRED = 1, SPLIT = 2 };
+
 template <bool NV>
 constexpr int SF_BLOCK = NV ? 2048 : 1024;   // a stage's scale atoms of 128 rows
 
@@ -64,6 +68,7 @@ struct Args {
   int sblk;          // row blocks of token scales that a copy brings
   int ksteps;        // MMAs along K (64 values each)
   int vec;           // 16-byte stores to y
+  int split;         // CTAs that share a tile's K
 };
 
 struct Ctl {
@@ -169,7 +174,15 @@ __device__ __forceinline__ uint32_t in_first(uint32_t addr) {
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void pair_sync() {
+// a float of this CTA's shared memory as CTA `rank` of the cluster has it
+__device__ __forceinline__ float peer_float(uint32_t addr, int rank) {
+  uint32_t r;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(r) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
 }
 
@@ -368,8 +381,9 @@ __device__ __forceinline__ void store_chunk(const Args& a, const uint32_t (&d)[3
   }
 }
 
-template <bool NV, bool SWIGLU, bool PAIR, typename T>
+template <bool NV, bool SWIGLU, Form FORM, typename T>
 __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_constant__ Args a) {
+  constexpr bool PAIR = FORM == PAIRED;
   extern __shared__ uint8_t raw[];
   // (both CTAs of a pair round the same address up, so that their stages lie at the same places)
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -380,7 +394,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
   Ctl& c = *reinterpret_cast<Ctl*>(sS + a.stages * s_bytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
-  const int first = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, stride = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+  const int piece = FORM == SPLIT ? (int)blockIdx.x % a.split : 0;
+  const int first = PAIR ? (int)(blockIdx.x >> 1) : FORM == SPLIT ? (int)blockIdx.x / a.split : (int)blockIdx.x;
+  const int stride = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;   // (SPLIT: one tile a cluster)
   const Fp4MmArgs& g = a.g;
 
   if (tid == 0) {
@@ -439,11 +455,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
   }
   fence_before();
   __syncthreads();
-  if constexpr (PAIR) pair_sync();
+  if constexpr (PAIR) cluster_sync();
   fence_after();
   const uint32_t tbase = c.tmem_base;
   const int total = c.tiles[g.mats];
-  const int kstages = (a.ksteps + 3) >> 2;
+  const int kall = (a.ksteps + 3) >> 2;
+  const int kbegin = FORM == SPLIT ? kall * piece / a.split : 0, kend = FORM == SPLIT ? kall * (piece + 1) / a.split : kall;
   volatile int* abortf = &c.abort;
 
   if (warp == CODE_WARP || warp == SCALE_WARP) {
@@ -461,7 +478,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
         const int wrow = t.mat * g.n + t.n0 + rank * 128, arow = t.row0 + t.t0 + rank * half;
         const int wblk = t.mat * ((g.n + 127) >> 7) + (t.n0 >> 7) + rank;
         const uint32_t bytes = (PAIR ? 2u : 1u) * (codes ? A_BYTES + nbox * a.box * 128 : s_bytes);
-        for (int k = 0; k < kstages; ++k, ++it) {
+        for (int k = kbegin; k < kend; ++k, ++it) {
           if (!wait(abortf, empty0 + 8 * s, ph)) {
             ok = false;
             break;
@@ -516,7 +533,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
           }
           fence_after();
           issue<NV, PAIR, decltype(blocks)::value, decltype(whole)::value>(tbase, acc, sfb, ad0 + s * (A_BYTES >> 4),
-                                                                           bd0 + s * b_step, sd0 + s * s_step, id, ktail, k == 0);
+                                                                           bd0 + s * b_step, sd0 + s * s_step, id, ktail, k == kbegin);
           commit_to<PAIR>(empty0 + 8 * s);
           if (++s == (uint32_t)a.stages) {
             s = 0;
@@ -524,8 +541,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
           }
         };
         auto tile = [&](auto blocks) {
-          for (int k = 0; ok && k < kfull; ++k) stage(blocks, std::true_type{}, k);
-          if (ok && ktail > 0) stage(blocks, std::false_type{}, kfull);
+          for (int k = kbegin; ok && k < min(kend, kfull); ++k) stage(blocks, std::true_type{}, k);
+          if (ok && kfull < kend) stage(blocks, std::false_type{}, kfull);
         };
         if ((t.t0 & 127) + t.cnt > 128) tile(std::integral_constant<int, 2>{});
         else tile(std::integral_constant<int, 1>{});
@@ -568,6 +585,18 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
       __syncwarp();
       if (!warp_wait(abortf, smem_addr(&c.accfull[q]), (n >> 1) & 1u)) break;
       fence_after();
+      if constexpr (FORM == SPLIT) {
+        // the products have read all stages: their place takes this piece's sums, [token][row]
+        float* part = reinterpret_cast<float*>(base);
+        for (int ch = half; ch * 32 < t.cnt; ch += 2) {
+          uint32_t d[32];
+          ld32(acc + ch * 32, d);
+          ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) part[(ch * 32 + j) * 128 + (warp & 3) * 32 + lane] = __uint_as_float(d[j]);
+        }
+        break;
+      }
       bool held = true;   // this warp has yet to read the accumulator's last chunk
       for (int ch = half, j = 0; ch * 32 < t.cnt; ch += 2, ++j) {
         uint32_t d[32];
@@ -597,7 +626,27 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
   }
   fence_before();
   __syncthreads();
-  if constexpr (PAIR) pair_sync();   // the other CTA's products read this one's shared memory to the end
+  if constexpr (FORM == SPLIT) {
+    // each CTA adds and stores its share of the tokens
+    cluster_sync();
+    if (first < total) {
+      const Tile t = tile_at<false>(a, c, first);
+      const uint32_t part = smem_addr(base);
+      const int mine = (t.cnt - piece + a.split - 1) / a.split * 128;
+      for (int i = tid; i < mine; i += NTHREADS) {
+        const int col = piece + (i >> 7) * a.split, r = i & 127, row = t.n0 + r;
+        float v = 0.f;
+        for (int p = 0; p < a.split; ++p) v += peer_float(part + (col * 128 + r) * 4, p);
+        if (row < g.n) {
+          float s = g.a_ts ? g.a_ts[g.a_ts_row ? t.t0 + col : 0] : 1.f;
+          if (g.w_ts) s *= g.w_ts[g.w_ts_n == 0 ? row : 0];
+          reinterpret_cast<T*>(g.y)[(int64_t)(t.t0 + col) * g.ldy + row] = to_out<T>(v * s);
+        }
+      }
+    }
+    cluster_sync();   // the others have read this CTA's sums
+  }
+  if constexpr (PAIR) cluster_sync();   // the other CTA's products read this one's shared memory to the end
   if (warp == MMA_WARP) {
     fence_after();
     if constexpr (PAIR) {
@@ -653,9 +702,9 @@ static cudaError_t scale_map(CUtensorMap* map, const void* base, uint64_t blocks
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-template <bool NV, bool SWIGLU, bool PAIR, typename T>
+template <bool NV, bool SWIGLU, fp4mm::Form FORM, typename T>
 static cudaError_t launch_mm(const fp4mm::Args& a, int grid, size_t smem, cudaStream_t st) {
-  const auto kernel = fp4mm::fp4_mm_kernel<NV, SWIGLU, PAIR, T>;
+  const auto kernel = fp4mm::fp4_mm_kernel<NV, SWIGLU, FORM, T>;
   // the limit belongs to the kernel on one device: set once for each
   static std::atomic<uint64_t> done{0};
   int dev = 0;
@@ -676,25 +725,27 @@ static cudaError_t launch_mm(const fp4mm::Args& a, int grid, size_t smem, cudaSt
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.x = FORM == fp4mm::PAIRED ? 2 : a.split;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = PAIR ? 2 : 1;
+  cfg.numAttrs = FORM == fp4mm::SINGLE ? 1 : 2;
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-template <bool PAIR, typename T>
+template <fp4mm::Form FORM, typename T>
 static cudaError_t launch_mm_t(const fp4mm::Args& a, int grid, size_t smem, cudaStream_t st) {
-  if (a.g.nv) return a.g.swiglu ? launch_mm<true, true, PAIR, T>(a, grid, smem, st) : launch_mm<true, false, PAIR, T>(a, grid, smem, st);
-  return a.g.swiglu ? launch_mm<false, true, PAIR, T>(a, grid, smem, st) : launch_mm<false, false, PAIR, T>(a, grid, smem, st);
+  if constexpr (FORM != fp4mm::SPLIT) {
+    if (a.g.swiglu) return a.g.nv ? launch_mm<true, true, FORM, T>(a, grid, smem, st) : launch_mm<false, true, FORM, T>(a, grid, smem, st);
+  }
+  return a.g.nv ? launch_mm<true, false, FORM, T>(a, grid, smem, st) : launch_mm<false, false, FORM, T>(a, grid, smem, st);
 }
 
-template <bool PAIR>
-static cudaError_t launch_mm_p(const fp4mm::Args& a, int dtype, int grid, size_t smem, cudaStream_t st) {
-  if (dtype == SB_F32) return launch_mm_t<PAIR, float>(a, grid, smem, st);
-  if (dtype == SB_F16) return launch_mm_t<PAIR, __half>(a, grid, smem, st);
-  return launch_mm_t<PAIR, __nv_bfloat16>(a, grid, smem, st);
+template <fp4mm::Form FORM>
+static cudaError_t launch_mm_f(const fp4mm::Args& a, int dtype, int grid, size_t smem, cudaStream_t st) {
+  if (dtype == SB_F32) return launch_mm_t<FORM, float>(a, grid, smem, st);
+  if (dtype == SB_F16) return launch_mm_t<FORM, __half>(a, grid, smem, st);
+  return launch_mm_t<FORM, __nv_bfloat16>(a, grid, smem, st);
 }
 
 cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
@@ -723,6 +774,11 @@ cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
   // Pairs where tiles of full width are many: they halve the token bytes per product, which is what bounds
   // those; narrow tiles are bound by the weights, which pairs do not share.
   const bool pair = a.nt >= 128 && g.m >= 128 * (int64_t)g.mats && tiles >= 2 * sms;
+  // K is split, for one token tile, as far as the SMs go and every piece keeps two stages (one token against 4096 x 8192:
+  // 12.0 us whole, see the split's time at the head of this file).
+  a.split = 1;
+  if (g.offsets == nullptr && tt == 1)
+    while (a.split < 8 && tiles * a.split * 2 <= sms && (a.ksteps + 3) / 4 >= a.split * 4) a.split *= 2;
   a.box = g.offsets ? BOX : (pair ? a.nt / 2 : a.nt);
   a.b_bytes = (pair ? a.nt / 2 : a.nt) * 128;
   a.sblk = a.nt > 128 ? 2 : 1;
@@ -740,8 +796,9 @@ cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
   if (e == cudaSuccess) e = scale_map(&a.map_ws, g.w_s, (uint64_t)g.mats * nb, (uint64_t)atoms, 1, along);
   if (e == cudaSuccess) e = scale_map(&a.map_as, g.a_s, a_blocks, (uint64_t)atoms, (uint32_t)a.sblk, along);
   if (e != cudaSuccess) return e;
-  if (pair) return launch_mm_p<true>(a, dtype, sms & ~1, smem, st);
-  return launch_mm_p<false>(a, dtype, (int)(tiles < sms ? tiles : sms), smem, st);
+  if (pair) return launch_mm_f<PAIRED>(a, dtype, sms & ~1, smem, st);
+  if (a.split > 1) return launch_mm_f<SPLIT>(a, dtype, (int)tiles * a.split, smem, st);
+  return launch_mm_f<SINGLE>(a, dtype, (int)(tiles < sms ? tiles : sms), smem, st);
 }
 
 cudaError_t fp4_mm_error(int* host_out, cudaStream_t st) {

@@ -138,6 +138,12 @@ def test_quant_strides_gather_and_shape(fmt):
     rows = torch.tensor([3, 3, 39, -1, 0, 40, 17], dtype=torch.int32)
     want = torch.stack([base[r].cpu() if 0 <= r < 40 else torch.zeros(333, dtype=torch.bfloat16) for r in rows.tolist()])
     _check_quant(want, fp4.quant(base, fmt, rows=rows.cuda()), fmt)
+    wide = base[:, :320].contiguous()         # rows of whole 16-byte vectors, and sources of NaN beside a missing row
+    wide[0] = math.nan
+    want = torch.stack([wide[r].cpu() if 0 <= r < 40 else torch.zeros(320, dtype=torch.bfloat16) for r in rows.tolist()])
+    _check_quant(want, fp4.quant(wide, fmt, rows=rows.cuda()), fmt)
+    none = fp4.quant(wide[:0], fmt, rows=rows.cuda())      # no row exists
+    assert bool((fp4.dequant(none) == 0).all())
 
 
 @gpu
