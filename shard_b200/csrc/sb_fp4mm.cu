@@ -69,6 +69,7 @@ struct Args {
   int ksteps;        // MMAs along K (64 values each)
   int vec;           // 16-byte stores to y
   int split;         // CTAs that share a tile's K
+  int ahead;         // stages of weights brought to L2 before the kernel before this one has ended
 };
 
 struct Ctl {
@@ -135,6 +136,13 @@ __device__ __forceinline__ void commit_to(uint32_t bar) {
         : "memory");
   else
     commit(bar);
+}
+
+// a box of codes into L2
+__device__ __forceinline__ void prefetch_2d(const CUtensorMap* map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1)
+               : "memory");
 }
 
 // tensor copies into this CTA's shared memory; a pair's complete on the first CTA's barrier
@@ -427,6 +435,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
     prefetch_map(&a.map_a);
     prefetch_map(&a.map_ws);
     prefetch_map(&a.map_as);
+    // The first weights on their way to L2 while the kernel before this one ends. Nothing is read yet: what it
+    // writes, were it these weights, is still seen by the copies behind the wait.
+    if (FORM != PAIRED && g.offsets == nullptr && a.ahead > 0) {
+      const int nb = (g.n + 127) >> 7, tile = FORM == SPLIT ? (int)blockIdx.x / a.split : (int)blockIdx.x;
+      const int all = (a.ksteps + 3) >> 2, k0 = FORM == SPLIT ? all * ((int)blockIdx.x % a.split) / a.split : 0;
+      for (int k = k0; k < min(all, k0 + a.ahead); ++k) prefetch_2d(&a.map_w, k * 128, (tile % nb) * 128);
+    }
   }
   pdl_wait();
   pdl_trigger();
@@ -779,6 +794,8 @@ cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
   a.split = 1;
   if (g.offsets == nullptr && tt == 1)
     while (a.split < 8 && tiles * a.split * 2 <= sms && (a.ksteps + 3) / 4 >= a.split * 4) a.split *= 2;
+  // (one token tile: a CTA's first tile is its own row block, whose stages it all reads)
+  a.ahead = g.offsets == nullptr && tt == 1 ? ((a.ksteps + 3) / 4 + a.split - 1) / a.split : 0;
   a.box = g.offsets ? BOX : (pair ? a.nt / 2 : a.nt);
   a.b_bytes = (pair ? a.nt / 2 : a.nt) * 128;
   a.sblk = a.nt > 128 ? 2 : 1;
