@@ -306,10 +306,13 @@ __device__ __forceinline__ void load_unit(Unit<T>& u, const T* row, int k, const
 
 // A row's wpr warps take its units (16 values a thread) in turn, V at a time with their loads issued together. With
 // one tensor scale per row the row is read twice, first for its largest value, then, from L1, for its
-// codes.
+// codes. (Blocks that take rows in turn, as many as fit at once: 45 us for 8192 x 7168 NVFP4; a block for every few
+// rows: 41.)
+constexpr int QUANT_WARPS = 8;
+
 template <typename T, bool NV, int V, bool VEC>
-__global__ void __launch_bounds__(1024) quant_kernel(QuantArgs a) {
-  __shared__ uint32_t red[32];
+__global__ void __launch_bounds__(QUANT_WARPS * 32, 4) quant_kernel(QuantArgs a) {
+  __shared__ uint32_t red[QUANT_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rpc = (blockDim.x >> 5) / a.wpr;
   const int rw = warp / a.wpr, tr = threadIdx.x - rw * a.wpr * 32;
@@ -358,7 +361,8 @@ __global__ void __launch_bounds__(1024) quant_kernel(QuantArgs a) {
       m = __reduce_max_sync(0xffffffffu, m);
       if (a.wpr > 1) {
         if (lane == 0) red[warp] = m;
-        __syncthreads();
+        // the row's warps alone
+        asm volatile("barrier.sync %0, %1;\n" ::"r"(rw + 1), "r"(step) : "memory");
         m = lane < a.wpr ? red[rw * a.wpr + lane] : 0u;
         m = __reduce_max_sync(0xffffffffu, m);
       }
@@ -500,11 +504,11 @@ cudaError_t launch_fp4_quant(const QuantArgs& args, int dtype, cudaStream_t st) 
   QuantArgs q = args;
   // Units per thread: one while the rows do not fill the GPU, up to eight at large sizes, where what a warp does once
   // per row counts (8192 x 7168 NVFP4: two units 49 us, eight 45; 1021 x 7168: 8.5 and 11.4). Two are in flight.
-  const int64_t per = q.rows * q.units / ((int64_t)num_sms() * 3072);
+  const int64_t per = q.rows * q.units / ((int64_t)num_sms() * 1536);
   const int each = per < 1 ? 1 : (per > 8 ? 8 : (int)per), v = each == 1 ? 1 : 2;
   q.wpr = (q.units + 32 * each - 1) / (32 * each);
-  if (q.wpr > 32) q.wpr = 32;
-  const int rpc = q.wpr >= 8 ? 1 : 8 / q.wpr;
+  if (q.wpr > fp4::QUANT_WARPS) q.wpr = fp4::QUANT_WARPS;
+  const int rpc = fp4::QUANT_WARPS / q.wpr;
   const dim3 grid((unsigned)((q.rows + rpc - 1) / rpc)), block(rpc * q.wpr * 32);
   const int es = dtype == SB_F32 ? 4 : 2;
   const bool vec = (reinterpret_cast<uintptr_t>(q.x) & 15u) == 0 && (q.stride * es) % 16 == 0 && q.k % 16 == 0 && q.src_rows > 0;
