@@ -72,7 +72,8 @@ SIGNATURES = {
     "sb_selftest_formats": (_int, [_vp, _vp]),
     "sb_debug_set_wait_limit": (_int, [_i64]),
     "sb_fp4_scale_bytes": (_sz, [_int, _i64, _i64, _i64, _i64]),
-    "sb_fp4_quant": (_int, [_int, _vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
+    "sb_fp4_quant_workspace_bytes": (_sz, [_int, _i64, _i64, _i64]),
+    "sb_fp4_quant": (_int, [_int, _vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "sb_fp4_dequant": (_int, [_int, _vp, _vp, _vp, _int, _i64, _i64, _vp, _int, _vp]),
     "sb_fp4_tile_scales": (_int, [_int, _vp, _vp, _i64, _i64, _i64, _vp]),
     "sb_fp4_gemm": (_int, [_int, _vp, _vp, _vp, _int, _i64, _vp, _vp, _vp, _int, _i64, _i64, _vp, _int, _i64, _vp]),

@@ -1130,9 +1130,16 @@ size_t sb_fp4_scale_bytes(int fmt, int64_t n_mat, int64_t rows, int64_t k, int64
   return (size_t)fp4_blocks(n_mat, rows, groups) * (size_t)fp4_atoms(fmt, k) * 512;
 }
 
+size_t sb_fp4_quant_workspace_bytes(int fmt, int64_t src_rows, int64_t rows, int64_t k) {
+  if (!fp4_fmt(fmt) || src_rows < 0 || src_rows > FP4_MAX_ROWS || rows < 0 || rows > FP4_MAX_ROWS || k < 1 || k > FP4_MAX_K)
+    return 0;
+  return sb::fp4_quant_workspace(src_rows, rows, fp4_kp(k) / 2, fp4_atoms(fmt, k));
+}
+
 int sb_fp4_quant(int fmt, const void* x, int dtype, int64_t src_rows, int64_t k, int64_t row_stride,
                  const int32_t* rows_in, int64_t rows, const float* tensor_scale, const int32_t* offsets,
-                 int64_t groups, void* codes, void* scales, float* row_scale, void* stream) {
+                 int64_t groups, void* codes, void* scales, float* row_scale, void* workspace, size_t workspace_bytes,
+                 void* stream) {
   if (int rc = fp4_common("fp4_quant", fmt, dtype, rows, k)) return rc;
   if (src_rows < 0 || src_rows > FP4_MAX_ROWS || row_stride < 0)
     return fail(SB_ERR_SHAPE, "fp4_quant: src_rows=%lld row_stride=%lld", (long long)src_rows, (long long)row_stride);
@@ -1147,6 +1154,11 @@ int sb_fp4_quant(int fmt, const void* x, int dtype, int64_t src_rows, int64_t k,
     return fail(SB_ERR_ARG, "fp4_quant: NULL pointer");
   if (!aligned16(codes) || !aligned16(scales)) return fail(SB_ERR_ARG, "fp4_quant: codes and scales must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(x) % (dtype == SB_F32 ? 4 : 2)) return fail(SB_ERR_ARG, "fp4_quant: x is misaligned");
+  const size_t need = rows_in ? sb_fp4_quant_workspace_bytes(fmt, src_rows, rows, k) : 0;
+  if (need == 0) workspace = nullptr;
+  if (workspace && workspace_bytes < need)
+    return fail(SB_ERR_WORKSPACE, "fp4_quant: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  if (!aligned16(workspace)) return fail(SB_ERR_ARG, "fp4_quant: the workspace must be 16-byte aligned");
   sb::QuantArgs q = {};
   q.x = x;
   q.stride = row_stride;
@@ -1165,7 +1177,7 @@ int sb_fp4_quant(int fmt, const void* x, int dtype, int64_t src_rows, int64_t k,
   q.row_bytes = fp4_kp(k) / 2;
   q.scales = (uint8_t*)scales;
   q.atoms = fp4_atoms(fmt, k);
-  return cuda_check(sb::launch_fp4_quant(q, dtype, (cudaStream_t)stream), "fp4_quant");
+  return cuda_check(sb::launch_fp4_quant(q, dtype, workspace, (cudaStream_t)stream), "fp4_quant");
 }
 
 int sb_fp4_dequant(int fmt, const void* codes, const void* scales, const float* ts, int ts_per_row, int64_t rows,
@@ -1307,8 +1319,7 @@ int sb_route_topk(const void* logits, int dtype, int64_t tokens, int64_t n_exper
 
 size_t sb_expert_order_workspace_bytes(int64_t pairs, int64_t n_experts) {
   if (pairs < 0 || pairs > INT32_MAX || n_experts < 1 || n_experts > 1024) return 0;
-  const int64_t b = sb::order_blocks(pairs);
-  return b > 1 ? (size_t)b * (size_t)n_experts * sizeof(int32_t) : 0;
+  return (size_t)sb::order_counts(pairs) * (size_t)n_experts * sizeof(int32_t);
 }
 
 int sb_expert_order(const int64_t* indices, int64_t tokens, int topk, int64_t n_experts, int32_t* offsets,

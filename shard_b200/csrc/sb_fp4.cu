@@ -304,6 +304,18 @@ __device__ __forceinline__ void load_unit(Unit<T>& u, const T* row, int k, const
   }
 }
 
+// The row's place among the scale atoms' rows, or -1 where it is none of the operand's (a whole warp's call).
+__device__ __forceinline__ int64_t place(const QuantArgs& a, int64_t row, int lane) {
+  if (row >= a.rows) return -1;
+  if (a.offsets == nullptr) return row;
+  int g = 0;   // the row's group: how many end at or before it
+  for (int i = lane; i < a.groups; i += 32) g += a.offsets[i + 1] <= row ? 1 : 0;
+  g = __reduce_add_sync(0xffffffffu, g);
+  if (g >= a.groups) return -1;
+  const int64_t o = a.offsets[g], pos = ((o >> 7) + g) * 128 + (row - o);
+  return o < 0 || o > row || pos >= a.blocks * 128 ? -1 : pos;
+}
+
 // A row's wpr warps take its units (16 values a thread) in turn, V at a time with their loads issued together. With
 // one tensor scale per row the row is read twice, first for its largest value, then, from L1, for its
 // codes. (Blocks that take rows in turn, as many as fit at once: 45 us for 8192 x 7168 NVFP4; a block for every few
@@ -320,20 +332,8 @@ __global__ void __launch_bounds__(QUANT_WARPS * 32, 4) quant_kernel(QuantArgs a)
   pdl_wait();
   pdl_trigger();
   int64_t src = row;
-  int64_t pos = row;    // the row's place among the scale atoms' rows
-  bool live = row < a.rows;
-  if (a.offsets != nullptr) {
-    // group of the row: how many groups end at or before it
-    int g = 0;
-    for (int i = lane; i < a.groups; i += 32) g += a.offsets[i + 1] <= row ? 1 : 0;
-    g = __reduce_add_sync(0xffffffffu, g);
-    live = live && g < a.groups;
-    if (live) {
-      const int64_t o = a.offsets[g];
-      pos = ((o >> 7) + g) * 128 + (row - o);
-      if (o < 0 || o > row || pos >= a.blocks * 128) live = false;
-    }
-  }
+  const int64_t pos = place(a, row, lane);
+  const bool live = pos >= 0;
   bool has = live;
   if (live && a.rows_in != nullptr) {
     src = a.rows_in[row];
@@ -377,7 +377,9 @@ __global__ void __launch_bounds__(QUANT_WARPS * 32, 4) quant_kernel(QuantArgs a)
   Leans ln = {0u, 0u};
   if (NV) ln = leans<T>(ts, lane);
   uint8_t* cr = a.codes + row * a.row_bytes;
-  uint8_t* sr = a.scales + ((pos >> 7) * a.atoms) * 512 + (pos & 31) * 16 + ((pos >> 5) & 3) * 4;
+  uint8_t* sr = a.flat ? a.scales + row * a.atoms * 4
+                       : a.scales + ((pos >> 7) * a.atoms) * 512 + (pos & 31) * 16 + ((pos >> 5) & 3) * 4;
+  const int64_t atom = a.flat ? 4 : 512;
   for (int base = 0; base < a.units; base += step * V) {
     Unit<T> u[V];
 #pragma unroll
@@ -396,7 +398,7 @@ __global__ void __launch_bounds__(QUANT_WARPS * 32, 4) quant_kernel(QuantArgs a)
         uint32_t w = sc << (8 * (k & 3));
         w |= __shfl_xor_sync(0xffffffffu, w, 1);
         w |= __shfl_xor_sync(0xffffffffu, w, 2);
-        if (k < a.units && (k & 3) == 0) *reinterpret_cast<uint32_t*>(sr + (int64_t)(k >> 2) * 512) = w;
+        if (k < a.units && (k & 3) == 0) *reinterpret_cast<uint32_t*>(sr + (k >> 2) * atom) = w;
       } else {
         const uint32_t m = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
         // amax = f 2^e: t = e - 2 for f <= 1.5, else e - 1; biased and floored at 2^-126
@@ -406,11 +408,42 @@ __global__ void __launch_bounds__(QUANT_WARPS * 32, 4) quant_kernel(QuantArgs a)
         uint32_t w = sc << (8 * ((k >> 1) & 3));
         w |= __shfl_xor_sync(0xffffffffu, w, 2);
         w |= __shfl_xor_sync(0xffffffffu, w, 4);
-        if (k < a.units && (k & 7) == 0) *reinterpret_cast<uint32_t*>(sr + (int64_t)(k >> 3) * 512) = w;
+        if (k < a.units && (k & 7) == 0) *reinterpret_cast<uint32_t*>(sr + (k >> 3) * atom) = w;
       }
       if (k < a.units) *reinterpret_cast<uint2*>(cr + (int64_t)k * 8) = c;
     }
   }
+}
+
+// Rows of an operand copied from the quantised source rows (codes, scale words row by row, tensor scales), a warp a row.
+__global__ void __launch_bounds__(256) gather_kernel(QuantArgs a, const uint8_t* __restrict__ codes,
+                                                     const uint32_t* __restrict__ words, const float* __restrict__ ts) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  pdl_wait();
+  pdl_trigger();
+  const int64_t pos = place(a, row, lane);
+  if (pos < 0) return;
+  const int64_t src = a.rows_in[row];
+  const bool has = src >= 0 && src < a.src_rows;
+  const uint4* from = reinterpret_cast<const uint4*>(codes + (has ? src : 0) * a.row_bytes);
+  uint4* to = reinterpret_cast<uint4*>(a.codes + row * a.row_bytes);
+  const int n = (int)(a.row_bytes / 16);
+#pragma unroll 4
+  for (int i = lane; i < n; i += 32) {
+    const uint4 v = __ldg(from + i);
+    to[i] = has ? v : make_uint4(0u, 0u, 0u, 0u);
+  }
+  const uint32_t* w = words + (has ? src : 0) * a.atoms;
+  uint8_t* sr = a.scales + ((pos >> 7) * a.atoms) * 512 + (pos & 31) * 16 + ((pos >> 5) & 3) * 4;
+  // (a missing row's scales are those of zeros: 0, or 2^-126)
+  const int nb = a.nv ? a.units : a.units / 2;
+#pragma unroll 4
+  for (int i = lane; i < a.atoms; i += 32) {
+    const uint32_t none = a.nv ? 0u : 0x01010101u >> (8 * max(0, 4 - (nb - 4 * i)));
+    *reinterpret_cast<uint32_t*>(sr + (int64_t)i * 512) = has ? __ldg(w + i) : none;
+  }
+  if (a.row_ts != nullptr && lane == 0) a.row_ts[row] = has ? ts[src] : 1.17549435e-38f;
 }
 
 template <typename T>
@@ -500,7 +533,7 @@ static cudaError_t launch_quant_t(const QuantArgs& q, int v, bool vec, dim3 grid
 
 }  // namespace fp4
 
-cudaError_t launch_fp4_quant(const QuantArgs& args, int dtype, cudaStream_t st) {
+static cudaError_t launch_rows(const QuantArgs& args, int dtype, cudaStream_t st) {
   QuantArgs q = args;
   // Units per thread: one while the rows do not fill the GPU, up to eight at large sizes, where what a warp does once
   // per row counts (8192 x 7168 NVFP4: two units 49 us, eight 45; 1021 x 7168: 8.5 and 11.4). Two are in flight.
@@ -515,6 +548,30 @@ cudaError_t launch_fp4_quant(const QuantArgs& args, int dtype, cudaStream_t st) 
   if (dtype == SB_F32) return fp4::launch_quant_t<float>(q, v, vec, grid, block, st);
   if (dtype == SB_F16) return fp4::launch_quant_t<__half>(q, v, vec, grid, block, st);
   return fp4::launch_quant_t<__nv_bfloat16>(q, v, vec, grid, block, st);
+}
+
+// A gather that takes each source row twice or more quantises the source once and copies (2048 rows of 4096, each
+// taken eight times, and their w13 product: 246 us without, 221 with).
+size_t fp4_quant_workspace(int64_t src_rows, int64_t rows, int64_t row_bytes, int64_t atoms) {
+  return rows >= 2 * src_rows && src_rows > 0 ? (size_t)(src_rows * (row_bytes + 4 * atoms + 4)) : 0;
+}
+
+cudaError_t launch_fp4_quant(const QuantArgs& a, int dtype, void* workspace, cudaStream_t st) {
+  if (a.rows_in == nullptr || workspace == nullptr) return launch_rows(a, dtype, st);
+  QuantArgs q = a;
+  q.rows = a.src_rows;
+  q.rows_in = nullptr;
+  q.offsets = nullptr;
+  q.codes = (uint8_t*)workspace;
+  q.scales = q.codes + a.src_rows * a.row_bytes;
+  q.row_ts = reinterpret_cast<float*>(q.scales + a.src_rows * a.atoms * 4);
+  q.flat = 1;
+  const cudaError_t e = launch_rows(q, dtype, st);
+  if (e != cudaSuccess) return e;
+  QuantArgs g = a;
+  if (a.ts != nullptr) g.row_ts = nullptr;
+  return launch_pdl(fp4::gather_kernel, dim3((unsigned)((a.rows + 7) / 8)), dim3(256), 0, st, g, q.codes,
+                    (const uint32_t*)q.scales, q.row_ts);
 }
 
 template <typename T>

@@ -26,6 +26,7 @@ struct QuantArgs {
   int64_t row_bytes;
   uint8_t* scales;
   int64_t atoms;
+  int flat;                  // scale words row by row, not in atoms
   int wpr;                   // warps per row (set by the launch)
 };
 
@@ -81,16 +82,18 @@ struct OrderArgs {
   int64_t pairs;
   int topk, experts;
   int blocks;                // set by the launch
-  int32_t* hist;             // [blocks][experts], blocks > 1
+  int32_t* hist;             // [order_counts][experts]
   int32_t* offsets;          // [experts + 1]
   int32_t* tokens;           // [pairs]
   int32_t* places;           // [pairs]
 };
 
-int64_t order_blocks(int64_t pairs);
+int64_t order_counts(int64_t pairs);   // blocks whose counts go through memory, 0: none
 cudaError_t launch_topk(const TopkArgs& a, int dtype, cudaStream_t st);
 cudaError_t launch_expert_order(const OrderArgs& a, cudaStream_t st);
-cudaError_t launch_fp4_quant(const QuantArgs& a, int dtype, cudaStream_t st);
+// bytes of the copy of a gather's quantised source rows, 0 where none is made
+size_t fp4_quant_workspace(int64_t src_rows, int64_t rows, int64_t row_bytes, int64_t atoms);
+cudaError_t launch_fp4_quant(const QuantArgs& a, int dtype, void* workspace, cudaStream_t st);
 cudaError_t launch_fp4_dequant(const DequantArgs& a, int dtype, cudaStream_t st);
 cudaError_t launch_fp4_tile_scales(const uint8_t* src, uint8_t* dst, int64_t mats, int64_t n, int64_t nb, cudaStream_t st);
 cudaError_t launch_fp4_mm(const Fp4MmArgs& a, int dtype, cudaStream_t st);

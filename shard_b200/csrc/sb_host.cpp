@@ -122,8 +122,12 @@ PyObject* quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int64_t end = p * ((k + 31) / 32) * 16, atoms_end = end + (int64_t)sb_fp4_scale_bytes(fmt, 1, p, k, groups);
   Tensor buf = empty({per_row ? atoms_end + 4 * p : atoms_end}, at::kByte, x);
   uint8_t* base = buf.data_ptr<uint8_t>();
+  const size_t need = rows ? sb_fp4_quant_workspace_bytes(fmt, m, p, k) : 0;
+  Tensor ws;
+  if (need) ws = empty({(int64_t)need}, at::kByte, x);
   const int rc = sb_fp4_quant(fmt, z.data_ptr(), dt, m, k, m > 1 ? z.stride(0) : k, rp, p, tp, op, groups, base, base + end,
-                              per_row ? reinterpret_cast<float*>(base + atoms_end) : nullptr, current_stream(x));
+                              per_row ? reinterpret_cast<float*>(base + atoms_end) : nullptr, need ? ws.data_ptr() : nullptr, need,
+                              current_stream(x));
   if (rc != SB_OK) return status(rc);
   const int64_t lead = rows ? 1 : x.dim() - 1;
   THPObjectPtr shape(PyTuple_New(lead));

@@ -9,7 +9,8 @@
 // scores of all experts took 20 us of 38). So a selection never hangs on how an exponential rounds.
 //
 // order_kernel: a stable counting sort of the pairs by expert, in blocks of 2048 pairs, no atomics
-// on anything the outputs depend on.
+// on anything the outputs depend on. Up to eight blocks form a cluster that reads one another's counts in
+// shared memory; more leave them in memory by a kernel before.
 #include <cfloat>
 
 #include "sb_device.cuh"
@@ -513,7 +514,7 @@ __global__ void __launch_bounds__(128) topk_kernel(TopkArgs a) {
 // ── expert order ───────────────────────────────────────────────────────────────────────────────
 constexpr int OSTEP = 8;            // pairs of a thread
 constexpr int OSEG = 32 * OSTEP;    // consecutive pairs of a warp
-constexpr int OW = 8;               // warps of a block (one block of 32 for 8192 pairs: 16 us, four of 8: 6)
+constexpr int OW = 8;               // warps of a block (one block of 32 for 8192 pairs: 16 us, four of 8: 7)
 constexpr int OBLOCK = OW * OSEG;
 
 // The warp's pairs' experts (-1: none), all loads in flight at once, and cnt[w][e], the pairs of expert e
@@ -550,8 +551,22 @@ __global__ void __launch_bounds__(OW * 32) order_count_kernel(OrderArgs a) {
   }
 }
 
+constexpr int OCLUSTER = 8;         // blocks of a cluster at most
+
+__device__ __forceinline__ int peer_int(const int* p, int rank) {
+  uint32_t r;
+  int v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.b32 %0, [%1];\n" : "=r"(v) : "r"(r) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
+}
+
+template <bool CLUSTER>
 __global__ void __launch_bounds__(OW * 32) order_kernel(OrderArgs a) {
-  extern __shared__ int cnt[];               // [OW][experts] counts, then [experts] all pairs of each expert
+  extern __shared__ int cnt[];               // [OW][experts] counts, [experts] all pairs of each, [experts] this block's
   __shared__ int wsum[OW];
   __shared__ int total;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -560,14 +575,33 @@ __global__ void __launch_bounds__(OW * 32) order_kernel(OrderArgs a) {
   int ex[OSTEP];
   // After order_count_kernel this starts while that one runs, which in turn began when the ids were written: they
   // can be read before the wait, the counts in memory after it.
-  if (a.blocks == 1) pdl_wait();
+  if (CLUSTER || a.blocks == 1) pdl_wait();
   segment(a, cnt, p0, ex);
-  if (a.blocks > 1) pdl_wait();
+  if (!CLUSTER && a.blocks > 1) pdl_wait();
   pdl_trigger();
+  if constexpr (CLUSTER) {
+    int* mine = all + a.experts;
+    for (int e = threadIdx.x; e < a.experts; e += OW * 32) {
+      int s = 0;
+#pragma unroll
+      for (int w = 0; w < OW; ++w) s += cnt[w * a.experts + e];
+      mine[e] = s;
+    }
+    cluster_sync();
+  }
   // counts become each segment's first place after the expert's base (below)
   for (int e = threadIdx.x; e < a.experts; e += OW * 32) {
     int sum = 0, at = 0;
-    if (a.blocks > 1) {
+    if constexpr (CLUSTER) {
+#pragma unroll
+      for (int b = 0; b < OCLUSTER; ++b) {
+        if (b < a.blocks) {
+          const int v = peer_int(all + a.experts + e, b);
+          sum += v;
+          at += b < (int)blockIdx.x ? v : 0;
+        }
+      }
+    } else if (a.blocks > 1) {
 #pragma unroll 16
       for (int b = 0; b < a.blocks; ++b) {
         const int v = a.hist[(int64_t)b * a.experts + e];
@@ -584,6 +618,7 @@ __global__ void __launch_bounds__(OW * 32) order_kernel(OrderArgs a) {
     }
     all[e] = a.blocks > 1 ? sum : here;
   }
+  if constexpr (CLUSTER) cluster_sync();   // all counts are read before a block ends
   __syncthreads();
   // exclusive scan of the experts' totals
   constexpr int PER = 1024 / (OW * 32);   // experts a thread
@@ -674,17 +709,38 @@ cudaError_t launch_topk(const TopkArgs& args, int dtype, cudaStream_t st) {
 }
 
 int64_t order_blocks(int64_t pairs) { return (pairs + topk::OBLOCK - 1) / topk::OBLOCK; }
+int64_t order_counts(int64_t pairs) {
+  const int64_t b = order_blocks(pairs);
+  return b > topk::OCLUSTER ? b : 0;
+}
 
 cudaError_t launch_expert_order(const OrderArgs& args, cudaStream_t st) {
   OrderArgs a = args;
   a.blocks = (int)(a.pairs > 0 ? order_blocks(a.pairs) : 1);
   const dim3 grid(a.blocks), block(topk::OW * 32);
-  const size_t smem = (size_t)(topk::OW + 1) * a.experts * sizeof(int);
+  const size_t smem = (size_t)(topk::OW + 2) * a.experts * sizeof(int);
+  if (a.blocks > 1 && a.blocks <= topk::OCLUSTER) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.blocks;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, topk::order_kernel<true>, a);
+  }
   if (a.blocks > 1) {
     const cudaError_t e = launch_pdl(topk::order_count_kernel, grid, block, smem, st, a);
     if (e != cudaSuccess) return e;
   }
-  return launch_pdl(topk::order_kernel, grid, block, smem, st, a);
+  return launch_pdl(topk::order_kernel<false>, grid, block, smem, st, a);
 }
 
 }  // namespace sb

@@ -23,8 +23,8 @@ def test_scale_bytes():
 
 
 def _quant(fmt=NV, x=FAKE, dtype=0, src=4, k=64, stride=64, rows_in=None, rows=4, ts=None, off=None, groups=0, codes=FAKE,
-           scales=FAKE, rs=FAKE):
-    return _lib.lib().sb_fp4_quant(fmt, x, dtype, src, k, stride, rows_in, rows, ts, off, groups, codes, scales, rs, None)
+           scales=FAKE, rs=FAKE, ws=None, n=0):
+    return _lib.lib().sb_fp4_quant(fmt, x, dtype, src, k, stride, rows_in, rows, ts, off, groups, codes, scales, rs, ws, n, None)
 
 
 def test_quant_refusals():
@@ -37,6 +37,11 @@ def test_quant_refusals():
                dict(fmt=MX, ts=FAKE)):
         assert _quant(**kw) == -1, kw
     assert _quant(rows=0, src=0, x=None, codes=None, scales=None) == 0
+    need = _lib.lib().sb_fp4_quant_workspace_bytes
+    assert need(NV, 4, 7, 64) == 0 and need(NV, 4, 8, 64) == 4 * (32 + 4 + 4) and need(MX, 4, 8, 129) == 4 * (80 + 8 + 4)
+    assert need(FP8, 4, 8, 64) == 0 and need(NV, 0, 8, 64) == 0 and need(NV, 4, 8, 0) == 0
+    assert _quant(rows_in=FAKE, rows=8, ws=FAKE, n=4 * 40 - 1) == -4
+    assert _quant(rows_in=FAKE, rows=8, ws=ODD, n=1 << 20) == -1
 
 
 def test_dequant_and_tile_refusals():
@@ -86,12 +91,12 @@ def test_route_refusals():
                dict(g=4, kg=0), dict(k=0), dict(k=17), dict(k=5, g=4, kg=1)):
         assert r(**kw) == -2, kw
     assert r(t=0, l=None) == 0
-    assert L.sb_expert_order_workspace_bytes(2048, 256) == 0 and L.sb_expert_order_workspace_bytes(2049, 256) == 2 * 256 * 4
+    assert L.sb_expert_order_workspace_bytes(16384, 256) == 0 and L.sb_expert_order_workspace_bytes(16385, 256) == 9 * 256 * 4
 
     def o(ids=FAKE, t=4, k=2, e=8, off=FAKE, tok=FAKE, pl=FAKE, ws=None, n=0):
         return L.sb_expert_order(ids, t, k, e, off, tok, pl, ws, n, None)
 
     assert o(t=-1) == -2 and o(k=0) == -2 and o(e=1025) == -2 and o(t=1 << 30, k=4) == -2
     assert o(ids=None) == -1 and o(off=None) == -1 and o(tok=None) == -1 and o(pl=None) == -1
-    assert o(t=8192, ws=None) == -4 and o(t=8192, ws=FAKE, n=8 * 8 * 4 - 1) == -4
-    assert o(t=8192, ws=ctypes.c_void_p(4097), n=1 << 20) == -1
+    assert o(t=16384, ws=None) == -4 and o(t=16384, ws=FAKE, n=16 * 8 * 4 - 1) == -4
+    assert o(t=16384, ws=ctypes.c_void_p(4097), n=1 << 20) == -1

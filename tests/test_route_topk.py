@@ -109,7 +109,8 @@ def test_topk_strides_and_large_batches():
 
 
 @gpu
-@pytest.mark.parametrize("t,k,e", [(0, 2, 4), (1, 1, 1), (3, 4, 16), (256, 8, 256), (257, 8, 7), (700, 8, 1024), (1024, 8, 256), (1025, 8, 256), (5000, 3, 100)])
+@pytest.mark.parametrize("t,k,e", [(0, 2, 4), (1, 1, 1), (3, 4, 16), (256, 8, 256), (257, 8, 7), (700, 8, 1024), (1024, 8, 256), (1025, 8, 256), (2048, 8, 64), (2049, 8, 64),
+                                   (5000, 3, 100), (9000, 8, 1024)])
 def test_expert_order(t, k, e):
     _need_gpu()
     gen = torch.Generator().manual_seed(t + e)
