@@ -321,7 +321,8 @@ int sb_moe_route(const sb_moe_layer* layer, const void* x, int64_t m, const int6
  * the tensor-core kernels' consumer-side waits (on operands and accumulators) make before they give
  * up: the kernel then sets the workspace error flag, drains its copies and MMAs in flight, frees its
  * tensor memory and returns, and the forward's output is incomplete. Waits for free slots and the
- * final drains keep their normal limits. polls = 0 restores each kernel's default. */
+ * final drains keep their normal limits. polls = 0 restores each kernel's default. (The fp4 x fp4 products set
+ * the flag that sb_fp4_error reads.) */
 int sb_debug_set_wait_limit(int64_t polls);
 
 /* Format self-test: decodes a fixed set of e2m1 / e4m3 / e8m0 codes on the device into out

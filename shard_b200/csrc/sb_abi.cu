@@ -1238,6 +1238,7 @@ int sb_fp4_gemm(int fmt, const void* a_codes, const void* a_scales, const float*
   g.kp = (int)fp4_kp(k);
   g.y = y;
   g.ldy = ldy;
+  g.probes = g_wait_limit.load(std::memory_order_relaxed);
   return cuda_check(sb::launch_fp4_mm(g, dtype, (cudaStream_t)stream), "fp4_gemm");
 }
 
@@ -1272,6 +1273,7 @@ int sb_fp4_grouped_gemm(int fmt, const void* a_codes, const void* a_scales, cons
   g.ldy = ldy;
   g.swiglu = swiglu;
   g.limit = limit;
+  g.probes = g_wait_limit.load(std::memory_order_relaxed);
   return cuda_check(sb::launch_fp4_mm(g, dtype, (cudaStream_t)stream), "fp4_grouped_gemm");
 }
 

@@ -59,6 +59,7 @@ struct Fp4MmArgs {
   int64_t ldy;
   int swiglu;                // rows 2i / 2i + 1 of W are gate / up
   float limit;               // swiglu: clamp, 0 for none
+  uint32_t probes;           // > 0: the consumers' waits give up after so many probes (for tests)
 };
 
 struct TopkArgs {

@@ -225,13 +225,15 @@ __device__ __forceinline__ int group_begin(const Fp4MmArgs& g, int mat) {
 }
 
 // The copying and issuing warps each run on one elected thread, whose waits need no vote of the warp (a vote and
-// a re-election per stage cost the issuing warp 100 ns of 330).
-__device__ __forceinline__ bool wait(volatile int* abortf, uint32_t bar, uint32_t parity) {
+// a re-election per stage cost the issuing warp 100 ns of 330). `probes` > 0 (a test's limit, on the consumers' waits):
+// that many probes without suspension instead.
+__device__ __forceinline__ bool wait(volatile int* abortf, uint32_t bar, uint32_t parity, uint32_t probes = 0u) {
+  if (probes > 0u) return wait_bounded<true>(abortf, &g_err, bar, parity, probes);
   return mbar_try_wait(bar, parity) || wait_bounded(abortf, &g_err, bar, parity, WAIT_LIMIT);
 }
 // one answer for the whole warp, whose next instructions need all of its lanes
-__device__ __forceinline__ bool warp_wait(volatile int* abortf, uint32_t bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, wait_bounded(abortf, &g_err, bar, parity, WAIT_LIMIT));
+__device__ __forceinline__ bool warp_wait(volatile int* abortf, uint32_t bar, uint32_t parity, uint32_t probes) {
+  return __all_sync(0xffffffffu, wait(abortf, bar, parity, probes));
 }
 
 // Tiles of one matrix run in bands of 12 weight blocks by all token tiles, so that the tiles in flight
@@ -542,7 +544,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
         if (!wait(abortf, smem_addr(&c.accempty[q]), ((n >> 1) & 1u) ^ 1u)) break;
         fence_after();
         auto stage = [&](auto blocks, auto whole, int k) {
-          if (!wait(abortf, full0 + 8 * s, ph)) {
+          if (!wait(abortf, full0 + 8 * s, ph, g.probes)) {
             ok = false;
             return;
           }
@@ -598,7 +600,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
         if (SWIGLU) wt[32 * j + lane] = w;
       }
       __syncwarp();
-      if (!warp_wait(abortf, smem_addr(&c.accfull[q]), (n >> 1) & 1u)) break;
+      if (!warp_wait(abortf, smem_addr(&c.accfull[q]), (n >> 1) & 1u, g.probes)) break;
       fence_after();
       if constexpr (FORM == SPLIT) {
         // the products have read all stages: their place takes this piece's sums, [token][row]

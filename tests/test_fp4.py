@@ -323,6 +323,56 @@ def test_pack_reads_the_canonical_form(fmt):
     assert torch.equal(v.canonical_scales().cpu(), inter)
 
 
+@gpu
+@pytest.mark.parametrize("m,n,k", [(5, 256, 64), (5, 256, 4096), (300, 256, 1024), (1024, 8192, 256)])
+def test_products_whose_waits_run_out(m, n, k):
+    """A consumer's wait that gives up at its first probe (one CTA a tile, K over a cluster, several tiles, CTA pairs):
+    the call ends, the error word says so, and the next call is whole again."""
+    _need_gpu()
+    from shard_b200 import _lib
+    L = _lib.lib()
+    codes, s, ts, _ = P.weights(NV, n, k, seed=1)
+    w = fp4.pack(NV, codes[0].cuda(), s[0].cuda(), ts[0].cuda())
+    a = fp4.quant(_acts(m, k, torch.bfloat16).cuda(), NV)
+    want = fp4.gemm(a, w)
+    assert fp4.device_error() == 0
+    try:
+        assert L.sb_debug_set_wait_limit(1) == 0
+        fp4.gemm(a, w)
+        torch.cuda.synchronize()
+    finally:
+        assert L.sb_debug_set_wait_limit(0) == 0
+    assert fp4.device_error() == 1 and fp4.device_error() == 0
+    assert torch.equal(fp4.gemm(a, w), want)
+    assert fp4.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+def test_pack_and_dequant_of_a_weight(fmt):
+    _need_gpu()
+    codes, s, ts, v = P.weights(fmt, 70, 96, seed=3)
+    w = fp4.pack(fmt, codes[0].cuda(), s[0].cuda(), None if ts is None else ts[0].cuda())
+    y = fp4.dequant(w, torch.float32).cpu()
+    # P.weights applies the tensor scale in 64 bits: the kernel rounds that product once
+    assert torch.equal(y, v[0].float())
+
+
+@gpu
+def test_gated_rows_of_nan_stay_nan():
+    """A clamp does not hide a NaN, and only its row has it."""
+    _need_gpu()
+    codes, s, ts, _ = P.weights(NV, 64, 64, seed=1, mats=2, halves=2)
+    bank = fp4.pack(NV, codes.cuda(), s.cuda(), ts.cuda(), kind=fp4.W13)
+    off = torch.tensor([0, 3, 9], dtype=torch.int32, device="cuda")
+    x = _acts(9, 64, torch.bfloat16, spread=0.1)
+    x[4, 20] = math.nan
+    for limit in (0.0, 1.5):
+        y = fp4.grouped_gemm(fp4.quant(x.cuda(), NV, offsets=off), bank, limit=limit).cpu()
+        assert torch.isnan(y).all(1).tolist() == [i == 4 for i in range(9)]
+        assert not bool(torch.isnan(y[[0, 1, 2, 3, 5, 6, 7, 8]]).any())
+
+
 def test_refusals_of_the_python_calls():
     """Arguments that no kernel may see are refused before the library is touched (no GPU needed)."""
     x = torch.zeros(4, 64, dtype=torch.bfloat16)
