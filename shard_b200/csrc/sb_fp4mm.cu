@@ -76,6 +76,7 @@ struct Ctl {
   uint64_t full[MAX_STAGES], empty[MAX_STAGES], accfull[2], accempty[2], drain;
   uint32_t tmem_base;
   int abort;
+  alignas(128) uint8_t turn[EPI_WARPS][2048];       // 32 rows x 32 outputs of 16 bits, to be turned
   alignas(16) float scale[EPI_WARPS][NT_MAX / 2];   // of each warp's tokens: tensor scale,
   alignas(16) float weight[EPI_WARPS][NT_MAX / 2];  // row weight
   int tiles[MAX_MATS + 1];   // tiles before each matrix
@@ -182,6 +183,12 @@ __device__ __forceinline__ uint32_t in_first(uint32_t addr) {
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
+// arrive on the accumulator's barrier where the MMAs are issued
+template <bool PAIR>
+__device__ __forceinline__ void release(uint32_t bar) {
+  if constexpr (PAIR) arrive_remote(in_first(bar));
+  else arrive(bar);
+}
 // a float of this CTA's shared memory as CTA `rank` of the cluster has it
 __device__ __forceinline__ float peer_float(uint32_t addr, int rank) {
   uint32_t r;
@@ -285,26 +292,17 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// v: one row's values of 8 columns, the lanes that differ in the bits M0, M1, M2 = M0 << 1, << 2 holding 8 rows.
-// Afterwards each of them holds 8 rows of one column (the one its three bits number), rounded.
-template <int M0, typename T>
-__device__ __forceinline__ uint4 transpose8(const float (&v)[8], int lane) {
-  const bool b0 = lane & M0, b1 = lane & (2 * M0), b2 = lane & (4 * M0);
-  uint32_t w[4], x[4];
-#pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    const float o = __shfl_xor_sync(0xffffffffu, b0 ? v[2 * p] : v[2 * p + 1], M0);
-    w[p] = pack2<T>(b0 ? o : v[2 * p], b0 ? v[2 * p + 1] : o);
-  }
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const uint32_t o = __shfl_xor_sync(0xffffffffu, b1 ? w[2 * q] : w[2 * q + 1], 2 * M0);
-    x[2 * q] = b1 ? o : w[2 * q];
-    x[2 * q + 1] = b1 ? w[2 * q + 1] : o;
-  }
-  const uint32_t o0 = __shfl_xor_sync(0xffffffffu, b2 ? x[0] : x[2], 4 * M0);
-  const uint32_t o1 = __shfl_xor_sync(0xffffffffu, b2 ? x[1] : x[3], 4 * M0);
-  return b2 ? make_uint4(o0, o1, x[2], x[3]) : make_uint4(x[0], x[1], o0, o1);
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// four 8 x 8 tiles of 16-bit values, read turned: lane l gets rows 2 (l % 4), + 1 of column l / 4 of each
+__device__ __forceinline__ uint4 read_turned(uint32_t addr) {
+  uint4 v;
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];\n"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
 }
 
 // silu(gate) * up of one pair of rows: the even lane holds gate, the odd lane up, of two tokens; each lane
@@ -316,51 +314,74 @@ __device__ __forceinline__ float gated(float v0, float v1, int lane, float lim) 
 }
 
 // 32 accumulator columns (tokens tok ..) of this thread's weight row to y; sc, wt: the tokens' scales and weights in
-// shared memory. 16-bit outputs are turned so that a lane stores 8 neighbouring ones at once: with a 2-byte
-// store per row and column the stores bound every tile of K <= 4096 (8.5 us a tile of 192 columns).
-template <bool SWIGLU, typename T>
+// shared memory. 16-bit outputs go through the warp's `turn` in shared memory, rows of 32 tokens in, tokens of up to
+// 8 neighbouring rows out: with a 2-byte store per row and column the stores bound every tile of K <= 4096 (8.5 us
+// a tile of 192 columns), and turned by shuffles (32 a chunk, against 8 accesses so) they took 3.7 us of
+// 3.7 at K = 2048. The 16-byte pieces of a row are placed so that neither side meets a bank conflict.
+template <bool SWIGLU, bool FULL, typename T>
 __device__ __forceinline__ void store_chunk(const Args& a, const uint32_t (&d)[32], int64_t tok, int row, int lane, int left,
-                                            bool vec, float wts, const float* sc, const float* wt) {
+                                            bool vec, float wts, const float* sc, const float* wt, uint32_t turn) {
   const Fp4MmArgs& g = a.g;
   T* y = reinterpret_cast<T*>(g.y);
   const int64_t ld = g.ldy;
   const float lim = g.limit > 0.f ? g.limit : INFINITY;
   if constexpr (sizeof(T) == 2) {
     if (vec) {
+      const int e = lane & 7, i = lane >> 3;   // this lane's part of an address list: row e of tile i
       if constexpr (SWIGLU) {
-        const int col = ((lane >> 1) & 7) * 2 + (lane & 1), base = ((row - lane) >> 1) + ((lane >> 4) << 3);
-        T* yp = y + (tok + col) * ld + base;
+        // rows of 16 results: tokens 0, 2, .. 30 (even lanes), then 1, 3, .. 31
+        const int hr = lane >> 1;
+        const uint32_t to = turn + hr * 64;
+        const uint32_t gw = (uint32_t)((hr >> 2) ^ ((hr >> 1) & 1)) & 3u;
 #pragma unroll
         for (int j = 0; j < 32; j += 16) {
-          if (j < left) {
-            float h[8];
+          float h[8];
 #pragma unroll
-            for (int m = 0; m < 8; ++m) {
-              const float2 s = *reinterpret_cast<const float2*>(sc + j + 2 * m);
-              h[m] = gated(__uint_as_float(d[j + 2 * m]) * (s.x * wts), __uint_as_float(d[j + 2 * m + 1]) * (s.y * wts),
-                           lane, lim) *
-                     wt[j + 2 * m + (lane & 1)];
-            }
-            const uint4 o = transpose8<2, T>(h, lane);
-            if (j + col < left && 2 * base < g.n) *reinterpret_cast<uint4*>(yp + (int64_t)j * ld) = o;
+          for (int m = 0; m < 8; ++m) {
+            const float2 s = *reinterpret_cast<const float2*>(sc + j + 2 * m);
+            h[m] = gated(__uint_as_float(d[j + 2 * m]) * (s.x * wts), __uint_as_float(d[j + 2 * m + 1]) * (s.y * wts), lane,
+                         lim) *
+                   wt[j + 2 * m + (lane & 1)];
           }
+          st_shared16(to + ((((lane & 1) * 2 + (j >> 4)) ^ gw) << 4), pack2<T>(h[0], h[1]), pack2<T>(h[2], h[3]),
+                      pack2<T>(h[4], h[5]), pack2<T>(h[6], h[7]));
+        }
+        __syncwarp();
+        const int r = 4 * (e >> 1) + 2 * (i & 1) + (e & 1), q = lane & 3;
+        const uint32_t from = turn + r * 64, gr = (uint32_t)((r >> 2) ^ ((r >> 1) & 1)) & 3u;
+        const int base = ((row - lane) >> 1) + 4 * q;
+        T* yp = y + tok * ld + base;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint4 o = read_turned(from + (((2 * u + (i >> 1)) ^ gr) << 4));
+          const int t0 = 2 * (lane >> 2) + u, t1 = t0 + 16;
+          if ((FULL || t0 < left) && 2 * base < g.n) *reinterpret_cast<uint2*>(yp + (int64_t)t0 * ld) = make_uint2(o.x, o.y);
+          if ((FULL || t1 < left) && 2 * base < g.n) *reinterpret_cast<uint2*>(yp + (int64_t)t1 * ld) = make_uint2(o.z, o.w);
         }
       } else {
-        const int col = lane & 7, base = row - lane + (lane & ~7);
-        T* yp = y + (tok + col) * ld + base;
+        const uint32_t to = turn + lane * 64, gw = (uint32_t)((lane >> 3) + (lane >> 1)) & 3u;
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
-          if (j < left) {
-            const float4 s0 = *reinterpret_cast<const float4*>(sc + j), s1 = *reinterpret_cast<const float4*>(sc + j + 4);
-            const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-            float v[8];
+          const float4 s0 = *reinterpret_cast<const float4*>(sc + j), s1 = *reinterpret_cast<const float4*>(sc + j + 4);
+          const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+          float v[8];
 #pragma unroll
-            for (int m = 0; m < 8; ++m) v[m] = __uint_as_float(d[j + m]) * (s[m] * wts);
-            const uint4 o = transpose8<1, T>(v, lane);
-            if (j + col < left && base < g.n) *reinterpret_cast<uint4*>(yp + (int64_t)j * ld) = o;
-          }
+          for (int m = 0; m < 8; ++m) v[m] = __uint_as_float(d[j + m]) * (s[m] * wts);
+          st_shared16(to + (((j >> 3) ^ gw) << 4), pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
+                      pack2<T>(v[6], v[7]));
+        }
+        __syncwarp();
+        const int r = 8 * (e >> 1) + 2 * i + (e & 1);
+        const uint32_t from = turn + r * 64, gr = (uint32_t)((r >> 3) + (r >> 1)) & 3u;
+        const int base = row - lane + 8 * (lane & 3);
+        T* yp = y + (tok + (lane >> 2)) * ld + base;
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          const uint4 o = read_turned(from + (((j >> 3) ^ gr) << 4));
+          if ((FULL || j + (lane >> 2) < left) && base < g.n) *reinterpret_cast<uint4*>(yp + (int64_t)j * ld) = o;
         }
       }
+      __syncwarp();
       return;
     }
   }
@@ -369,23 +390,23 @@ __device__ __forceinline__ void store_chunk(const Args& a, const uint32_t (&d)[3
     T* yp = y + (tok + (lane & 1)) * ld + (row >> 1);
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
-      if (j < left) {
+      if (FULL || j < left) {
         const float2 s = *reinterpret_cast<const float2*>(sc + j);
         const float h = gated(__uint_as_float(d[j]) * (s.x * wts), __uint_as_float(d[j + 1]) * (s.y * wts), lane, lim) *
                         wt[j + (lane & 1)];
-        if (in && j + (lane & 1) < left) yp[(int64_t)j * ld] = to_out<T>(h);
+        if (in && (FULL || j + (lane & 1) < left)) yp[(int64_t)j * ld] = to_out<T>(h);
       }
     }
   } else {
     T* yp = y + tok * ld + row;
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
-      if (j < left) {
+      if (FULL || j < left) {
         const float4 s = *reinterpret_cast<const float4*>(sc + j);
         const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
         for (int m = 0; m < 4; ++m)
-          if (in && j + m < left) yp[(int64_t)(j + m) * ld] = to_out<T>(__uint_as_float(d[j + m]) * (v[m] * wts));
+          if (in && (FULL || j + m < left)) yp[(int64_t)(j + m) * ld] = to_out<T>(__uint_as_float(d[j + m]) * (v[m] * wts));
       }
     }
   }
@@ -572,34 +593,50 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
     }
     __syncwarp();
   } else {
+    constexpr int CHUNKS = NT_MAX / 64;
     uint32_t n = 0;
     const int half = warp >> 2;   // this warp's 32-column chunks: half, half + 2, ...
     const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t turn = smem_addr(c.turn[warp]);
     float* sc = c.scale[warp];
     float* wt = c.weight[warp];
+    // a tile's place, scales and weights are found while the one before it is stored (1900 cycles a tile otherwise)
+    Tile next;
+    float s_next[CHUNKS], w_next[CHUNKS], wts_next = 1.f;
+    auto look_ahead = [&](int i) {
+      if (i >= total) return;
+      next = tile_at<PAIR>(a, c, i);
+      const int row = next.n0 + rank * 128 + (warp & 3) * 32 + lane;
+      wts_next = 1.f;
+      if (g.w_ts != nullptr && row < g.n)
+        wts_next = g.w_ts[g.w_ts_n == 0 ? row : next.mat * g.w_ts_n + (g.w_ts_n == 2 ? (row & 1) : 0)];
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j) {
+        const int col = 32 * (half + 2 * j) + lane;
+        const int64_t tok = (int64_t)next.row0 + next.t0 + col;
+        s_next[j] = w_next[j] = 1.f;
+        if (col < next.cnt) {
+          if (g.a_ts != nullptr) s_next[j] = g.a_ts[g.a_ts_row ? tok : 0];
+          if (g.row_weight != nullptr) w_next[j] = g.row_weight[tok];
+        }
+      }
+    };
+    look_ahead(first);
     for (int i = first; i < total; i += stride, ++n) {
-      const Tile t = tile_at<PAIR>(a, c, i);
+      const Tile t = next;
+      const float wts = wts_next;
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j) {
+        sc[32 * j + lane] = SWIGLU ? s_next[j] : s_next[j] * w_next[j];
+        if (SWIGLU) wt[32 * j + lane] = w_next[j];
+      }
+      __syncwarp();
+      if constexpr (FORM != SPLIT) look_ahead(i + stride);
       const uint32_t q = n & 1u;
       const uint32_t acc = tbase + q * NT_MAX + quarter;
       const int row = t.n0 + rank * 128 + (warp & 3) * 32 + lane;
       const bool vec = a.vec && (t.n0 + rank * 128 + 128 <= g.n || (SWIGLU ? g.n % 16 : g.n % 8) == 0);
-      float wts = 1.f;
-      if (g.w_ts != nullptr && row < g.n)
-        wts = g.w_ts[g.w_ts_n == 0 ? row : t.mat * g.w_ts_n + (g.w_ts_n == 2 ? (row & 1) : 0)];
-      // the tokens' scales and weights, in shared memory before the products are done
       const int64_t tok0 = (int64_t)t.row0 + t.t0;
-#pragma unroll
-      for (int j = 0; j < NT_MAX / 64; ++j) {
-        const int col = 32 * (half + 2 * j) + lane;
-        float s = 1.f, w = 1.f;
-        if (col < t.cnt) {
-          if (g.a_ts != nullptr) s = g.a_ts[g.a_ts_row ? tok0 + col : 0];
-          if (g.row_weight != nullptr) w = g.row_weight[tok0 + col];
-        }
-        sc[32 * j + lane] = SWIGLU ? s : s * w;
-        if (SWIGLU) wt[32 * j + lane] = w;
-      }
-      __syncwarp();
       if (!warp_wait(abortf, smem_addr(&c.accfull[q]), (n >> 1) & 1u, g.probes)) break;
       fence_after();
       if constexpr (FORM == SPLIT) {
@@ -623,20 +660,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
           held = false;
           fence_before();
           __syncwarp();
-          if (lane == 0) {
-            if constexpr (PAIR) arrive_remote(in_first(smem_addr(&c.accempty[q])));
-            else arrive(smem_addr(&c.accempty[q]));
-          }
+          if (lane == 0) release<PAIR>(smem_addr(&c.accempty[q]));
         }
-        store_chunk<SWIGLU, T>(a, d, tok0 + ch * 32, row, lane, min(32, t.cnt - ch * 32), vec, wts, sc + 32 * j, wt + 32 * j);
+        const int left = t.cnt - ch * 32;
+        if (left >= 32) store_chunk<SWIGLU, true, T>(a, d, tok0 + ch * 32, row, lane, 32, vec, wts, sc + 32 * j, wt + 32 * j, turn);
+        else store_chunk<SWIGLU, false, T>(a, d, tok0 + ch * 32, row, lane, left, vec, wts, sc + 32 * j, wt + 32 * j, turn);
       }
       if (held) {
         fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR) arrive_remote(in_first(smem_addr(&c.accempty[q])));
-          else arrive(smem_addr(&c.accempty[q]));
-        }
+        if (lane == 0) release<PAIR>(smem_addr(&c.accempty[q]));
       }
       __syncwarp();
     }
