@@ -831,7 +831,9 @@ cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
     while (a.split < 8 && tiles * a.split * 2 <= sms && (a.ksteps + 3) / 4 >= a.split * 4) a.split *= 2;
   // (one token tile: a CTA's first tile is its own row block, whose stages it all reads)
   a.ahead = g.offsets == nullptr && tt == 1 ? ((a.ksteps + 3) / 4 + a.split - 1) / a.split : 0;
-  a.box = g.offsets ? BOX : (pair ? a.nt / 2 : a.nt);
+  // Token rows of a copy: a whole tile's (of a pair's half), but with narrow groups 32 at a time, as many as the group has.
+  // (Three copies of 32 rows in place of one of 96 made the copying thread the bound: 0.33 us a stage, one copy 0.26.)
+  a.box = pair ? a.nt / 2 : g.offsets ? BOX : a.nt;
   a.b_bytes = (pair ? a.nt / 2 : a.nt) * 128;
   a.sblk = a.nt > 128 ? 2 : 1;
   a.vec = (reinterpret_cast<uintptr_t>(g.y) & 15u) == 0 && g.ldy % 8 == 0;
