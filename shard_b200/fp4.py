@@ -67,6 +67,14 @@ def _fmt(fmt: Union[int, str]) -> int:
     return f
 
 
+def _away(what: str, t: torch.Tensor, stream) -> bool:
+    """Whether a call on `t` has to make another device or stream current first."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"{what}: the tensors must be on a CUDA device")
+    return stream is not None or dev != _current_device()
+
+
 @contextlib.contextmanager
 def _elsewhere(device, stream):
     """`device` made current, and `stream` when one is given (also for the allocations of the call)."""
@@ -139,9 +147,7 @@ def quant(x: torch.Tensor, fmt: Union[int, str] = F.FMT_NVFP4, tensor_scale: Opt
     f = _FMT.get(fmt)
     if f is None:
         f = _fmt(fmt)
-    if stream is not None or x.get_device() != _current_device():
-        if not x.is_cuda:
-            raise ValueError("quant: x must be a CUDA tensor of bf16, fp16 or fp32")
+    if _away("quant", x, stream):
         with _elsewhere(x.device, stream):
             return quant(x, f, tensor_scale, rows, offsets)
     r = (_HOST or host()).quant(x, f, tensor_scale, rows, offsets)
@@ -165,7 +171,7 @@ def dequant(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, stream=None) -> t
     if dt is None:
         raise ValueError(f"dequant: dtype {dtype}")
     buf = q._buf
-    if stream is not None or buf.get_device() != _current_device():
+    if _away("dequant", buf, stream):
         with _elsewhere(buf.device, stream):
             return dequant(q, dtype)
     y = (_HOST or host()).dequant(buf, q.fmt, q.codes_ptr, q.scales_ptr, q.ts_ptr, q.per_row, q.rows, q.k, q.shape, dt)
@@ -199,7 +205,7 @@ def pack(fmt: Union[int, str], codes: torch.Tensor, scales: torch.Tensor, ts: Op
             raise ValueError(f"pack: {ts.shape[1]} tensor scales a matrix")
     if kind not in (PLAIN, W13) or (kind == W13 and n % 2):
         raise ValueError("pack: kind is PLAIN, or W13 with an even number of rows")
-    if stream is not None or codes.get_device() != _current_device():
+    if _away("pack", codes, stream):
         with _elsewhere(codes.device, stream):
             return pack(fmt, codes, scales, ts, kind)
     c, s = c.reshape(mats, n, k // 2), s.reshape(mats, n, nb)
@@ -237,7 +243,7 @@ def gemm(a: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, ou
     if a.offsets is not None or w.offsets is not None or w.mats != 1 or w.kind != PLAIN:
         raise ValueError("gemm: plain operands of one matrix (grouped_gemm takes banks and expert groups)")
     buf = a._buf
-    if stream is not None or buf.get_device() != _current_device():
+    if _away("gemm", buf, stream):
         with _elsewhere(buf.device, stream):
             return gemm(a, w, out_dtype, out)
     y = (_HOST or host()).gemm(buf, a.fmt, a.codes_ptr, a.scales_ptr, a.ts_ptr, a.per_row, a.rows, a.shape, a.k, w.codes_ptr,
@@ -260,7 +266,7 @@ def grouped_gemm(a: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bflo
     if not limit >= 0.0:
         raise ValueError("grouped_gemm: limit must be >= 0")
     buf = a._buf
-    if stream is not None or buf.get_device() != _current_device():
+    if _away("grouped_gemm", buf, stream):
         with _elsewhere(buf.device, stream):
             return grouped_gemm(a, w, out_dtype, row_weight, limit, out)
     y = (_HOST or host()).grouped_gemm(buf, a.fmt, a.codes_ptr, a.scales_ptr, a.ts_ptr, a.per_row, a.rows, a.k, off, w.codes_ptr,

@@ -15,10 +15,9 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import _lib
+from . import _lib, fp4
 from ._lib import check
-from . import fp4
-from .fp4 import _current_device, _elsewhere
+from .fp4 import _away, _elsewhere
 
 _SCORE = _lib.SCORE
 _GROUP_SCORE = {"max": 0, "top2": 1}
@@ -47,9 +46,7 @@ def topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, scor
     sc, gs = _SCORE.get(score), _GROUP_SCORE.get(group_score)
     if sc is None or gs is None:
         raise ValueError(f"topk: score {score!r}, group_score {group_score!r}")
-    if stream is not None or logits.get_device() != _current_device():
-        if not logits.is_cuda:
-            raise ValueError("topk: logits must be a CUDA tensor [T, E] of bf16, fp16 or fp32")
+    if _away("topk", logits, stream):
         with _elsewhere(logits.device, stream):
             return topk(logits, k, bias, score, n_group, topk_group, group_score, renormalize, scale)
     r = (fp4._HOST or fp4.host()).topk(logits, k, bias, sc, n_group, topk_group, gs, renormalize, scale)
@@ -61,9 +58,7 @@ def topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, scor
 def expert_order(indices: torch.Tensor, n_experts: int, stream=None) -> ExpertOrder:
     """indices int64 [T, k] -> ExpertOrder. Pairs whose id is outside [0, n_experts) (dropped tokens, padding) are
     left out."""
-    if stream is not None or indices.get_device() != _current_device():
-        if not indices.is_cuda:
-            raise ValueError("expert_order: indices must be a contiguous CUDA int64 tensor [T, k]")
+    if _away("expert_order", indices, stream):
         with _elsewhere(indices.device, stream):
             return expert_order(indices, n_experts)
     r = (fp4._HOST or fp4.host()).expert_order(indices, n_experts)
