@@ -261,7 +261,7 @@ size_t sb_fp4_scale_bytes(int fmt, int64_t n_mat, int64_t rows, int64_t k, int64
  * [0, src_rows) the row is zero. tensor_scale (NVFP4): fp32 [1], or NULL for one per row,
  * max(2^-126, amax / 2688), written to row_scale fp32 [rows]. Rows behind offsets[groups] are not
  * written. A block that holds a non-finite value gets a NaN scale. The workspace (16-byte aligned) of
- * sb_fp4_quant_workspace_bytes, or NULL: with it a gather that takes its source rows twice or more quantises
+ * sb_fp4_quant_workspace_bytes, or NULL: with it a large gather that takes its source rows twice or more quantises
  * them once and copies; the results are the same. It is the call's own until it has run. */
 size_t sb_fp4_quant_workspace_bytes(int fmt, int64_t src_rows, int64_t rows, int64_t k);
 int sb_fp4_quant(int fmt, const void* x, int dtype, int64_t src_rows, int64_t k, int64_t row_stride,

@@ -550,10 +550,13 @@ static cudaError_t launch_rows(const QuantArgs& args, int dtype, cudaStream_t st
   return fp4::launch_quant_t<__nv_bfloat16>(q, v, vec, grid, block, st);
 }
 
-// A gather that takes each source row twice or more quantises the source once and copies (2048 rows of 4096, each
-// taken eight times, and their w13 product: 246 us without, 221 with).
+// A gather that takes each source row twice or more quantises the source once and copies, from 4 M values on (2048 rows
+// of 4096, each taken eight times, and their w13 product: 246 us without, 221 with; below, the second launch
+// costs more than it saves).
 size_t fp4_quant_workspace(int64_t src_rows, int64_t rows, int64_t row_bytes, int64_t atoms) {
-  return rows >= 2 * src_rows && src_rows > 0 ? (size_t)(src_rows * (row_bytes + 4 * atoms + 4)) : 0;
+  return rows >= 2 * src_rows && src_rows > 0 && rows * row_bytes >= (2 << 20)
+             ? (size_t)(src_rows * (row_bytes + 4 * atoms + 4))
+             : 0;
 }
 
 cudaError_t launch_fp4_quant(const QuantArgs& a, int dtype, void* workspace, cudaStream_t st) {

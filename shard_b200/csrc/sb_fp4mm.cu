@@ -315,9 +315,10 @@ __device__ __forceinline__ float gated(float v0, float v1, int lane, float lim) 
 
 // 32 accumulator columns (tokens tok ..) of this thread's weight row to y; sc, wt: the tokens' scales and weights in
 // shared memory. 16-bit outputs go through the warp's `turn` in shared memory, rows of 32 tokens in, tokens of up to
-// 8 neighbouring rows out: with a 2-byte store per row and column the stores bound every tile of K <= 4096 (8.5 us
-// a tile of 192 columns), and turned by shuffles (32 a chunk, against 8 accesses so) they took 3.7 us of
-// 3.7 at K = 2048. The 16-byte pieces of a row are placed so that neither side meets a bank conflict.
+// 8 neighbouring rows out, the 16-byte pieces of a row placed so that neither side meets a bank conflict. This
+// readback bounds tiles of K <= 2048: 8192 x 4096 x 2048 took 62 us turned by shuffles (32 of them a chunk, against 8
+// accesses so), now 46; with a 2-byte store per row and column a tile of 192 columns took 8.5 us. FULL: a whole
+// chunk, without a branch per group of columns, which would keep the groups from overlapping.
 template <bool SWIGLU, bool FULL, typename T>
 __device__ __forceinline__ void store_chunk(const Args& a, const uint32_t (&d)[32], int64_t tok, int row, int lane, int left,
                                             bool vec, float wts, const float* sc, const float* wt, uint32_t turn) {
@@ -821,11 +822,11 @@ cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
   const int64_t nb = (g.n + 127) / 128;
   const int64_t tt = g.offsets ? (int64_t)g.m / a.nt + (g.mats < g.m ? g.mats : g.m) : (g.m + a.nt - 1) / a.nt;
   const int64_t tiles = tt * nb;
-  // Pairs where tiles of full width are many: they halve the token bytes per product, which is what bounds
-  // those; narrow tiles are bound by the weights, which pairs do not share.
+  // Pairs where tiles of full width are many: they halve the token bytes that each SM copies and reads per product
+  // (8192 cubed: 274 us without, 248 with); narrow tiles are bound by the weights, which pairs do not share.
   const bool pair = a.nt >= 128 && g.m >= 128 * (int64_t)g.mats && tiles >= 2 * sms;
   // K is split, for one token tile, as far as the SMs go and every piece keeps two stages (one token against 4096 x 8192:
-  // 12.0 us whole, see the split's time at the head of this file).
+  // 12.0 us whole, 9.3 in four pieces, 8.6 with the weights ahead in L2).
   a.split = 1;
   if (g.offsets == nullptr && tt == 1)
     while (a.split < 8 && tiles * a.split * 2 <= sms && (a.ksteps + 3) / 4 >= a.split * 4) a.split *= 2;

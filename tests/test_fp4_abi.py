@@ -38,10 +38,12 @@ def test_quant_refusals():
         assert _quant(**kw) == -1, kw
     assert _quant(rows=0, src=0, x=None, codes=None, scales=None) == 0
     need = _lib.lib().sb_fp4_quant_workspace_bytes
-    assert need(NV, 4, 7, 64) == 0 and need(NV, 4, 8, 64) == 4 * (32 + 4 + 4) and need(MX, 4, 8, 129) == 4 * (80 + 8 + 4)
-    assert need(FP8, 4, 8, 64) == 0 and need(NV, 0, 8, 64) == 0 and need(NV, 4, 8, 0) == 0
-    assert _quant(rows_in=FAKE, rows=8, ws=FAKE, n=4 * 40 - 1) == -4
-    assert _quant(rows_in=FAKE, rows=8, ws=ODD, n=1 << 20) == -1
+    p = 1 << 16                     # from 2^22 values on, each source row taken twice or more
+    assert need(NV, 4, p, 64) == 4 * (32 + 4 + 4) and need(MX, 4, p, 129) == 4 * (80 + 8 + 4) and need(NV, p // 2, p, 64) > 0
+    assert need(NV, 4, p - 1, 64) == 0 and need(NV, p // 2 + 1, p, 64) == 0
+    assert need(FP8, 4, p, 64) == 0 and need(NV, 0, p, 64) == 0 and need(NV, 4, p, 0) == 0
+    assert _quant(rows_in=FAKE, rows=p, ws=FAKE, n=4 * 40 - 1) == -4
+    assert _quant(rows_in=FAKE, rows=p, ws=ODD, n=1 << 20) == -1
 
 
 def test_dequant_and_tile_refusals():
