@@ -331,9 +331,9 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
       load_bias<C>(a, lane, b);
 #pragma unroll
       for (int i = 0; i < C; ++i) {
-        const float t = gv[i] + b[i];
-        most = fmaxf(most, gv[i] + fabsf(b[i]));
+        const float t = gv[i] + b[i], mag = gv[i] + fabsf(b[i]);
         v[i] = gv[i] = l[i] > -INFINITY && t == t ? t : -INFINITY;
+        most = fmaxf(most, v[i] > -INFINITY ? mag : 0.f);   // (a bias of -inf masks its expert)
       }
     } else {
 #pragma unroll

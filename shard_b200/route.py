@@ -42,7 +42,8 @@ def topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, scor
     renormalize  divide the chosen experts' unbiased scores by their sum; then times `scale`
 
     Values are compared as real numbers, ties go to the lower id. An expert whose logit is NaN, -inf or the
-    type's lowest value is masked: after all others of the kept groups, with weight 0."""
+    type's lowest value is masked: after all others of the kept groups, with weight 0. A bias of -inf keeps an
+    expert behind the others too."""
     sc, gs = _SCORE.get(score), _GROUP_SCORE.get(group_score)
     if sc is None or gs is None:
         raise ValueError(f"topk: score {score!r}, group_score {group_score!r}")

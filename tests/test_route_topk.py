@@ -91,6 +91,22 @@ def test_topk_masks(dtype, score):
 
 
 @gpu
+def test_topk_biases_without_end():
+    """-inf keeps experts (whole groups too) behind the others, +inf puts one first; weights are the scores all the same."""
+    _need_gpu()
+    gen = torch.Generator().manual_seed(8)
+    logits = torch.randn(40, 64, generator=gen)
+    bias = 0.2 * torch.randn(64, generator=gen)
+    bias[::3] = -math.inf
+    bias[16:24] = -math.inf
+    for g, kept in ((1, 1), (8, 3)):
+        for gs in ("max", "top2"):
+            _check(logits, 6, bias, n_group=g, topk_group=kept, group_score=gs)
+    bias[5] = math.inf
+    _check(logits, 6, bias)
+
+
+@gpu
 def test_topk_strides_and_large_batches():
     _need_gpu()
     gen = torch.Generator().manual_seed(6)
