@@ -250,8 +250,8 @@ int sb_residual_rmsnorm(void* x, const void* y, int64_t rows, int64_t dim, const
  * scales (row r's four bytes at 16 (r % 32) + 4 (r / 32 % 4) of its atom; the atoms of a row block lie
  * along K, row blocks follow one another; an expert bank pads each matrix to whole row blocks); for
  * NVFP4 an fp32 tensor scale: one, or one per row. With expert groups (row p of group e iff
- * offsets[e] <= p < offsets[e+1]; int32 on the device, ascending, offsets[0] = 0), group e's scales
- * start at row block offsets[e] / 128 + e. Codes and scales are 16-byte aligned. */
+ * offsets[e] <= p < offsets[e+1]; int32 on the device, ascending), group e's scales start at row block
+ * offsets[e] / 128 + e. Codes and scales are 16-byte aligned. */
 enum sb_dtype { SB_BF16 = 0, SB_F16 = 1, SB_F32 = 2 };
 /* Bytes of an operand's scales: n_mat matrices of `rows` rows (groups = 0), or one of `rows` rows in
  * `groups` expert groups (n_mat = 1). 0 for arguments that the calls below refuse. */
@@ -259,7 +259,7 @@ size_t sb_fp4_scale_bytes(int fmt, int64_t n_mat, int64_t rows, int64_t k, int64
 /* x [src_rows, K] of `dtype`, rows row_stride elements apart -> operand of `rows` rows, K in 1..65536.
  * rows_in (int32 [rows], or NULL: row p is x's row p): the row of x that row p takes; outside
  * [0, src_rows) the row is zero. tensor_scale (NVFP4): fp32 [1], or NULL for one per row,
- * max(2^-126, amax / 2688), written to row_scale fp32 [rows]. Rows behind offsets[groups] are not
+ * max(2^-126, amax / 2688), written to row_scale fp32 [rows]. Rows of no group are not
  * written. A block that holds a non-finite value gets a NaN scale. The workspace (16-byte aligned) of
  * sb_fp4_quant_workspace_bytes, or NULL: with it a large gather that takes its source rows twice or more quantises
  * them once and copies; the results are the same. It is the call's own until it has run. */
@@ -279,8 +279,8 @@ int sb_fp4_tile_scales(int fmt, const void* src, void* dst, int64_t n_mat, int64
 int sb_fp4_gemm(int fmt, const void* a_codes, const void* a_scales, const float* a_ts, int a_ts_per_row, int64_t m,
                 const void* w_codes, const void* w_scales, const float* w_ts, int w_ts_per_row, int64_t n, int64_t k,
                 void* y, int dtype, int64_t ldy, void* stream);
-/* The same with one W [N, K] per expert of a bank and A's rows in expert groups. Rows behind
- * offsets[n_experts] are left as they are. w_ts: fp32 [n_experts, w_ts_n] or NULL. row_weight: fp32 [M]
+/* The same with one W [N, K] per expert of a bank and A's rows in expert groups. Rows of no group are left
+ * as they are. w_ts: fp32 [n_experts, w_ts_n] or NULL. row_weight: fp32 [M]
  * (each output row times its weight) or NULL. swiglu: W holds w1's and w3's rows in turn (row 2i: w1,
  * 2i + 1: w3; w_ts_n 2 gives each its scale) and y [M, N/2] = silu(min(g, limit)) * clip(u, +-limit)
  * (limit 0: no clamp; Expert.forward, model.py:601-611). n_experts <= 1024. */

@@ -1172,7 +1172,7 @@ int sb_fp4_quant(int fmt, const void* x, int dtype, int64_t src_rows, int64_t k,
   q.groups = (int)groups;
   q.blocks = fp4_blocks(1, rows, groups);
   q.ts = tensor_scale;
-  q.row_ts = row_scale;
+  q.row_ts = nv && !tensor_scale ? row_scale : nullptr;
   q.codes = (uint8_t*)codes;
   q.row_bytes = fp4_kp(k) / 2;
   q.scales = (uint8_t*)scales;

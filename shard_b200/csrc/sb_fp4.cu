@@ -571,9 +571,7 @@ cudaError_t launch_fp4_quant(const QuantArgs& a, int dtype, void* workspace, cud
   q.flat = 1;
   const cudaError_t e = launch_rows(q, dtype, st);
   if (e != cudaSuccess) return e;
-  QuantArgs g = a;
-  if (a.ts != nullptr) g.row_ts = nullptr;
-  return launch_pdl(fp4::gather_kernel, dim3((unsigned)((a.rows + 7) / 8)), dim3(256), 0, st, g, q.codes,
+  return launch_pdl(fp4::gather_kernel, dim3((unsigned)((a.rows + 7) / 8)), dim3(256), 0, st, a, q.codes,
                     (const uint32_t*)q.scales, q.row_ts);
 }
 

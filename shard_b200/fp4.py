@@ -143,7 +143,7 @@ def quant(x: torch.Tensor, fmt: Union[int, str] = F.FMT_NVFP4, tensor_scale: Opt
     tensor_scale  NVFP4: calibrated fp32 scale (one value) in place of the rows' own
     rows          int32 [P]: operand row p is x's row rows[p] (a gather in the same pass); outside x: zeros
     offsets       int32 [E + 1]: expert e's rows are offsets[e] .. offsets[e + 1] - 1 (for grouped_gemm);
-                  rows behind offsets[E] are left as they are"""
+                  rows of no expert are left as they are"""
     f = _FMT.get(fmt)
     if f is None:
         f = _fmt(fmt)
@@ -258,7 +258,7 @@ def grouped_gemm(a: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bflo
                  stream=None) -> torch.Tensor:
     """Row p of expert e (offsets[e] <= p < offsets[e+1]) against W_e of the bank: y [P, N], or for a W13 bank
     y [P, N/2] = silu(min(g, limit)) * clip(u, -limit, limit) (limit 0: no clamp). row_weight fp32 [P]
-    multiplies the output rows. Rows behind offsets[E] are left as they are."""
+    multiplies the output rows. Rows of no expert are left as they are."""
     dt = _operands("grouped_gemm", a, w, out_dtype)
     off = a.offsets
     if off is None or off.shape[0] != w.mats + 1 or w.per_row or w.offsets is not None:

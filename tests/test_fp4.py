@@ -313,6 +313,23 @@ def test_grouped_gemm(fmt, w13, counts):
 
 @gpu
 @pytest.mark.parametrize("fmt", [NV, MX])
+def test_groups_that_begin_late(fmt):
+    """Offsets of some of the experts of an order: rows before the first group and behind the last are left alone."""
+    _need_gpu()
+    codes, s, ts, _ = P.weights(fmt, 64, 128, seed=6, mats=6)
+    one = lambda lo, hi: fp4.pack(fmt, codes[lo:hi].cuda(), s[lo:hi].cuda(), None if ts is None else ts[lo:hi].cuda())  # noqa: E731
+    x = _acts(400, 128, torch.bfloat16, seed=6).cuda()
+    off = torch.tensor([0, 130, 131, 131, 290, 300, 400], dtype=torch.int32, device="cuda")
+    whole = fp4.grouped_gemm(fp4.quant(x, fmt, offsets=off), one(0, 6))
+    part = off[1:5].contiguous()
+    out = torch.full((400, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    fp4.grouped_gemm(fp4.quant(x, fmt, offsets=part), one(1, 4), out=out)
+    assert torch.equal(out[130:290], whole[130:290])
+    assert bool((out[:130] == 5).all()) and bool((out[290:] == 5).all())
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
 def test_pack_reads_the_canonical_form(fmt):
     """Tiling and back; a plain product equals one with the operand that quant makes of the same values."""
     _need_gpu()
