@@ -82,14 +82,14 @@ struct OrderArgs {
   const int64_t* ids;        // [pairs]
   int64_t pairs;
   int topk, experts;
-  int blocks;                // set by the launch
+  int blocks, scanned;       // set by the launch
   int32_t* hist;             // [order_counts][experts]
   int32_t* offsets;          // [experts + 1]
   int32_t* tokens;           // [pairs]
   int32_t* places;           // [pairs]
 };
 
-int64_t order_counts(int64_t pairs);   // blocks whose counts go through memory, 0: none
+int64_t order_counts(int64_t pairs);   // rows of counts that go through memory, 0: none
 cudaError_t launch_topk(const TopkArgs& a, int dtype, cudaStream_t st);
 cudaError_t launch_expert_order(const OrderArgs& a, cudaStream_t st);
 // bytes of the copy of a gather's quantised source rows, 0 where none is made

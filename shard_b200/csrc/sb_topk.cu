@@ -10,7 +10,7 @@
 //
 // order_kernel: a stable counting sort of the pairs by expert, in blocks of 2048 pairs, no atomics
 // on anything the outputs depend on. Up to eight blocks form a cluster that reads one another's counts in
-// shared memory; more leave them in memory by a kernel before.
+// shared memory; more leave them in memory by a kernel before, and many have them summed by one between.
 #include <cfloat>
 
 #include "sb_device.cuh"
@@ -551,6 +551,63 @@ __global__ void __launch_bounds__(OW * 32) order_count_kernel(OrderArgs a) {
   }
 }
 
+// Counts [blocks][experts] to the counts of the blocks before, in place, and behind them each expert's total. A block
+// takes SE experts (a row's 32 bytes), its threads SC runs of neighbouring counts.
+constexpr int SE = 8, SC = 128;
+
+__global__ void __launch_bounds__(SE * SC) order_scan_kernel(OrderArgs a) {
+  __shared__ int part[SE][SC];
+  const int x = threadIdx.x % SE, run = threadIdx.x / SE, e = blockIdx.x * SE + x;
+  const bool in = e < a.experts;
+  const int b0 = (int)((int64_t)a.blocks * run / SC), b1 = (int)((int64_t)a.blocks * (run + 1) / SC);
+  int* h = a.hist + (in ? e : 0);
+  pdl_wait();
+  pdl_trigger();
+  int sum = 0;
+  if (in) {
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) sum += h[(int64_t)b * a.experts];
+  }
+  part[x][run] = sum;
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp < SE) {   // the runs of one expert
+    constexpr int PER = SC / 32;
+    int v[PER], mine = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      v[j] = part[warp][lane * PER + j];
+      mine += v[j];
+    }
+    int at = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += u;
+    }
+    if (lane == 31 && blockIdx.x * SE + warp < a.experts)
+      a.hist[(int64_t)a.blocks * a.experts + blockIdx.x * SE + warp] = at;
+    at -= mine;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      part[warp][lane * PER + j] = at;
+      at += v[j];
+    }
+  }
+  __syncthreads();
+  int at = part[x][run];
+  for (int b = b0; in && b < b1; b += 8) {
+    int v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = b + j < b1 ? h[(int64_t)(b + j) * a.experts] : 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (b + j < b1) h[(int64_t)(b + j) * a.experts] = at;
+      at += v[j];
+    }
+  }
+}
+
 constexpr int OCLUSTER = 8;         // blocks of a cluster at most
 
 __device__ __forceinline__ int peer_int(const int* p, int rank) {
@@ -573,8 +630,8 @@ __global__ void __launch_bounds__(OW * 32) order_kernel(OrderArgs a) {
   const int64_t p0 = (int64_t)blockIdx.x * OBLOCK;
   int* all = cnt + OW * a.experts;
   int ex[OSTEP];
-  // After order_count_kernel this starts while that one runs, which in turn began when the ids were written: they
-  // can be read before the wait, the counts in memory after it.
+  // After order_count_kernel (and order_scan_kernel) this starts while they run, which in turn began when the ids were
+  // written: they can be read before the wait, the counts in memory after it.
   if (CLUSTER || a.blocks == 1) pdl_wait();
   segment(a, cnt, p0, ex);
   if (!CLUSTER && a.blocks > 1) pdl_wait();
@@ -601,6 +658,9 @@ __global__ void __launch_bounds__(OW * 32) order_kernel(OrderArgs a) {
           at += b < (int)blockIdx.x ? v : 0;
         }
       }
+    } else if (a.scanned) {
+      at = a.hist[(int64_t)blockIdx.x * a.experts + e];
+      sum = a.hist[(int64_t)a.blocks * a.experts + e];
     } else if (a.blocks > 1) {
 #pragma unroll 16
       for (int b = 0; b < a.blocks; ++b) {
@@ -711,7 +771,7 @@ cudaError_t launch_topk(const TopkArgs& args, int dtype, cudaStream_t st) {
 int64_t order_blocks(int64_t pairs) { return (pairs + topk::OBLOCK - 1) / topk::OBLOCK; }
 int64_t order_counts(int64_t pairs) {
   const int64_t b = order_blocks(pairs);
-  return b > topk::OCLUSTER ? b : 0;
+  return b > topk::OCLUSTER ? b + 1 : 0;   // (and the totals)
 }
 
 cudaError_t launch_expert_order(const OrderArgs& args, cudaStream_t st) {
@@ -737,7 +797,12 @@ cudaError_t launch_expert_order(const OrderArgs& args, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, topk::order_kernel<true>, a);
   }
   if (a.blocks > 1) {
-    const cudaError_t e = launch_pdl(topk::order_count_kernel, grid, block, smem, st, a);
+    cudaError_t e = launch_pdl(topk::order_count_kernel, grid, block, smem, st, a);
+    // Up to 64 blocks each adds up the counts before its own; more would read a quadratic number of them (256 experts, 64
+    // blocks: 9.0 us, 9.1 with the scan; 32: 7.8 and 8.8; 256: 19 and 14; 4096, 8.4 M pairs: 1194 and 114).
+    a.scanned = a.blocks > 64;
+    if (e == cudaSuccess && a.scanned)
+      e = launch_pdl(topk::order_scan_kernel, dim3((a.experts + topk::SE - 1) / topk::SE), dim3(topk::SE * topk::SC), 0, st, a);
     if (e != cudaSuccess) return e;
   }
   return launch_pdl(topk::order_kernel<false>, grid, block, smem, st, a);

@@ -126,7 +126,7 @@ def test_topk_strides_and_large_batches():
 
 @gpu
 @pytest.mark.parametrize("t,k,e", [(0, 2, 4), (1, 1, 1), (3, 4, 16), (256, 8, 256), (257, 8, 7), (700, 8, 1024), (1024, 8, 256), (1025, 8, 256), (2048, 8, 64), (2049, 8, 64),
-                                   (5000, 3, 100), (9000, 8, 1024)])
+                                   (5000, 3, 100), (9000, 8, 1024), (16384, 8, 60), (16385, 8, 60), (40000, 9, 1), (50001, 16, 1001)])
 def test_expert_order(t, k, e):
     _need_gpu()
     gen = torch.Generator().manual_seed(t + e)
@@ -140,6 +140,24 @@ def test_expert_order(t, k, e):
     assert o.offsets.tolist() == offsets
     assert o.tokens.tolist() == tokens
     assert o.places.reshape(-1).tolist() == places
+
+
+@gpu
+def test_expert_order_of_many_pairs():
+    """30 M pairs: the counts of 14649 blocks."""
+    _need_gpu()
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    ids = torch.randint(-1, 256, (3_000_000, 10), generator=gen, device="cuda")
+    o = route.expert_order(ids, 256)
+    flat = ids.reshape(-1)
+    counts = torch.bincount(flat[flat >= 0], minlength=256)
+    assert torch.equal(o.offsets[1:].long(), counts.cumsum(0)) and int(o.offsets[0]) == 0
+    at = torch.sort(torch.where(flat >= 0, flat, 256), stable=True).indices
+    n = int(counts.sum())
+    assert torch.equal(o.tokens[:n].long(), at[:n] // 10) and bool((o.tokens[n:] == -1).all())
+    places = torch.full_like(flat, -1)
+    places[at[:n]] = torch.arange(n, device="cuda")
+    assert torch.equal(o.places.reshape(-1).long(), places)
 
 
 def _order_fast(ids, e):
