@@ -609,6 +609,9 @@ __global__ void __launch_bounds__(SE * SC) order_scan_kernel(OrderArgs a) {
 }
 
 constexpr int OCLUSTER = 8;         // blocks of a cluster at most
+// Up to so many blocks each adds up the counts before its own; more would read a quadratic number of them (256 experts, 64
+// blocks: 9.0 us, 9.1 with the scan; 32: 7.8 and 8.8; 256: 19 and 14; 4096, 8.4 M pairs: 1194 and 114).
+constexpr int OSCAN = 64;
 
 __device__ __forceinline__ int peer_int(const int* p, int rank) {
   uint32_t r;
@@ -771,7 +774,7 @@ cudaError_t launch_topk(const TopkArgs& args, int dtype, cudaStream_t st) {
 int64_t order_blocks(int64_t pairs) { return (pairs + topk::OBLOCK - 1) / topk::OBLOCK; }
 int64_t order_counts(int64_t pairs) {
   const int64_t b = order_blocks(pairs);
-  return b > topk::OCLUSTER ? b + 1 : 0;   // (and the totals)
+  return b > topk::OCLUSTER ? b + (b > topk::OSCAN ? 1 : 0) : 0;   // (and the totals)
 }
 
 cudaError_t launch_expert_order(const OrderArgs& args, cudaStream_t st) {
@@ -798,9 +801,7 @@ cudaError_t launch_expert_order(const OrderArgs& args, cudaStream_t st) {
   }
   if (a.blocks > 1) {
     cudaError_t e = launch_pdl(topk::order_count_kernel, grid, block, smem, st, a);
-    // Up to 64 blocks each adds up the counts before its own; more would read a quadratic number of them (256 experts, 64
-    // blocks: 9.0 us, 9.1 with the scan; 32: 7.8 and 8.8; 256: 19 and 14; 4096, 8.4 M pairs: 1194 and 114).
-    a.scanned = a.blocks > 64;
+    a.scanned = a.blocks > topk::OSCAN;
     if (e == cudaSuccess && a.scanned)
       e = launch_pdl(topk::order_scan_kernel, dim3((a.experts + topk::SE - 1) / topk::SE), dim3(topk::SE * topk::SC), 0, st, a);
     if (e != cudaSuccess) return e;
