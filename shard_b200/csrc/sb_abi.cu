@@ -1086,6 +1086,8 @@ constexpr int64_t FP4_MAX_K = 65536;      // a row's values stay in the register
 constexpr int64_t FP4_MAX_ROWS = 1 << 30;
 constexpr int64_t FP4_MAX_GROUPS = 1024;
 
+bool off_grid(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+int dtype_bytes(int dtype) { return dtype == SB_F32 ? 4 : 2; }
 bool fp4_fmt(int fmt) { return fmt == SB_FMT_NVFP4 || fmt == SB_FMT_MXFP4; }
 bool fp4_dtype(int dtype) { return dtype == SB_BF16 || dtype == SB_F16 || dtype == SB_F32; }
 int64_t fp4_kp(int64_t k) { return (k + 31) / 32 * 32; }
@@ -1117,6 +1119,7 @@ int fp4_product(const char* what, int fmt, int dtype, const void* const* ptrs, i
   for (int i = 0; i < n_ptrs; ++i) {
     if (!ptrs[i]) return fail(SB_ERR_ARG, "%s: NULL pointer", what);
     if (i < 4 && !aligned16(ptrs[i])) return fail(SB_ERR_ARG, "%s: codes and scales must be 16-byte aligned", what);
+    if (off_grid(ptrs[i], i == 4 ? dtype_bytes(dtype) : 4)) return fail(SB_ERR_ARG, "%s: a misaligned pointer", what);
   }
   return SB_OK;
 }
@@ -1153,7 +1156,9 @@ int sb_fp4_quant(int fmt, const void* x, int dtype, int64_t src_rows, int64_t k,
   if ((!x && src_rows > 0) || !codes || !scales || (nv && !tensor_scale && !row_scale))
     return fail(SB_ERR_ARG, "fp4_quant: NULL pointer");
   if (!aligned16(codes) || !aligned16(scales)) return fail(SB_ERR_ARG, "fp4_quant: codes and scales must be 16-byte aligned");
-  if (reinterpret_cast<uintptr_t>(x) % (dtype == SB_F32 ? 4 : 2)) return fail(SB_ERR_ARG, "fp4_quant: x is misaligned");
+  if (off_grid(x, dtype_bytes(dtype)) || off_grid(rows_in, 4) || off_grid(tensor_scale, 4) || off_grid(offsets, 4) ||
+      off_grid(row_scale, 4))
+    return fail(SB_ERR_ARG, "fp4_quant: a misaligned pointer");
   const size_t need = rows_in ? sb_fp4_quant_workspace_bytes(fmt, src_rows, rows, k) : 0;
   if (need == 0) workspace = nullptr;
   if (workspace && workspace_bytes < need)
@@ -1187,7 +1192,7 @@ int sb_fp4_dequant(int fmt, const void* codes, const void* scales, const float* 
   if (rows == 0) return SB_OK;
   if (!codes || !scales || !y) return fail(SB_ERR_ARG, "fp4_dequant: NULL pointer");
   if (!aligned16(codes) || !aligned16(scales)) return fail(SB_ERR_ARG, "fp4_dequant: codes and scales must be 16-byte aligned");
-  if (reinterpret_cast<uintptr_t>(y) % (dtype == SB_F32 ? 4 : 2)) return fail(SB_ERR_ARG, "fp4_dequant: y is misaligned");
+  if (off_grid(y, dtype_bytes(dtype)) || off_grid(ts, 4)) return fail(SB_ERR_ARG, "fp4_dequant: a misaligned pointer");
   sb::DequantArgs d = {};
   d.codes = (const uint8_t*)codes;
   d.scales = (const uint8_t*)scales;
@@ -1221,6 +1226,7 @@ int sb_fp4_gemm(int fmt, const void* a_codes, const void* a_scales, const float*
   const void* ptrs[] = {a_codes, a_scales, w_codes, w_scales, y};
   if (int rc = fp4_product("fp4_gemm", fmt, dtype, ptrs, 5, m, 1, n, k, n, ldy)) return rc;
   if (fmt == SB_FMT_MXFP4 && (a_ts || w_ts)) return fail(SB_ERR_ARG, "fp4_gemm: MXFP4 has no tensor scale");
+  if (off_grid(a_ts, 4) || off_grid(w_ts, 4)) return fail(SB_ERR_ARG, "fp4_gemm: a misaligned pointer");
   if (m == 0) return SB_OK;
   sb::Fp4MmArgs g = {};
   g.w = (const uint8_t*)w_codes;
@@ -1249,6 +1255,7 @@ int sb_fp4_grouped_gemm(int fmt, const void* a_codes, const void* a_scales, cons
   const void* ptrs[] = {a_codes, a_scales, w_codes, w_scales, y, offsets};
   if (int rc = fp4_product("fp4_grouped_gemm", fmt, dtype, ptrs, 6, m, n_experts, n, k, swiglu ? n / 2 : n, ldy)) return rc;
   if (fmt == SB_FMT_MXFP4 && (a_ts || w_ts)) return fail(SB_ERR_ARG, "fp4_grouped_gemm: MXFP4 has no tensor scale");
+  if (off_grid(a_ts, 4) || off_grid(w_ts, 4) || off_grid(row_weight, 4)) return fail(SB_ERR_ARG, "fp4_grouped_gemm: a misaligned pointer");
   if (swiglu && n % 2) return fail(SB_ERR_SHAPE, "fp4_grouped_gemm: swiglu needs an even N (%lld)", (long long)n);
   if (w_ts && w_ts_n != 1 && w_ts_n != 2) return fail(SB_ERR_ARG, "fp4_grouped_gemm: w_ts_n %d", w_ts_n);
   if (!(limit >= 0.f)) return fail(SB_ERR_ARG, "fp4_grouped_gemm: limit must be >= 0");
@@ -1300,7 +1307,8 @@ int sb_route_topk(const void* logits, int dtype, int64_t tokens, int64_t n_exper
     return fail(SB_ERR_SHAPE, "route_topk: topk %d must lie in 1..16 and in the kept groups' experts", topk);
   if (tokens == 0) return SB_OK;
   if (!logits || !weights || !indices) return fail(SB_ERR_ARG, "route_topk: NULL pointer");
-  if (reinterpret_cast<uintptr_t>(logits) % (dtype == SB_F32 ? 4 : 2)) return fail(SB_ERR_ARG, "route_topk: logits are misaligned");
+  if (off_grid(logits, dtype_bytes(dtype)) || off_grid(bias, 4) || off_grid(weights, 4) || off_grid(indices, 8))
+    return fail(SB_ERR_ARG, "route_topk: a misaligned pointer");
   sb::TopkArgs a = {};
   a.logits = logits;
   a.stride = row_stride;
@@ -1334,7 +1342,8 @@ int sb_expert_order(const int64_t* indices, int64_t tokens, int topk, int64_t n_
   const size_t need = sb_expert_order_workspace_bytes(pairs, n_experts);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(SB_ERR_WORKSPACE, "expert_order: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
-  if (reinterpret_cast<uintptr_t>(workspace) & 3u) return fail(SB_ERR_ARG, "expert_order: workspace must be 4-byte aligned");
+  if (off_grid(workspace, 4) || off_grid(indices, 8) || off_grid(offsets, 4) || off_grid(sorted_tokens, 4) || off_grid(places, 4))
+    return fail(SB_ERR_ARG, "expert_order: a misaligned pointer");
   sb::OrderArgs a = {};
   a.ids = indices;
   a.pairs = pairs;

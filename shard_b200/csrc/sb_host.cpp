@@ -66,6 +66,11 @@ int64_t as_int(PyObject* o) {
   if (v == -1 && PyErr_Occurred()) throw python_error();
   return v;
 }
+// a C int of the entries: what lies outside is refused as the nearest one is
+int as_c_int(PyObject* o) {
+  const int64_t v = as_int(o);
+  return (int)(v < INT32_MIN ? INT32_MIN : v > INT32_MAX ? INT32_MAX : v);
+}
 double as_float(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw python_error();
@@ -220,14 +225,15 @@ PyObject* topk(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Tensor l = tensor(args[0], "topk");
   const int dt = dtype_code(l.scalar_type());
   if (dt < 0 || !l.is_cuda() || l.dim() != 2) REFUSE("topk: logits must be a CUDA tensor [T, E] of bf16, fp16 or fp32");
-  const int64_t t = l.size(0), e = l.size(1), k = as_int(args[1]);
+  const int64_t t = l.size(0), e = l.size(1);
+  const int k = as_c_int(args[1]);
   const Tensor* bias = optional(args[2], "topk");
   const float* bp = bias ? float_values("topk", "bias", l, *bias, e) : nullptr;
   if (e > 1 && l.stride(1) != 1) l = l.contiguous();
-  const int64_t room = k < 0 ? 0 : k;   // (the entry refuses such k)
+  const int64_t room = k < 0 || k > e ? 0 : k;   // (the entry refuses such k)
   Tensor w = empty({t, room}, at::kFloat, l), ids = empty({t, room}, at::kLong, l);
-  const int rc = sb_route_topk(l.data_ptr(), dt, t, e, t > 1 ? l.stride(0) : e, bp, (int)k, (int)as_int(args[3]),
-                               (int)as_int(args[4]), (int)as_int(args[5]), (int)as_int(args[6]), as_bool(args[7]),
+  const int rc = sb_route_topk(l.data_ptr(), dt, t, e, t > 1 ? l.stride(0) : e, bp, k, as_c_int(args[3]),
+                               as_c_int(args[4]), as_c_int(args[5]), as_c_int(args[6]), as_bool(args[7]),
                                (float)as_float(args[8]), w.data_ptr<float>(), ids.data_ptr<int64_t>(), current_stream(l));
   if (rc != SB_OK) return status(rc);
   return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(w)), THPVariable_Wrap(std::move(ids)));
@@ -242,11 +248,11 @@ PyObject* expert_order(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!ids.is_cuda() || ids.scalar_type() != at::kLong || ids.dim() != 2 || !ids.is_contiguous() || ids.size(1) < 1)
     REFUSE("expert_order: indices must be a contiguous CUDA int64 tensor [T, k]");
   const int64_t t = ids.size(0), k = ids.size(1), pairs = t * k, e = as_int(args[1]);
-  const size_t need = sb_expert_order_workspace_bytes(pairs, e);   // (0 for an e that the entry refuses)
-  Tensor offsets = empty({e < 0 ? 0 : e + 1}, at::kInt, ids), tokens = empty({pairs}, at::kInt, ids), places = empty({t, k}, at::kInt, ids);
+  const size_t need = sb_expert_order_workspace_bytes(pairs, e);   // (0 for an e that the entry refuses; e <= 1024)
+  Tensor offsets = empty({e < 0 || e > 1024 ? 0 : e + 1}, at::kInt, ids), tokens = empty({pairs}, at::kInt, ids), places = empty({t, k}, at::kInt, ids);
   Tensor ws;
   if (need) ws = empty({(int64_t)need}, at::kByte, ids);
-  const int rc = sb_expert_order(ids.data_ptr<int64_t>(), t, (int)k, e, offsets.data_ptr<int32_t>(), tokens.data_ptr<int32_t>(),
+  const int rc = sb_expert_order(ids.data_ptr<int64_t>(), t, k > INT32_MAX ? 0 : (int)k, e, offsets.data_ptr<int32_t>(), tokens.data_ptr<int32_t>(),
                                  places.data_ptr<int32_t>(), need ? ws.data_ptr() : nullptr, need, current_stream(ids));
   if (rc != SB_OK) return status(rc);
   return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(offsets)), THPVariable_Wrap(std::move(tokens)),

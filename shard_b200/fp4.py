@@ -23,7 +23,8 @@ per 32 values, the smallest with amax <= 6 s. Roundings are to nearest, ties to 
 non-finite value comes back as NaN, and a row of zeros as zeros.
 
 Every call runs on the tensors' device, on its current stream or on `stream`, allocates its outputs
-through torch and does not synchronise; it can be captured into a CUDA graph. CUDA tensors only.
+through torch and does not synchronise; it can be captured into a CUDA graph. CUDA tensors only. As with
+torch's own operators, the caller orders streams and keeps inputs of another stream until the call has run.
 """
 from __future__ import annotations
 
@@ -78,6 +79,8 @@ def _away(what: str, t: torch.Tensor, stream) -> bool:
 @contextlib.contextmanager
 def _elsewhere(device, stream):
     """`device` made current, and `stream` when one is given (also for the allocations of the call)."""
+    if stream is not None and stream.device != device:
+        raise ValueError(f"a stream of {stream.device} for tensors on {device}")
     with torch.cuda.device(device):
         if stream is None:
             yield

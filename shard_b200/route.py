@@ -41,7 +41,7 @@ def topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, scor
                  scored by its best expert ("max") or the sum of its two best ("top2")
     renormalize  divide the chosen experts' unbiased scores by their sum; then times `scale`
 
-    Values are compared as real numbers, ties go to the lower id. An expert whose logit is NaN, -inf or the
+    Values are compared as real numbers (sums with a bias, or of two: in 64 bits), ties go to the lower id. An expert whose logit is NaN, -inf or the
     type's lowest value is masked: after all others of the kept groups, with weight 0. A bias of -inf keeps an
     expert behind the others too."""
     sc, gs = _SCORE.get(score), _GROUP_SCORE.get(group_score)

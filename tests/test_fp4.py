@@ -7,13 +7,14 @@ tensor core adds K / 64 partial sums in fp32, each with an error of at most 2^-2
     |y - exact| <= (K / 64 + 2) 2^-22 S + (eps_out / 2 + 2^-23) |exact|
 """
 import math
+import types
 
 import pytest
 import torch
 
 import fp4_plain as P
 from shard_b200 import formats as F
-from shard_b200 import fp4
+from shard_b200 import fp4, route
 
 NV, MX = F.FMT_NVFP4, F.FMT_MXFP4
 gpu = pytest.mark.gpu
@@ -59,6 +60,26 @@ def test_quant_and_dequant_are_exact(fmt, dtype, m, k):
         d = (fp4.dequant(q, out).cpu().double() - v).abs()
         lim = v.abs() * (torch.finfo(out).eps / 2 + 2.0 ** -24) + torch.finfo(out).smallest_normal * torch.finfo(out).eps
         assert bool((d <= lim)[v.abs() < torch.finfo(out).max].all())
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k", [(3, 16), (5, 48), (40, 1040), (700, 4112)])
+def test_rows_that_end_inside_a_block_of_32(fmt, dtype, m, k):
+    """K = 16 more than a multiple of 32, loads of 16 bytes; the last half block is the largest, or not finite."""
+    _need_gpu()
+    x = _acts(m, k, dtype, seed=k)
+    x[1, -16:] *= 64
+    x[2, -1] = math.inf
+    _check_quant(x, fp4.quant(x.cuda(), fmt), fmt)
+    rows = torch.tensor([0, m, 2, -1, 1], dtype=torch.int32)
+    q = fp4.quant(x.cuda(), fmt, rows=rows.cuda())
+    z = torch.cat([x, x.new_zeros(1, k)])[[0, m, 2, m, 1]]
+    _check_quant(z, q, fmt)
+    w = fp4.quant(_acts(24, k, dtype, seed=1).cuda(), fmt)
+    y = fp4.gemm(q, w, out_dtype=torch.float32)
+    assert bool((y[[1, 3]] == 0).all()) and bool(y[2].isnan().all()) and bool(y[[0, 4]].isfinite().all())
 
 
 @gpu
@@ -377,6 +398,47 @@ def test_pack_and_dequant_of_a_weight(fmt):
 
 
 @gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+def test_a_bank_of_one_matrix(fmt):
+    _need_gpu()
+    codes, s, ts, _ = P.weights(fmt, 80, 96, seed=4, mats=1)
+    bank = fp4.pack(fmt, codes.cuda(), s.cuda(), None if ts is None else ts.cuda())
+    x = _acts(70, 96, torch.bfloat16, seed=4).cuda()
+    plain = fp4.gemm(fp4.quant(x, fmt), bank)
+    off = torch.tensor([0, 70], dtype=torch.int32, device="cuda")
+    assert torch.equal(fp4.grouped_gemm(fp4.quant(x, fmt, offsets=off), bank), plain)
+
+
+@gpu
+def test_calls_on_two_streams_at_once():
+    """Products of all three forms and a large order, in flight on two streams: each gives what it gives alone."""
+    _need_gpu()
+    x = _acts(2048, 4096, torch.bfloat16, seed=2).cuda()
+    w = fp4.quant(_acts(4096, 4096, torch.bfloat16, seed=3).cuda())
+    ids = torch.randint(0, 256, (40000, 8), device="cuda")
+    off = torch.tensor([0, 700, 701, 2048], dtype=torch.int32, device="cuda")
+    bank = fp4.pack(NV, w.codes.view(1, 4096, -1).repeat(3, 1, 1), w.canonical_scales().view(1, 4096, -1).repeat(3, 1, 1))
+
+    def work():
+        return [fp4.gemm(fp4.quant(x[:m]), w) for m in (1, 40, 2048)] + \
+            [fp4.grouped_gemm(fp4.quant(x, offsets=off), bank), *route.expert_order(ids, 256)]
+
+    want = work()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(4):
+        for st, g in zip(streams, got):
+            with torch.cuda.stream(st):
+                g.append(work())
+    torch.cuda.synchronize()
+    assert fp4.device_error() == 0
+    for g in got:
+        for outs in g:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@gpu
 def test_gated_rows_of_nan_stay_nan():
     """A clamp does not hide a NaN, and only its row has it."""
     _need_gpu()
@@ -438,3 +500,7 @@ def test_refusals_of_tensors():
         fp4.gemm(a, a, out=torch.zeros(4, 5, dtype=torch.bfloat16, device="cuda"))
     with pytest.raises(ValueError):
         fp4.gemm(a, a, out=torch.zeros(4, 4, dtype=torch.bfloat16, device="cuda").t()[:, :])
+    other = types.SimpleNamespace(device=torch.device("cuda", 7 if x.device.index != 7 else 0))
+    for call in (lambda: fp4.quant(x, stream=other), lambda: fp4.gemm(a, a, stream=other), lambda: fp4.dequant(a, stream=other)):
+        with pytest.raises(ValueError, match="stream"):
+            call()

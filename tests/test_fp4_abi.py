@@ -102,3 +102,25 @@ def test_route_refusals():
     assert o(ids=None) == -1 and o(off=None) == -1 and o(tok=None) == -1 and o(pl=None) == -1
     assert o(t=16384, ws=None) == -4 and o(t=16384, ws=FAKE, n=16 * 8 * 4 - 1) == -4
     assert o(t=16384, ws=ctypes.c_void_p(4097), n=1 << 20) == -1
+
+
+def test_misaligned_pointers_are_refused():
+    L = _lib.lib()
+    at = lambda n: ctypes.c_void_p((1 << 12) + n)  # noqa: E731
+    for kw in (dict(rows_in=at(2)), dict(ts=at(2)), dict(off=at(1), groups=2), dict(rs=at(2)), dict(x=at(2), dtype=2)):
+        assert _quant(**kw) == -1, kw
+    assert L.sb_fp4_dequant(NV, FAKE, FAKE, at(2), 0, 4, 64, FAKE, 0, None) == -1
+    for ats, wts, y, dt in ((at(2), None, FAKE, 0), (None, at(1), FAKE, 0), (None, None, at(1), 0), (None, None, at(2), 2)):
+        assert L.sb_fp4_gemm(NV, FAKE, FAKE, ats, 1, 4, FAKE, FAKE, wts, 0, 8, 64, y, dt, 8, None) == -1
+    for off, rw in ((at(2), None), (FAKE, at(2))):
+        assert L.sb_fp4_grouped_gemm(NV, FAKE, FAKE, None, 0, 4, off, FAKE, FAKE, None, 1, 2, 8, 64, 0, 0.0, rw, FAKE, 0, 8, None) == -1
+    for bias, w, i in ((at(2), FAKE, FAKE), (None, at(2), FAKE), (None, FAKE, at(4))):
+        assert L.sb_route_topk(FAKE, 2, 2, 16, 16, bias, 4, 1, 1, 1, 0, 1, 1.0, w, i, None) == -1
+    for ids, off, tok, pl in ((at(4), FAKE, FAKE, FAKE), (FAKE, at(2), FAKE, FAKE), (FAKE, FAKE, at(1), FAKE), (FAKE, FAKE, FAKE, at(2))):
+        assert L.sb_expert_order(ids, 4, 2, 8, off, tok, pl, None, 0, None) == -1
+
+
+def test_expert_order_workspace_holds_the_counts_and_their_totals():
+    f = _lib.lib().sb_expert_order_workspace_bytes
+    assert f(64 * 2048, 256) == 64 * 256 * 4 and f(64 * 2048 + 1, 256) == 66 * 256 * 4
+    assert f(2 ** 31 - 1, 1024) == (2 ** 20 + 1) * 1024 * 4

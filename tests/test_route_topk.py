@@ -200,3 +200,10 @@ def test_refusals_of_tensors():
         route.expert_order(torch.zeros(2, 2, dtype=torch.int32, device="cuda"), 4)
     with pytest.raises(Exception, match="1024"):
         route.expert_order(torch.zeros(2, 2, dtype=torch.int64, device="cuda"), 1025)
+    for k in (2 ** 32 + 1, -2 ** 40):       # not cut to 32 bits, and nothing of that size is allocated
+        with pytest.raises(Exception, match="topk"):
+            route.topk(l, k)
+    with pytest.raises(Exception, match="n_group"):
+        route.topk(l, 2, n_group=2 ** 32 + 1)
+    with pytest.raises(Exception, match="1024"):
+        route.expert_order(torch.zeros(2, 2, dtype=torch.int64, device="cuda"), 2 ** 40)
