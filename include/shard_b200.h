@@ -296,7 +296,7 @@ int sb_fp4_error(int* host_out, void* stream);
 enum sb_group_score { SB_GROUP_MAX = 0, SB_GROUP_TOP2 = 1 };
 /* logits [T, E] of `dtype`, rows row_stride elements apart -> weights fp32 [T, k], indices int64 [T, k] in
  * ranking order. score: sb_score of each logit; selection by score + bias (fp32 [E] or NULL) as real
- * numbers, ties to the lower id; with n_group > 1 (a divisor of E, <= 32) only the experts of the
+ * numbers (sums in 64 bits), ties to the lower id; with n_group > 1 (a divisor of E, <= 32) only the experts of the
  * topk_group best groups (scored by their best expert, or by the sum of their two best) compete. Weights
  * are the unbiased scores, divided by their sum if renormalize, times route_scale. An expert whose logit
  * is NaN, -inf or the type's lowest value is masked: it comes after every other of the kept groups, with
