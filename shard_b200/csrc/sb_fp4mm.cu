@@ -14,9 +14,9 @@
 // Stages hold 256 K: 128 weight rows and the token rows of 128 bytes each, landed by TMA in the 128-byte-
 // swizzled K-major form, and their scale atoms. Roles (352 threads): warp 8 copies codes, warp 9 scales,
 // warp 10 moves scale atoms to tensor memory and issues the MMAs, warps 0-7 read the accumulator (a
-// thread: one weight row, every other 32 columns) and store. Two accumulators of up to 192 columns
-// alternate, so that one tile's readback overlaps the next tile's products; 192 and not 256 leaves room
-// for the scales beside two of them.
+// thread: one weight row, every other 32 columns) and store. Two accumulators alternate, so that one tile's
+// readback overlaps the next tile's products: of up to 192 columns each, or in pairs of 256, which share 64
+// columns to leave room for the scales; the readback begins with those and releases them at once.
 //
 // Every wait is bounded: on timeout the CTA sets the device's error word and winds down.
 #include <cudaTypedefs.h>
@@ -39,13 +39,14 @@ constexpr int CODE_WARP = 8;         // copies codes,
 constexpr int SCALE_WARP = 9;        // and their scales
 constexpr int MMA_WARP = 10;
 constexpr int NTHREADS = 352;
-constexpr int NT_MAX = 192;          // token columns of a tile
+constexpr int NT_MAX = 256;          // token columns of a tile: 256 in a pair, elsewhere up to
+constexpr int NT_APART = 192;        // so many, whose two accumulators lie side by side
 constexpr int BOX = 32;              // token rows of one copy with expert groups
 constexpr int A_BYTES = 128 * 128;   // a stage's weight rows
 constexpr int MAX_STAGES = 10;
 constexpr int MAX_MATS = 1024;
 constexpr int TMEM_COLS = 512;
-constexpr int SFA_COL = 2 * NT_MAX;  // scale factors: 4 atoms x 4 columns of the weights,
+constexpr int SFA_COL = NT_APART + NT_MAX;  // scale factors: 4 atoms x 4 columns of the weights,
 constexpr int SFB_COL = SFA_COL + 16;  // 4 atoms x 8 columns of the tokens (two row blocks)
 constexpr uint32_t WAIT_LIMIT = 1u << 16;
 constexpr int SMEM_LIMIT = 232448;
@@ -73,7 +74,7 @@ struct Args {
 };
 
 struct Ctl {
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES], accfull[2], accempty[2], drain;
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], accfull[2], accempty[2], shared, drain;
   uint32_t tmem_base;
   int abort;
   alignas(128) uint8_t turn[EPI_WARPS][2048];       // 32 rows x 32 outputs of 16 bits, to be turned
@@ -260,8 +261,10 @@ __device__ __forceinline__ Tile tile_at(const Args& a, const Ctl& c, int i) {
   t.mat = lo;
   t.n0 = (band * 12 + left % wide) * MT;
   t.row0 = c.rows[lo];
-  t.t0 = left / wide * a.nt;
-  t.cnt = min(c.rows[lo + 1] - t.row0 - t.t0, a.nt);
+  // a group's tokens in tiles alike, of whole 64-row steps of the scale atoms
+  const int all = c.rows[lo + 1] - t.row0, each = tb > 1 ? ((all + tb - 1) / tb + 63) & ~63 : a.nt;
+  t.t0 = left / wide * each;
+  t.cnt = min(all - t.t0, each);
   t.blk = (a.g.offsets ? (t.row0 >> 7) + lo : 0) + (t.t0 >> 7);
   return t;
 }
@@ -440,6 +443,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
       mbar_init(smem_addr(&c.accfull[q]), 1);
       mbar_init(smem_addr(&c.accempty[q]), PAIR ? 2 * EPI_WARPS : EPI_WARPS);
     }
+    mbar_init(smem_addr(&c.shared), 2 * EPI_WARPS);
     mbar_init(smem_addr(&c.drain), 1);
     c.abort = 0;
     mbar_init_fence();
@@ -560,10 +564,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
       const int kfull = a.ksteps >> 2, ktail = a.ksteps & 3;
       for (int i = first; ok && i < total; i += stride, ++n) {
         const Tile t = tile_at<PAIR>(a, c, i);
-        const uint32_t q = n & 1u, acc = tbase + q * NT_MAX;
+        const uint32_t q = n & 1u, acc = tbase + q * NT_APART;
         const uint32_t sfb = tbase + SFB_COL + ((t.t0 & 127) >> 5);
         const uint32_t id = idesc<NV, PAIR>(PAIR ? (uint32_t)(t.cnt + 15) & ~15u : (uint32_t)(t.cnt + 7) & ~7u);
         if (!wait(abortf, smem_addr(&c.accempty[q]), ((n >> 1) & 1u) ^ 1u)) break;
+        if (PAIR && a.nt > NT_APART && n > 0 && !wait(abortf, smem_addr(&c.shared), (n - 1) & 1u)) break;
         fence_after();
         auto stage = [&](auto blocks, auto whole, int k) {
           if (!wait(abortf, full0 + 8 * s, ph, g.probes)) {
@@ -634,7 +639,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
       __syncwarp();
       if constexpr (FORM != SPLIT) look_ahead(i + stride);
       const uint32_t q = n & 1u;
-      const uint32_t acc = tbase + q * NT_MAX + quarter;
+      const uint32_t acc = tbase + q * NT_APART + quarter;
       const int row = t.n0 + rank * 128 + (warp & 3) * 32 + lane;
       const bool vec = a.vec && (t.n0 + rank * 128 + 128 <= g.n || (SWIGLU ? g.n % 16 : g.n % 8) == 0);
       const int64_t tok0 = (int64_t)t.row0 + t.t0;
@@ -652,24 +657,29 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
         }
         break;
       }
-      bool held = true;   // this warp has yet to read the accumulator's last chunk
-      for (int ch = half, j = 0; ch * 32 < t.cnt; ch += 2, ++j) {
+      // This warp's chunks, those in the columns that the next tile's accumulator shares first: the last ones of the lower
+      // accumulator, the first ones of the upper.
+      const int mine = ((t.cnt + 31) / 32 - half + 1) >> 1;
+      const bool overlaps = PAIR && a.nt > NT_APART;
+      for (int u = 0; u < mine; ++u) {
+        const int j = overlaps && q == 0 ? mine - 1 - u : u, ch = half + 2 * j;
         uint32_t d[32];
         ld32(acc + ch * 32, d);
         ld_wait();
-        if ((ch + 2) * 32 >= t.cnt) {
-          held = false;
+        if (u == mine - 1 || (overlaps && u == 0)) {
           fence_before();
           __syncwarp();
-          if (lane == 0) release<PAIR>(smem_addr(&c.accempty[q]));
+          if (lane == 0 && overlaps && u == 0) release<PAIR>(smem_addr(&c.shared));
+          if (lane == 0 && u == mine - 1) release<PAIR>(smem_addr(&c.accempty[q]));
         }
         const int left = t.cnt - ch * 32;
         if (left >= 32) store_chunk<SWIGLU, true, T>(a, d, tok0 + ch * 32, row, lane, 32, vec, wts, sc + 32 * j, wt + 32 * j, turn);
         else store_chunk<SWIGLU, false, T>(a, d, tok0 + ch * 32, row, lane, left, vec, wts, sc + 32 * j, wt + 32 * j, turn);
       }
-      if (held) {
+      if (mine <= 0) {
         fence_before();
         __syncwarp();
+        if (lane == 0 && overlaps) release<PAIR>(smem_addr(&c.shared));
         if (lane == 0) release<PAIR>(smem_addr(&c.accempty[q]));
       }
       __syncwarp();
@@ -812,7 +822,7 @@ cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
   if (g.offsets != nullptr) {
     const int avg = (g.m + g.mats - 1) / g.mats;
     a.nt = avg > 128 ? 192 : 128;
-  } else if (g.m <= NT_MAX) {
+  } else if (g.m <= NT_APART) {
     a.nt = (g.m + 15) & ~15;
   } else {
     const int c128 = (g.m + 127) / 128 * 128, c192 = (g.m + 191) / 192 * 192;
@@ -825,6 +835,9 @@ cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
   // Pairs where tiles of full width are many: they halve the token bytes that each SM copies and reads per product
   // (8192 cubed: 274 us without, 248 with); narrow tiles are bound by the weights, which pairs do not share.
   const bool pair = a.nt >= 128 && g.m >= 128 * (int64_t)g.mats && tiles >= 2 * sms;
+  // A pair's tiles have 256 tokens: fewer bytes of shared memory per product than 192, which have both accumulators to
+  // themselves (8192 x 4096 x 8192: 104 us and 124; x 2048: 45 and 54; x 512: even; 32 groups of 512 tokens: even).
+  if (pair) a.nt = 256;
   // K is split, for one token tile, as far as the SMs go and every piece keeps two stages (one token against 4096 x 8192:
   // 12.0 us whole, 9.3 in four pieces, 8.6 with the weights ahead in L2).
   a.split = 1;
