@@ -45,6 +45,7 @@ constexpr int BOX = 32;              // token rows of one copy with expert group
 constexpr int A_BYTES = 128 * 128;   // a stage's weight rows
 constexpr int MAX_STAGES = 10;
 constexpr int MAX_MATS = 1024;
+constexpr int RING = 16;             // tiles found ahead of their products and readback: more than MAX_STAGES + 3
 constexpr int TMEM_COLS = 512;
 constexpr int SFA_COL = NT_APART + NT_MAX;  // scale factors: 4 atoms x 4 columns of the weights,
 constexpr int SFB_COL = SFA_COL + 16;  // 4 atoms x 8 columns of the tokens (two row blocks)
@@ -74,12 +75,14 @@ struct Args {
 };
 
 struct Ctl {
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES], accfull[2], accempty[2], shared, drain;
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], accfull[2], accempty[2], shared, drain, told[RING];
   uint32_t tmem_base;
   int abort;
   alignas(128) uint8_t turn[EPI_WARPS][2048];       // 32 rows x 32 outputs of 16 bits, to be turned
   alignas(16) float scale[EPI_WARPS][NT_MAX / 2];   // of each warp's tokens: tensor scale,
   alignas(16) float weight[EPI_WARPS][NT_MAX / 2];  // row weight
+  int4 tile[RING];           // of each tile: matrix, first weight row, first row of its tokens, tokens
+  int tile_t0[RING];         // and its first token in the group
   int tiles[MAX_MATS + 1];   // tiles before each matrix
   int rows[MAX_MATS + 1];    // first token row of each matrix's group, and the end of the last
 };
@@ -181,8 +184,10 @@ __device__ __forceinline__ uint32_t in_first(uint32_t addr) {
   asm("mapa.shared::cluster.u32 %0, %1, 0;\n" : "=r"(r) : "r"(addr));
   return r;
 }
+// Without release: what it follows are reads of tensor memory, whose values this thread holds. (A release at cluster scope
+// waits for the stores to y before it: 1000 cycles twice a tile, in the readback and in the products that wait for it.)
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
 // arrive on the accumulator's barrier where the MMAs are issued
 template <bool PAIR>
@@ -444,6 +449,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
       mbar_init(smem_addr(&c.accempty[q]), PAIR ? 2 * EPI_WARPS : EPI_WARPS);
     }
     mbar_init(smem_addr(&c.shared), 2 * EPI_WARPS);
+    for (int r = 0; r < RING; ++r) mbar_init(smem_addr(&c.told[r]), 1);
     mbar_init(smem_addr(&c.drain), 1);
     c.abort = 0;
     mbar_init_fence();
@@ -508,13 +514,21 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
 
   if (warp == CODE_WARP || warp == SCALE_WARP) {
     if (elect_one()) {
-      uint32_t it = 0, s = 0, ph = 1;
+      uint32_t it = 0, s = 0, ph = 1, n = 0;
       bool ok = true;
       const bool codes = warp == CODE_WARP;
       const uint32_t own0 = smem_addr(&c.full[0]), full0 = PAIR ? in_first(own0) : own0, empty0 = smem_addr(&c.empty[0]);
       const uint32_t a0 = smem_addr(sA), b0 = smem_addr(sB), s0 = smem_addr(sS);
-      for (int i = first; ok && i < total; i += stride) {
+      for (int i = first; ok && i < total; i += stride, ++n) {
         const Tile t = tile_at<PAIR>(a, c, i);
+        if (!codes) {
+          // For the products and the readback, which would find it in 700 to 1100 cycles a tile. The place is free: the last
+          // stage of the tile before was, so that a tile at most MAX_STAGES before that one was begun, and the readback
+          // of the second before it is over.
+          c.tile[n % RING] = make_int4(t.mat, t.n0, t.row0 + t.t0, t.cnt);
+          c.tile_t0[n % RING] = t.t0;
+          arrive(smem_addr(&c.told[n % RING]));
+        }
         // token rows that this CTA brings: all, or its half of the pair's columns
         const int half = PAIR ? ((t.cnt + 15) >> 4) << 3 : t.cnt;
         const int nbox = (half + a.box - 1) / a.box;
@@ -563,10 +577,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
       const uint32_t full0 = smem_addr(&c.full[0]), empty0 = smem_addr(&c.empty[0]);
       const int kfull = a.ksteps >> 2, ktail = a.ksteps & 3;
       for (int i = first; ok && i < total; i += stride, ++n) {
-        const Tile t = tile_at<PAIR>(a, c, i);
+        if (!wait(abortf, smem_addr(&c.told[n % RING]), (n / RING) & 1u)) break;
+        const int cnt = c.tile[n % RING].w, t0 = c.tile_t0[n % RING];
         const uint32_t q = n & 1u, acc = tbase + q * NT_APART;
-        const uint32_t sfb = tbase + SFB_COL + ((t.t0 & 127) >> 5);
-        const uint32_t id = idesc<NV, PAIR>(PAIR ? (uint32_t)(t.cnt + 15) & ~15u : (uint32_t)(t.cnt + 7) & ~7u);
+        const uint32_t sfb = tbase + SFB_COL + ((t0 & 127) >> 5);
+        const uint32_t id = idesc<NV, PAIR>(PAIR ? (uint32_t)(cnt + 15) & ~15u : (uint32_t)(cnt + 7) & ~7u);
         if (!wait(abortf, smem_addr(&c.accempty[q]), ((n >> 1) & 1u) ^ 1u)) break;
         if (PAIR && a.nt > NT_APART && n > 0 && !wait(abortf, smem_addr(&c.shared), (n - 1) & 1u)) break;
         fence_after();
@@ -588,7 +603,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
           for (int k = kbegin; ok && k < min(kend, kfull); ++k) stage(blocks, std::true_type{}, k);
           if (ok && kfull < kend) stage(blocks, std::false_type{}, kfull);
         };
-        if ((t.t0 & 127) + t.cnt > 128) tile(std::integral_constant<int, 2>{});
+        if ((t0 & 127) + cnt > 128) tile(std::integral_constant<int, 2>{});
         else tile(std::integral_constant<int, 1>{});
         if (ok) commit_to<PAIR>(smem_addr(&c.accfull[q]));
       }
@@ -606,30 +621,33 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
     const uint32_t turn = smem_addr(c.turn[warp]);
     float* sc = c.scale[warp];
     float* wt = c.weight[warp];
-    // a tile's place, scales and weights are found while the one before it is stored (1900 cycles a tile otherwise)
-    Tile next;
+    // a tile's place, scales and weights are fetched while the one before it is stored (1900 cycles a tile otherwise)
+    int4 next = make_int4(0, 0, 0, 0);
     float s_next[CHUNKS], w_next[CHUNKS], wts_next = 1.f;
-    auto look_ahead = [&](int i) {
-      if (i >= total) return;
-      next = tile_at<PAIR>(a, c, i);
-      const int row = next.n0 + rank * 128 + (warp & 3) * 32 + lane;
+    auto look_ahead = [&](int i, uint32_t n) {
+      if (i >= total) return true;
+      if (!warp_wait(abortf, smem_addr(&c.told[n % RING]), (n / RING) & 1u, 0u)) return false;
+      next = c.tile[n % RING];
+      const int row = next.y + rank * 128 + (warp & 3) * 32 + lane;
       wts_next = 1.f;
       if (g.w_ts != nullptr && row < g.n)
-        wts_next = g.w_ts[g.w_ts_n == 0 ? row : next.mat * g.w_ts_n + (g.w_ts_n == 2 ? (row & 1) : 0)];
+        wts_next = g.w_ts[g.w_ts_n == 0 ? row : next.x * g.w_ts_n + (g.w_ts_n == 2 ? (row & 1) : 0)];
 #pragma unroll
       for (int j = 0; j < CHUNKS; ++j) {
         const int col = 32 * (half + 2 * j) + lane;
-        const int64_t tok = (int64_t)next.row0 + next.t0 + col;
+        const int64_t tok = (int64_t)next.z + col;
         s_next[j] = w_next[j] = 1.f;
-        if (col < next.cnt) {
+        if (col < next.w) {
           if (g.a_ts != nullptr) s_next[j] = g.a_ts[g.a_ts_row ? tok : 0];
           if (g.row_weight != nullptr) w_next[j] = g.row_weight[tok];
         }
       }
+      return true;
     };
-    look_ahead(first);
-    for (int i = first; i < total; i += stride, ++n) {
-      const Tile t = next;
+    bool ok = look_ahead(first, 0u);
+    for (int i = first; ok && i < total; i += stride, ++n) {
+      const int n0 = next.y + rank * 128, cnt = next.w;
+      const int64_t tok0 = next.z;
       const float wts = wts_next;
 #pragma unroll
       for (int j = 0; j < CHUNKS; ++j) {
@@ -637,18 +655,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
         if (SWIGLU) wt[32 * j + lane] = w_next[j];
       }
       __syncwarp();
-      if constexpr (FORM != SPLIT) look_ahead(i + stride);
+      if constexpr (FORM != SPLIT) ok = look_ahead(i + stride, n + 1);
       const uint32_t q = n & 1u;
       const uint32_t acc = tbase + q * NT_APART + quarter;
-      const int row = t.n0 + rank * 128 + (warp & 3) * 32 + lane;
-      const bool vec = a.vec && (t.n0 + rank * 128 + 128 <= g.n || (SWIGLU ? g.n % 16 : g.n % 8) == 0);
-      const int64_t tok0 = (int64_t)t.row0 + t.t0;
-      if (!warp_wait(abortf, smem_addr(&c.accfull[q]), (n >> 1) & 1u, g.probes)) break;
+      const int row = n0 + (warp & 3) * 32 + lane;
+      const bool vec = a.vec && (n0 + 128 <= g.n || (SWIGLU ? g.n % 16 : g.n % 8) == 0);
+      if (!ok || !warp_wait(abortf, smem_addr(&c.accfull[q]), (n >> 1) & 1u, g.probes)) break;
       fence_after();
       if constexpr (FORM == SPLIT) {
         // the products have read all stages: their place takes this piece's sums, [token][row]
         float* part = reinterpret_cast<float*>(base);
-        for (int ch = half; ch * 32 < t.cnt; ch += 2) {
+        for (int ch = half; ch * 32 < cnt; ch += 2) {
           uint32_t d[32];
           ld32(acc + ch * 32, d);
           ld_wait();
@@ -659,7 +676,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
       }
       // This warp's chunks, those in the columns that the next tile's accumulator shares first: the last ones of the lower
       // accumulator, the first ones of the upper.
-      const int mine = ((t.cnt + 31) / 32 - half + 1) >> 1;
+      const int mine = ((cnt + 31) / 32 - half + 1) >> 1;
       const bool overlaps = PAIR && a.nt > NT_APART;
       for (int u = 0; u < mine; ++u) {
         const int j = overlaps && q == 0 ? mine - 1 - u : u, ch = half + 2 * j;
@@ -672,7 +689,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
           if (lane == 0 && overlaps && u == 0) release<PAIR>(smem_addr(&c.shared));
           if (lane == 0 && u == mine - 1) release<PAIR>(smem_addr(&c.accempty[q]));
         }
-        const int left = t.cnt - ch * 32;
+        const int left = cnt - ch * 32;
         if (left >= 32) store_chunk<SWIGLU, true, T>(a, d, tok0 + ch * 32, row, lane, 32, vec, wts, sc + 32 * j, wt + 32 * j, turn);
         else store_chunk<SWIGLU, false, T>(a, d, tok0 + ch * 32, row, lane, left, vec, wts, sc + 32 * j, wt + 32 * j, turn);
       }
