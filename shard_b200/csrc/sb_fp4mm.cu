@@ -62,6 +62,7 @@ __device__ int g_err;
 struct Args {
   CUtensorMap map_w, map_a;     // codes
   CUtensorMap map_ws, map_as;   // scale atoms
+  CUtensorMap map_n;            // token codes of a pair's narrower tiles
   Fp4MmArgs g;
   int nt;            // token columns of a full tile (a multiple of 64 when a matrix has several)
   int box;           // token rows of one copy
@@ -531,10 +532,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
         }
         // token rows that this CTA brings: all, or its half of the pair's columns
         const int half = PAIR ? ((t.cnt + 15) >> 4) << 3 : t.cnt;
-        const int nbox = (half + a.box - 1) / a.box;
+        const bool narrow = PAIR && half <= NT_APART / 2;
+        const int box = narrow ? NT_APART / 2 : a.box, nbox = (half + box - 1) / box;
+        const CUtensorMap* map_a = narrow ? &a.map_n : &a.map_a;
         const int wrow = t.mat * g.n + t.n0 + rank * 128, arow = t.row0 + t.t0 + rank * half;
         const int wblk = t.mat * ((g.n + 127) >> 7) + (t.n0 >> 7) + rank;
-        const uint32_t bytes = (PAIR ? 2u : 1u) * (codes ? A_BYTES + nbox * a.box * 128 : s_bytes);
+        const uint32_t bytes = (PAIR ? 2u : 1u) * (codes ? A_BYTES + nbox * box * 128 : s_bytes);
         for (int k = kbegin; k < kend; ++k, ++it) {
           if (!wait(abortf, empty0 + 8 * s, ph)) {
             ok = false;
@@ -545,7 +548,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
           if (codes) {
             load_2d<PAIR>(a0 + s * A_BYTES, &a.map_w, k * 128, wrow, full);
             const uint32_t dst = b0 + s * a.b_bytes;
-            for (int b = 0; b < nbox; ++b) load_2d<PAIR>(dst + b * a.box * 128, &a.map_a, k * 128, arow + b * a.box, full);
+            for (int b = 0; b < nbox; ++b) load_2d<PAIR>(dst + b * box * 128, map_a, k * 128, arow + b * box, full);
           } else {
             const uint32_t dst = s0 + s * s_bytes;
             const int at = k * (NV ? 4 : 2);
@@ -878,6 +881,7 @@ cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
   const uint32_t along = g.nv ? 4 : 2;
   cudaError_t e = code_map(&a.map_w, g.w, (uint64_t)g.mats * g.n, row_bytes, 128);
   if (e == cudaSuccess) e = code_map(&a.map_a, g.a, (uint64_t)g.m, row_bytes, (uint32_t)a.box);
+  if (e == cudaSuccess && pair) e = code_map(&a.map_n, g.a, (uint64_t)g.m, row_bytes, NT_APART / 2);
   if (e == cudaSuccess) e = scale_map(&a.map_ws, g.w_s, (uint64_t)g.mats * nb, (uint64_t)atoms, 1, along);
   if (e == cudaSuccess) e = scale_map(&a.map_as, g.a_s, a_blocks, (uint64_t)atoms, (uint32_t)a.sblk, along);
   if (e != cudaSuccess) return e;
