@@ -852,9 +852,11 @@ cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
   const int64_t nb = (g.n + 127) / 128;
   const int64_t tt = g.offsets ? (int64_t)g.m / a.nt + (g.mats < g.m ? g.mats : g.m) : (g.m + a.nt - 1) / a.nt;
   const int64_t tiles = tt * nb;
-  // Pairs where tiles of full width are many: they halve the token bytes that each SM copies and reads per product
-  // (8192 cubed: 274 us without, 248 with); narrow tiles are bound by the weights, which pairs do not share.
-  const bool pair = a.nt >= 128 && g.m >= 128 * (int64_t)g.mats && tiles >= 2 * sms;
+  // Pairs where tiles of full width need more than one round of the SMs: they halve the token bytes that each SM copies and
+  // reads per product (1024 x 4096 x 8192: 18.0 us, 26.3 without; 2048 x 2048 x 4096: 12.7 and 16.0). With fewer tiles single
+  // CTAs use more SMs (256 x 8192 x 8192: 15.0, pairs 17.8), and narrow tiles are bound by the weights, which pairs do not
+  // share.
+  const bool pair = a.nt >= 128 && g.m >= 128 * (int64_t)g.mats && tiles > sms;
   // A pair's tiles have 256 tokens: fewer bytes of shared memory per product than 192, which have both accumulators to
   // themselves (8192 x 4096 x 8192: 104 us and 124; x 2048: 45 and 54; x 512: even; 32 groups of 512 tokens: even).
   if (pair) a.nt = 256;
