@@ -18,6 +18,8 @@
 // its own atoms and any row finds its place from the offsets alone.
 //
 // Both directions are bound by HBM at prompt sizes and by launch latency at one row.
+#include <type_traits>
+
 #include "sb_device.cuh"
 #include "sb_fp4.h"
 #include "sb_launch.h"
@@ -144,12 +146,16 @@ struct Unit {
       w[i] = a | (b << 16);
     }
   }
-  // bits of the largest magnitude as fp32 (0x7F800000 and above: not finite)
-  __device__ __forceinline__ uint32_t amax() const {
+  // bits of the largest magnitude (INF and above: not finite)
+  __device__ __forceinline__ uint32_t hmax() const {
     uint32_t m = w[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) m = Traits<T>::max2(m, w[i]);
-    const uint32_t h = max(m & 0x7FFFu, (m >> 16) & 0x7FFFu);
+    return max(m & 0x7FFFu, (m >> 16) & 0x7FFFu);
+  }
+  // and as fp32 (0x7F800000 and above: not finite)
+  __device__ __forceinline__ uint32_t amax() const {
+    const uint32_t h = hmax();
     return h >= Traits<T>::INF ? 0x7FC00000u : __float_as_uint(Traits<T>::f(h));
   }
   __device__ __forceinline__ float get(int i) const {
@@ -193,75 +199,75 @@ constexpr uint32_t F32_INF = 0x7F800000u;
 // one factor serves). With one scale per row such values are common: there 6 p is the row's largest value in
 // its own block.
 template <typename T>
-__device__ __forceinline__ uint32_t lean(float p, float e) {
+__device__ __forceinline__ uint32_t lean(float p, float e, float first) {   // of the mantissas first (1 or 5) and first + 2
   uint32_t need = 0u;
 #pragma unroll
-  for (int m = 1; m < 8; m += 2) {
-    const float k = (float)m;
+  for (int m = 0; m < 2; ++m) {
+    const float k = m ? first + 2.f : first;
     const uint32_t b = __float_as_uint(p * k);
     const float g = __uint_as_float((b + (Traits<T>::BELOW + 1u) / 2u) & ~Traits<T>::BELOW);
     const float r = fmaf(-k, e, fmaf(-k, p, g));
-    const uint32_t side = r > 0.f || (r == 0.f && (m & 2)) ? 2u : 1u;
+    const uint32_t side = r > 0.f || (r == 0.f && m) ? 2u : 1u;
     if (((b + 16u) & Traits<T>::BELOW) <= 32u) need |= side;
   }
   return need;
 }
-template <>
-__device__ __forceinline__ uint32_t lean<float>(float, float) { return 3u; }
 
-// lean() depends on the mantissas of s and ts alone, and an e4m3 value has one of eight: for a row's ts, bit m of
-// `down` and `up` is its answer for the mantissa 1 + m / 8 (each lane finds one: 66 instructions a unit otherwise).
-struct Leans {
-  uint32_t down, up;
-};
+// What x is multiplied by for the scale s ts, turned as lean() says, but for s's exponent: for a row's ts, lane m < 8 holds
+// it for the subnormal scale m / 8 2^-6, lane 8 + m for the mantissa 1 + m / 8 (times 2^-7). Below 0: no one factor
+// serves. (Found once per row, each half warp two of lean()'s borders: as many as 66 instructions a unit otherwise.)
 template <typename T>
-__device__ __forceinline__ Leans leans(float ts, int lane) {
-  const float s = 1.f + 0.125f * (float)(lane & 7), p = s * ts;
-  const uint32_t need = lean<T>(p, fmaf(s, ts, -p));
-  return {__ballot_sync(0xffffffffu, need & 1u), __ballot_sync(0xffffffffu, need & 2u)};
+__device__ __forceinline__ float factors(float ts, int lane) {
+  const float s = (float)((lane & 7) + (lane & 8)) * ((lane & 8) ? 0.0009765625f : 0.001953125f);
+  const float p = s * ts, inv = rcp(p), e = fmaf(s, ts, -p);
+  uint32_t need = lean<T>(p, e, lane < 16 ? 1.f : 5.f);
+  need |= __shfl_xor_sync(0xffffffffu, need, 16);
+  const float f = need == 0u ? inv : need == 1u ? inv * (1.f - 4.8e-7f) : need == 2u ? inv * (1.f + 4.8e-7f) : -inv;
+  return s == 0.f ? 0.f : f;
 }
 
-// the unit's 16 codes for the scale s ts (NVFP4)
+// the unit's 16 codes of x f
 template <typename T>
-__device__ __forceinline__ uint2 codes_nv(const Unit<T>& u, float s, float ts, bool mid, const Leans& ln) {
+__device__ __forceinline__ uint2 codes_by(const Unit<T>& u, float f) {
+  uint32_t out[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float a[8];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) mul2(u.get(8 * h + i), u.get(8 * h + i + 1), f, a[i], a[i + 1]);
+    out[h] = cvt8(a);
+  }
+  return make_uint2(out[0], out[1]);
+}
+
+// the unit's 16 codes for the scale s ts (NVFP4), from both ends of an interval around each quotient; mid: ts in mid_range
+template <typename T>
+__device__ __forceinline__ uint2 codes_nv(const Unit<T>& u, float s, float ts, bool mid) {
   if (s == 0.f) return make_uint2(0u, 0u);
   uint32_t out[2];
   if (mid) {
     const float p = s * ts, inv = rcp(p);
-    const uint32_t m = (__float_as_uint(s) >> 20) & 7u;
-    const bool down = (ln.down >> m) & 1u, up = (ln.up >> m) & 1u;
-    if (!(down && up)) {
-      const float f = down ? inv * (1.f - 4.8e-7f) : (up ? inv * (1.f + 4.8e-7f) : inv);
+    const float e = fmaf(s, ts, -p);   // s ts = p + e exactly
+    const float lo = inv * (1.f - 9.6e-7f), hi = inv * (1.f + 9.6e-7f);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float a[8];
+    for (int h = 0; h < 2; ++h) {
+      float a[8], b[8];
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) mul2(u.get(8 * h + i), u.get(8 * h + i + 1), f, a[i], a[i + 1]);
-        out[h] = cvt8(a);
+      for (int i = 0; i < 8; i += 2) {
+        const float x0 = u.get(8 * h + i), x1 = u.get(8 * h + i + 1);
+        mul2(x0, x1, lo, a[i], a[i + 1]);
+        mul2(x0, x1, hi, b[i], b[i + 1]);
       }
-    } else {
-      const float e = fmaf(s, ts, -p);   // s ts = p + e exactly
-      const float lo = inv * (1.f - 9.6e-7f), hi = inv * (1.f + 9.6e-7f);
+      out[h] = cvt8(a);
+      const uint32_t diff = out[h] ^ cvt8(b);
+      if (diff != 0u) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float a[8], b[8];
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const float x0 = u.get(8 * h + i), x1 = u.get(8 * h + i + 1);
-          mul2(x0, x1, lo, a[i], a[i + 1]);
-          mul2(x0, x1, hi, b[i], b[i + 1]);
-        }
-        out[h] = cvt8(a);
-        const uint32_t diff = out[h] ^ cvt8(b);
-        if (diff != 0u) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if ((diff >> (4 * i)) & 0xFu) {
-              // |x| - m (p + e): the first difference is exact this near to the border m p
-              const uint32_t c = (out[h] >> (4 * i)) & 7u;
-              const float m = border(c), r = fmaf(-m, e, fmaf(-m, p, fabsf(u.get(8 * h + i))));
-              if (r > 0.f || (r == 0.f && (c & 1u))) out[h] += 1u << (4 * i);
-            }
+        for (int i = 0; i < 8; ++i) {
+          if ((diff >> (4 * i)) & 0xFu) {
+            // |x| - m (p + e): the first difference is exact this near to the border m p
+            const uint32_t c = (out[h] >> (4 * i)) & 7u;
+            const float m = border(c), r = fmaf(-m, e, fmaf(-m, p, fabsf(u.get(8 * h + i))));
+            if (r > 0.f || (r == 0.f && (c & 1u))) out[h] += 1u << (4 * i);
           }
         }
       }
@@ -279,6 +285,15 @@ __device__ __forceinline__ uint2 codes_nv(const Unit<T>& u, float s, float ts, b
     }
   }
   return make_uint2(out[0], out[1]);
+}
+// Out of line, for the units whose scale lies next to a border or whose codes no one factor serves, and those that are not
+// finite: codes, scale.
+template <typename T>
+__device__ __noinline__ uint3 unit_rare(Unit<T> u, uint32_t h, float ts, float inv6) {
+  if (h >= Traits<T>::INF) return make_uint3(0u, 0u, 0x7Fu);
+  const uint32_t sc = scale_code(Traits<T>::f(h), ts, inv6, true);
+  const uint2 c = codes_nv<T>(u, e4m3_to_f32(sc), ts, true);
+  return make_uint3(c.x, c.y, sc);
 }
 
 template <typename T>
@@ -316,19 +331,22 @@ __device__ __forceinline__ int64_t place(const QuantArgs& a, int64_t row, int la
   return o < 0 || o > row || pos >= a.blocks * 128 ? -1 : pos;
 }
 
-// A row's wpr warps take its units (16 values a thread) in turn, V at a time with their loads issued together. With
-// one tensor scale per row the row is read twice, first for its largest value, then, from L1, for its
-// codes. (Blocks that take rows in turn, as many as fit at once: 45 us for 8192 x 7168 NVFP4; a block for every few
-// rows: 41.)
-constexpr int QUANT_WARPS = 8;
+// A row's warps take its units (16 values a thread) in turn, V at a time with their loads issued together. With
+// one tensor scale per row the row is read twice, first for its largest value and each unit's, which are kept in shared
+// memory, then, from L1 or L2, for its codes. 118 instructions a unit and 250 a warp and row bound it (NVFP4, 8192 x
+// 7168: 37 us, 4.1 TB/s; with the caller's scale 29; MXFP4 25). (Blocks that take rows in turn: 45 against 41 at the time.)
+constexpr int QUANT_WARPS = 8;    // warps of a row at most
+constexpr int QUANT_FIRST = 4;    // units in flight while a row's largest value is found
 
 template <typename T, bool NV, int V, bool VEC>
 __global__ void __launch_bounds__(QUANT_WARPS * 32, 4) quant_kernel(QuantArgs a) {
+  // 16-bit values with a scale per row: the units' largest magnitudes, of each thread's own
+  constexpr bool HALF = NV && sizeof(T) == 2;
+  constexpr int W = V == 1 ? 1 : QUANT_FIRST;
   __shared__ uint32_t red[QUANT_WARPS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rpc = (blockDim.x >> 5) / a.wpr;
-  const int rw = warp / a.wpr, tr = threadIdx.x - rw * a.wpr * 32;
-  const int64_t row = (int64_t)blockIdx.x * rpc + rw;
+  extern __shared__ uint16_t stash[];
+  const int lane = threadIdx.x & 31, rw = threadIdx.y, tr = threadIdx.x;   // a block: some rows' threads
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + rw;
   pdl_wait();
   pdl_trigger();
   int64_t src = row;
@@ -341,31 +359,57 @@ __global__ void __launch_bounds__(QUANT_WARPS * 32, 4) quant_kernel(QuantArgs a)
   }
   // (a row without a source reads row 0, and its values count as zeros)
   const T* xr = reinterpret_cast<const T*>(a.x) + (has ? src : 0) * a.stride;
-  const int step = a.wpr * 32, whole = has ? (a.k + 15) / 16 : 0;   // units with values
+  const int step = blockDim.x, whole = has ? (a.k + 15) / 16 : 0;   // units with values
   float ts = 1.f;
+  bool empty = false;   // a row of zeros (and blocks that are not finite)
   if (NV) {
     if (a.ts != nullptr) {
       ts = *a.ts;
     } else {
       uint32_t m = 0u;
-      for (int k0 = tr; k0 < a.units; k0 += step * V) {
-        Unit<T> u[V];
+      if constexpr (HALF) {
+        uint16_t* to = stash + rw * a.stash + tr;
+        const T* p = xr + tr * 16;
+        auto turn = [&](int k0, auto full) {
+          Unit<T> u[W];
 #pragma unroll
-        for (int i = 0; i < V; ++i) load_unit<T, VEC>(u[i], xr, k0 + i * step, a, has);
+          for (int i = 0; i < W; ++i) {
+            if (VEC && decltype(full)::value) u[i].load(p + i * step * 16);
+            else load_unit<T, VEC>(u[i], xr, k0 + i * step, a, has);
+          }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const uint32_t am = u[i].amax();
-          m = max(m, am < F32_INF ? am : 0u);
+          for (int i = 0; i < W; ++i) {
+            const uint32_t h = u[i].hmax();
+            to[i * step] = (uint16_t)h;
+            m = max(m, h < Traits<T>::INF ? h : 0u);
+          }
+          to += W * step;
+          p += W * step * 16;
+        };
+        int k0 = tr;
+        for (const int last = a.k / 16 - (W - 1) * step; k0 < last; k0 += W * step) turn(k0, std::true_type{});
+        for (; k0 < a.units; k0 += W * step) turn(k0, std::false_type{});
+        m = __float_as_uint(Traits<T>::f(m));
+      } else {
+        for (int k0 = tr; k0 < a.units; k0 += step * V) {
+          Unit<T> u[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) load_unit<T, VEC>(u[i], xr, k0 + i * step, a, has);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const uint32_t am = u[i].amax();
+            m = max(m, am < F32_INF ? am : 0u);
+          }
         }
       }
       m = __reduce_max_sync(0xffffffffu, m);
       if (a.wpr > 1) {
-        if (lane == 0) red[warp] = m;
-        // the row's warps alone
-        asm volatile("barrier.sync %0, %1;\n" ::"r"(rw + 1), "r"(step) : "memory");
+        if (lane == 0) red[rw * a.wpr + (tr >> 5)] = m;
+        __syncthreads();   // (all rows' warps: barriers of the rows' own, by number, cost the SM half of its blocks)
         m = lane < a.wpr ? red[rw * a.wpr + lane] : 0u;
         m = __reduce_max_sync(0xffffffffu, m);
       }
+      empty = !has || m == 0u;
       ts = fmaxf(__fdiv_rn(has ? __uint_as_float(m) : 0.f, 2688.f), 1.17549435e-38f);
       if (live && tr == 0) a.row_ts[row] = ts;
     }
@@ -374,12 +418,62 @@ __global__ void __launch_bounds__(QUANT_WARPS * 32, 4) quant_kernel(QuantArgs a)
   const bool ts_ok = ts > 0.f && __float_as_uint(ts) < F32_INF;
   const bool ts_mid = mid_range(ts);
   const float inv6 = NV ? rcp(6.f * ts) : 0.f;
-  Leans ln = {0u, 0u};
-  if (NV) ln = leans<T>(ts, lane);
   uint8_t* cr = a.codes + row * a.row_bytes;
   uint8_t* sr = a.flat ? a.scales + row * a.atoms * 4
                        : a.scales + ((pos >> 7) * a.atoms) * 512 + (pos & 31) * 16 + ((pos >> 5) & 3) * 4;
   const int64_t atom = a.flat ? 4 : 512;
+  if constexpr (HALF) {
+    if (ts_mid || empty) {
+      const float fs = empty ? 0.f : factors<T>(ts, lane);
+      const uint16_t* from = stash + rw * a.stash + tr;
+      const int end = (a.units + 3) & ~3;   // (the last scale word is written whole)
+      uint8_t* st = sr + (tr >> 2) * atom + (tr & 3);
+      const int64_t st_step = (step >> 2) * atom;
+      uint2* ct = reinterpret_cast<uint2*>(cr) + tr;
+      auto units = [&](int base, auto full, auto own) {   // own: the row's scale is its own, the largest values are at hand
+        constexpr bool FULL = decltype(full)::value, OWN = decltype(own)::value;
+        Unit<T> u[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if (FULL && VEC) u[i].load(xr + (base + tr + i * step) * 16);
+          else load_unit<T, VEC>(u[i], xr, base + tr + i * step, a, has);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int k = base + tr + i * step;
+          const bool in = FULL || k < whole;
+          uint32_t h = OWN ? from[i * step] : u[i].hmax();
+          if (!in) h = 0u;
+          const float v = Traits<T>::f(h) * inv6;
+          const uint32_t two =
+              __nv_cvt_float2_to_fp8x2(make_float2(v * (1.f - 9.6e-7f), v * (1.f + 9.6e-7f)), __NV_SATFINITE, __NV_E4M3);
+          uint32_t sc = two & 0xFFu;
+          const float f0 = __shfl_sync(0xffffffffu, fs, (int)min(sc, (sc & 7u) | 8u));
+          const float f = __uint_as_float(__float_as_uint(f0) - ((sc & 0x78u) << 20));
+          uint2 c = codes_by<T>(u[i], f);
+          if (two >> 8 != sc || f < 0.f || h >= Traits<T>::INF) {
+            const uint3 r = unit_rare<T>(u[i], h, ts, inv6);
+            c = make_uint2(r.x, r.y);
+            sc = r.z;
+          }
+          if (!in) c = make_uint2(0u, 0u);
+          if (FULL || k < end) st[i * st_step] = (uint8_t)sc;
+          if (FULL || k < a.units) ct[i * step] = c;
+        }
+        from += V * step;
+        st += V * st_step;
+        ct += V * step;
+      };
+      auto row_units = [&](auto own) {
+        int base = 0;
+        for (; base + step * V <= whole; base += step * V) units(base, std::true_type{}, own);
+        for (; base < a.units; base += step * V) units(base, std::false_type{}, own);
+      };
+      if (a.ts == nullptr) row_units(std::true_type{});
+      else row_units(std::false_type{});
+      return;
+    }
+  }
   for (int base = 0; base < a.units; base += step * V) {
     Unit<T> u[V];
 #pragma unroll
@@ -393,7 +487,7 @@ __global__ void __launch_bounds__(QUANT_WARPS * 32, 4) quant_kernel(QuantArgs a)
       if (NV) {
         const bool fine = am < F32_INF && ts_ok;
         sc = fine ? scale_code(__uint_as_float(am), ts, inv6, ts_mid) : 0x7Fu;
-        if (fine) c = codes_nv<T>(u[i], e4m3_to_f32(sc), ts, ts_mid, ln);
+        if (fine) c = codes_nv<T>(u[i], e4m3_to_f32(sc), ts, ts_mid);
         if (k >= a.units) sc = 0u;
         uint32_t w = sc << (8 * (k & 3));
         w |= __shfl_xor_sync(0xffffffffu, w, 1);
@@ -520,9 +614,16 @@ __global__ void __launch_bounds__(256) tile_scales_kernel(const uint8_t* __restr
 }
 
 template <typename T, bool NV, bool VEC>
-static cudaError_t launch_quant_v(const QuantArgs& q, int v, dim3 grid, dim3 block, cudaStream_t st) {
-  if (v == 1) return launch_pdl(quant_kernel<T, NV, 1, VEC>, grid, block, 0, st, q);
-  return launch_pdl(quant_kernel<T, NV, 2, VEC>, grid, block, 0, st, q);
+static cudaError_t launch_quant_v(QuantArgs q, int v, dim3 grid, dim3 block, cudaStream_t st) {
+  // each thread's units, whole turns of them
+  size_t smem = 0;
+  if (NV && sizeof(T) == 2 && q.ts == nullptr) {
+    const int w = v == 1 ? 1 : QUANT_FIRST, turns = (q.units + q.wpr * 32 * w - 1) / (q.wpr * 32 * w);
+    q.stash = turns * w * (int)block.x;
+    smem = (size_t)q.stash * block.y * sizeof(uint16_t);
+  }
+  if (v == 1) return launch_pdl(quant_kernel<T, NV, 1, VEC>, grid, block, smem, st, q);
+  return launch_pdl(quant_kernel<T, NV, 2, VEC>, grid, block, smem, st, q);
 }
 
 template <typename T>
@@ -535,14 +636,15 @@ static cudaError_t launch_quant_t(const QuantArgs& q, int v, bool vec, dim3 grid
 
 static cudaError_t launch_rows(const QuantArgs& args, int dtype, cudaStream_t st) {
   QuantArgs q = args;
-  // Units per thread: one while the rows do not fill the GPU, up to eight at large sizes, where what a warp does once
-  // per row counts (8192 x 7168 NVFP4: two units 49 us, eight 45; 1021 x 7168: 8.5 and 11.4). Two are in flight.
+  // Units per thread: one while the rows do not fill the GPU, up to four at large sizes, where what a warp does once per
+  // row counts (8192 x 7168 NVFP4: two 47 us, four 37, eight, whose rows outgrow L1 between their two readings, 39).
+  // Two are in flight. Blocks of four warps, or of a row's (of eight: 40 us).
   const int64_t per = q.rows * q.units / ((int64_t)num_sms() * 1536);
-  const int each = per < 1 ? 1 : (per > 8 ? 8 : (int)per), v = each == 1 ? 1 : 2;
+  const int each = per < 1 ? 1 : (per > 4 ? 4 : (int)per), v = each == 1 ? 1 : 2;
   q.wpr = (q.units + 32 * each - 1) / (32 * each);
   if (q.wpr > fp4::QUANT_WARPS) q.wpr = fp4::QUANT_WARPS;
-  const int rpc = fp4::QUANT_WARPS / q.wpr;
-  const dim3 grid((unsigned)((q.rows + rpc - 1) / rpc)), block(rpc * q.wpr * 32);
+  const int rpc = q.wpr < 4 ? 4 / q.wpr : 1;
+  const dim3 grid((unsigned)((q.rows + rpc - 1) / rpc)), block(q.wpr * 32, rpc);
   const int es = dtype == SB_F32 ? 4 : 2;
   const bool vec = (reinterpret_cast<uintptr_t>(q.x) & 15u) == 0 && (q.stride * es) % 16 == 0 && q.k % 16 == 0 && q.src_rows > 0;
   if (dtype == SB_F32) return fp4::launch_quant_t<float>(q, v, vec, grid, block, st);

@@ -27,7 +27,7 @@ struct QuantArgs {
   uint8_t* scales;
   int64_t atoms;
   int flat;                  // scale words row by row, not in atoms
-  int wpr;                   // warps per row (set by the launch)
+  int wpr, stash;            // warps per row, shared halfwords per row (set by the launch)
 };
 
 struct DequantArgs {
