@@ -260,17 +260,23 @@ __device__ __forceinline__ Tile tile_at(const Args& a, const Ctl& c, int i) {
     const int mid = (lo + hi) >> 1;
     if (c.tiles[mid] <= i) lo = mid; else hi = mid;
   }
-  const int r = i - c.tiles[lo], nb = (a.g.n + MT - 1) / MT;
-  const int tb = (c.tiles[lo + 1] - c.tiles[lo]) / nb;
-  const int band = r / (12 * tb), left = r - band * 12 * tb, wide = min(12, nb - band * 12);
+  const int r = i - c.tiles[lo], nb = (a.g.n + MT - 1) / MT, tiles = c.tiles[lo + 1] - c.tiles[lo];
   Tile t;
   t.mat = lo;
-  t.n0 = (band * 12 + left % wide) * MT;
   t.row0 = c.rows[lo];
-  // a group's tokens in tiles alike, of whole 64-row steps of the scale atoms
-  const int all = c.rows[lo + 1] - t.row0, each = tb > 1 ? ((all + tb - 1) / tb + 63) & ~63 : a.nt;
-  t.t0 = left / wide * each;
-  t.cnt = min(all - t.t0, each);
+  const int all = c.rows[lo + 1] - t.row0;
+  if (tiles == nb) {   // one token tile (the divisions below cost small products 0.5 us)
+    t.n0 = r * MT;
+    t.t0 = 0;
+    t.cnt = min(all, a.nt);
+  } else {
+    const int tb = tiles / nb, band = r / (12 * tb), left = r - band * 12 * tb, wide = min(12, nb - band * 12);
+    // a group's tokens in tiles alike, of whole 64-row steps of the scale atoms
+    const int each = ((all + tb - 1) / tb + 63) & ~63;
+    t.n0 = (band * 12 + left % wide) * MT;
+    t.t0 = left / wide * each;
+    t.cnt = min(all - t.t0, each);
+  }
   t.blk = (a.g.offsets ? (t.row0 >> 7) + lo : 0) + (t.t0 >> 7);
   return t;
 }
@@ -440,19 +446,21 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
   const int stride = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;   // (SPLIT: one tile a cluster)
   const Fp4MmArgs& g = a.g;
 
-  if (tid == 0) {
-    for (int s = 0; s < a.stages; ++s) {
-      mbar_init(smem_addr(&c.full[s]), 2);
-      mbar_init(smem_addr(&c.empty[s]), 1);
+  if (warp == 0) {
+    if (lane < a.stages) {
+      mbar_init(smem_addr(&c.full[lane]), 2);
+      mbar_init(smem_addr(&c.empty[lane]), 1);
     }
-    for (int q = 0; q < 2; ++q) {
-      mbar_init(smem_addr(&c.accfull[q]), 1);
-      mbar_init(smem_addr(&c.accempty[q]), PAIR ? 2 * EPI_WARPS : EPI_WARPS);
+    if (lane < RING) mbar_init(smem_addr(&c.told[lane]), 1);
+    if (lane < 2) {
+      mbar_init(smem_addr(&c.accfull[lane]), 1);
+      mbar_init(smem_addr(&c.accempty[lane]), PAIR ? 2 * EPI_WARPS : EPI_WARPS);
     }
-    mbar_init(smem_addr(&c.shared), 2 * EPI_WARPS);
-    for (int r = 0; r < RING; ++r) mbar_init(smem_addr(&c.told[r]), 1);
-    mbar_init(smem_addr(&c.drain), 1);
-    c.abort = 0;
+    if (lane == 0) {
+      mbar_init(smem_addr(&c.shared), 2 * EPI_WARPS);
+      mbar_init(smem_addr(&c.drain), 1);
+      c.abort = 0;
+    }
     mbar_init_fence();
   }
   if (warp == MMA_WARP) {
