@@ -239,6 +239,61 @@ def test_gemm(fmt, m, n, k):
 
 @gpu
 @pytest.mark.parametrize("fmt", [NV, MX])
+@pytest.mark.parametrize("m,n,k", [(150, 19000, 64), (300, 12808, 96), (513, 8200, 160), (3000, 1300, 544), (1000, 5000, 2080),
+                                   (1500, 8196, 288), (2000, 4096, 4096)])
+def test_gemm_of_many_tiles(fmt, m, n, k):
+    """Tiles for more than one round of the SMs: pairs of CTAs, one to several tiles each, token tiles of 129 to 256."""
+    _need_gpu()
+    w = fp4.quant(_acts(n, k, torch.bfloat16, seed=n, spread=0.5).cuda(), fmt)
+    a = fp4.quant(_acts(m, k, torch.bfloat16, seed=m).cuda(), fmt)
+    av, wv = _values(a).cuda(), _values(w).cuda()
+    exact = av @ wv.T
+    for out in (torch.float32, torch.bfloat16):
+        buf = torch.full((m + 1, n + 8), 3.0, dtype=out, device="cuda")
+        y = fp4.gemm(a, w, out_dtype=out, out=buf[:m, :n])
+        assert bool(((y.double() - exact).abs() <= _tol(av, wv, exact, k, out)).all())
+        assert bool((buf[m:] == 3).all()) and bool((buf[:, n:] == 3).all())
+    assert fp4.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+@pytest.mark.parametrize("w13", [False, True])
+@pytest.mark.parametrize("counts,n,k", [([300, 0, 513, 190, 64, 1000, 1, 257], 2064, 160), ([256, 512, 768, 255, 257], 2048, 1024),
+                                        ([0, 0, 0, 900], 6160, 96)])
+def test_grouped_gemm_of_many_tiles(fmt, w13, counts, n, k):
+    """Pairs of CTAs on groups of every width of tile; errors of the gated form as in test_grouped_gemm."""
+    _need_gpu()
+    e, p = len(counts), sum(counts)
+    codes, s, ts, wv = P.weights(fmt, n, k, seed=k, mats=e, halves=2 if w13 else 1)
+    bank = fp4.pack(fmt, codes.cuda(), s.cuda(), None if ts is None else ts.cuda(), kind=fp4.W13 if w13 else fp4.PLAIN)
+    off = torch.tensor([0] + counts).cumsum(0).to(torch.int32)
+    x = (_acts(p, k, torch.bfloat16, seed=p, spread=0.3) * 0.02).to(torch.bfloat16)
+    a = fp4.quant(x.cuda(), fmt, offsets=off.cuda())
+    c, sb, t = P.quant(x, fmt)
+    av = P.values(c, sb, fmt, t).cuda()
+    limit = 2.5 if w13 else 0.0
+    for out in (torch.float32, torch.bfloat16):
+        y = fp4.grouped_gemm(a, bank, out_dtype=out, limit=limit).double()
+        for i in range(e):
+            lo, hi = int(off[i]), int(off[i + 1])
+            w = wv[i].cuda()
+            r = av[lo:hi] @ w.T
+            tol = _tol(av[lo:hi], w, r, k, torch.float32 if w13 else out)
+            if w13:
+                g, u = r[:, :n // 2].clamp_max(limit), r[:, n // 2:].clamp(-limit, limit)
+                dg, du = tol[:, :n // 2], tol[:, n // 2:]
+                silu = g / (1 + torch.exp(-g))
+                r = silu * u
+                # (g below -64: silu's own size bounds what the fast exponential can add)
+                tol = 1.1 * dg * u.abs() + silu.abs() * du + (2.0 ** -19 + torch.finfo(out).eps / 2) * r.abs() * (g > -64) + \
+                    1.01 * r.abs() * (g <= -64) + 1e-26
+            assert bool(((y[lo:hi] - r).abs() <= tol).all())
+    assert fp4.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
 @pytest.mark.parametrize("calibrated", [False, True])
 def test_gemm_of_two_quantised_matrices(fmt, calibrated):
     """K 100: both operands are padded to 128 with zero codes. Tensor scales: one, or one per row of either."""
