@@ -331,8 +331,8 @@ __device__ __forceinline__ float gated(float v0, float v1, int lane, float lim) 
 // 32 accumulator columns (tokens tok ..) of this thread's weight row to y; sc, wt: the tokens' scales and weights in
 // shared memory. 16-bit outputs go through the warp's `turn` in shared memory, rows of 32 tokens in, tokens of up to
 // 8 neighbouring rows out, the 16-byte pieces of a row placed so that neither side meets a bank conflict. This
-// readback bounds tiles of K <= 2048: 8192 x 4096 x 2048 took 62 us turned by shuffles (32 of them a chunk, against 8
-// accesses so), now 46; with a 2-byte store per row and column a tile of 192 columns took 8.5 us. FULL: a whole
+// readback bounds tiles of K <= 1024 (690 cycles a chunk, gated 1330; a stage takes 520): 8192 x 4096 x 2048 took 62 us
+// turned by shuffles (32 of them a chunk, against 8 accesses so), 46 at the time, now 34; with a 2-byte store per row and column a tile of 192 columns took 8.5 us. FULL: a whole
 // chunk, without a branch per group of columns, which would keep the groups from overlapping.
 template <bool SWIGLU, bool FULL, typename T>
 __device__ __forceinline__ void store_chunk(const Args& a, const uint32_t (&d)[32], int64_t tok, int row, int lane, int left,
@@ -866,7 +866,8 @@ cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
   // share.
   const bool pair = a.nt >= 128 && g.m >= 128 * (int64_t)g.mats && tiles > sms;
   // A pair's tiles have 256 tokens: fewer bytes of shared memory per product than 192, which have both accumulators to
-  // themselves (8192 x 4096 x 8192: 104 us and 124; x 2048: 45 and 54; x 512: even; 32 groups of 512 tokens: even).
+  // themselves (when this was chosen, 8192 x 4096 x 8192: 104 us and 124; x 2048: 45 and 54; x 512 and 32 groups of 512
+  // tokens: even; now 98, 34).
   if (pair) a.nt = 256;
   // K is split, for one token tile, as far as the SMs go and every piece keeps two stages (one token against 4096 x 8192:
   // 12.0 us whole, 9.3 in four pieces, 8.6 with the weights ahead in L2).
