@@ -352,7 +352,9 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
   uint32_t kept = 0xffffffffu;
   if (a.groups > 1) {
     float gs = -INFINITY;   // lane g: the score of group g
-    uint32_t near = 0u;     // this lane's experts that may be among their group's two best
+    // This lane's experts that may be among their group's two best: also those that no comparison tells from the
+    // second (biases of +inf on two experts make the difference NaN).
+    uint32_t near = 0u;
     if (a.span > 0) {
       float b1 = -INFINITY, b2 = -INFINITY;
 #pragma unroll
@@ -363,7 +365,7 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
       }
       gs = __shfl_sync(0xffffffffu, a.group_two && b2 > -INFINITY ? b1 + b2 : b1, (lane * a.span) & 31);
 #pragma unroll
-      for (int i = 0; i < C; ++i) near |= gv[i] > -INFINITY && gv[i] >= b2 - eps ? 1u << i : 0u;
+      for (int i = 0; i < C; ++i) near |= gv[i] > -INFINITY && !(gv[i] < b2 - eps) ? 1u << i : 0u;
     } else {
       for (int g = 0; g < a.groups; ++g) {
         float b1 = -INFINITY, b2 = -INFINITY;
@@ -381,7 +383,7 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           const int e = lane * C + i;
-          if (e >= g * a.size && e < (g + 1) * a.size && gv[i] > -INFINITY && gv[i] >= b2 - eps) near |= 1u << i;
+          if (e >= g * a.size && e < (g + 1) * a.size && gv[i] > -INFINITY && !(gv[i] < b2 - eps)) near |= 1u << i;
         }
       }
     }

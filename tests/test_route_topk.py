@@ -107,6 +107,25 @@ def test_topk_biases_without_end():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group_score", ["max", "top2"])
+@pytest.mark.parametrize("e,g", [(64, 8), (96, 8), (60, 4), (1024, 16)])
+def test_topk_groups_with_several_biases_of_inf(e, g, group_score, dtype):
+    """Two of a group's experts at +inf, all of them, and several such groups, which come before every other; groups of
+    whole lanes and groups that share them."""
+    _need_gpu()
+    gen = torch.Generator().manual_seed(e)
+    s = e // g
+    logits = torch.randn(20, e, generator=gen).to(dtype)
+    for forced in ([2 * s, 2 * s + 3], list(range(2 * s, 3 * s)), [s, s + 1, 3 * s + 2, 3 * s + 4], [0, 3 * s, 3 * s + 1],
+                   list(range(e))):
+        bias = 0.2 * torch.randn(e, generator=gen)
+        bias[forced] = math.inf
+        for kept in (1, 3):
+            _check(logits, 4, bias, n_group=g, topk_group=kept, group_score=group_score)
+
+
+@gpu
 def test_topk_strides_and_large_batches():
     _need_gpu()
     gen = torch.Generator().manual_seed(6)
