@@ -328,6 +328,15 @@ __device__ __forceinline__ float gated(float v0, float v1, int lane, float lim) 
   return __fdividef(gate, 1.f + __expf(-gate)) * up;
 }
 
+// Outputs are (d w) s, d the accumulator, w the weight row's scale, s the token's: with w between 2^-50 and 2^50, d w is a plain
+// number for any sum of products and s scales it with one rounding. (s w by itself is subnormal or inf where the
+// output is not: off by 1.4e-3 at rows of 1e-35 and weight scales of 4e-5.) Whether w is none of these:
+__device__ __forceinline__ bool odd_row(float w) {
+  return (__float_as_uint(w) & 0x7FFFFFFFu) - ((127u - 50u) << 23) > (100u << 23);
+}
+// s times a row weight that left fp32's range (or is 0)
+__device__ __forceinline__ bool odd_col(float s) { return !(fabsf(s) >= 1.17549435e-38f && fabsf(s) < INFINITY); }
+
 // 32 accumulator columns (tokens tok ..) of this thread's weight row to y; sc, wt: the tokens' scales and weights in
 // shared memory. 16-bit outputs go through the warp's `turn` in shared memory, rows of 32 tokens in, tokens of up to
 // 8 neighbouring rows out, the 16-byte pieces of a row placed so that neither side meets a bank conflict. This
@@ -355,8 +364,7 @@ __device__ __forceinline__ void store_chunk(const Args& a, const uint32_t (&d)[3
 #pragma unroll
           for (int m = 0; m < 8; ++m) {
             const float2 s = *reinterpret_cast<const float2*>(sc + j + 2 * m);
-            h[m] = gated(__uint_as_float(d[j + 2 * m]) * (s.x * wts), __uint_as_float(d[j + 2 * m + 1]) * (s.y * wts), lane,
-                         lim) *
+            h[m] = gated(__uint_as_float(d[j + 2 * m]) * wts * s.x, __uint_as_float(d[j + 2 * m + 1]) * wts * s.y, lane, lim) *
                    wt[j + 2 * m + (lane & 1)];
           }
           st_shared16(to + ((((lane & 1) * 2 + (j >> 4)) ^ gw) << 4), pack2<T>(h[0], h[1]), pack2<T>(h[2], h[3]),
@@ -382,7 +390,7 @@ __device__ __forceinline__ void store_chunk(const Args& a, const uint32_t (&d)[3
           const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
           float v[8];
 #pragma unroll
-          for (int m = 0; m < 8; ++m) v[m] = __uint_as_float(d[j + m]) * (s[m] * wts);
+          for (int m = 0; m < 8; ++m) v[m] = __uint_as_float(d[j + m]) * wts * s[m];
           st_shared16(to + (((j >> 3) ^ gw) << 4), pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
                       pack2<T>(v[6], v[7]));
         }
@@ -408,7 +416,7 @@ __device__ __forceinline__ void store_chunk(const Args& a, const uint32_t (&d)[3
     for (int j = 0; j < 32; j += 2) {
       if (FULL || j < left) {
         const float2 s = *reinterpret_cast<const float2*>(sc + j);
-        const float h = gated(__uint_as_float(d[j]) * (s.x * wts), __uint_as_float(d[j + 1]) * (s.y * wts), lane, lim) *
+        const float h = gated(__uint_as_float(d[j]) * wts * s.x, __uint_as_float(d[j + 1]) * wts * s.y, lane, lim) *
                         wt[j + (lane & 1)];
         if (in && (FULL || j + (lane & 1) < left)) yp[(int64_t)j * ld] = to_out<T>(h);
       }
@@ -422,10 +430,62 @@ __device__ __forceinline__ void store_chunk(const Args& a, const uint32_t (&d)[3
         const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
         for (int m = 0; m < 4; ++m)
-          if (in && (FULL || j + m < left)) yp[(int64_t)(j + m) * ld] = to_out<T>(__uint_as_float(d[j + m]) * (v[m] * wts));
+          if (in && (FULL || j + m < left)) yp[(int64_t)(j + m) * ld] = to_out<T>(__uint_as_float(d[j + m]) * wts * v[m]);
       }
     }
   }
+}
+
+// The same for an odd_row or odd_cols, in 64 bits, where s w is exact and the result rounds once. False, and nothing is done,
+// where all that such scales multiply is zero and they are small (weight rows of zeros have the smallest scale), or a
+// token's weight is zero. s: what store_chunk would take; weight: the lane's token's; odd: 32 floats of the warp's. Rare,
+// out of line: within the loop it cost products of K 512 6%.
+struct Chunk {
+  uint32_t d[32];
+};
+template <bool SWIGLU, typename T>
+__device__ __noinline__ bool store_wide(const Args& a, Chunk v, int64_t tok, int row, int lane, int left, float wts, float s,
+                                        float weight, float* odd) {
+  const Fp4MmArgs& g = a.g;
+  const bool in = row < g.n, col_odd = !SWIGLU && weight != 0.f && odd_col(s), row_odd = wts != 0.f && odd_row(wts);
+  odd[lane] = col_odd ? 1.f : 0.f;
+  __syncwarp();
+  float sum = (col_odd && !(fabsf(s) < 1.f)) || (row_odd && !(fabsf(wts) < 1.f)) ? 1.f : 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    const float4 f = *reinterpret_cast<const float4*>(odd + j);
+    const float w[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+    for (int m = 0; m < 4; ++m) sum = fmaf(fabsf(__uint_as_float(v.d[j + m])), row_odd ? 1.f : w[m], sum);
+  }
+  __syncwarp();
+  if (!__any_sync(0xffffffffu, sum != 0.f)) return false;
+  s = weight = 1.f;
+  if (lane < left) {
+    if (g.a_ts != nullptr) s = g.a_ts[g.a_ts_row ? tok + lane : 0];
+    if (g.row_weight != nullptr) weight = g.row_weight[tok + lane];
+  }
+  T* yp = reinterpret_cast<T*>(g.y) + tok * g.ldy;
+  const float lim = g.limit > 0.f ? g.limit : INFINITY;
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    float h[2], w[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      w[m] = __shfl_sync(0xffffffffu, weight, j + m);
+      const double f = (double)__shfl_sync(0xffffffffu, s, j + m) * (double)wts;
+      h[m] = (float)((double)__uint_as_float(v.d[j + m]) * f * (SWIGLU ? 1.0 : (double)w[m]));
+    }
+    if constexpr (SWIGLU) {
+      const float o = gated(h[0], h[1], lane, lim) * w[lane & 1];
+      if (in && j + (lane & 1) < left) yp[(j + (lane & 1)) * g.ldy + (row >> 1)] = to_out<T>(o);
+    } else {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        if (in && j + m < left) yp[(j + m) * g.ldy + row] = to_out<T>(h[m]);
+    }
+  }
+  return true;
 }
 
 template <bool NV, bool SWIGLU, Form FORM, typename T>
@@ -665,6 +725,15 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
         sc[32 * j + lane] = SWIGLU ? s_next[j] : s_next[j] * w_next[j];
         if (SWIGLU) wt[32 * j + lane] = w_next[j];
       }
+      bool odd = odd_row(wts);   // or, with weights, a column
+      if (!SWIGLU && g.row_weight != nullptr) {
+#pragma unroll
+        for (int j = 0; j < CHUNKS; ++j) {
+          wt[32 * j + lane] = w_next[j];
+          odd |= odd_col(s_next[j] * w_next[j]);
+        }
+      }
+      const bool wide = __any_sync(0xffffffffu, odd);
       __syncwarp();
       if constexpr (FORM != SPLIT) ok = look_ahead(i + stride, n + 1);
       const uint32_t q = n & 1u;
@@ -701,6 +770,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
           if (lane == 0 && u == mine - 1) release<PAIR>(smem_addr(&c.accempty[q]));
         }
         const int left = cnt - ch * 32;
+        if (wide) {
+          Chunk v;
+#pragma unroll
+          for (int m = 0; m < 32; ++m) v.d[m] = d[m];
+          if (store_wide<SWIGLU, T>(a, v, tok0 + ch * 32, row, lane, min(left, 32), wts, sc[32 * j + lane],
+                                    g.row_weight != nullptr ? wt[32 * j + lane] : 1.f, reinterpret_cast<float*>(c.turn[warp])))
+            continue;
+        }
         if (left >= 32) store_chunk<SWIGLU, true, T>(a, d, tok0 + ch * 32, row, lane, 32, vec, wts, sc + 32 * j, wt + 32 * j, turn);
         else store_chunk<SWIGLU, false, T>(a, d, tok0 + ch * 32, row, lane, left, vec, wts, sc + 32 * j, wt + 32 * j, turn);
       }
@@ -727,9 +804,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
         float v = 0.f;
         for (int p = 0; p < a.split; ++p) v += peer_float(part + (col * 128 + r) * 4, p);
         if (row < g.n) {
-          float s = g.a_ts ? g.a_ts[g.a_ts_row ? t.t0 + col : 0] : 1.f;
-          if (g.w_ts) s *= g.w_ts[g.w_ts_n == 0 ? row : 0];
-          reinterpret_cast<T*>(g.y)[(int64_t)(t.t0 + col) * g.ldy + row] = to_out<T>(v * s);
+          const float s = g.a_ts ? g.a_ts[g.a_ts_row ? t.t0 + col : 0] : 1.f;
+          const float w = g.w_ts ? g.w_ts[g.w_ts_n == 0 ? row : 0] : 1.f;
+          v = !odd_row(w) ? v * w * s : (float)((double)v * ((double)s * (double)w));
+          reinterpret_cast<T*>(g.y)[(int64_t)(t.t0 + col) * g.ldy + row] = to_out<T>(v);
         }
       }
     }

@@ -559,3 +559,95 @@ def test_refusals_of_tensors():
     for call in (lambda: fp4.quant(x, stream=other), lambda: fp4.gemm(a, a, stream=other), lambda: fp4.dequant(a, stream=other)):
         with pytest.raises(ValueError, match="stream"):
             call()
+
+
+def _rows_of_all_sizes(rows, k, lo, hi, seed):
+    """Rows from 10^lo to 10^hi, in no order of size."""
+    g = torch.Generator().manual_seed(seed)
+    size = torch.pow(10.0, torch.linspace(lo, hi, rows, dtype=torch.float64))[torch.randperm(rows, generator=g)]
+    return (torch.randn(rows, k, generator=g).clamp(-3, 3) * size[:, None]).float()
+
+
+# of the output type, behind its fp32 rounding: half a step of its smallest values
+TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133}
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (5, 256, 4096), (300, 256, 1024), (1024, 8192, 256)])
+@pytest.mark.parametrize("ts", [None, 4e-5, 1e-30, 1e28])
+def test_gemm_of_tiny_and_huge_rows(m, n, k, ts):
+    """The two tensor scales' own product leaves fp32's range where the output does not: rows of either operand near both
+    ends of it (or one scale ts of the weights), one of zeros, in every form of the kernel, within _tol."""
+    _need_gpu()
+    x = _rows_of_all_sizes(m, k, -37.5, 37.5, m) if m > 1 else _rows_of_all_sizes(1, k, -34, -34, 1)
+    if m > 3:
+        x[2] = 0
+    a = fp4.quant(x.cuda(), NV)
+    if ts is None:
+        wx = _rows_of_all_sizes(n, k, -33, 33, n)
+        wx[n // 3] = 0
+        w = fp4.quant(wx.cuda(), NV)
+        wv = _values(w).cuda()
+    else:
+        codes, s, _, _ = P.weights(NV, n, k, seed=n + k)
+        t = torch.tensor([ts])
+        w = fp4.pack(NV, codes[0].cuda(), s[0].cuda(), t.cuda())
+        wv = P.values(P.unpack(codes[0]), s[0], NV, t).cuda()
+    av = _values(a).cuda()
+    exact = av @ wv.T
+    for out in (torch.float32, torch.bfloat16):
+        tol = _tol(av, wv, exact, k, out) + TINY[out]
+        y = fp4.gemm(a, w, out_dtype=out).double()
+        fits = exact.abs() + tol < torch.finfo(out).max
+        assert float(fits.double().mean()) > 0.3
+        assert bool(((y - exact).abs() <= tol)[fits].all())
+    assert fp4.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("counts,n,k", [([5, 0, 40, 130], 272, 96), ([513, 256, 0, 600], 2176, 64)])
+@pytest.mark.parametrize("w13", [False, True])
+def test_grouped_gemm_of_tiny_and_huge_rows(counts, n, k, w13):
+    """The same with expert groups, with weights of the rows (0 among them) far from one. Gated rows: the exponential's argument
+    is |g| 2^-23 of itself off, it, the division and the products 2^-20; below -87 its reciprocal may count as 0."""
+    _need_gpu()
+    e, p = len(counts), sum(counts)
+    codes, s, _, _ = P.weights(NV, n, k, seed=k, mats=e)
+    ts = torch.tensor([[1e-5, 1e30], [1e25, 1e-5], [1.0, 1.0], [1e-30, 1e-20]]) if w13 else torch.tensor([[1e-5], [1e25], [1.0], [1e-30]])
+    bank = fp4.pack(NV, codes.cuda(), s.cuda(), ts.cuda(), kind=fp4.W13 if w13 else fp4.PLAIN)
+    off = torch.tensor([0] + counts).cumsum(0).to(torch.int32)
+    x = _rows_of_all_sizes(p, k, -37.5, 37.5, p)
+    x[7] = 0
+    a = fp4.quant(x.cuda(), NV, offsets=off.cuda())
+    c, sb, t = P.quant(x, NV)
+    av = P.values(c, sb, NV, t).cuda()
+    rw = torch.pow(10.0, torch.linspace(-25, 25, p, dtype=torch.float64))[torch.randperm(p, generator=torch.Generator().manual_seed(1))].float()
+    rw[::9] = 0
+    rw[1::3] = 0.25
+    for out in (torch.float32, torch.bfloat16):
+        y = fp4.grouped_gemm(a, bank, out_dtype=out, row_weight=rw.cuda()).double()
+        for i in range(e):
+            lo, hi = int(off[i]), int(off[i + 1])
+            if lo == hi:
+                continue
+            h = ts.shape[1]
+            w = (P.values(P.unpack(codes[i]), s[i], NV).view(h, n // h, k) * ts[i].double().view(h, 1, 1)).view(n, k).cuda()
+            f = rw[lo:hi, None].double().cuda()
+            r = av[lo:hi] @ w.T
+            if w13:
+                d = _tol(av[lo:hi], w, r, k, torch.float32) + 2.0 ** -149
+                fits = (r.abs() + d < 3e38).view(hi - lo, 2, -1).all(1)
+                g, u = r[:, :n // 2], r[:, n // 2:]
+                silu = g / (1 + torch.exp(-g))
+                q = silu * u
+                tol = 1.1 * d[:, :n // 2] * u.abs() + silu.abs() * d[:, n // 2:] + \
+                    torch.where(g > -87, (g.abs() * 2.0 ** -23).clamp_max(2.0 ** -16) + 2.0 ** -20, 1.01) * q.abs() + 2.0 ** -149
+                fits &= q.abs() < 3e38
+            else:
+                q, tol = r, _tol(av[lo:hi], w, r, k, torch.float32)
+                fits = r.abs() + tol < 3e38
+            r, tol = q * f, tol * f + (2.0 ** -23 + torch.finfo(out).eps / 2) * (q * f).abs() + TINY[out]
+            fits &= r.abs() + tol < 3e38
+            assert float(fits.double().mean()) > 0.1
+            assert bool(((y[lo:hi] - r).abs() <= tol)[fits].all()), f"expert {i}"
+    assert fp4.device_error() == 0
