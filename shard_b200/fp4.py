@@ -192,6 +192,9 @@ def pack(fmt: Union[int, str], codes: torch.Tensor, scales: torch.Tensor, ts: Op
     f = _fmt(fmt)
     if not codes.is_cuda or codes.dim() not in (2, 3):
         raise ValueError("pack: codes must be a CUDA tensor [N, K/2] or [E, N, K/2]")
+    if _away("pack", codes, stream):      # before any conversion: those run there, too
+        with _elsewhere(codes.device, stream):
+            return pack(fmt, codes, scales, ts, kind)
     c, s = codes.view(torch.uint8), scales.view(torch.uint8)
     for t in (scales, ts):
         if t is not None and t.device != codes.device:
@@ -208,9 +211,6 @@ def pack(fmt: Union[int, str], codes: torch.Tensor, scales: torch.Tensor, ts: Op
             raise ValueError(f"pack: {ts.shape[1]} tensor scales a matrix")
     if kind not in (PLAIN, W13) or (kind == W13 and n % 2):
         raise ValueError("pack: kind is PLAIN, or W13 with an even number of rows")
-    if _away("pack", codes, stream):
-        with _elsewhere(codes.device, stream):
-            return pack(fmt, codes, scales, ts, kind)
     c, s = c.reshape(mats, n, k // 2), s.reshape(mats, n, nb)
     if kind == W13:
         c, s = (t.view(mats, 2, n // 2, -1).transpose(1, 2).reshape(mats, n, -1) for t in (c, s))

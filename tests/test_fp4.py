@@ -651,3 +651,46 @@ def test_grouped_gemm_of_tiny_and_huge_rows(counts, n, k, w13):
             assert float(fits.double().mean()) > 0.1
             assert bool(((y[lo:hi] - r).abs() <= tol)[fits].all()), f"expert {i}"
     assert fp4.device_error() == 0
+
+
+def test_pack_is_on_its_stream_before_it_touches_a_tensor(monkeypatch):
+    """Conversions of the scales belong to the given stream, as the products behind them do (no GPU needed)."""
+    class Reached(Exception):
+        pass
+
+    class Tensor:
+        is_cuda, device = True, torch.device("cuda", 0)
+
+        def dim(self):
+            return 2
+
+        def get_device(self):
+            return 0
+
+    def elsewhere(device, stream):
+        raise Reached
+
+    monkeypatch.setattr(fp4, "_elsewhere", elsewhere)
+    with pytest.raises(Reached):
+        fp4.pack(NV, Tensor(), Tensor(), Tensor(), stream=object())
+
+
+@gpu
+@pytest.mark.parametrize("kind", [fp4.PLAIN, fp4.W13])
+def test_pack_on_a_stream(kind):
+    """Tensor scales that have to be converted (64 bits, not contiguous), while the current stream is busy."""
+    _need_gpu()
+    codes, s, ts, _ = P.weights(NV, 64, 128, seed=3, mats=4, halves=2 if kind == fp4.W13 else 1)
+    off = torch.tensor([0, 3, 3, 8, 9], dtype=torch.int32, device="cuda")
+    c, sc = codes.cuda(), s.cuda()
+    wide = ts.double().repeat(1, 2).cuda()[:, ::2] if kind == fp4.PLAIN else ts.double().t().contiguous().cuda().t()
+    a = fp4.quant(_acts(9, 128, torch.bfloat16).cuda(), NV, offsets=off)
+    want = fp4.grouped_gemm(a, fp4.pack(NV, c, sc, ts.cuda(), kind=kind))
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    fp4.pack(NV, c, sc, wide, kind=kind, stream=st)      # (what is loaded or allocated at the first call waits for the device)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)          # about 0.1 s
+    got = fp4.grouped_gemm(a, fp4.pack(NV, c, sc, wide, kind=kind, stream=st), stream=st)
+    st.synchronize()
+    assert torch.equal(got, want)
