@@ -1109,7 +1109,7 @@ int fp4_common(const char* what, int fmt, int dtype, int64_t rows, int64_t k) {
 int fp4_product(const char* what, int fmt, int dtype, const void* const* ptrs, int n_ptrs, int64_t m, int64_t mats,
                 int64_t n, int64_t k, int64_t width, int64_t ldy) {
   if (int rc = fp4_common(what, fmt, dtype, m, k)) return rc;
-  if (n < 1 || mats < 1 || mats > FP4_MAX_GROUPS || mats * n > FP4_MAX_ROWS)
+  if (n < 1 || mats < 1 || mats > FP4_MAX_GROUPS || n > FP4_MAX_ROWS / mats)
     return fail(SB_ERR_SHAPE, "%s: need N >= 1, 1..%lld matrices and at most 2^30 weight rows (matrices=%lld N=%lld)",
                 what, (long long)FP4_MAX_GROUPS, (long long)mats, (long long)n);
   if ((m / 128 + mats) * ((n + 127) / 128) > FP4_MAX_ROWS)
@@ -1128,7 +1128,7 @@ int fp4_product(const char* what, int fmt, int dtype, const void* const* ptrs, i
 
 size_t sb_fp4_scale_bytes(int fmt, int64_t n_mat, int64_t rows, int64_t k, int64_t groups) {
   if (!fp4_fmt(fmt) || n_mat < 1 || rows < 0 || rows > FP4_MAX_ROWS || n_mat > FP4_MAX_ROWS || k < 1 ||
-      k > FP4_MAX_K || groups < 0 || groups > FP4_MAX_GROUPS || (groups > 0 && n_mat != 1))
+      k > FP4_MAX_K || groups < 0 || groups > FP4_MAX_GROUPS || (groups > 0 && n_mat != 1) || (rows > 0 && n_mat > FP4_MAX_ROWS / rows))
     return 0;
   return (size_t)fp4_blocks(n_mat, rows, groups) * (size_t)fp4_atoms(fmt, k) * 512;
 }
@@ -1210,7 +1210,7 @@ int sb_fp4_dequant(int fmt, const void* codes, const void* scales, const float* 
 
 int sb_fp4_tile_scales(int fmt, const void* src, void* dst, int64_t n_mat, int64_t n, int64_t k, void* stream) {
   if (int rc = fp4_common("fp4_tile_scales", fmt, SB_BF16, n, k)) return rc;
-  if (k % 32 || n_mat < 1 || n < 1 || n_mat * n > FP4_MAX_ROWS)
+  if (k % 32 || n_mat < 1 || n < 1 || n_mat > FP4_MAX_ROWS / n)
     return fail(SB_ERR_SHAPE, "fp4_tile_scales: need K %% 32 == 0 and 1..2^30 rows (n_mat=%lld n=%lld k=%lld)",
                 (long long)n_mat, (long long)n, (long long)k);
   if (!src || !dst) return fail(SB_ERR_ARG, "fp4_tile_scales: NULL pointer");

@@ -124,3 +124,20 @@ def test_expert_order_workspace_holds_the_counts_and_their_totals():
     f = _lib.lib().sb_expert_order_workspace_bytes
     assert f(64 * 2048, 256) == 64 * 256 * 4 and f(64 * 2048 + 1, 256) == 66 * 256 * 4
     assert f(2 ** 31 - 1, 1024) == (2 ** 20 + 1) * 1024 * 4
+
+
+def test_sizes_whose_products_leave_64_bits_are_refused():
+    L = _lib.lib()
+    for n_mat, n in ((1 << 34, 1 << 30), (1 << 60, 16), ((1 << 62) + 1, 4), ((1 << 63) - 1, 2)):
+        assert L.sb_fp4_tile_scales(NV, FAKE, FAKE, n_mat, n, 64, None) == -2, (n_mat, n)
+    f = L.sb_fp4_scale_bytes
+    assert f(NV, 1 << 30, 1 << 30, 64, 0) == 0 and f(NV, 1 << 20, (1 << 10) + 1, 64, 0) == 0 and f(NV, 1 << 34, 1 << 30, 64, 0) == 0
+    assert f(NV, 1 << 20, 1 << 10, 64, 0) == (1 << 20) * 8 * 512 and f(MX, 1 << 30, 1, 65536, 0) == (1 << 30) * 512 * 512
+
+    def gg(e, n, m=4, ld=None):
+        return L.sb_fp4_grouped_gemm(NV, FAKE, FAKE, None, 0, m, FAKE, FAKE, FAKE, None, 1, e, n, 64, 0, 0.0, None, FAKE, 0,
+                                     n if ld is None else ld, None)
+
+    for e, n, m in ((4, 1 << 62, 508 * 128), (1024, 1 << 54, 4), (1, (1 << 63) - 1, 4), (2, 1 << 62, 4)):
+        assert gg(e, n, m) == -2, (e, n)
+        assert L.sb_fp4_gemm(NV, FAKE, FAKE, None, 0, m, FAKE, FAKE, None, 0, n, 64, FAKE, 0, n, None) == -2
