@@ -4,8 +4,8 @@
 // topk_kernel: one warp per token, lane l holds experts C l .. C l + C - 1. Selection values are exact
 // without a bias (the scores ascend with the logits, so the logits themselves are compared). With a
 // bias, or for groups scored by a sum, they are fp32 sums of rounded scores: the gaps that decide are
-// compared with the error bound of those sums, and where one is smaller the candidates in doubt are
-// compared again in 64 bits (a fraction of a percent of the tokens; selecting those tokens anew from 64-bit
+// compared with the error bounds of the values on their two sides, and where one is smaller the candidates in doubt
+// are compared again in 64 bits (a fraction of a percent of the tokens; selecting those tokens anew from 64-bit
 // scores of all experts took 20 us of 38). So a selection never hangs on how an exponential rounds.
 //
 // order_kernel: a stable counting sort of the pairs by expert, in blocks of 2048 pairs, no atomics
@@ -217,6 +217,24 @@ __device__ __forceinline__ void scores32(const float (&l)[C], float mx, float rs
   for (int i = 0; i < C; ++i) s[i] = score32(FUNC, l[i], mx, rsum);
 }
 
+// How far fp32 selection values may be from the real ones: a score by k times the row's largest, its sum with a bias (and that of
+// two such values) by a rounding more of itself. In units of 2^-24: sigmoid 7 (the exponential 4, the sum 1, the reciprocal 2),
+// sqrtsoftplus 5; softmax 4 for the exponential and its argument, 3 for the division, 20 for the exponentials in
+// the sum (each 2 (2 + 1.173 d) and d for its argument, d below the largest logit; of 1024 experts at one d the mean
+// is largest at d = 5.4) and C + 4 for the C + 5 additions of a lane and the warp; the factor of 6.1e-8 is 2% above
+// 2^-24. value +- of(value) ascends with the value, so that neighbours in a ranking are all that has to be compared.
+struct Bound {
+  float ks;   // k times the largest score
+  __device__ __forceinline__ float rounding(float v) const { return 6.1e-8f * fminf(fabsf(v), FLT_MAX); }
+  __device__ __forceinline__ float of(float v) const { return rounding(v) + ks; }
+  // a > b for certain (never of two infinities)
+  __device__ __forceinline__ bool above(float a, float b) const { return a - b > of(a) + of(b); }
+};
+template <int C>
+__device__ __forceinline__ float bound_of_scores(int func, float largest) {
+  return 6.1e-8f * (func == SCORE_SOFTMAX ? (float)(C + 32) : 8.f) * largest;
+}
+
 template <int C>
 __device__ __forceinline__ void load_bias(const TopkArgs& a, int lane, float (&b)[C]) {
   if (C % 4 == 0 && a.vec_bias) {
@@ -249,7 +267,7 @@ __device__ __forceinline__ double sum_exact(const TopkArgs& a, const float (&l)[
   return sum;
 }
 
-// The groups kept, from exact scores of the experts that can be among a group's two best: near[i], those within eps
+// The groups kept, from exact scores of the experts that can be among a group's two best: near[i], those within the bounds
 // of its second best fp32 value (rare, out of line).
 template <int C, typename T>
 __device__ __noinline__ uint32_t kept_exact(const TopkArgs& a, const T* row, int lane, float lowest, float mx, uint32_t near) {
@@ -320,25 +338,33 @@ template <int C, typename T>
 __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const float (&l)[C], int lane, float lowest, float mx,
                                       float sum) {
   const bool biased = a.bias != nullptr, scored = biased || (a.groups > 1 && a.group_two);
-  float v[C], gv[C], most = 0.f;
+  float v[C], gv[C];
+  Bound err = {0.f};
   if (scored) {
     // (one branch for the whole row, not one per expert)
     if (a.score == SCORE_SOFTMAX) scores32<C, SCORE_SOFTMAX>(l, mx, rcp(sum), gv);
     else if (a.score == SCORE_SIGMOID) scores32<C, SCORE_SIGMOID>(l, mx, 1.f, gv);
     else scores32<C, SCORE_SQRTSOFTPLUS>(l, mx, 1.f, gv);
+    float largest = 0.f;
+    if (a.score == SCORE_SOFTMAX) {
+      largest = rcp(sum);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) largest = fmaxf(largest, gv[i]);
+      largest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(largest)));
+    }
+    err.ks = bound_of_scores<C>(a.score, largest);
     if (biased) {
       float b[C];
       load_bias<C>(a, lane, b);
 #pragma unroll
       for (int i = 0; i < C; ++i) {
-        const float t = gv[i] + b[i], mag = gv[i] + fabsf(b[i]);
-        v[i] = gv[i] = l[i] > -INFINITY && t == t ? t : -INFINITY;
-        most = fmaxf(most, v[i] > -INFINITY ? mag : 0.f);   // (a bias of -inf masks its expert)
+        const float t = gv[i] + b[i];
+        v[i] = gv[i] = l[i] > -INFINITY && t == t ? t : -INFINITY;   // (a bias of -inf masks its expert)
       }
     } else {
 #pragma unroll
       for (int i = 0; i < C; ++i) {
-        most = fmaxf(most, gv[i]);
         gv[i] = l[i] > -INFINITY ? gv[i] : -INFINITY;
         v[i] = l[i];
       }
@@ -347,14 +373,17 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] = gv[i] = l[i];
   }
-  // rounding errors of a score and its sum, twice (two of them are compared) and for pairs of experts
-  const float eps = scored ? 2e-6f * __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most))) : 0.f;
   uint32_t kept = 0xffffffffu;
   if (a.groups > 1) {
-    float gs = -INFINITY;   // lane g: the score of group g
-    // This lane's experts that may be among their group's two best: also those that no comparison tells from the
-    // second (biases of +inf on two experts make the difference NaN).
+    float gs = -INFINITY, ge = 0.f;   // lane g: the score of group g, and its bound
+    // This lane's experts that may be among their group's two best. (Four bounds of the second best: two of its own, and
+    // two for an expert below it.)
     uint32_t near = 0u;
+    auto group = [&](float b1, float b2, float& score, float& bound) {
+      const bool two = a.group_two && b2 > -INFINITY;
+      score = two ? b1 + b2 : b1;
+      bound = two ? err.of(b1) + err.of(b2) + err.rounding(score) : err.of(b1);
+    };
     if (a.span > 0) {
       float b1 = -INFINITY, b2 = -INFINITY;
 #pragma unroll
@@ -363,9 +392,12 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
         const float c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
         merge(b1, b2, c1, c2);
       }
-      gs = __shfl_sync(0xffffffffu, a.group_two && b2 > -INFINITY ? b1 + b2 : b1, (lane * a.span) & 31);
+      group(b1, b2, gs, ge);
+      gs = __shfl_sync(0xffffffffu, gs, (lane * a.span) & 31);
+      ge = __shfl_sync(0xffffffffu, ge, (lane * a.span) & 31);
+      const float from = b2 - 4.f * err.of(b2);
 #pragma unroll
-      for (int i = 0; i < C; ++i) near |= gv[i] > -INFINITY && !(gv[i] < b2 - eps) ? 1u << i : 0u;
+      for (int i = 0; i < C; ++i) near |= gv[i] > -INFINITY && !(gv[i] < from) ? 1u << i : 0u;
     } else {
       for (int g = 0; g < a.groups; ++g) {
         float b1 = -INFINITY, b2 = -INFINITY;
@@ -379,26 +411,29 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
           const float c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
           merge(b1, b2, c1, c2);
         }
-        if (lane == g) gs = a.group_two && b2 > -INFINITY ? b1 + b2 : b1;
+        if (lane == g) group(b1, b2, gs, ge);
+        const float from = b2 - 4.f * err.of(b2);
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           const int e = lane * C + i;
-          if (e >= g * a.size && e < (g + 1) * a.size && gv[i] > -INFINITY && !(gv[i] < b2 - eps)) near |= 1u << i;
+          if (e >= g * a.size && e < (g + 1) * a.size && gv[i] > -INFINITY && !(gv[i] < from)) near |= 1u << i;
         }
       }
     }
-    uint32_t gk = lane < a.groups ? key_of(gs) : 0u, low = 0u;
+    uint32_t gk = lane < a.groups ? key_of(gs) : 0u;
     kept = 0u;
     for (int j = 0; j < a.kept; ++j) {
-      low = __reduce_max_sync(0xffffffffu, gk);
-      const int w = __ffs(__ballot_sync(0xffffffffu, gk == low)) - 1;
+      const uint32_t top = __reduce_max_sync(0xffffffffu, gk);
+      const int w = __ffs(__ballot_sync(0xffffffffu, gk == top)) - 1;
       kept |= 1u << w;
       if (lane == w) gk = 0u;
     }
     if (scored && a.kept < a.groups) {
-      const uint32_t high = __reduce_max_sync(0xffffffffu, gk);
-      if (high > key_of(-INFINITY) && !(value_of(low) - value_of(high) > eps))
-        kept = kept_exact<C, T>(a, row, lane, lowest, mx, near);
+      // the least that a kept group can be, the most of the others (masked ones are what they are)
+      const bool in = (kept >> lane) & 1u;
+      const uint32_t low = __reduce_min_sync(0xffffffffu, in ? key_of(gs - ge) : 0xffffffffu);
+      const uint32_t high = __reduce_max_sync(0xffffffffu, !in && gk > key_of(-INFINITY) ? key_of(gs + ge) : 0u);
+      if (high >= low) kept = kept_exact<C, T>(a, row, lane, lowest, mx, near);
     }
   }
   uint32_t key[C], own[C];
@@ -459,14 +494,14 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
     // order is that of their ids. Else all that may belong to the k best are ordered by their exact values.
     const uint32_t nk = __shfl_down_sync(0xffffffffu, got, 1);
     const int ne = __shfl_down_sync(0xffffffffu, mine, 1);
-    bool near = lane < a.topk && got > 1u && nk > 1u && !(value_of(got) - value_of(nk) > eps);
+    bool near = lane < a.topk && got > 1u && nk > 1u && !err.above(value_of(got), value_of(nk));
     if (near && a.bias[mine] == a.bias[ne] && row[mine] == row[ne]) near = false;
     if (__any_sync(0xffffffffu, near)) {
       const uint32_t last = __shfl_sync(0xffffffffu, got, a.topk - 1);
       uint32_t top = __shfl_sync(0xffffffffu, got, a.topk);
       int n = rounds;
-      while (n < 32 && last > 1u && top > 1u && !(value_of(last) - value_of(top) > eps)) top = round(n++);
-      if (last > 1u && top > 1u && !(value_of(last) - value_of(top) > eps)) return select_exact<C, T>(a, row, lane, lowest);
+      while (n < 32 && last > 1u && top > 1u && !err.above(value_of(last), value_of(top))) top = round(n++);
+      if (last > 1u && top > 1u && !err.above(value_of(last), value_of(top))) return select_exact<C, T>(a, row, lane, lowest);
       mine = expert();
       mine = order_exact<C, T>(a, row, lane, lowest, mx, mine, lane < n ? (got > 1u ? 2 : (int)got) : 0, n);
     }

@@ -126,6 +126,43 @@ def test_topk_groups_with_several_biases_of_inf(e, g, group_score, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("above", [False, True])
+def test_topk_softmax_sums_that_lose_their_small_terms(above):
+    """Two experts of 1 in lanes whose 31 others, just below 2^-24, are lost in the lane's fp32 sum: the group's score is 1.8e-6
+    above the real one, further than one rounding of each value explains. The other group lies between the two, or above."""
+    _need_gpu()
+    e, g = 1024, 16
+    logits = torch.full((1, e), -math.inf)
+    logits[0, :64] = math.log(5.9e-8)
+    logits[0, 0] = logits[0, 32] = 0.0
+    logits[0, 64:128] = -30.0
+    bias = torch.zeros(e)
+    bias[64] = bias[65] = 0.5 + (1e-7 if above else -0.75e-6)
+    _check(logits, 2, bias, score="softmax", n_group=g, topk_group=1, group_score="top2")
+
+
+@gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid", "sqrtsoftplus"])
+@pytest.mark.parametrize("e,g", [(64, 8), (60, 4), (256, 8), (1024, 16)])
+def test_topk_finite_masks_and_large_biases(score, e, g):
+    """Biases of -1e9 and fp32's lowest value, on some experts and whole groups, and of 1e9 and 1e30 on a few."""
+    _need_gpu()
+    gen = torch.Generator().manual_seed(e)
+    s = e // g
+    logits = 1.5 * torch.randn(16, e, generator=gen)
+    for low in (-1e9, torch.finfo(torch.float32).min):
+        bias = 0.2 * torch.randn(e, generator=gen)
+        bias[::5] = low
+        bias[s:2 * s] = low
+        for high in (0.1, 1e9, 1e30):
+            bias[2 * s + 1] = bias[3 * s + 2] = high
+            _check(logits, 6, bias, score=score)
+            for gs in ("max", "top2"):
+                for kept in (2, g - 1):
+                    _check(logits, 6, bias, score=score, n_group=g, topk_group=kept, group_score=gs)
+
+
+@gpu
 def test_topk_strides_and_large_batches():
     _need_gpu()
     gen = torch.Generator().manual_seed(6)
