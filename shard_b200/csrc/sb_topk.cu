@@ -43,23 +43,30 @@ __device__ __forceinline__ float rcp(float v) {
   return r;
 }
 
-// The score of a logit: for the selection (each within a few 2^-24 of itself, softmax of the row's largest), as an
-// output, and in 64 bits; mx, sum: the row's softmax statistics.
+// sqrt(softplus(l)). Below FAR e^l is a subnormal number or 0, whose root is not: e^(l / 2) is the score to within e^l of itself.
+constexpr float FAR = -80.f;
+__device__ __forceinline__ float sqrtsoftplus(float l) {
+  const float t = expf(l < FAR ? 0.5f * l : -fabsf(l));
+  return l < FAR ? t : sqrtf(fmaxf(l, 0.f) + log1pf(t));
+}
+
+// The score of a logit: for the selection (each within a few 2^-24 of itself, softmax of the row's largest; sigmoids below
+// 2^-126 count as 0), as an output, and in 64 bits; mx, sum: the row's softmax statistics.
 __device__ __forceinline__ float score32(int func, float l, float mx, float rsum) {
   if (func == SCORE_SOFTMAX) return l > -INFINITY ? __expf(l - mx) * rsum : 0.f;
   if (func == SCORE_SIGMOID) return rcp(1.f + expf(-l));
-  return sqrtf(fmaxf(l, 0.f) + log1pf(expf(-fabsf(l))));
+  return sqrtsoftplus(l);
 }
 __device__ __forceinline__ float score_weight(int func, float l, float mx, float sum) {
   if (func == SCORE_SOFTMAX) return __fdiv_rn(expf(l - mx), sum);
-  if (func == SCORE_SIGMOID) return __fdiv_rn(1.f, 1.f + expf(-l));
-  return sqrtf(fmaxf(l, 0.f) + log1pf(expf(-fabsf(l))));
+  if (func == SCORE_SIGMOID) return l < FAR ? expf(l) : __fdiv_rn(1.f, 1.f + expf(-l));   // (expf(-l) may be inf there)
+  return sqrtsoftplus(l);
 }
 __device__ __noinline__ double score64(int func, float l, double mx, double sum) {
   const double x = (double)l;
   if (func == SCORE_SOFTMAX) return exp(x - mx) / sum;
   if (func == SCORE_SIGMOID) return 1.0 / (1.0 + exp(-x));
-  return sqrt(fmax(x, 0.0) + log1p(exp(-fabs(x))));
+  return l < FAR ? exp(0.5 * x) : sqrt(fmax(x, 0.0) + log1p(exp(-fabs(x))));
 }
 
 __device__ __forceinline__ float logit(const float* p) { return *p; }
@@ -222,7 +229,7 @@ __device__ __forceinline__ void scores32(const float (&l)[C], float mx, float rs
 // sqrtsoftplus 5; softmax 4 for the exponential and its argument, 3 for the division, 20 for the exponentials in
 // the sum (each 2 (2 + 1.173 d) and d for its argument, d below the largest logit; of 1024 experts at one d the mean
 // is largest at d = 5.4) and C + 4 for the C + 5 additions of a lane and the warp; the factor of 6.1e-8 is 2% above
-// 2^-24. value +- of(value) ascends with the value, so that neighbours in a ranking are all that has to be compared.
+// 2^-24. Where all scores are tiny: 2.4e-38 for one that counts as 0. value +- of(value) ascends with the value, so that neighbours in a ranking are all that has to be compared.
 struct Bound {
   float ks;   // k times the largest score
   __device__ __forceinline__ float rounding(float v) const { return 6.1e-8f * fminf(fabsf(v), FLT_MAX); }
@@ -232,7 +239,7 @@ struct Bound {
 };
 template <int C>
 __device__ __forceinline__ float bound_of_scores(int func, float largest) {
-  return 6.1e-8f * (func == SCORE_SOFTMAX ? (float)(C + 32) : 8.f) * largest;
+  return 6.1e-8f * (func == SCORE_SOFTMAX ? (float)(C + 32) : 8.f) * largest + 2.4e-38f;
 }
 
 template <int C>

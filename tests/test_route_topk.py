@@ -163,6 +163,33 @@ def test_topk_finite_masks_and_large_biases(score, e, g):
 
 
 @gpu
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("lo,hi", [(-120, -100), (-160, -80), (-100, 3)])
+def test_topk_sqrtsoftplus_of_far_logits(lo, hi, renormalize):
+    """e^l is subnormal or 0 where the score, its root, is a plain number."""
+    _need_gpu()
+    gen = torch.Generator().manual_seed(-lo)
+    l = lo + (hi - lo) * torch.rand(9, 64, generator=gen)
+    for scale in (1.0, 1e20):
+        _check(l, 6, score="sqrtsoftplus", renormalize=renormalize, scale=scale)
+        _check(l, 6, (l.mean() / 2).exp() * torch.rand(64, generator=gen), score="sqrtsoftplus", renormalize=renormalize, scale=scale)
+
+
+@gpu
+def test_topk_sigmoids_near_the_end_of_the_range():
+    """Scores on both sides of 2^-126, with biases of their size: the selection is still that of the real sums."""
+    _need_gpu()
+    gen = torch.Generator().manual_seed(1)
+    l = -87 - 2 * torch.rand(40, 64, generator=gen)
+    _check(l, 6, 1e-38 * torch.rand(64, generator=gen), renormalize=False)
+    _check(l, 6, 1e-38 * torch.rand(64, generator=gen), n_group=8, topk_group=3, group_score="top2", renormalize=False)
+    l = -75 - 20 * torch.rand(40, 64, generator=gen)
+    w, ids = route.topk(l.cuda(), 6, renormalize=False)
+    want = 1 / (1 + torch.exp(-l.double().gather(1, ids.cpu())))
+    assert bool(((w.cpu().double() - want).abs() <= 16 * 2.0 ** -23 * want + 2.0 ** -149).all())
+
+
+@gpu
 def test_topk_strides_and_large_batches():
     _need_gpu()
     gen = torch.Generator().manual_seed(6)
