@@ -516,6 +516,23 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
   return mine;
 }
 
+// Chosen scores over their sum where fp32 scores lose bits or vanish (sigmoids of logits below -69, softmax of experts that far
+// below one that is not chosen): in 64 bits, each score over e^(the largest chosen logit) before they are added (rare,
+// out of line). x: the lane's chosen logit, -inf: none, or masked.
+__device__ __noinline__ float far_weight(int func, float x) {
+  const double top = (double)warp_max(x), c = func == SCORE_SOFTMAX ? top : fmin(top, 0.0), l = (double)x;
+  double e = 0.0;
+  if (x > -INFINITY) {
+    if (func == SCORE_SOFTMAX) e = exp(l - c);
+    else if (func == SCORE_SIGMOID) e = x < 0.f ? exp(l - c) / (1.0 + exp(l)) : 1.0 / (1.0 + exp(-l));
+    else e = x < FAR ? exp(0.5 * (l - c)) : sqrt(fmax(l, 0.0) + log1p(exp(-fabs(l)))) * exp(-0.5 * c);
+  }
+  double sum = e;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return (float)(e / sum);
+}
+
 // One warp per token; the chain of its rounds and its instructions bound it.
 template <int C, typename T>
 __global__ void __launch_bounds__(128) topk_kernel(TopkArgs a) {
@@ -538,16 +555,20 @@ __global__ void __launch_bounds__(128) topk_kernel(TopkArgs a) {
   }
   const int mine = select<C, T>(a, row, l, lane, lowest, mx, sum);
   // weights of the chosen ones, from their unbiased scores
-  float w = 0.f;
+  float w = 0.f, x = -INFINITY;
   if (lane < a.topk) {
-    const float x = clean(logit(row + mine), lowest);
+    x = clean(logit(row + mine), lowest);
     if (x > -INFINITY) w = score_weight(a.score, x, mx, sum);
   }
   if (a.renorm) {
-    float s = w;   // lanes 16 and above hold zeros
+    if (__any_sync(0xffffffffu, x > -INFINITY && w < 1e-30f)) {
+      w = far_weight(a.score, x);
+    } else {
+      float s = w;   // lanes 16 and above hold zeros
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    w = s > 0.f ? __fdiv_rn(w, s) : 0.f;
+      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      w = s > 0.f ? __fdiv_rn(w, s) : 0.f;
+    }
   }
   if (lane < a.topk) {
     a.weights[t * a.topk + lane] = w * a.scale;

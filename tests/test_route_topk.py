@@ -190,6 +190,30 @@ def test_topk_sigmoids_near_the_end_of_the_range():
 
 
 @gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid", "sqrtsoftplus"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lo,hi", [(-98, -92), (-300, -90), (-110, 5), (-400, -60)])
+def test_topk_renormalised_weights_of_far_logits(score, dtype, lo, hi):
+    """Rows whose chosen scores are all subnormal or 0 in fp32 have weights that sum to one all the same; so do the experts
+    far below one that a bias of -inf, or its group, leaves out."""
+    _need_gpu()
+    gen = torch.Generator().manual_seed(-lo)
+    l = (lo + (hi - lo) * torch.rand(12, 64, generator=gen)).to(dtype)
+    l[1::3, 5] = 12
+    l[2, :] = -math.inf
+    l[3, 7:] = -math.inf
+    l[6, 3:] = -math.inf
+    b = torch.zeros(64)
+    b[5] = -math.inf
+    for bias in (None, b, b + 0.1 * torch.rand(64, generator=gen)):
+        _check(l, 6, bias, score=score, scale=2.5)
+        _check(l, 6, bias, score=score, n_group=8, topk_group=3, group_score="top2")
+    w, _ = route.topk(l.cuda(), 6, bias=b.cuda(), score=score)
+    total = w.double().sum(1).cpu()
+    assert bool(((total - 1).abs() <= 6 * 2.0 ** -23)[[i for i in range(12) if i != 2]].all()) and float(total[2]) == 0
+
+
+@gpu
 def test_topk_strides_and_large_batches():
     _need_gpu()
     gen = torch.Generator().manual_seed(6)
