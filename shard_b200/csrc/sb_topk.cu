@@ -108,7 +108,7 @@ __device__ __forceinline__ float row_max(const float (&l)[C]) {
   return warp_max(mx);
 }
 
-// A token's selection in 64 bits: lane j < k gets the expert of rank j. Out of line: it is rare, and its
+// A token's selection with a bias, in 64 bits: lane j < k gets the expert of rank j. Out of line: it is rare, and its
 // registers are not the others'.
 template <int C, typename T>
 __device__ __noinline__ int select_exact(const TopkArgs& a, const T* row, int lane, float lowest) {
@@ -120,15 +120,14 @@ __device__ __noinline__ int select_exact(const TopkArgs& a, const T* row, int la
   for (int i = 0; i < C; ++i) sum += l[i] > -INFINITY ? exp((double)l[i] - mx) : 0.0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  double v[C], gv[C];      // what the experts, and what their groups, are compared by
+  double v[C];             // what the experts, and their groups, are compared by
 #pragma unroll 1
   for (int i = 0; i < C; ++i) {
     const int e = lane * C + i;
-    v[i] = gv[i] = NONE;
+    v[i] = NONE;
     if (e < a.experts && l[i] > -INFINITY) {
-      const double s = score64(a.score, l[i], mx, sum), t = a.bias != nullptr ? s + (double)a.bias[e] : (double)l[i];
+      const double t = score64(a.score, l[i], mx, sum) + (double)a.bias[e];
       v[i] = t == t ? t : NONE;
-      gv[i] = a.bias == nullptr && a.group_two ? s : v[i];
     }
   }
   uint32_t kept = 0xffffffffu;
@@ -140,7 +139,7 @@ __device__ __noinline__ int select_exact(const TopkArgs& a, const T* row, int la
 #pragma unroll 1
       for (int i = 0; i < C; ++i) {
         const int e = lane * C + i;
-        if (e >= g * size && e < (g + 1) * size) merge(b1, b2, gv[i], NONE);
+        if (e >= g * size && e < (g + 1) * size) merge(b1, b2, v[i], NONE);
       }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
