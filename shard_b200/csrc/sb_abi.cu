@@ -1082,7 +1082,7 @@ int sb_residual_rmsnorm(void* x, const void* y, int64_t rows, int64_t dim, const
 
 namespace {
 
-constexpr int64_t FP4_MAX_K = 65536;      // a row's values stay in the registers of one CTA
+constexpr int64_t FP4_MAX_K = 65536;      // the quantiser keeps a row's 4096 largest magnitudes of 16 in shared memory
 constexpr int64_t FP4_MAX_ROWS = 1 << 30;
 constexpr int64_t FP4_MAX_GROUPS = 1024;
 

@@ -51,6 +51,7 @@ constexpr int SFA_COL = NT_APART + NT_MAX;  // scale factors: 4 atoms x 4 column
 constexpr int SFB_COL = SFA_COL + 16;  // 4 atoms x 8 columns of the tokens (two row blocks)
 constexpr uint32_t WAIT_LIMIT = 1u << 16;
 constexpr int SMEM_LIMIT = 232448;
+constexpr int64_t L2_AHEAD = 32 << 20;
 
 enum Form { SINGLE = 0, PAIRED = 1, SPLIT = 2 };
 
@@ -952,8 +953,13 @@ cudaError_t launch_fp4_mm(const Fp4MmArgs& g, int dtype, cudaStream_t st) {
   a.split = 1;
   if (g.offsets == nullptr && tt == 1)
     while (a.split < 8 && tiles * a.split * 2 <= sms && (a.ksteps + 3) / 4 >= a.split * 4) a.split *= 2;
-  // (one token tile: a CTA's first tile is its own row block, whose stages it all reads)
-  a.ahead = g.offsets == nullptr && tt == 1 ? ((a.ksteps + 3) / 4 + a.split - 1) / a.split : 0;
+  // (one token tile: a CTA's first tile is its own row block, whose stages it all reads; no more than a quarter of L2 in all,
+  // or the first ones leave it before they are copied: 1 x 18944 x 32768 took 88 us without this limit, 76 with it)
+  if (g.offsets == nullptr && tt == 1) {
+    const int64_t ctas = tiles * a.split < sms ? tiles * a.split : sms, most = L2_AHEAD / (ctas * A_BYTES);
+    a.ahead = ((a.ksteps + 3) / 4 + a.split - 1) / a.split;
+    if (a.ahead > most) a.ahead = (int)most;
+  }
   // Token rows of a copy: a whole tile's (of a pair's half), but with narrow groups 32 at a time, as many as the group has.
   // (Three copies of 32 rows in place of one of 96 made the copying thread the bound: 0.33 us a stage, one copy 0.26.)
   a.box = pair ? a.nt / 2 : g.offsets ? BOX : a.nt;

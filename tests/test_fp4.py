@@ -694,3 +694,21 @@ def test_pack_on_a_stream(kind):
     got = fp4.grouped_gemm(a, fp4.pack(NV, c, sc, wide, kind=kind, stream=st), stream=st)
     st.synchronize()
     assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+@pytest.mark.parametrize("m,n,k", [(1, 300, 65536), (3, 19000, 16384), (64, 19000, 8224)])
+def test_gemm_of_long_rows(fmt, m, n, k):
+    """Few tokens against weights that outgrow L2, and the longest K."""
+    _need_gpu()
+    w = fp4.quant(torch.randn(n, k, generator=torch.Generator("cuda").manual_seed(n), device="cuda", dtype=torch.bfloat16), fmt)
+    a = fp4.quant(_acts(m, k, torch.bfloat16, seed=m).cuda(), fmt)
+    y = fp4.gemm(a, w, out_dtype=torch.float32).double()
+    at = torch.cat([torch.arange(0, n, 97), torch.arange(n - 130, n)])
+    wv, av = fp4.dequant(w, torch.float32)[at].double(), fp4.dequant(a, torch.float32).double()
+    exact = av @ wv.T
+    # (values of 32 bits: each 2^-24 off, two in a product)
+    tol = _tol(av, wv, exact, k, torch.float32) + 2.0 ** -22 * (av.abs() @ wv.abs().T)
+    assert bool(((y[:, at] - exact).abs() <= tol).all())
+    assert fp4.device_error() == 0
