@@ -114,7 +114,7 @@ class Fp4Tensor:
     @property
     def codes(self) -> torch.Tensor:
         if self._codes is None:
-            self._codes = self._buf[:self._parts[0]].view(self.rows, -1)
+            self._codes = self._buf[:self._parts[0]].view(self.rows, -(-self.k // 32) * 16)
         return self._codes
 
     @property
@@ -134,8 +134,9 @@ class Fp4Tensor:
         if self.offsets is not None:
             raise ValueError("canonical_scales: rows in expert groups")
         nb = self.codes.shape[1] // (8 if self.fmt == F.FMT_NVFP4 else 16)
-        s = self.scales.view(self.mats, -(-self.rows // 128), -1, 32, 4, 4)     # mat, block, atom, lane, quarter, byte
-        s = s.permute(0, 1, 4, 3, 2, 5).reshape(self.mats, -1, s.shape[2] * 4)
+        blocks, atoms = -(-self.rows // 128), -(-nb // 4)
+        s = self.scales.view(self.mats, blocks, atoms, 32, 4, 4)                # mat, block, atom, lane, quarter, byte
+        s = s.permute(0, 1, 4, 3, 2, 5).reshape(self.mats, blocks * 128, atoms * 4)
         return s[:, :self.rows, :nb].reshape(self.mats * self.rows, nb).contiguous()
 
 

@@ -712,3 +712,25 @@ def test_gemm_of_long_rows(fmt, m, n, k):
     tol = _tol(av, wv, exact, k, torch.float32) + 2.0 ** -22 * (av.abs() @ wv.abs().T)
     assert bool(((y[:, at] - exact).abs() <= tol).all())
     assert fp4.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+@pytest.mark.parametrize("k", [33, 64, 4096])
+def test_operands_of_no_rows(fmt, k):
+    """A batch of no tokens through every call, and its parts' shapes."""
+    _need_gpu()
+    x = torch.empty(2, 0, k, device="cuda", dtype=torch.bfloat16)
+    q = fp4.quant(x, fmt)
+    kp = -(-k // 32) * 32
+    assert q.codes.shape == (0, kp // 2) and q.canonical_scales().shape == (0, kp // (16 if fmt == NV else 32))
+    assert q.ts is None if fmt == MX else q.ts.shape == (0,)
+    assert fp4.dequant(q).shape == (2, 0, k)
+    w = fp4.quant(_acts(24, k, torch.bfloat16).cuda(), fmt)
+    assert fp4.gemm(q, w).shape == (2, 0, 24)
+    off = torch.zeros(4, dtype=torch.int32, device="cuda")
+    codes, s, ts, _ = P.weights(fmt, 24, kp, seed=1, mats=3)
+    bank = fp4.pack(fmt, codes.cuda(), s.cuda(), None if ts is None else ts.cuda())
+    bank.k = k
+    assert fp4.grouped_gemm(fp4.quant(x[0], fmt, offsets=off), bank).shape == (0, 24)
+    torch.cuda.synchronize()
