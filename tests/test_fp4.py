@@ -734,3 +734,20 @@ def test_operands_of_no_rows(fmt, k):
     bank.k = k
     assert fp4.grouped_gemm(fp4.quant(x[0], fmt, offsets=off), bank).shape == (0, 24)
     torch.cuda.synchronize()
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+def test_a_gather_of_no_rows(fmt):
+    _need_gpu()
+    x = _acts(3, 64, torch.bfloat16).cuda()
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    q = fp4.quant(x, fmt, rows=none)
+    assert q.rows == 0 and fp4.dequant(q).shape == (0, 64) and q.codes.shape == (0, 32)
+    off = torch.zeros(4, dtype=torch.int32, device="cuda")
+    codes, s, ts, _ = P.weights(fmt, 24, 64, seed=1, mats=3)
+    bank = fp4.pack(fmt, codes.cuda(), s.cuda(), None if ts is None else ts.cuda())
+    assert fp4.grouped_gemm(fp4.quant(x, fmt, rows=none, offsets=off), bank).shape == (0, 24)
+    o = route.expert_order(torch.empty(0, 2, dtype=torch.int64, device="cuda"), 3)
+    assert fp4.grouped_gemm(fp4.quant(x[:0], fmt, rows=o.tokens, offsets=o.offsets), bank).shape == (0, 24)
+    torch.cuda.synchronize()
