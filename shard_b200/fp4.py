@@ -189,7 +189,8 @@ def pack(fmt: Union[int, str], codes: torch.Tensor, scales: torch.Tensor, ts: Op
     """Canonical weights -> operand, once at load time. codes uint8 [N, K/2] or [E, N, K/2], scales as bytes or
     in their own type [.., K/16] (NVFP4) / [.., K/32] (MXFP4), ts fp32: one per matrix, or for w13 banks
     [E, 2] (w1, w3). K % 32 == 0. kind W13: the rows are w1's, then w3's; they are interleaved, so that one
-    pass of grouped_gemm forms silu(w1 x) * (w3 x). PLAIN operands share the codes given."""
+    pass of grouped_gemm forms silu(w1 x) * (w3 x). PLAIN operands share the codes given, if these are contiguous and
+    16-byte aligned."""
     f = _fmt(fmt)
     if not codes.is_cuda or codes.dim() not in (2, 3):
         raise ValueError("pack: codes must be a CUDA tensor [N, K/2] or [E, N, K/2]")
@@ -216,6 +217,8 @@ def pack(fmt: Union[int, str], codes: torch.Tensor, scales: torch.Tensor, ts: Op
     if kind == W13:
         c, s = (t.view(mats, 2, n // 2, -1).transpose(1, 2).reshape(mats, n, -1) for t in (c, s))
     c, s = c.contiguous().view(mats * n, k // 2), s.contiguous()
+    if c.data_ptr() % 16:                 # (a view into a larger buffer: the products copy from 16-byte addresses)
+        c = c.clone()
     L = lib()
     out = torch.empty(L.sb_fp4_scale_bytes(f, mats, n, k, 0), dtype=torch.uint8, device=c.device)
     check(L.sb_fp4_tile_scales(f, s.data_ptr(), out.data_ptr(), mats, n, k, torch.cuda.current_stream().cuda_stream),

@@ -751,3 +751,28 @@ def test_a_gather_of_no_rows(fmt):
     o = route.expert_order(torch.empty(0, 2, dtype=torch.int64, device="cuda"), 3)
     assert fp4.grouped_gemm(fp4.quant(x[:0], fmt, rows=o.tokens, offsets=o.offsets), bank).shape == (0, 24)
     torch.cuda.synchronize()
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+def test_pack_of_views(fmt):
+    """Codes and scales inside larger buffers: at odd addresses, and every other matrix of a bank."""
+    _need_gpu()
+    codes, s, ts, _ = P.weights(fmt, 40, 96, seed=5, mats=4)
+    t = None if ts is None else ts.cuda()
+    off = torch.tensor([0, 3, 3, 8, 9], dtype=torch.int32, device="cuda")
+    a = fp4.quant(_acts(9, 96, torch.bfloat16).cuda(), fmt, offsets=off)
+    want = fp4.grouped_gemm(a, fp4.pack(fmt, codes.cuda(), s.cuda(), t))
+
+    def inside(v, at):
+        b = torch.empty(v.numel() + at, dtype=torch.uint8, device="cuda")
+        w = b[at:].view(v.shape)
+        w.copy_(v)
+        return w
+
+    for at in (1, 8, 16):
+        assert torch.equal(fp4.grouped_gemm(a, fp4.pack(fmt, inside(codes, at), inside(s, at), t)), want)
+    apart = lambda v: torch.stack([v, v], 1).cuda()[:, 1]  # noqa: E731
+    assert torch.equal(fp4.grouped_gemm(a, fp4.pack(fmt, apart(codes), apart(s), t)), want)
+    c = codes.cuda()
+    assert fp4.pack(fmt, c, s.cuda(), t).codes.data_ptr() == c.data_ptr()
