@@ -530,11 +530,13 @@ __global__ void __launch_bounds__(256) gather_kernel(QuantArgs a, const uint8_t*
   }
   const uint32_t* w = words + (has ? src : 0) * a.atoms;
   uint8_t* sr = a.scales + ((pos >> 7) * a.atoms) * 512 + (pos & 31) * 16 + ((pos >> 5) & 3) * 4;
-  // (a missing row's scales are those of zeros: 0, or 2^-126)
+  // (a missing row's scales are those of zeros: 0, or 2^-126; NaN where the caller's tensor scale is no scale)
   const int nb = a.nv ? a.units : a.units / 2;
+  const float ts1 = a.ts != nullptr ? *a.ts : 1.f;
+  const uint32_t zeros = !a.nv ? 0x01010101u : ts1 > 0.f && ts1 < INFINITY ? 0u : 0x7F7F7F7Fu;
 #pragma unroll 4
   for (int i = lane; i < a.atoms; i += 32) {
-    const uint32_t none = a.nv ? 0u : 0x01010101u >> (8 * max(0, 4 - (nb - 4 * i)));
+    const uint32_t none = zeros >> (8 * max(0, 4 - (nb - 4 * i)));
     *reinterpret_cast<uint32_t*>(sr + (int64_t)i * 512) = has ? __ldg(w + i) : none;
   }
   if (a.row_ts != nullptr && lane == 0) a.row_ts[row] = has ? ts[src] : 1.17549435e-38f;

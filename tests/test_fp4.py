@@ -776,3 +776,17 @@ def test_pack_of_views(fmt):
     assert torch.equal(fp4.grouped_gemm(a, fp4.pack(fmt, apart(codes), apart(s), t)), want)
     c = codes.cuda()
     assert fp4.pack(fmt, c, s.cuda(), t).codes.data_ptr() == c.data_ptr()
+
+
+@gpu
+@pytest.mark.parametrize("n", [8, 1 << 17])
+@pytest.mark.parametrize("ts", [math.nan, 0.0, -1.0, math.inf])
+def test_rows_under_a_tensor_scale_that_is_none(ts, n):
+    """NaN, in a small gather and in one that quantises its source rows once; missing rows and rows of zeros too."""
+    _need_gpu()
+    x = _acts(7, 80, torch.bfloat16).cuda()
+    x[1] = 0
+    rows = torch.arange(n) % 8
+    rows = torch.where(rows == 7, -1, rows).to(torch.int32).cuda()
+    q = fp4.quant(x, NV, tensor_scale=torch.tensor([ts], device="cuda"), rows=rows)
+    assert bool((q.canonical_scales()[:, :5] == 0x7F).all()) and bool(fp4.dequant(q).isnan().all())
