@@ -289,7 +289,8 @@ int sb_fp4_grouped_gemm(int fmt, const void* a_codes, const void* a_scales, cons
                         const float* w_ts, int w_ts_n, int64_t n_experts, int64_t n, int64_t k, int swiglu,
                         float limit, const float* row_weight, void* y, int dtype, int64_t ldy, void* stream);
 /* *host_out = 1 if a kernel of the two products gave up a bounded wait on the current device since the
- * last call (outputs since then may be incomplete), else 0. Synchronises the stream. */
+ * last call (outputs since then may be incomplete), or found offsets that descend (it then writes nothing), else
+ * 0. Synchronises the stream. */
 int sb_fp4_error(int* host_out, void* stream);
 
 /* ── routing from the caller's logits ───────────────────────────────────────────────────────────── */

@@ -18,7 +18,7 @@
 // readback overlaps the next tile's products: of up to 192 columns each, or in pairs of 256, which share 64
 // columns to leave room for the scales; the readback begins with those and releases them at once.
 //
-// Every wait is bounded: on timeout the CTA sets the device's error word and winds down.
+// Every wait is bounded: on timeout the CTA sets the device's error word and winds down. Offsets that descend set it, too.
 #include <cudaTypedefs.h>
 #include <string.h>
 
@@ -553,9 +553,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
     // tiles before each matrix
     const int nb = (g.n + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
     int run = 0;
+    bool down = false;
     for (int m0 = 0; m0 < g.mats; m0 += 32) {
       const int m = m0 + lane;
-      const int r0 = m < g.mats ? group_begin(g, m) : 0, cnt = m < g.mats ? max(group_begin(g, m + 1) - r0, 0) : 0;
+      const int r0 = m < g.mats ? group_begin(g, m) : 0, cnt = m < g.mats ? group_begin(g, m + 1) - r0 : 0;
+      down |= cnt < 0;
       const int v = (cnt + a.nt - 1) / a.nt * nb;
       int inc = v;
 #pragma unroll
@@ -570,7 +572,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
       }
       run += __shfl_sync(0xffffffffu, inc, 31);
     }
-    if (lane == 0) c.tiles[g.mats] = run;
+    // Offsets that descend name rows more than once, in all perhaps more than the tiles can be counted: no tile is made.
+    down = __any_sync(0xffffffffu, down);
+    if (lane == 0) c.tiles[g.mats] = down ? 0 : run;
+    if (lane == 0 && down) atomicExch(&g_err, 1);
   }
   fence_before();
   __syncthreads();

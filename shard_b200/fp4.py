@@ -285,7 +285,8 @@ def grouped_gemm(a: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bflo
 
 
 def device_error(device=None) -> int:
-    """1 if a product's kernel gave up a bounded wait on the device since the last call, else 0. Synchronises."""
+    """1 if a product's kernel gave up a bounded wait on the device since the last call, or found offsets that descend
+    (it then writes nothing), else 0. Synchronises."""
     with torch.cuda.device(device):
         v = ctypes.c_int(0)
         check(lib().sb_fp4_error(ctypes.byref(v), torch.cuda.current_stream().cuda_stream), "sb_fp4_error")

@@ -790,3 +790,23 @@ def test_rows_under_a_tensor_scale_that_is_none(ts, n):
     rows = torch.where(rows == 7, -1, rows).to(torch.int32).cuda()
     q = fp4.quant(x, NV, tensor_scale=torch.tensor([ts], device="cuda"), rows=rows)
     assert bool((q.canonical_scales()[:, :5] == 0x7F).all()) and bool(fp4.dequant(q).isnan().all())
+
+
+@gpu
+@pytest.mark.parametrize("offsets", [[0, 5, 3, 9], [9, 0, 9, 0], [0, 9, 9, -4], [0, 2 ** 31 - 1, -2 ** 31, 9]])
+def test_offsets_that_descend(offsets):
+    """They name rows more than once: nothing is written, and the error word says so. Ends outside the rows are cut."""
+    _need_gpu()
+    codes, s, ts, _ = P.weights(NV, 40, 64, seed=5, mats=3)
+    bank = fp4.pack(NV, codes.cuda(), s.cuda(), ts.cuda())
+    x = _acts(9, 64, torch.bfloat16).cuda()
+    assert fp4.device_error() == 0
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    out = torch.full((9, 40), 3.0, dtype=torch.bfloat16, device="cuda")
+    fp4.grouped_gemm(fp4.quant(x, NV, offsets=off), bank, out=out)
+    assert bool((out == 3).all()) and fp4.device_error() == 1 and fp4.device_error() == 0
+    good = torch.tensor([0, 4, 9, 9], dtype=torch.int32, device="cuda")
+    a = fp4.quant(x, NV, offsets=good)
+    want = fp4.grouped_gemm(a, bank)
+    a.offsets = torch.tensor([0, 4, 12, 15], dtype=torch.int32, device="cuda")
+    assert torch.equal(fp4.grouped_gemm(a, bank)[:9], want) and fp4.device_error() == 0
