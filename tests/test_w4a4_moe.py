@@ -107,3 +107,29 @@ def test_a_given_stream_orders_the_call():
     h = fp4.grouped_gemm(a, w13, stream=st)
     st.synchronize()
     assert torch.equal(h, want[2]) and torch.equal(ids, want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [F.FMT_NVFP4, F.FMT_MXFP4])
+def test_moe_with_dropped_pairs(fmt):
+    """Ids outside the experts (dropped tokens, padding) add nothing, whatever the rows that no expert wrote hold."""
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    x, logits, bias, w13, w2, _, _ = _setup(fmt, 40)
+    x, logits, bias = x.cuda(), logits.cuda(), bias.cuda()
+    w, ids = route.topk(logits, K, bias=bias, n_group=4, topk_group=2, group_score="top2")
+
+    def run(ids, w):
+        o = route.expert_order(ids, E)
+        h = fp4.grouped_gemm(fp4.quant(x, fmt, rows=o.tokens, offsets=o.offsets), w13)
+        out = torch.full((ids.numel(), H), float("nan"), device="cuda")
+        fp4.grouped_gemm(fp4.quant(h, fmt, offsets=o.offsets), w2, out_dtype=torch.float32, out=out)
+        at = o.places.long()[..., None]
+        return torch.where(at >= 0, out[at[..., 0]] * w[..., None], 0).sum(1)
+
+    whole = run(ids, w)
+    drop = torch.zeros(40, K, dtype=torch.bool, device="cuda")
+    drop[3], drop[7, 1], drop[20:24, 2:], drop[39, 3] = True, True, True, True
+    part = run(torch.where(drop, -1, ids), w)
+    kept = run(ids, w * ~drop)
+    assert torch.equal(part, kept) and bool((part[3] == 0).all()) and torch.equal(part[0], whole[0])
