@@ -186,8 +186,11 @@ __device__ __forceinline__ uint32_t in_first(uint32_t addr) {
   asm("mapa.shared::cluster.u32 %0, %1, 0;\n" : "=r"(r) : "r"(addr));
   return r;
 }
-// Without release: what it follows are reads of tensor memory, whose values this thread holds. (A release at cluster scope
-// waits for the stores to y before it: 1000 cycles twice a tile, in the readback and in the products that wait for it.)
+// Without release: what it follows are reads of tensor memory, complete at tcgen05.wait::ld in every lane (their values are in
+// registers) and ordered before the arrival by fence::before_thread_sync and, between the lanes, __syncwarp. It hands over
+// nothing else: a read or write of shared or global memory that the other CTA had to see or wait for would need a release
+// here. (A release at cluster scope waits for the stores to y before it: 1000 cycles twice a tile, in the readback and
+// in the products that wait for it.)
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
@@ -322,7 +325,8 @@ __device__ __forceinline__ uint4 read_turned(uint32_t addr) {
 }
 
 // silu(gate) * up of one pair of rows: the even lane holds gate, the odd lane up, of two tokens; each lane
-// gets one of the tokens' results
+// gets one of the tokens' results. The fast exponential and division are off by |gate| 2^-23 + 2^-20 of the result (less
+// than a rounding to 16 bits); for gates below -87, where silu is below 1e-35, the division may give 0.
 __device__ __forceinline__ float gated(float v0, float v1, int lane, float lim) {
   const float o = __shfl_xor_sync(0xffffffffu, (lane & 1) ? v0 : v1, 1);
   const float gate = clamp_hi((lane & 1) ? o : v0, lim), up = clamp_lo(clamp_hi((lane & 1) ? v1 : o, lim), -lim);

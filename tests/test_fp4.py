@@ -810,3 +810,41 @@ def test_offsets_that_descend(offsets):
     want = fp4.grouped_gemm(a, bank)
     a.offsets = torch.tensor([0, 4, 12, 15], dtype=torch.int32, device="cuda")
     assert torch.equal(fp4.grouped_gemm(a, bank)[:9], want) and fp4.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", [NV, MX])
+@pytest.mark.parametrize("e,t,k,n,kind", [(256, 16, 1024, 512, fp4.W13), (384, 16, 512, 256, fp4.PLAIN), (384, 700, 512, 256, fp4.W13),
+                                          (1024, 300, 64, 64, fp4.PLAIN)])
+def test_banks_of_many_experts(fmt, e, t, k, n, kind):
+    """Verify chunks and larger ones over banks of as many experts as layers have, through the order of their routed pairs."""
+    _need_gpu()
+    h = 2 if kind == fp4.W13 else 1
+    codes, s, ts, _ = P.weights(fmt, n, k, seed=e, mats=e, halves=h)
+    codes, s, ts = codes.cuda(), s.cuda(), None if ts is None else ts.cuda()
+    g = torch.Generator().manual_seed(e + t)
+    ids = torch.stack([torch.randperm(e, generator=g)[:8] for _ in range(t)]).cuda()
+    o = route.expert_order(ids, e)
+    x = (_acts(t, k, torch.bfloat16, seed=t, spread=0.3) * 0.02).to(torch.bfloat16).cuda()
+    a = fp4.quant(x, fmt, rows=o.tokens, offsets=o.offsets)
+    y = fp4.grouped_gemm(a, fp4.pack(fmt, codes, s, ts, kind=kind), out_dtype=torch.float32).double()
+    av = fp4.dequant(fp4.quant(x, fmt), torch.float32).double()[o.tokens.long()]
+    off = o.offsets.tolist()
+    for i in range(e):
+        lo, hi = off[i], off[i + 1]
+        if lo == hi:
+            continue
+        half = lambda v, j: v[i, j * (n // h):(j + 1) * (n // h)]  # noqa: E731
+        w = torch.cat([fp4.dequant(fp4.pack(fmt, half(codes, j), half(s, j), None if ts is None else ts[i, j:j + 1]), torch.float32)
+                       for j in range(h)]).double()
+        r = av[lo:hi] @ w.T
+        # (values of 32 bits: each 2^-24 off, two in a product)
+        tol = _tol(av[lo:hi], w, r, k, torch.float32) + 2.0 ** -22 * (av[lo:hi].abs() @ w.abs().T)
+        if h == 2:
+            gate, up, dg, du = r[:, :n // 2], r[:, n // 2:], tol[:, :n // 2], tol[:, n // 2:]
+            silu = gate / (1 + torch.exp(-gate))
+            r = silu * up
+            tol = 1.1 * dg * up.abs() + silu.abs() * du + \
+                torch.where(gate > -87, gate.abs() * 2.0 ** -23 + 2.0 ** -20, 1.01) * r.abs() + 2.0 ** -149
+        assert bool(((y[lo:hi] - r).abs() <= tol).all()), f"expert {i}"
+    assert fp4.device_error() == 0
