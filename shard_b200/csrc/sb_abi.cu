@@ -1128,7 +1128,8 @@ int fp4_product(const char* what, int fmt, int dtype, const void* const* ptrs, i
 
 size_t sb_fp4_scale_bytes(int fmt, int64_t n_mat, int64_t rows, int64_t k, int64_t groups) {
   if (!fp4_fmt(fmt) || n_mat < 1 || rows < 0 || rows > FP4_MAX_ROWS || n_mat > FP4_MAX_ROWS || k < 1 ||
-      k > FP4_MAX_K || groups < 0 || groups > FP4_MAX_GROUPS || (groups > 0 && n_mat != 1) || (rows > 0 && n_mat > FP4_MAX_ROWS / rows))
+      k > FP4_MAX_K || groups < 0 || groups > FP4_MAX_GROUPS || (groups > 0 && n_mat != 1) ||
+      (rows > 0 && n_mat > FP4_MAX_ROWS / rows))
     return 0;
   return (size_t)fp4_blocks(n_mat, rows, groups) * (size_t)fp4_atoms(fmt, k) * 512;
 }

@@ -131,7 +131,8 @@ PyObject* quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Tensor ws;
   if (need) ws = empty({(int64_t)need}, at::kByte, x);
   // (a gather of no rows has no pointer, which the entry takes for none: no source rows, then)
-  const int rc = sb_fp4_quant(fmt, z.data_ptr(), dt, rows && p == 0 ? 0 : m, k, m > 1 ? z.stride(0) : k, rp, p, tp, op, groups, base, base + end,
+  const int64_t src = rows && p == 0 ? 0 : m;
+  const int rc = sb_fp4_quant(fmt, z.data_ptr(), dt, src, k, m > 1 ? z.stride(0) : k, rp, p, tp, op, groups, base, base + end,
                               per_row ? reinterpret_cast<float*>(base + atoms_end) : nullptr, need ? ws.data_ptr() : nullptr, need,
                               current_stream(x));
   if (rc != SB_OK) return status(rc);

@@ -228,7 +228,8 @@ __device__ __forceinline__ void scores32(const float (&l)[C], float mx, float rs
 // sqrtsoftplus 5; softmax 4 for the exponential and its argument, 3 for the division, 20 for the exponentials in
 // the sum (each 2 (2 + 1.173 d) and d for its argument, d below the largest logit; of 1024 experts at one d the mean
 // is largest at d = 5.4) and C + 4 for the C + 5 additions of a lane and the warp; the factor of 6.1e-8 is 2% above
-// 2^-24. Where all scores are tiny: 2.4e-38 for one that counts as 0. value +- of(value) ascends with the value, so that neighbours in a ranking are all that has to be compared.
+// 2^-24. Where all scores are tiny: 2.4e-38 for one that counts as 0. value +- of(value) ascends with the value, so that
+// neighbours in a ranking are all that has to be compared.
 struct Bound {
   float ks;   // k times the largest score
   __device__ __forceinline__ float rounding(float v) const { return 6.1e-8f * fminf(fabsf(v), FLT_MAX); }
@@ -497,11 +498,12 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
   int mine = expert();
   if (biased) {
     // Neighbours in the ranking, to the first one left out: far enough apart, or the same logit and bias, whose
-    // order is that of their ids. Else all that may belong to the k best are ordered by their exact values.
+    // order is that of their ids (not at the last place: whoever comes behind the two is compared with neither).
+    // Else all that may belong to the k best are ordered by their exact values.
     const uint32_t nk = __shfl_down_sync(0xffffffffu, got, 1);
     const int ne = __shfl_down_sync(0xffffffffu, mine, 1);
     bool near = lane < a.topk && got > 1u && nk > 1u && !err.above(value_of(got), value_of(nk));
-    if (near && a.bias[mine] == a.bias[ne] && row[mine] == row[ne]) near = false;
+    if (near && lane + 1 < a.topk && a.bias[mine] == a.bias[ne] && row[mine] == row[ne]) near = false;
     if (__any_sync(0xffffffffu, near)) {
       const uint32_t last = __shfl_sync(0xffffffffu, got, a.topk - 1);
       uint32_t top = __shfl_sync(0xffffffffu, got, a.topk);

@@ -214,6 +214,22 @@ def test_topk_renormalised_weights_of_far_logits(score, dtype, lo, hi):
 
 
 @gpu
+@pytest.mark.parametrize("copies", [1, 2, 3, 17, 40])
+@pytest.mark.parametrize("k", [1, 2, 5, 16])
+def test_topk_equal_experts_before_a_better_one(copies, k):
+    """Experts of one logit and bias, whose fp32 sums are also that of experts behind them that are a little better: the equal
+    ones are in order among themselves, and still behind those."""
+    _need_gpu()
+    logits = torch.full((1, 128), -2.0)
+    bias = torch.zeros(128)
+    logits[0, :copies], bias[:copies] = -0.25, 0.562176525592804            # 1.0000000247
+    logits[0, 60:63], bias[60:63] = 0.5, 0.3775407075881958                 # 1.0000000388
+    logits[0, 100:100 + copies // 3], bias[100:100 + copies // 3] = -0.25, 0.562176525592804
+    for g, kept in ((1, 1), (8, 8)):
+        _check(logits, k, bias, n_group=g, topk_group=kept)
+
+
+@gpu
 def test_topk_strides_and_large_batches():
     _need_gpu()
     gen = torch.Generator().manual_seed(6)
