@@ -386,10 +386,12 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
     // This lane's experts that may be among their group's two best. (Four bounds of the second best: two of its own, and
     // two for an expert below it.)
     uint32_t near = 0u;
+    // (halves in place of sums: two biases of the lowest value add up to -inf, which is a masked group's)
+    const float part = a.group_two ? 0.5f : 1.f;
     auto group = [&](float b1, float b2, float& score, float& bound) {
       const bool two = a.group_two && b2 > -INFINITY;
-      score = two ? b1 + b2 : b1;
-      bound = two ? err.of(b1) + err.of(b2) + err.rounding(score) : err.of(b1);
+      score = part * b1 + (two ? part * b2 : 0.f);
+      bound = part * (err.of(b1) + (two ? err.of(b2) : 0.f)) + err.rounding(score);
     };
     if (a.span > 0) {
       float b1 = -INFINITY, b2 = -INFINITY;

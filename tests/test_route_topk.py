@@ -230,6 +230,29 @@ def test_topk_equal_experts_before_a_better_one(copies, k):
 
 
 @gpu
+@pytest.mark.parametrize("e,g", [(64, 8), (60, 4), (16, 8)])
+def test_topk_group_sums_below_the_range(e, g):
+    """Groups whose two best have a bias of fp32's lowest value come behind the others and before masked ones, in the order of
+    their real sums."""
+    _need_gpu()
+    gen = torch.Generator().manual_seed(e)
+    s = e // g
+    logits = torch.randn(12, e, generator=gen)
+    low = torch.finfo(torch.float32).min
+    bias = torch.full((e,), low)
+    for own, factor in ((0, 1.0), (1, 1.0), (1, 0.75), (2, 0.75)):
+        b = bias.clone()
+        b[:own * s] = 0.1 * torch.randn(own * s, generator=gen)
+        b[s * (g - 1):] = low * factor
+        l = logits.clone()
+        l[3:6, s:2 * s] = -math.inf
+        l[6:9, s + 1:2 * s] = -math.inf
+        l[9:, : s * (g - 1)] = -math.inf
+        for kept in range(1, g):
+            _check(l, min(6, kept * s), b, n_group=g, topk_group=kept, group_score="top2")
+
+
+@gpu
 def test_topk_strides_and_large_batches():
     _need_gpu()
     gen = torch.Generator().manual_seed(6)
