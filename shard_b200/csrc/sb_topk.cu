@@ -500,19 +500,23 @@ __device__ __forceinline__ int select(const TopkArgs& a, const T* row, const flo
   int mine = expert();
   if (biased) {
     // Neighbours in the ranking, to the first one left out: far enough apart, or the same logit and bias, whose
-    // order is that of their ids (not at the last place: whoever comes behind the two is compared with neither).
-    // Else all that may belong to the k best are ordered by their exact values.
+    // order is that of their ids. Else all that may belong to the k best are ordered by their exact values.
     const uint32_t nk = __shfl_down_sync(0xffffffffu, got, 1);
     const int ne = __shfl_down_sync(0xffffffffu, mine, 1);
-    bool near = lane < a.topk && got > 1u && nk > 1u && !err.above(value_of(got), value_of(nk));
-    if (near && lane + 1 < a.topk && a.bias[mine] == a.bias[ne] && row[mine] == row[ne]) near = false;
-    if (__any_sync(0xffffffffu, near)) {
+    const bool near = lane < a.topk && got > 1u && nk > 1u && !err.above(value_of(got), value_of(nk));
+    const bool other = near && !(a.bias[mine] == a.bias[ne] && row[mine] == row[ne]);
+    const uint32_t others = __ballot_sync(0xffffffffu, other), nears = __ballot_sync(0xffffffffu, near);
+    if (others != 0u || ((nears >> (a.topk - 1)) & 1u)) {
       const uint32_t last = __shfl_sync(0xffffffffu, got, a.topk - 1);
       uint32_t top = __shfl_sync(0xffffffffu, got, a.topk);
       int n = rounds;
       while (n < 32 && last > 1u && top > 1u && !err.above(value_of(last), value_of(top))) top = round(n++);
       if (last > 1u && top > 1u && !err.above(value_of(last), value_of(top))) return select_exact<C, T>(a, row, lane, lowest);
       mine = expert();
+      // nothing but equals of the last one behind it: the ids order them, too
+      const int ml = __shfl_sync(0xffffffffu, mine, a.topk - 1);
+      const bool apart = lane >= a.topk && lane < n - 1 && !(a.bias[mine] == a.bias[ml] && row[mine] == row[ml]);
+      if (others == 0u && !__any_sync(0xffffffffu, apart)) return mine;
       mine = order_exact<C, T>(a, row, lane, lowest, mx, mine, lane < n ? (got > 1u ? 2 : (int)got) : 0, n);
     }
   }
