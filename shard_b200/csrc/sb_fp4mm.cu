@@ -439,6 +439,7 @@ __device__ __forceinline__ void store_chunk(const Args& a, const uint32_t (&d)[3
       }
     }
   }
+  __syncwarp();   // the warp's next read of tensor memory needs all of its lanes
 }
 
 // The same for an odd_row or odd_cols, in 64 bits, where s w is exact and the result rounds once. False, and nothing is done,
@@ -490,6 +491,7 @@ __device__ __noinline__ bool store_wide(const Args& a, Chunk v, int64_t tok, int
         if (in && j + m < left) yp[(j + m) * g.ldy + row] = to_out<T>(h[m]);
     }
   }
+  __syncwarp();
   return true;
 }
 
