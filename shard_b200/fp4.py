@@ -130,7 +130,7 @@ class Fp4Tensor:
         return self._ts
 
     def canonical_scales(self) -> torch.Tensor:
-        """uint8 [mats * rows, K / 16 or K / 32]: the scales row by row (no expert groups)."""
+        """uint8 [mats * rows, kp / 16 or kp / 32]: the scales row by row (no expert groups)."""
         if self.offsets is not None:
             raise ValueError("canonical_scales: rows in expert groups")
         nb = self.codes.shape[1] // (8 if self.fmt == F.FMT_NVFP4 else 16)
@@ -188,7 +188,7 @@ def pack(fmt: Union[int, str], codes: torch.Tensor, scales: torch.Tensor, ts: Op
          kind: int = PLAIN, stream=None) -> Fp4Tensor:
     """Canonical weights -> operand, once at load time. codes uint8 [N, K/2] or [E, N, K/2], scales as bytes or
     in their own type [.., K/16] (NVFP4) / [.., K/32] (MXFP4), ts fp32: one per matrix, or for w13 banks
-    [E, 2] (w1, w3). K % 32 == 0. kind W13: the rows are w1's, then w3's; they are interleaved, so that one
+    [E, 2] (w1, w3). K is whole blocks of scales (16 or 32; rows are padded to 32 with zeros). kind W13: the rows are w1's, then w3's; they are interleaved, so that one
     pass of grouped_gemm forms silu(w1 x) * (w3 x). PLAIN operands share the codes given, if these are contiguous and
     16-byte aligned."""
     f = _fmt(fmt)
@@ -202,9 +202,10 @@ def pack(fmt: Union[int, str], codes: torch.Tensor, scales: torch.Tensor, ts: Op
         if t is not None and t.device != codes.device:
             raise ValueError(f"pack: tensors on {t.device} and {codes.device}")
     mats, n, k = (1 if c.dim() == 2 else c.shape[0]), c.shape[-2], 2 * c.shape[-1]
-    nb = k // (16 if f == F.FMT_NVFP4 else 32)
-    if k % 32 or tuple(s.shape) != (*c.shape[:-1], nb):
-        raise ValueError(f"pack: scales {tuple(s.shape)} for codes {tuple(c.shape)} (K % 32 == 0 is needed)")
+    block = 16 if f == F.FMT_NVFP4 else 32
+    nb = k // block
+    if k % block or tuple(s.shape) != (*c.shape[:-1], nb):
+        raise ValueError(f"pack: scales {tuple(s.shape)} for codes {tuple(c.shape)} (K % {block} == 0 is needed)")
     if ts is not None:
         if f != F.FMT_NVFP4:
             raise ValueError("pack: MXFP4 has no tensor scale")
@@ -213,15 +214,18 @@ def pack(fmt: Union[int, str], codes: torch.Tensor, scales: torch.Tensor, ts: Op
             raise ValueError(f"pack: {ts.shape[1]} tensor scales a matrix")
     if kind not in (PLAIN, W13) or (kind == W13 and n % 2):
         raise ValueError("pack: kind is PLAIN, or W13 with an even number of rows")
-    c, s = c.reshape(mats, n, k // 2), s.reshape(mats, n, nb)
+    kp = -(-k // 32) * 32
+    if kp != k:
+        c, s = torch.nn.functional.pad(c, (0, (kp - k) // 2)), torch.nn.functional.pad(s, (0, (kp - k) // block))
+    c, s = c.reshape(mats, n, kp // 2), s.reshape(mats, n, kp // block)
     if kind == W13:
         c, s = (t.view(mats, 2, n // 2, -1).transpose(1, 2).reshape(mats, n, -1) for t in (c, s))
-    c, s = c.contiguous().view(mats * n, k // 2), s.contiguous()
+    c, s = c.contiguous().view(mats * n, kp // 2), s.contiguous()
     if c.data_ptr() % 16:                 # (a view into a larger buffer: the products copy from 16-byte addresses)
         c = c.clone()
     L = lib()
-    out = torch.empty(L.sb_fp4_scale_bytes(f, mats, n, k, 0), dtype=torch.uint8, device=c.device)
-    check(L.sb_fp4_tile_scales(f, s.data_ptr(), out.data_ptr(), mats, n, k, torch.cuda.current_stream().cuda_stream),
+    out = torch.empty(L.sb_fp4_scale_bytes(f, mats, n, kp, 0), dtype=torch.uint8, device=c.device)
+    check(L.sb_fp4_tile_scales(f, s.data_ptr(), out.data_ptr(), mats, n, kp, torch.cuda.current_stream().cuda_stream),
           "sb_fp4_tile_scales")
     return Fp4Tensor(f, mats, n, k, c, out, ts, None, kind, tuple(codes.shape[:-1]))
 

@@ -848,3 +848,34 @@ def test_banks_of_many_experts(fmt, e, t, k, n, kind):
                 torch.where(gate > -87, gate.abs() * 2.0 ** -23 + 2.0 ** -20, 1.01) * r.abs() + 2.0 ** -149
         assert bool(((y[lo:hi] - r).abs() <= tol).all()), f"expert {i}"
     assert fp4.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("k", [16, 48, 4112])
+def test_pack_of_nvfp4_rows_that_end_inside_a_block_of_32(k):
+    """K = 16 more than a multiple of 32: the operand, its values, and products with activations of that K."""
+    _need_gpu()
+    codes, s, ts, wv = P.weights(NV, 72, k, seed=k, mats=3, halves=2)
+    c, sc, t = codes.cuda(), s.cuda(), ts.cuda()
+    one = fp4.pack(NV, c[0, :36], sc[0, :36], t[0, :1])
+    assert one.k == k and torch.equal(fp4.dequant(one, torch.float32).cpu(), wv[0, :36].float())
+    x = (_acts(40, k, torch.bfloat16, seed=k, spread=0.3) * 0.05).to(torch.bfloat16)
+    a = fp4.quant(x.cuda(), NV)
+    av = _values(a)[:, :k]
+    exact = av @ wv[0, :36].T
+    assert bool(((fp4.gemm(a, one, out_dtype=torch.float32).cpu().double() - exact).abs()
+                 <= _tol(av, wv[0, :36], exact, k, torch.float32)).all())
+    off = torch.tensor([0, 7, 7, 40], dtype=torch.int32, device="cuda")
+    y = fp4.grouped_gemm(fp4.quant(x.cuda(), NV, offsets=off), fp4.pack(NV, c, sc, t, kind=fp4.W13), out_dtype=torch.float32)
+    for i, (lo, hi) in enumerate(((0, 7), (7, 7), (7, 40))):
+        r = av[lo:hi] @ wv[i].T
+        d = _tol(av[lo:hi], wv[i], r, k, torch.float32)
+        gate, up, dg, du = r[:, :36], r[:, 36:], d[:, :36], d[:, 36:]
+        silu = gate / (1 + torch.exp(-gate))
+        tol = 1.1 * dg * up.abs() + silu.abs() * du + \
+            torch.where(gate > -87, gate.abs() * 2.0 ** -23 + 2.0 ** -20, 1.01) * (silu * up).abs() + 2.0 ** -149
+        assert bool(((y[lo:hi].cpu().double() - silu * up).abs() <= tol).all())
+    with pytest.raises(ValueError, match="32"):
+        fp4.pack(MX, c[0], torch.zeros(72, k // 32 + 1, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(ValueError, match="16"):
+        fp4.pack(NV, c[0, :, :4].contiguous(), sc[0, :, :0].contiguous())
