@@ -346,8 +346,9 @@ __device__ __forceinline__ bool odd_col(float s) { return !(fabsf(s) >= 1.175494
 // shared memory. 16-bit outputs go through the warp's `turn` in shared memory, rows of 32 tokens in, tokens of up to
 // 8 neighbouring rows out, the 16-byte pieces of a row placed so that neither side meets a bank conflict. This
 // readback bounds tiles of K <= 1024 (690 cycles a chunk, gated 1330; a stage takes 520): 8192 x 4096 x 2048 took 62 us
-// turned by shuffles (32 of them a chunk, against 8 accesses so), 46 at the time, now 34; with a 2-byte store per row and column a tile of 192 columns took 8.5 us. FULL: a whole
-// chunk, without a branch per group of columns, which would keep the groups from overlapping.
+// turned by shuffles (32 of them a chunk, against 8 accesses so), 46 at the time, now 34; with a 2-byte store per row and
+// column a tile of 192 columns took 8.5 us. FULL: a whole chunk, without a branch per group of columns, which would
+// keep the groups from overlapping.
 template <bool SWIGLU, bool FULL, typename T>
 __device__ __forceinline__ void store_chunk(const Args& a, const uint32_t (&d)[32], int64_t tok, int row, int lane, int left,
                                             bool vec, float wts, const float* sc, const float* wt, uint32_t turn) {
@@ -790,8 +791,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) fp4_mm_kernel(const __grid_consta
                                     g.row_weight != nullptr ? wt[32 * j + lane] : 1.f, reinterpret_cast<float*>(c.turn[warp])))
             continue;
         }
-        if (left >= 32) store_chunk<SWIGLU, true, T>(a, d, tok0 + ch * 32, row, lane, 32, vec, wts, sc + 32 * j, wt + 32 * j, turn);
-        else store_chunk<SWIGLU, false, T>(a, d, tok0 + ch * 32, row, lane, left, vec, wts, sc + 32 * j, wt + 32 * j, turn);
+        if (left >= 32)
+          store_chunk<SWIGLU, true, T>(a, d, tok0 + ch * 32, row, lane, 32, vec, wts, sc + 32 * j, wt + 32 * j, turn);
+        else
+          store_chunk<SWIGLU, false, T>(a, d, tok0 + ch * 32, row, lane, left, vec, wts, sc + 32 * j, wt + 32 * j, turn);
       }
       if (mine <= 0) {
         fence_before();

@@ -188,9 +188,9 @@ def pack(fmt: Union[int, str], codes: torch.Tensor, scales: torch.Tensor, ts: Op
          kind: int = PLAIN, stream=None) -> Fp4Tensor:
     """Canonical weights -> operand, once at load time. codes uint8 [N, K/2] or [E, N, K/2], scales as bytes or
     in their own type [.., K/16] (NVFP4) / [.., K/32] (MXFP4), ts fp32: one per matrix, or for w13 banks
-    [E, 2] (w1, w3). K is whole blocks of scales (16 or 32; rows are padded to 32 with zeros). kind W13: the rows are w1's, then w3's; they are interleaved, so that one
-    pass of grouped_gemm forms silu(w1 x) * (w3 x). PLAIN operands share the codes given, if these are contiguous and
-    16-byte aligned."""
+    [E, 2] (w1, w3). K is whole blocks of scales (16 or 32; rows are padded to 32 with zeros). kind W13: the rows
+    are w1's, then w3's; they are interleaved, so that one pass of grouped_gemm forms silu(w1 x) * (w3 x). PLAIN
+    operands share the codes given, if these are contiguous, 16-byte aligned and not padded."""
     f = _fmt(fmt)
     if not codes.is_cuda or codes.dim() not in (2, 3):
         raise ValueError("pack: codes must be a CUDA tensor [N, K/2] or [E, N, K/2]")
